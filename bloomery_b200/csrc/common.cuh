@@ -28,6 +28,7 @@ enum FaultSite : unsigned {
   FS_PAGE = 6,
   FS_WAIT_TIMEOUT = 7,
   FS_SAMPLER = 8,
+  FS_BEAM = 9,
 };
 
 __device__ __forceinline__ void raise_fault(unsigned* fault, int layer, unsigned site) {

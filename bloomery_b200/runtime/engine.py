@@ -32,7 +32,7 @@ FAULT_CLEAN = 0xFFFFFFFF
 
 FAULT_SITES = {1: "token id out of range", 2: "non-finite activation", 3: "non-finite router logit",
                4: "expert id out of range", 5: "key count out of range", 6: "KV page missing",
-               7: "device wait ran out", 8: "sampler"}
+               7: "device wait ran out", 8: "sampler", 9: "beam reordering out of range"}
 
 
 class EngineFault(RuntimeError):
