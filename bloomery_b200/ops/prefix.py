@@ -52,11 +52,22 @@ class PrefixPlan:
         self.device = torch.device(device)
         if self.rows > 1024:
             raise ValueError("at most 1024 rows")
-        rows, first = [], 0
+        # units: the rows of a group that read its keys together, as many as two tiles of 128 (row, head) pairs of a key head hold
+        per = 128 // (n_q // n_kv)
+        rows, units, first = [], [], 0
         for n, p in zip(group_rows, prefix_len):
-            rows += [(first, n, p)] * n
+            for i in range(n):
+                u, at = (len(units) + i // (2 * per), i % (2 * per)) if p else (-1, 0)
+                rows.append((first, n, p, u, at // per * 128 + at % per * (n_q // n_kv)))
+            if p:
+                units += [(first + i, min(2 * per, n - i), p, first, n) for i in range(0, n, 2 * per)]
             first += n
-        self.meta = torch.tensor(rows, dtype=torch.int32).to(self.device)          # [rows][first row, rows, positions] of its group
+        self.n_units = len(units)
+        self.meta = torch.tensor(rows + units, dtype=torch.int32).to(self.device)
+        self.n_cta = sm_count(self.device) if self.device.type == "cuda" else 1
+        fn = cuda().bl_prefix_work_bytes
+        fn.restype = ctypes.c_long
+        self.work = torch.empty(fn(head, n_q, n_kv, self.rows, self.n_units, self.n_cta), dtype=torch.uint8, device=self.device)
 
 
 def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, row_pos: torch.Tensor, row_seq: torch.Tensor,
@@ -85,7 +96,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if plan.max_prefix > block_table.shape[1] * PAGE:
         raise ValueError("the prefix is longer than a table row")
     rc = _fn()(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), row_pos.data_ptr(), row_seq.data_ptr(), block_table.data_ptr(),
-               block_table.shape[0], block_table.shape[1], k_cache.shape[0], head, plan.n_q, n_kv, plan.rows, plan.meta.data_ptr(), 0, None,
-               1 if q8 else 0, out.data_ptr(), sm_count(plan.device), fault.data_ptr() if fault is not None else None, layer,
+               block_table.shape[0], block_table.shape[1], k_cache.shape[0], head, plan.n_q, n_kv, plan.rows, plan.meta.data_ptr(), plan.n_units, plan.work.data_ptr(),
+               1 if q8 else 0, out.data_ptr(), plan.n_cta, fault.data_ptr() if fault is not None else None, layer,
                torch.cuda.current_stream(plan.device).cuda_stream)
     check(rc, "bl_prefix_attention")
