@@ -16,103 +16,284 @@ namespace bl {
 
 constexpr int kMaxBeams = 64;
 
+constexpr int kBmThreads = 256;
+constexpr int kBmList = 512;                              // survivors that are ranked side by side
+constexpr int kBmMaxCells = 4096;                         // chunks of a row x beams: what one block merges
+
+struct BeamCell { float value; int id; };
+
 struct BeamArgs {
   const float* logits; long stride; int V, G, B;
   const float* scores;                                    // [G][B], -inf: no beam
   const int* done; const int* lengths;                    // optional [G][B]
   int eos; float alpha;
+  int n_chunks, chunk;                                    // of a row; values of a chunk (a multiple of 4 unless there is one)
+  BeamCell* cells;                                        // [G * B][n_chunks][B], best first
+  float2* sums;                                           // [G * B][n_chunks]: maximum, sum of exponentials
+  BeamCell* best;                                         // [G * B][B]
   double* lse;                                            // [G * B]
+  int* tickets;                                           // [G * B] chunks, then [G] rows; zero between calls
   int* parent; int* token; float* out_scores; int* out_done; int* out_lengths;
   unsigned* fault;
 };
 
-// grid (G * B), 512 threads: lse of a row; NaN where a logit is NaN or +inf
-__global__ void __launch_bounds__(512) beam_lse_kernel(const BeamArgs a) {
-  __shared__ float s_m[16];
-  __shared__ double s_l[16];
-  const int r = blockIdx.x, tid = threadIdx.x;
-  pdl_wait();
-  pdl_launch();
-  const float* x = a.logits + (long)r * a.stride;
-  if ((a.done && a.done[r]) || a.scores[r] == -INFINITY) return;
-  float m = -INFINITY;
-  bool bad = false;
-  for (int t = tid; t < a.V; t += 512) { bad |= !(x[t] < INFINITY); m = fmaxf(m, x[t]); }
-  m = warp_max(m);
-  if ((tid & 31) == 0) s_m[tid >> 5] = m;
-  bad = __syncthreads_or(bad);
-  for (int w = 0; w < 16; ++w) m = fmaxf(m, s_m[w]);
-  float l = 0.f;
-  if (m > -INFINITY) for (int t = tid; t < a.V; t += 512) l += expf(x[t] - m);
-  const double d = warp_sum_d((double)l);
-  if ((tid & 31) == 0) s_l[tid >> 5] = d;
+// The k best of a block's values, best first, ties to the lower id: store(rank, value, id) for each of the min(k, n) there are
+// (values of -inf are none).  A bound that k values at least reach comes from 8, 16, 32 or 64 groups of lanes, each of which
+// has a maximum: the smallest of them.  The few values from there on are listed and each counts the ones before it.  Data that
+// let more than the list through (an ascending row, say) are taken in k rounds instead.
+template <typename T, int E, typename Id, typename Store>
+__device__ __forceinline__ void block_best(const T (&v)[E], int k, T* s_value, int* s_id, T* s_group, int* s_n, Id id, Store store) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  const T none = (T)-INFINITY;
+  T mine = none;
+#pragma unroll
+  for (int i = 0; i < E; ++i) mine = v[i] > mine ? v[i] : mine;
+  const int lanes = k <= 8 ? 32 : k <= 16 ? 16 : k <= 32 ? 8 : 4;
+  T top = mine;
+  for (int o = lanes >> 1; o > 0; o >>= 1) { const T u = __shfl_xor_sync(0xffffffffu, top, o); top = u > top ? u : top; }
+  if ((lane & (lanes - 1)) == 0) s_group[tid / lanes] = top;
+  if (tid == 0) *s_n = 0;
   __syncthreads();
-  if (tid == 0) {
-    double all = 0.0;
-    for (int w = 0; w < 16; ++w) all += s_l[w];
-    a.lse[r] = bad ? (double)NAN : (double)m + log(all);
+  const int groups = kBmThreads / lanes;
+  T bound = s_group[lane % groups];
+  if (groups == 64) { const T u = s_group[lane + 32]; bound = u < bound ? u : bound; }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) { const T u = __shfl_xor_sync(0xffffffffu, bound, o); bound = u < bound ? u : bound; }
+  if (mine >= bound && mine > none) {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (v[i] >= bound && v[i] > none) {
+        const int at = atomicAdd(s_n, 1);
+        if (at < kBmList) { s_value[at] = v[i]; s_id[at] = id(i); }
+      }
   }
+  __syncthreads();
+  const int n = *s_n;
+  if (n <= kBmList) {
+    for (int e = tid; e < n; e += kBmThreads) {
+      const T value = s_value[e];
+      const int where = s_id[e];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += s_value[j] > value || (s_value[j] == value && s_id[j] < where);
+      if (rank < k) store(rank, value, where);
+    }
+    __syncthreads();
+    return;
+  }
+  T last = (T)INFINITY;
+  int last_id = -1;
+  for (int round = 0; round < k; ++round) {
+    T best = none;
+    int where = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int w = id(i);
+      if ((v[i] < last || (v[i] == last && w > last_id)) && (v[i] > best || (v[i] == best && v[i] > none && w < where))) { best = v[i]; where = w; }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const T u = __shfl_xor_sync(0xffffffffu, best, o);
+      const int w = __shfl_xor_sync(0xffffffffu, where, o);
+      if (u > best || (u == best && w < where)) { best = u; where = w; }
+    }
+    __syncthreads();
+    if (lane == 0) { s_value[tid >> 5] = best; s_id[tid >> 5] = where; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kBmThreads / 32; ++w)
+      if (s_value[w] > best || (s_value[w] == best && s_id[w] < where)) { best = s_value[w]; where = s_id[w]; }
+    if (best == none) break;
+    if (tid == 0) store(round, best, where);
+    last = best;
+    last_id = where;
+  }
+  __syncthreads();
 }
 
-// grid (G), 1024 threads: B rounds, each finds the best candidate behind the last one
-__global__ void __launch_bounds__(1024) beam_pick_kernel(const BeamArgs a) {
-  __shared__ double s_fac[kMaxBeams], s_key[32];
-  __shared__ long s_at[32];
-  const int g = blockIdx.x, tid = threadIdx.x, B = a.B, V = a.V, r0 = g * B;
+// True in the block that arrives last of `n`: what the others wrote before they arrived is visible to it.
+__device__ __forceinline__ bool block_last(int* ticket, int n, int* s_last) {
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    *s_last = atomicAdd(ticket, 1) == n - 1;
+    if (*s_last) *ticket = 0;                             // ready for the next call
+  }
+  __syncthreads();
+  const bool last = *s_last;
+  if (last) __threadfence();
+  return last;
+}
+
+// grid (n_chunks, G * B).  A block takes the sum of exponentials and the B best of a chunk; the last block of a row merges the
+// row's; the last row of a search ranks the B x B candidates that are left.
+template <int E>
+__global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamArgs a) {
+  __shared__ double s_value[kBmList], s_group[64], s_sum[8];
+  __shared__ double s_fac[kMaxBeams], s_lse[kMaxBeams];
+  __shared__ int s_id[kBmList], s_pick[kMaxBeams], s_n, s_last;
+  __shared__ float s_max[8], s_score[kMaxBeams];
+  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int B = a.B, V = a.V, g = r / B;
   pdl_wait();
   pdl_launch();
+  const bool over = a.done && a.done[r];
+  const float score = a.scores[r];
+  const bool reads = !over && score > -INFINITY;          // a beam with candidates among its logits
+  if (!reads && c > 0) return;
+  if (reads) {
+    const float* x = a.logits + (long)r * a.stride;
+    const int lo = c * a.chunk, hi = min(V, lo + a.chunk);
+    const bool vec = ((uintptr_t)x & 15) == 0;
+    float m = -INFINITY, sum = 0.f;                       // of what this thread has seen
+    float v[E + 1];                                       // a tile's values, and one of the best so far
+    v[E] = -INFINITY;
+    int carried = 0;
+    for (int t0 = lo; t0 < hi; t0 += E * kBmThreads) {
+      const int n = hi - t0;
+      if (vec) {
+#pragma unroll
+        for (int i = 0; i < E; i += 4) {
+          const int e = (tid + i / 4 * kBmThreads) * 4;
+          if (e + 4 <= n) {
+            const float4 q = __ldg(reinterpret_cast<const float4*>(x + t0 + e));
+            v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i + j] = e + j < n ? __ldg(x + t0 + e + j) : -INFINITY;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = tid + i * kBmThreads < n ? __ldg(x + t0 + tid + i * kBmThreads) : -INFINITY;
+      }
+      float top = v[0];
+#pragma unroll
+      for (int i = 1; i < E; ++i) top = fmaxf(top, v[i]);
+      top = fmaxf(top, m);
+      if (top > -INFINITY) {                              // NaN and +inf end up as a NaN of the sum
+        sum *= __expf(m - top);
+#pragma unroll
+        for (int i = 0; i < E; ++i) sum += __expf(v[i] - top);
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) sum += v[i] == -INFINITY ? 0.f : v[i];
+      }
+      m = top;
+      BeamCell* out = a.cells + ((long)r * a.n_chunks + c) * B;
+      block_best<float, E + 1>(v, B, reinterpret_cast<float*>(s_value), s_id, reinterpret_cast<float*>(s_group), &s_n,
+          [&](int i) { return i == E ? carried : t0 + (vec ? (tid + i / 4 * kBmThreads) * 4 + i % 4 : tid + i * kBmThreads); },
+          [&](int rank, float value, int id) { out[rank] = BeamCell{value, id}; });
+      const int had = min(B, s_n);
+      if (tid >= had && tid < B) out[tid] = BeamCell{-INFINITY, 0x7fffffff};
+      if (t0 + E * kBmThreads < hi) {                     // the best so far take part in the next tile's choice
+        __syncthreads();
+        v[E] = -INFINITY;
+        if (tid < had) { v[E] = out[tid].value; carried = out[tid].id; }
+        __syncthreads();
+      }
+    }
+    // the block's sum
+    float all = warp_max(m);
+    if (lane == 0) s_max[warp] = all;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) all = fmaxf(all, s_max[w]);
+    const double part = warp_sum_d(m > -INFINITY ? (double)(sum * __expf(m - all)) : (double)sum);
+    if (lane == 0) s_sum[warp] = part;
+    __syncthreads();
+    if (tid == 0) {
+      double l = 0.0;
+      for (int w = 0; w < 8; ++w) l += s_sum[w];
+      a.sums[(long)r * a.n_chunks + c] = make_float2(all, (float)l);
+    }
+    if (!block_last(a.tickets + r, a.n_chunks, &s_last)) return;
+    // ---- the row: its log-sum and the best of its chunks' best
+    const float2* sums = a.sums + (long)r * a.n_chunks;
+    float top = -INFINITY;
+    for (int i = tid; i < a.n_chunks; i += kBmThreads) top = fmaxf(top, __ldcg(sums + i).x);
+    top = warp_max(top);
+    if (lane == 0) s_max[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) top = fmaxf(top, s_max[w]);
+    double l = 0.0;
+    for (int i = tid; i < a.n_chunks; i += kBmThreads) {
+      const float2 s = __ldcg(sums + i);
+      l += s.x > -INFINITY ? (double)s.y * exp((double)s.x - (double)top) : (double)s.y;
+    }
+    l = warp_sum_d(l);
+    if (lane == 0) s_sum[warp] = l;
+    __syncthreads();
+    if (tid == 0) {
+      double total = 0.0;
+      for (int w = 0; w < 8; ++w) total += s_sum[w];
+      a.lse[r] = (double)top + log(total);                // -inf where every id is masked; NaN where a logit is not finite
+    }
+    constexpr int EC = kBmMaxCells / kBmThreads;
+    const BeamCell* cells = a.cells + (long)r * a.n_chunks * B;
+    float w[EC];
+    int at[EC];
+#pragma unroll
+    for (int i = 0; i < EC; ++i) {
+      const int e = tid + i * kBmThreads;
+      w[i] = -INFINITY;
+      at[i] = 0x7fffffff;
+      if (e < a.n_chunks * B) { const float2 q = __ldcg(reinterpret_cast<const float2*>(cells + e)); w[i] = q.x; at[i] = __float_as_int(q.y); }
+    }
+    BeamCell* best = a.best + (long)r * B;
+    block_best<float, EC>(w, B, reinterpret_cast<float*>(s_value), s_id, reinterpret_cast<float*>(s_group), &s_n,
+                          [&](int i) { return at[i]; }, [&](int rank, float value, int id) { best[rank] = BeamCell{value, id}; });
+    const int had = min(B, s_n);
+    if (tid >= had && tid < B) best[tid] = BeamCell{-INFINITY, 0x7fffffff};
+  }
+  if (!block_last(a.tickets + a.G * B + g, B, &s_last)) return;
+  // ---- the search
+  const int r0 = g * B;
   bool bad = false;
   if (tid < B) {
-    const int r = r0 + tid;
-    const bool over = a.done && a.done[r];
-    const float sc = a.scores[r];
-    bad = !(sc < INFINITY) || (!over && sc > -INFINITY && a.lse[r] != a.lse[r]);
-    s_fac[tid] = a.alpha != 0.f ? pow((double)max(1, a.lengths[r] + (over ? 0 : 1)), -(double)a.alpha) : 1.0;
+    const int q = r0 + tid;
+    const bool ended = a.done && a.done[q];
+    const float sc = a.scores[q];
+    s_score[tid] = sc;
+    s_lse[tid] = sc == -INFINITY || ended ? 0.0 : __ldcg(a.lse + q);
+    bad = !(sc < INFINITY) || s_lse[tid] != s_lse[tid];
+    s_fac[tid] = a.alpha != 0.f ? pow((double)max(1, a.lengths[q] + (ended ? 0 : 1)), -(double)a.alpha) : 1.0;
+    s_pick[tid] = -1;
   }
   bad = __syncthreads_or(bad);
-  double last = INFINITY;
-  long last_at = -1;
-  for (int i = 0; i < B; ++i) {
-    double best = -INFINITY;
-    long at = -1;
-    auto offer = [&](double key, long where) {
-      if (key > -INFINITY && (key < last || (key == last && where > last_at)) && (key > best || (key == best && where < at))) { best = key; at = where; }
-    };
-    for (int b = 0; !bad && b < B; ++b) {
-      const int r = r0 + b;
-      const double sc = a.scores[r];
-      if (sc == -INFINITY) continue;
-      if (a.done && a.done[r]) {
-        if (tid == 0) offer(sc * s_fac[b], (long)b * V + a.eos);
-        continue;
+  auto cand = [&](int b, float value) { return (double)s_score[b] + ((double)value - s_lse[b]); };
+  constexpr int EB = kMaxBeams * kMaxBeams / kBmThreads;
+  double v[EB];
+#pragma unroll
+  for (int i = 0; i < EB; ++i) {
+    const int e = tid + i * kBmThreads;
+    v[i] = -INFINITY;
+    if (!bad && e < B * B) {
+      const int b = e / B, j = e % B;
+      const bool ended = a.done && a.done[r0 + b];
+      if (s_score[b] > -INFINITY) {
+        if (ended) v[i] = j == 0 ? (double)s_score[b] * s_fac[b] : -INFINITY;
+        else {
+          const float value = __ldcg(&a.best[(long)(r0 + b) * B + j].value);
+          if (value > -INFINITY) v[i] = cand(b, value) * s_fac[b];
+        }
       }
-      for (int t = tid; t < V; t += 1024) offer((sc + ((double)a.logits[(long)r * a.stride + t] - a.lse[r])) * s_fac[b], (long)b * V + t);
     }
-    for (int o = 16; o > 0; o >>= 1) {
-      const double k = __shfl_xor_sync(0xffffffffu, best, o);
-      const long w = __shfl_xor_sync(0xffffffffu, at, o);
-      if (w >= 0 && (at < 0 || k > best || (k == best && w < at))) { best = k; at = w; }
-    }
-    __syncthreads();
-    if ((tid & 31) == 0) { s_key[tid >> 5] = best; s_at[tid >> 5] = at; }
-    __syncthreads();
-    for (int w = 0; w < 32; ++w)
-      if (s_at[w] >= 0 && (at < 0 || s_key[w] > best || (s_key[w] == best && s_at[w] < at))) { best = s_key[w]; at = s_at[w]; }
-    if (tid == 0) {
-      const int p = at < 0 ? i : (int)(at / V), t = at < 0 ? max(a.eos, 0) : (int)(at % V), r = r0 + p;
-      const bool over = a.done && a.done[r];
-      a.parent[r0 + i] = p;
-      a.token[r0 + i] = t;
-      a.out_scores[r0 + i] = bad ? __int_as_float(0x7fc00000) : at < 0 ? -INFINITY : over ? a.scores[r]
-                             : (float)((double)a.scores[r] + ((double)a.logits[(long)r * a.stride + t] - a.lse[r]));
-      if (a.out_done) a.out_done[r0 + i] = at < 0 || over || t == a.eos;
-      if (a.out_lengths) a.out_lengths[r0 + i] = a.lengths[r] + (at < 0 || over ? 0 : 1);
-      if (bad && i == 0) raise_fault(a.fault, 0, FS_SAMPLER);
-    }
-    last = best;
-    last_at = at;
-    if (at < 0) last = -INFINITY;
   }
+  // within a beam the places are in order of logit and id, so that of equal ranks the lower place comes first
+  block_best<double, EB>(v, B, s_value, s_id, s_group, &s_n, [&](int i) { return tid + i * kBmThreads; },
+                         [&](int rank, double value, int id) { s_pick[rank] = id; });
+  if (tid < B) {
+    const int e = s_pick[tid], b = e < 0 ? tid : e / B, q = r0 + b;
+    const bool ended = a.done && a.done[q];
+    const BeamCell cell = e < 0 || ended ? BeamCell{0.f, max(a.eos, 0)} : BeamCell{__ldcg(&a.best[(long)q * B + e % B].value), __ldcg(&a.best[(long)q * B + e % B].id)};
+    a.parent[r0 + tid] = b;
+    a.token[r0 + tid] = cell.id;
+    a.out_scores[r0 + tid] = bad ? __int_as_float(0x7fc00000) : e < 0 ? -INFINITY : ended ? s_score[b] : (float)cand(b, cell.value);
+    if (a.out_done) a.out_done[r0 + tid] = e < 0 || ended || cell.id == a.eos;
+    if (a.out_lengths) a.out_lengths[r0 + tid] = a.lengths[q] + (e < 0 || ended ? 0 : 1);
+  }
+  if (bad && tid == 0) raise_fault(a.fault, 0, FS_SAMPLER);
 }
 
 // ---- states -----------------------------------------------------------------------------------------------
@@ -200,17 +381,44 @@ using namespace bl;
 
 extern "C" {
 
+static void beam_chunks(int V, int rows, int B, int sms, int& tile, int& n, int& chunk) {
+  // 8,192 values a block cost less than 4,096 (the choice of the best is once a block) where both fill the processors
+  tile = (long)rows * ((V + 8191) / 8192) >= 2L * sms ? 8192 : 4096;
+  n = (V + tile - 1) / tile;
+  if (n > kBmMaxCells / B) n = kBmMaxCells / B;
+  chunk = ((V + n - 1) / n + 3) / 4 * 4;
+  n = (V + chunk - 1) / chunk;
+}
+
+// Bytes of scratch that bl_beam_select takes; zeroed once.
+long bl_beam_work_bytes(int V, int G, int B, int sms) {
+  int tile, n, chunk;
+  beam_chunks(V, G * B, B, sms, tile, n, chunk);
+  const long R = (long)G * B;
+  return R * 8 + R * n * 8 + R * n * B * 8 + R * B * 8 + (R + G) * 4;
+}
+
 int bl_beam_select(const float* logits, long stride, int V, int G, int B, const float* scores, const int* done, const int* lengths,
-                   int eos, float alpha, void* work, int* parent, int* token, float* out_scores, int* out_done, int* out_lengths,
-                   unsigned* fault, cudaStream_t st) {
-  BL_REQUIRE(V >= 1 && G >= 1 && B >= 1 && stride >= V, BL_ERR_SHAPE);
+                   int eos, float alpha, void* work, int sms, int* parent, int* token, float* out_scores, int* out_done,
+                   int* out_lengths, unsigned* fault, cudaStream_t st) {
+  BL_REQUIRE(V >= 1 && G >= 1 && B >= 1 && stride >= V && sms >= 1, BL_ERR_SHAPE);
   BL_REQUIRE(B <= kMaxBeams && (long)G * B <= 65535, BL_ERR_LIMIT);
   BL_REQUIRE(eos < V && (!done || eos >= 0) && (alpha == 0.f || lengths) && (!out_lengths || lengths), BL_ERR_SHAPE);
-  BeamArgs a{logits, stride, V, G, B, scores, done, lengths, eos, alpha, (double*)work, parent, token, out_scores, out_done,
-             out_lengths, fault};
-  cudaError_t e = launch(beam_lse_kernel, dim3(G * B), dim3(512), 0, st, a);
-  if (e != cudaSuccess) return (int)e;
-  return (int)launch(beam_pick_kernel, dim3(G), dim3(1024), 0, st, a);
+  BL_REQUIRE(((uintptr_t)logits & 3) == 0 && ((uintptr_t)work & 7) == 0, BL_ERR_ALIGN);
+  BeamArgs a{logits, stride, V, G, B, scores, done, lengths, eos, alpha};
+  int tile;
+  beam_chunks(V, G * B, B, sms, tile, a.n_chunks, a.chunk);
+  const long R = (long)G * B;
+  uint8_t* w = (uint8_t*)work;
+  a.lse = (double*)w; w += R * 8;
+  a.sums = (float2*)w; w += R * a.n_chunks * 8;
+  a.cells = (BeamCell*)w; w += R * a.n_chunks * B * 8;
+  a.best = (BeamCell*)w; w += R * B * 8;
+  a.tickets = (int*)w;
+  a.parent = parent; a.token = token; a.out_scores = out_scores; a.out_done = out_done; a.out_lengths = out_lengths; a.fault = fault;
+  const dim3 grid(a.n_chunks, (unsigned)R);
+  if (tile == 8192) return (int)launch(beam_select_kernel<32>, grid, dim3(kBmThreads), 0, st, a);
+  return (int)launch(beam_select_kernel<16>, grid, dim3(kBmThreads), 0, st, a);
 }
 
 int bl_beam_reorder(void* k, void* v, long k_row, long v_row, int n_layer, int n_pages, int n_kv, const int* table, int* table_out,

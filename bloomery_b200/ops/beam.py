@@ -8,6 +8,7 @@ import torch
 
 from ..runtime.kv import PAGE
 from ._lib import check, cuda
+from .decode import sm_count
 
 MAX_BEAMS = 64
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
@@ -36,7 +37,12 @@ class BeamScratch:
             raise ValueError(f"searches of 1 to {MAX_BEAMS} beams")
         self.groups, self.beams, self.vocab = groups, beams, vocab
         self.device = torch.device(device)
-        self.work = torch.zeros(groups * beams, dtype=torch.float64, device=self.device)
+        if groups * beams > 65535:
+            raise ValueError("at most 65,535 beams in all")
+        self.sms = sm_count(self.device) if self.device.type == "cuda" else 1
+        size = _fn("bl_beam_work_bytes", _I, _I, _I, _I)
+        size.restype = _L
+        self.work = torch.zeros(size(vocab, groups, beams, self.sms), dtype=torch.uint8, device=self.device)
 
 
 def _same(name: str, t: torch.Tensor, dtype, n: int) -> None:
@@ -73,9 +79,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, scratch: BeamScratch
         raise ValueError("finished beams need the id of the end")
     if lengths is None and (alpha != 0.0 or out_lengths is not None):
         raise ValueError("a rank by length needs the lengths")
-    fn = _fn("bl_beam_select", _P, _L, _I, _I, _I, _P, _P, _P, _I, _F, _P, _P, _P, _P, _P, _P, _P, _P)
+    fn = _fn("bl_beam_select", _P, _L, _I, _I, _I, _P, _P, _P, _I, _F, _P, _I, _P, _P, _P, _P, _P, _P, _P)
     check(fn(logits.data_ptr(), max(logits.stride(0), scratch.vocab), scratch.vocab, G, B, scores.data_ptr(), _ptr(done), _ptr(lengths), eos,
-             alpha, scratch.work.data_ptr(), parent.data_ptr(), token.data_ptr(), out_scores.data_ptr(), _ptr(out_done),
+             alpha, scratch.work.data_ptr(), scratch.sms, parent.data_ptr(), token.data_ptr(), out_scores.data_ptr(), _ptr(out_done),
              _ptr(out_lengths), _ptr(fault), torch.cuda.current_stream(scratch.device).cuda_stream), "bl_beam_select")
 
 
