@@ -52,22 +52,21 @@ class PrefixPlan:
         self.device = torch.device(device)
         if self.rows > 1024:
             raise ValueError("at most 1024 rows")
-        # units: the rows of a group that read its keys together, as many as two tiles of 128 (row, head) pairs of a key head hold
-        per = 128 // (n_q // n_kv)
+        # units: rows of a group that read all of their keys together, as many as two tiles of 128 (row, head) pairs of a key
+        # head hold
+        G = n_q // n_kv
+        per = 128 // G
         rows, units, first = [], [], 0
         for n, p in zip(group_rows, prefix_len):
-            for i in range(n):
-                u, at = (len(units) + i // (2 * per), i % (2 * per)) if p else (-1, 0)
-                rows.append((first, n, p, u, at // per * 128 + at % per * (n_q // n_kv)))
-            if p:
-                units += [(first + i, min(2 * per, n - i), p, first, n) for i in range(0, n, 2 * per)]
+            rows += [(first, n, p, len(units) + i // (2 * per), i % (2 * per) // per * 128 + i % per * G) for i in range(n)]
+            units += [(first + i, min(2 * per, n - i), p, first, n) for i in range(0, n, 2 * per)]
             first += n
         self.n_units = len(units)
         self.meta = torch.tensor(rows + units, dtype=torch.int32).to(self.device)
         self.n_cta = sm_count(self.device) if self.device.type == "cuda" else 1
         fn = cuda().bl_prefix_work_bytes
         fn.restype = ctypes.c_long
-        self.work = torch.empty(fn(head, n_q, n_kv, self.rows, self.n_units, self.n_cta), dtype=torch.uint8, device=self.device)
+        self.work = torch.empty(fn(head, n_kv, self.n_units, self.n_cta), dtype=torch.uint8, device=self.device)
 
 
 def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, row_pos: torch.Tensor, row_seq: torch.Tensor,

@@ -225,6 +225,36 @@ def test_rows_that_cannot_be_served_get_nan_and_a_fault():
         assert int(c.fault) == (3 << 8 | (6 if change == "page" else 5)), change
 
 
+@gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("bad", [NAN, math.inf, -math.inf])
+def test_what_one_row_holds_does_not_reach_another(bad, q8):
+    """Values and keys that are not finite, in one row's own pages and behind the end of a row inside the prefix."""
+    c = Case([(128, [100, 200, 150, 128, 260])], 32, 4, 128, q8, seed=16)
+    c.check(c.run())
+    want, tol = c.reference()
+    own, shared = c.rows[1][1][2], c.rows[1][1][1]
+    raw = torch.tensor([bad], dtype=torch.float16, device=DEV).view(torch.uint8) if q8 else bad
+    for cache in (c.k, c.v):
+        if q8:
+            cache[own, :, 3, :2] = raw
+            cache[own, :, 3, 8:40] = 1
+        else:
+            cache[own, :, 3] = raw
+    out = c.run()
+    fine = [0, 2, 3, 4]
+    assert ((out.double() - want).abs() - tol)[fine].max() <= 0
+    assert not torch.isfinite(out[1]).all()
+    if q8:
+        c.v[shared, :, 50, :2] = raw
+        c.v[shared, :, 50, 8:40] = 1
+    else:
+        c.v[shared, :, 50] = raw                       # position 114: behind row 0's end, seen by all others
+    out = c.run()
+    assert ((out.double() - want).abs() - tol)[0].max() <= 0
+    assert not torch.isfinite(out[2]).all()
+
+
 def _cpu_call(**kw):
     from bloomery_b200.ops.prefix import PrefixPlan, prefix_attention
     plan = PrefixPlan([2], [64], 4, 2, 64, "cpu")
