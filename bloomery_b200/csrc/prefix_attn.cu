@@ -13,12 +13,12 @@
 //   S = Q K^T     tcgen05.mma kind::f16, M = N = 128, into one of two score buffers in tensor memory
 //   softmax       one thread per query row; the probabilities go back as f16 into the score columns they came from
 //   O += P V      P from tensor memory, V as it lies in the cache: rows of keys, the MN-major form of a B operand
-// The scores of the job after the next are multiplied behind a job's second product, so that one job's softmax runs under the
-// products of its neighbours, whether two tiles of rows take turns or one goes on alone.
+// Two tiles of rows take a score buffer each, and one's softmax runs under the other's products; a tile that is alone takes both
+// in turn.
 // The work of a call is one line of tiles, unit after unit; every CTA takes an equal stretch of it, whatever the lengths, and
 // goes through the fragments that its stretch cuts.
 // Roles: warps 0..3 softmax of the first tile of rows, 4..7 of the second (warp id modulo 4 = TMEM lane quarter), warp 8 the TMA
-// producer (two-stage rings for keys and values, 128 KB in flight), warp 9 the MMA issuer and TMEM owner.
+// producer (two-stage rings for keys and values, 128 KB in flight), warps 9 and 10 the MMA issuers of either tile; 9 owns the TMEM.
 // Queries and probabilities are rounded to f16 (11 bits; queries scaled by a power of two a row): less than the output's 8 bits.
 // A value that is not finite would reach the masked rows of its tile as 0 x inf; rows whose output is not finite are summed again
 // key by key, over their own keys alone.
@@ -28,7 +28,7 @@
 namespace bl {
 
 constexpr int kPxPage = 64;
-constexpr int kPxMaxRows = 1024;
+constexpr int kPxMaxRows = 512;
 constexpr float kPxLog2e = 1.4426950408889634f;
 constexpr float kPxLazy = 8.0f;                         // the maximum may lag by 2^8 before the output is rescaled
 
@@ -118,6 +118,8 @@ struct PxLine {
   int* keys;                      // [M] keys of a row
   int* pages;                     // [M + 1] running sum of the rows' own pages
   int* tiles;                     // [n_units + 1] running sum of the units' tiles
+  int* seq;                       // [M]
+  int* units;                     // [n_units][kPxUnit]
   int n_units, n_kv, S, T, n_cta, cta, g, end;
 
   __device__ __forceinline__ static int find(const int* cum, int n, int at) {      // the last i with cum[i] <= at
@@ -137,29 +139,34 @@ struct PxLine {
     }
     if (lane == 0) cum[0] = 0;
   }
-  __device__ __forceinline__ int unit_pages(const PrefixArgs& a, int u) const {
-    const int* unit = a.units + u * kPxUnit;
-    int live = 0;                                               // a unit without a live row reads nothing
-    for (int m = unit[0]; !live && m < unit[0] + unit[1]; ++m) live = keys[m];
-    return live ? unit[2] / kPxPage + pages[unit[0] + unit[1]] - pages[unit[0]] : 0;
-  }
-  // whole block; `mem` holds 2 M + n_units + 2 words
+  __host__ __device__ static constexpr int words(int M, int n_units) { return 3 * M + 1 + n_units + 1 + n_units * kPxUnit; }
+  // whole block; `mem` holds words(M, n_units)
   __device__ __forceinline__ void build(const PrefixArgs& a, int* mem, bool raise) {
-    keys = mem; pages = keys + a.M; tiles = pages + a.M + 1;
+    keys = mem; pages = keys + a.M; tiles = pages + a.M + 1; seq = tiles + a.n_units + 1; units = seq + a.M;
     n_units = a.n_units; n_kv = a.n_kv;
+    for (int i = threadIdx.x; i < n_units * kPxUnit; i += blockDim.x) units[i] = a.units[i];
     for (int m = threadIdx.x; m < a.M; m += blockDim.x) {
+      const int shared = a.meta[m * kPxMeta + 2];
       bool bad;
       const int n = px_keys(a, m, bad);
       if (bad && raise) raise_fault(a.fault, a.layer, FS_KEY_COUNT);
       keys[m] = n;
-      pages[m + 1] = max(0, n - a.meta[m * kPxMeta + 2] + kPxPage - 1) / kPxPage;
+      seq[m] = a.row_seq[m];
+      pages[m + 1] = max(0, n - shared + kPxPage - 1) / kPxPage;
     }
     __syncthreads();
-    if (threadIdx.x < 32) running(pages, a.M);
-    __syncthreads();
-    for (int u = threadIdx.x; u < n_units; u += blockDim.x) tiles[u + 1] = (unit_pages(a, u) + 1) / 2;
-    __syncthreads();
-    if (threadIdx.x < 32) running(tiles, n_units);
+    if (threadIdx.x < 32) {
+      running(pages, a.M);
+      __syncwarp();
+      for (int u = threadIdx.x; u < n_units; u += 32) {
+        const int* unit = units + u * kPxUnit;
+        int live = 0;                                           // a unit without a live row reads nothing
+        for (int m = unit[0]; !live && m < unit[0] + unit[1]; ++m) live = keys[m];
+        tiles[u + 1] = live ? (unit[2] / kPxPage + pages[unit[0] + unit[1]] - pages[unit[0]] + 1) / 2 : 0;
+      }
+      __syncwarp();
+      running(tiles, n_units);
+    }
     __syncthreads();
     S = tiles[n_units];
     T = n_kv * S;
@@ -188,13 +195,22 @@ struct PxLine {
 struct PxWalk {
   const int* keys; const int* pages;
   int row0, rows, shared, total, row;                           // shared, total: pages
-  __device__ __forceinline__ void start(const PrefixArgs& a, const PxLine& line, int u, int page) {
-    const int* unit = a.units + u * kPxUnit;
+  __device__ __forceinline__ void start(const PxLine& line, int u, int page) {
+    const int* unit = line.units + u * kPxUnit;
     keys = line.keys; pages = line.pages;
     row0 = unit[0]; rows = unit[1]; shared = unit[2] / kPxPage;
     total = shared + pages[row0 + rows] - pages[row0];
     row = row0;
     if (page > shared) row = row0 + PxLine::find(pages + row0, rows, pages[row0] + page - shared);
+  }
+  // Both pages of a tile at once; for shared pages, most of a long walk, nothing is looked up.
+  __device__ __forceinline__ void tile(int t, int& o0, int& c0, int& n0, int& o1, int& c1, int& n1) {
+    if (2 * t + 2 <= shared) {
+      o0 = o1 = -1; c0 = 2 * t; c1 = 2 * t + 1; n0 = n1 = kPxPage;
+    } else {
+      page(2 * t, o0, c0, n0);
+      page(2 * t + 1, o1, c1, n1);
+    }
   }
   // owner: row of the unit, -1 all of them, -2 no page; col: page of the sequence; n: its keys.  Pages are asked for in order.
   __device__ __forceinline__ void page(int p, int& owner, int& col, int& n) {
@@ -209,6 +225,10 @@ struct PxWalk {
     }
   }
 };
+// The same value in a uniform register, which is where the tensor instructions take their operands from: what comes from memory
+// or a shuffle, and what is branched on it, would be moved there for each of them (the issuer took 2,300 clocks a job).
+__device__ __forceinline__ int px_uniform(int v) { return (int)__reduce_or_sync(0xffffffffu, (unsigned)v); }
+
 // tiles of rows that a page concerns, one bit each
 __device__ __forceinline__ unsigned px_tiles(int owner, int rows_tile, int n_x) {
   return owner == -2 ? 0u : owner == -1 ? (n_x == 2 ? 3u : 1u) : owner < rows_tile ? 1u : 2u;
@@ -244,17 +264,21 @@ __device__ __forceinline__ void px_st16(uint32_t taddr, const uint32_t (&r)[16])
                "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 
-constexpr int kPxThreads = 320;
+constexpr int kPxThreads = 384;                          // of warps 8 to 11 two work; all four give registers to the softmax
 constexpr int kPxHalf = 128 * 128;                      // 16 KB: 128 rows of 64 f16 values, one swizzle atom wide
 constexpr int px_tile(int head) { return head / 64 * kPxHalf; }
-constexpr int px_smem(int head, int n_units, int M) { return 6 * px_tile(head) + 1024 + (n_units + 2 * M + 2) * 4; }
+constexpr int px_smem(int head, int n_units, int M) { return 6 * px_tile(head) + 1024 + PxLine::words(M, n_units) * 4; }
+
+// 3 x 168 registers a lane at the launch = 104 + 200 + 200
+__device__ __forceinline__ void px_give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 104;"); }
+__device__ __forceinline__ void px_take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 200;"); }
 
 template <int HEAD>
 __global__ void __launch_bounds__(kPxThreads, 1)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const PrefixArgs a) {
   constexpr int NH = HEAD / 64, TILE = px_tile(HEAD), PAGE_BYTES = kPxPage * 128;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[4], p_full[2], pv_done[4];
+  __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[4], p_full[8], pv_done[4], frag_start;
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort, s_bad[8];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -262,13 +286,14 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
   uint8_t* sK = sQ + 2 * TILE;       // [2 stages][NH][128 keys][128 bytes]
   uint8_t* sV = sK + 2 * TILE;       // [2 stages][2 pages][NH][64 keys][128 bytes]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int G = a.n_q / a.n_kv, rows_tile = 128 / G;
+  const int G = a.n_q / a.n_kv, rows_tile = 128 / G, inv_G = 65536 / G + 1;     // i * inv_G >> 16 is i / G for i < 128
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 4); mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1); mbar_init(&s_full[i], 1); mbar_init(&s_full[2 + i], 1); mbar_init(&p_full[i], 4); mbar_init(&pv_done[i], 1); mbar_init(&pv_done[2 + i], 1);
+      mbar_init(&q_full[i], 4); mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 2); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 2);
     }
+    for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&pv_done[i], 1); mbar_init(&p_full[i], 4); mbar_init(&p_full[4 + i], 4); }
+    mbar_init(&frag_start, 2);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -289,192 +314,216 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
   PxFrag f;
   PxWalk w;
 
-  if (warp == 8) {
-    // ---- producer: all lanes walk, lane 0 waits and copies
-    int tile = 0;
-    bool ok = true;
-    for (int nf = 0; ok && line.next(f); ++nf) {
-      w.start(a, line, f.unit, 2 * f.t_lo);
-      const int* unit = a.units + f.unit * kPxUnit;
-      int lead = -1;                                            // sequence of the first row of the group that has a table
-      for (int i = 0; lead < 0 && i < unit[4]; i += 32) {
-        const int mine = i + lane < unit[4] ? a.row_seq[unit[3] + i + lane] : -1;
-        const unsigned live = __ballot_sync(0xffffffffu, mine >= 0 && mine < a.n_slots);
-        if (live) lead = __shfl_sync(0xffffffffu, mine, __ffs(live) - 1);
+  if (warp >= 8) {
+    px_give_registers();
+    if (warp == 8) {
+      // ---- producer: all lanes walk, lane 0 waits and copies
+      int tile = 0;
+      bool ok = true;
+      for (int nf = 0; ok && line.next(f); ++nf) {
+        w.start(line, f.unit, 2 * f.t_lo);
+        const int* unit = line.units + f.unit * kPxUnit;
+        int lead = -1;                                            // sequence of the first row of the group that has a table
+        for (int i = 0; lead < 0 && i < unit[4]; i += 32) {
+          const int mine = i + lane < unit[4] ? line.seq[unit[3] + i + lane] : -1;
+          const unsigned live = __ballot_sync(0xffffffffu, mine >= 0 && mine < a.n_slots);
+          if (live) lead = __shfl_sync(0xffffffffu, mine, __ffs(live) - 1);
+        }
+        int ids = 0;                                              // pages of the next 16 tiles, one a lane
+        bool bad = false;
+        for (int t = 0; ok && t < f.n_t; ++t, ++tile) {
+          if ((t & 15) == 0) {
+            PxWalk ahead = w;
+            int owner = -2, col = 0, n;
+            const int p = 2 * (f.t_lo + t) + lane;
+            if (p < ahead.shared) { owner = -1; col = p; }
+            else if (p < ahead.total && lane < 2 * (f.n_t - t)) {
+              ahead.row = w.row0 + PxLine::find(w.pages + w.row0, w.rows, w.pages[w.row0] + p - w.shared);
+              ahead.page(p, owner, col, n);
+            }
+            const int seq = owner == -1 ? lead : owner >= 0 ? line.seq[w.row0 + owner] : -1;
+            ids = seq >= 0 ? a.table[(long)seq * a.max_pages + col] : 0;
+            const bool off = owner > -2 && lane < 2 * (f.n_t - t) && (ids < 0 || ids >= a.n_pages);
+            if (ids < 0 || ids >= a.n_pages) ids = 0;
+            if (off) raise_fault(a.fault, a.layer, FS_PAGE);
+            bad = bad || __any_sync(0xffffffffu, off);
+          }
+          const int p0 = __shfl_sync(0xffffffffu, ids, 2 * t & 31), p1 = __shfl_sync(0xffffffffu, ids, (2 * t + 1) & 31);
+          const int n_p = min(2, w.total - 2 * (f.t_lo + t));
+          const int st = tile & 1;
+          const uint32_t par = (uint32_t)((tile >> 1) & 1);
+          if (lane == 0) {
+            ok = mbar_wait(&k_empty[st], par ^ 1, abort_flag);
+            if (ok) {
+              // behind this wait the softmax of four fragments ago is over: the flag may be used again
+              if (t == 0 || bad) s_bad[nf & 7] = bad;
+              mbar_expect_tx(&k_full[st], n_p * NH * PAGE_BYTES);
+              for (int p = 0; p < n_p; ++p)
+                for (int h = 0; h < NH; ++h)
+                  tma_load_2d(sK + st * TILE + h * kPxHalf + p * PAGE_BYTES, &tma_k, h * 64, ((p ? p1 : p0) * a.n_kv + f.kvh) * kPxPage, &k_full[st]);
+              ok = mbar_wait(&v_empty[st], par ^ 1, abort_flag);
+            }
+            if (ok) {
+              mbar_expect_tx(&v_full[st], n_p * NH * PAGE_BYTES);
+              for (int p = 0; p < n_p; ++p)
+                for (int h = 0; h < NH; ++h)
+                  tma_load_2d(sV + st * TILE + (p * NH + h) * PAGE_BYTES, &tma_v, h * 64, ((p ? p1 : p0) * a.n_kv + f.kvh) * kPxPage, &v_full[st]);
+            }
+          }
+          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        }
       }
-      int ids = 0;                                              // pages of the next 16 tiles, one a lane
-      bool bad = false;
-      for (int t = 0; ok && t < f.n_t; ++t, ++tile) {
-        if ((t & 15) == 0) {
-          PxWalk ahead = w;
-          int owner = -2, col = 0, n;
-          const int p = 2 * (f.t_lo + t) + lane;
-          if (p < ahead.shared) { owner = -1; col = p; }
-          else if (p < ahead.total && lane < 2 * (f.n_t - t)) {
-            ahead.row = w.row0 + PxLine::find(w.pages + w.row0, w.rows, w.pages[w.row0] + p - w.shared);
-            ahead.page(p, owner, col, n);
-          }
-          const int seq = owner == -1 ? lead : owner >= 0 ? a.row_seq[w.row0 + owner] : -1;
-          ids = seq >= 0 ? a.table[(long)seq * a.max_pages + col] : 0;
-          const bool off = owner > -2 && lane < 2 * (f.n_t - t) && (ids < 0 || ids >= a.n_pages);
-          if (ids < 0 || ids >= a.n_pages) ids = 0;
-          if (off) raise_fault(a.fault, a.layer, FS_PAGE);
-          bad = bad || __any_sync(0xffffffffu, off);
-        }
-        const int p0 = __shfl_sync(0xffffffffu, ids, 2 * t & 31), p1 = __shfl_sync(0xffffffffu, ids, (2 * t + 1) & 31);
-        const int n_p = min(2, w.total - 2 * (f.t_lo + t));
-        const int st = tile & 1;
-        const uint32_t par = (uint32_t)((tile >> 1) & 1);
-        if (lane == 0) {
-          ok = mbar_wait(&k_empty[st], par ^ 1, abort_flag);
-          if (ok) {
-            // behind this wait the softmax of four fragments ago is over: the flag may be used again
-            if (t == 0 || bad) s_bad[nf & 7] = bad;
-            mbar_expect_tx(&k_full[st], n_p * NH * PAGE_BYTES);
-            for (int p = 0; p < n_p; ++p)
-              for (int h = 0; h < NH; ++h)
-                tma_load_2d(sK + st * TILE + h * kPxHalf + p * PAGE_BYTES, &tma_k, h * 64, ((p ? p1 : p0) * a.n_kv + f.kvh) * kPxPage, &k_full[st]);
-            ok = mbar_wait(&v_empty[st], par ^ 1, abort_flag);
-          }
-          if (ok) {
-            mbar_expect_tx(&v_full[st], n_p * NH * PAGE_BYTES);
-            for (int p = 0; p < n_p; ++p)
-              for (int h = 0; h < NH; ++h)
-                tma_load_2d(sV + st * TILE + (p * NH + h) * PAGE_BYTES, &tma_v, h * 64, ((p ? p1 : p0) * a.n_kv + f.kvh) * kPxPage, &v_full[st]);
-          }
-        }
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      if (*abort_flag) {
+        // copies of ours may still be landing: give them a bounded moment before the block's memory goes away
+        const unsigned long long t0 = globaltimer();
+        while (globaltimer() - t0 < 2000000ull) { }
       }
-    }
-    if (*abort_flag) {
-      // copies of ours may still be landing: give them a bounded moment before the block's memory goes away
-      const unsigned long long t0 = globaltimer();
-      while (globaltimer() - t0 < 2000000ull) { }
-    }
-  } else if (warp == 9) {
-    // ---- issuer: one cursor for the first products, one for the second, two jobs behind
-    constexpr uint32_t idesc_s = px_idesc(128, 128, false), idesc_o = px_idesc(128, HEAD, true);
-    struct Cursor { PxWalk w; int t, tile, job; unsigned left; bool two; };
-    Cursor qk, pv;
-    qk.tile = pv.tile = -1;                                     // tiles through the rings
-    qk.job = pv.job = 0;
-    int n_q0 = 0, n_q1 = 0, n_s0 = 0, n_s1 = 0, n_o0 = 0, n_o1 = 0;      // query tiles, first and second products of either tile of rows
-    bool ok = true;
-    while (ok && line.next(f)) {
-      w.start(a, line, f.unit, 2 * f.t_lo);
-      const int n_x = w.rows > rows_tile ? 2 : 1;
-      // the next job of a cursor: its tile of rows, and whether it is the tile's first and last
-      auto next = [&](Cursor& c, int& x, bool& first, bool& last) {
-        first = false;
-        while (c.left == 0) {
-          if (++c.t >= f.n_t) return false;
-          ++c.tile;
-          int o0, o1, col, n;
-          c.w.page(2 * (f.t_lo + c.t), o0, col, n);
-          c.w.page(2 * (f.t_lo + c.t) + 1, o1, col, n);
-          c.left = px_tiles(o0, rows_tile, n_x) | px_tiles(o1, rows_tile, n_x);
-          c.two = o1 != -2;
-          first = true;
+    } else if (warp <= 10) {
+      // ---- issuers: one for each tile of rows, so that neither's waits and look-ups hold the other's products up
+      const int x = px_uniform(warp - 9);
+      constexpr uint32_t idesc_s = px_idesc(128, 128, false), idesc_o = px_idesc(128, HEAD, true);
+      const uint32_t uS = (uint32_t)px_uniform((int)tS0), uO = uS + 256 + x * HEAD;
+      int tile = 0, n_q = 0, n_s = 0, n_o = 0, n_f = 0;         // tiles through the rings; query tiles, first and second products; fragments
+      bool ok = true;
+      for (int g = px_uniform(line.g), g_end = px_uniform(line.end); ok && g < g_end; ++n_f) {
+        line.next(f);
+        w.start(line, f.unit, 2 * f.t_lo);
+        const int n_x = px_uniform(w.rows > rows_tile ? 2 : 1), n_t = px_uniform(f.n_t), t_lo = px_uniform(f.t_lo), pages = px_uniform(w.total);
+        const int shared = px_uniform(w.shared), tile0 = tile;
+        g += n_t;
+        tile += n_t;
+        // S = Q K^T of tile t into score buffer b
+        auto first_product = [&](int t, int b) {
+          const int st = (tile0 + t) & 1;
+          ok = ok && mbar_wait_warp(&k_full[st], (uint32_t)(((tile0 + t) >> 1) & 1), abort_flag);
+          if (!ok) return;
+          tc_fence_after();
+#pragma unroll
+          for (int h = 0; h < NH; ++h) {
+            const uint64_t dq = umma_desc(smem_u32(sQ + x * TILE + h * kPxHalf)), dk = umma_desc(smem_u32(sK + st * TILE + h * kPxHalf));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma_bf16(uS + b * 128, dq + (uint64_t)(k * 2), dk + (uint64_t)(k * 2), idesc_s, h + k > 0 ? 1u : 0u);
+          }
+          // Two barriers, for every other job.  The softmax waits for its scores but not for every second product; when it comes
+          // to a barrier, the job before the last is known to be complete (these scores were issued behind it), the last one is
+          // not, and a wait by parity must not be two phases off.
+          umma_commit(&s_full[2 * x + (n_s++ & 1)]);
+          umma_commit(&k_empty[st]);
+        };
+        // O += P V of tile t out of buffer b, the halves as their probabilities arrive
+        auto second_product = [&](int t, int b, uint32_t old) {
+          const int st = (tile0 + t) & 1, half = 2 * x + (n_o & 1);
+          const uint32_t par = (uint32_t)((n_o >> 1) & 1);
+          ok = ok && mbar_wait_warp(&v_full[st], (uint32_t)(((tile0 + t) >> 1) & 1), abort_flag) && mbar_wait_warp(&p_full[half], par, abort_flag);
+          if (!ok) return;
+          tc_fence_after();
+          const uint32_t tP = uS + b * 128;
+          const uint64_t dv = px_desc_v(smem_u32(sV + st * TILE)), dw = px_desc_v(smem_u32(sV + st * TILE + NH * PAGE_BYTES));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_bf16_ta(uO, tP + k * 8, dv + (uint64_t)(k * 128), idesc_o, k > 0 ? 1u : old);
+          ok = mbar_wait_warp(&p_full[4 + half], par, abort_flag);
+          if (!ok) return;
+          tc_fence_after();
+          if (2 * (t_lo + t) + 1 < pages) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma_bf16_ta(uO, tP + 32 + k * 8, dw + (uint64_t)(k * 128), idesc_o, 1u);
+          }
+          umma_commit(&pv_done[2 * x + (n_o++ & 1)]);
+          umma_commit(&v_empty[st]);
+        };
+        // a tile that this tile of rows takes no part in
+        auto pass = [&](int t) {
+          const int st = (tile0 + t) & 1;
+          const uint32_t par = (uint32_t)(((tile0 + t) >> 1) & 1);
+          ok = ok && mbar_wait_warp(&k_full[st], par, abort_flag);
+          if (ok && lane == 0) mbar_arrive(&k_empty[st]);
+          ok = ok && mbar_wait_warp(&v_full[st], par, abort_flag);
+          if (ok && lane == 0) mbar_arrive(&v_empty[st]);
+        };
+        // both are through with what the last fragment left in the score buffers
+        if (lane == 0) mbar_arrive(&frag_start);
+        ok = mbar_wait_warp(&frag_start, (uint32_t)(n_f & 1), abort_flag);
+        if (n_x == 2) {
+          bool asked = false;
+          for (int t = 0; ok && t < n_t; ++t) {
+            bool part = true;
+            if (2 * (t_lo + t) + 2 > shared) {
+              int o0, o1, c0, c1, k0, k1;
+              w.tile(t_lo + t, o0, c0, k0, o1, c1, k1);
+              part = px_uniform((int)((px_tiles(o0, rows_tile, 2) | px_tiles(o1, rows_tile, 2)) >> x & 1)) != 0;
+            }
+            if (!part) { pass(t); continue; }
+            if (!asked) ok = mbar_wait_warp(&q_full[x], (uint32_t)(n_q & 1), abort_flag);
+            first_product(t, x);
+            second_product(t, x, asked);
+            n_q += !asked;
+            asked = true;
+          }
+        } else if (x == 0) {
+          // alone: both score buffers in turn, the scores of the tile after the next behind a tile's second product
+          ok = ok && mbar_wait_warp(&q_full[0], (uint32_t)(n_q++ & 1), abort_flag);
+          first_product(0, 0);
+          if (n_t > 1) first_product(1, 1);
+          for (int t = 0; ok && t < n_t; ++t) {
+            second_product(t, t & 1, t > 0);
+            if (t + 2 < n_t) first_product(t + 2, t & 1);
+          }
+        } else {
+          for (int t = 0; ok && t < n_t; ++t) pass(t);
         }
-        x = c.left & 1 ? 0 : 1;
-        c.left &= c.left - 1;
-        last = c.left == 0;
-        return true;
-      };
-      unsigned asked = 0, begun = 0;                            // tiles of rows whose queries are there; whose output holds something
-      auto first_product = [&]() {
-        int x;
-        bool first, last;
-        if (!next(qk, x, first, last)) return;
-        const int st = qk.tile & 1, b = qk.job++ & 1;
-        if (first) ok = mbar_wait_warp(&k_full[st], (uint32_t)((qk.tile >> 1) & 1), abort_flag);
-        if (ok && !(asked >> x & 1)) ok = mbar_wait_warp(&q_full[x], (uint32_t)((x ? n_q1++ : n_q0++) & 1), abort_flag);
-        if (!ok) return;
-        asked |= 1u << x;
-        tc_fence_after();
-#pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          const uint64_t dq = umma_desc(smem_u32(sQ + x * TILE + h * kPxHalf)), dk = umma_desc(smem_u32(sK + st * TILE + h * kPxHalf));
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16(tS0 + b * 128, dq + (uint64_t)(k * 2), dk + (uint64_t)(k * 2), idesc_s, h + k > 0 ? 1u : 0u);
-        }
-        // Barriers for every other job of a tile of rows.  Its warps wait for their own jobs alone and not for every second
-        // product; when they come to a barrier, the job before the last is known to be complete (these scores were issued behind
-        // it), the last one is not, and a wait by parity must not be two phases off.
-        umma_commit(&s_full[2 * x + ((x ? n_s1++ : n_s0++) & 1)]);
-        if (last) umma_commit(&k_empty[st]);
-      };
-      qk.w = pv.w = w;
-      qk.t = pv.t = -1;
-      qk.left = pv.left = 0;
-      first_product();
-      if (ok) first_product();
-      int x;
-      bool first, last;
-      while (ok && next(pv, x, first, last)) {
-        const int st = pv.tile & 1, b = pv.job & 1;
-        if (first) ok = mbar_wait_warp(&v_full[st], (uint32_t)((pv.tile >> 1) & 1), abort_flag);
-        ok = ok && mbar_wait_warp(&p_full[b], (uint32_t)((pv.job >> 1) & 1), abort_flag);
-        if (!ok) break;
-        ++pv.job;
-        tc_fence_after();
-        const uint32_t tP = tS0 + b * 128, tO = tO0 + x * HEAD, old = begun >> x & 1;
-        const uint64_t dv = px_desc_v(smem_u32(sV + st * TILE)), dw = px_desc_v(smem_u32(sV + st * TILE + NH * PAGE_BYTES));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) umma_bf16_ta(tO, tP + k * 8, dv + (uint64_t)(k * 128), idesc_o, k > 0 ? 1u : old);
-        if (pv.two) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16_ta(tO, tP + 32 + k * 8, dw + (uint64_t)(k * 128), idesc_o, 1u);
-        }
-        begun |= 1u << x;
-        umma_commit(&pv_done[2 * x + ((x ? n_o1++ : n_o0++) & 1)]);
-        if (last) umma_commit(&v_empty[st]);
-        first_product();
       }
     }
   } else {
+    px_take_registers();
     // ---- softmax: a thread per query row ------------------------------------------------------------------
     const int x = warp >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;                          // row of the tile
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint32_t tO = tO0 + x * HEAD + lane_base;
-    int tile = 0, job = 0, mine = 0;                            // tiles; jobs of both tiles of rows; jobs of this one
+    int tile = 0, mine = 0;                                     // tiles; jobs of this tile of rows
     bool ok = true;
     for (int nf = 0; ok && line.next(f); ++nf) {
-      w.start(a, line, f.unit, 2 * f.t_lo);
+      w.start(line, f.unit, 2 * f.t_lo);
       const int n_x = w.rows > rows_tile ? 2 : 1;
       const int live = max(0, min(rows_tile, w.rows - x * rows_tile)) * G;      // query rows of this tile
-      const int my = r < live ? x * rows_tile + r / G : -3;     // row of the unit
+      const int my = r < live ? x * rows_tile + (r * inv_G >> 16) : -3;     // row of the unit
       const int n_keys = r < live ? w.keys[w.row0 + my] : 0;
       const bool busy = quarter * 32 < live;
       float to_log2 = 0.f;
+      // queries to f16: four lanes a row, scaled by a power of two to a largest element in [512, 1024); all loads at once
       auto put_queries = [&]() {
         if (busy) {
-          // queries to f16: four lanes a row, scaled by a power of two to a largest element in [512, 1024)
-#pragma unroll 2
-          for (int p = 0; p < 4; ++p) {
-            const int i = quarter * 32 + p * 8 + (lane >> 2);
-            float4 v[HEAD / 16];
-            float top = 0.f;
-            const float* src = a.q + ((long)(w.row0 + x * rows_tile + i / G) * a.n_q + f.kvh * G + i % G) * HEAD + (lane & 3) * 4;
+          float4 v[4][HEAD / 16];
 #pragma unroll
-            for (int c = 0; c < HEAD / 16; ++c) {
-              v[c] = i < live ? __ldg(reinterpret_cast<const float4*>(src + c * 16)) : make_float4(0.f, 0.f, 0.f, 0.f);
-              top = fmaxf(top, fmaxf(fmaxf(fabsf(v[c].x), fabsf(v[c].y)), fmaxf(fabsf(v[c].z), fabsf(v[c].w))));
-            }
+          for (int p = 0; p < 4; ++p) {
+            const int i = quarter * 32 + p * 8 + (lane >> 2), row = i * inv_G >> 16;
+            const float4* src = reinterpret_cast<const float4*>(a.q + ((long)(w.row0 + x * rows_tile + row) * a.n_q + f.kvh * G + i - row * G) * HEAD) + (lane & 3);
+#pragma unroll
+            for (int c = 0; c < HEAD / 16; ++c) v[p][c] = i < live ? __ldg(src + c * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            if (quarter * 32 + p * 8 >= live) break;
+            const int i = quarter * 32 + p * 8 + (lane >> 2);
+            float top = 0.f;
+#pragma unroll
+            for (int c = 0; c < HEAD / 16; ++c)
+              top = fmaxf(top, fmaxf(fmaxf(fabsf(v[p][c].x), fabsf(v[p][c].y)), fmaxf(fabsf(v[p][c].z), fabsf(v[p][c].w))));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = (int)(__float_as_uint(top) >> 23);      // top >= 0
-            const int se = e == 0 ? 127 : min(254, 263 - e);
+            const int e = (int)(__float_as_uint(top) >> 23);    // top >= 0
+            const int se = e == 0 ? 127 : min(253, 263 - e);
             const float scale = __uint_as_float((unsigned)se << 23);
-            const float back = kPxLog2e / scale;
+            const float back = kPxLog2e * __uint_as_float((unsigned)(254 - se) << 23);
             const float given = __shfl_sync(0xffffffffu, back, (lane & 7) * 4);
             if ((lane >> 3) == p) to_log2 = given;
+            uint8_t* dst = sQ + x * TILE + i * 128 + ((lane & 1) << 3);
 #pragma unroll
             for (int c = 0; c < HEAD / 16; ++c) {
-              const int col = (lane & 3) * 4 + c * 16;            // four values: 8 bytes of 16-byte chunk (col % 64) / 8
-              uint8_t* dst = sQ + x * TILE + (col >> 6) * kPxHalf + i * 128 + ((((col & 63) >> 3) ^ (i & 7)) << 4) + ((col & 4) << 1);
-              *reinterpret_cast<uint2*>(dst) = make_uint2(px_pack(v[c].x * scale, v[c].y * scale), px_pack(v[c].z * scale, v[c].w * scale));
+              // values 4 (lane & 3) + 16 c ..: 8 bytes of 16-byte chunk 2 c + (lane & 3) / 2, swizzled within 64 values
+              const int chunk = 2 * c + ((lane >> 1) & 1);
+              *reinterpret_cast<uint2*>(dst + (chunk >> 3) * kPxHalf + (((chunk & 7) ^ (i & 7)) << 4)) =
+                  make_uint2(px_pack(v[p][c].x * scale, v[p][c].y * scale), px_pack(v[p][c].z * scale, v[p][c].w * scale));
             }
           }
           fence_async_smem();
@@ -486,17 +535,34 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
       bool begun = false;
       for (int t = 0; t < f.n_t; ++t, ++tile) {
         int o0, c0, k0, o1, c1, k1;
-        w.page(2 * (f.t_lo + t), o0, c0, k0);
-        w.page(2 * (f.t_lo + t) + 1, o1, c1, k1);
+        w.tile(f.t_lo + t, o0, c0, k0, o1, c1, k1);
         const unsigned who = px_tiles(o0, rows_tile, n_x) | px_tiles(o1, rows_tile, n_x);
-        const int at = job + (x == 1 && (who & 1));             // number of this tile's job
-        job += __popc(who);
         if (!(who >> x & 1)) continue;
-        const int b = at & 1;
+        const int b = n_x == 2 ? x : t & 1;
         const uint32_t tS = tS0 + b * 128 + lane_base;
         // keys of either page that this thread's row attends to
         const int n0 = o0 == my ? k0 : o0 == -1 ? min(kPxPage, max(0, n_keys - kPxPage * c0)) : 0;
         const int n1 = o1 == my ? k1 : o1 == -1 ? min(kPxPage, max(0, n_keys - kPxPage * c1)) : 0;
+        // Half p of the probabilities is written.  Where a page ends inside the tile, what lies behind its keys may be anything,
+        // and zero times that must be zero: the first tile of rows that takes part clears it in the value tile.
+        auto finish = [&](int p) {
+          const int n = p ? k1 : k0;
+          if (n > 0 && n < kPxPage && x == (who & 1 ? 0 : 1)) {
+            const int st = tile & 1;
+            ok = mbar_wait_warp(&v_full[st], (uint32_t)((tile >> 1) & 1), abort_flag);
+            if (!ok) return false;
+            uint8_t* page = sV + st * TILE + p * NH * PAGE_BYTES;
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+              for (int i = n * 8 + r; i < kPxPage * 8; i += 128) *reinterpret_cast<uint4*>(page + h * PAGE_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
+            fence_async_smem();
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[4 * p + 2 * x + (mine & 1)]);
+          return true;
+        };
         if (!begun) put_queries();
         ok = mbar_wait_warp(&s_full[2 * x + (mine & 1)], (uint32_t)((mine >> 1) & 1), abort_flag);
         if (!ok) break;
@@ -522,6 +588,21 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
           if (m != -INFINITY && (m_new - m) * to_log2 <= kPxLazy) m_new = m;
           const float mb = (m_new == -INFINITY) ? 0.f : m_new * to_log2;      // a row with no key yet keeps zeros
           const float corr = (m == -INFINITY || m == m_new) ? 1.f : px_ex2(m * to_log2 - mb);
+          if (begun && __any_sync(0xffffffffu, corr != 1.0f)) {
+            // the output is scaled in tensor memory, behind the tile's last product
+            ok = mbar_wait_warp(&pv_done[2 * x + ((mine - 1) & 1)], (uint32_t)(((mine - 1) >> 1) & 1), abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HEAD / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tO + c * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_st32(tO + c * 32, o);
+            }
+          }
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -538,25 +619,13 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
               pk[i >> 1] = px_pack(p0, p1);
             }
             px_st16(tS + 16 * c, pk);
-          }
-          if (begun && __any_sync(0xffffffffu, corr != 1.0f)) {
-            // the output is scaled in tensor memory, behind the tile's last product
-            ok = mbar_wait_warp(&pv_done[2 * x + ((mine - 1) & 1)], (uint32_t)(((mine - 1) >> 1) & 1), abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < HEAD / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(tO + c * 32, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-              tmem_st32(tO + c * 32, o);
+            if (c == 1) {                                       // the first page's half of the second product may begin
+              if (!finish(0)) break;
             }
           }
+          if (!ok) break;
           l = l * corr + ((sum[0] + sum[2]) + (sum[1] + sum[3]));
           m = m_new;
-          tmem_st_wait();
         } else {
           // no row of this warp attends to these pages
           uint32_t zero[16];
@@ -564,30 +633,11 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
           for (int i = 0; i < 16; ++i) zero[i] = 0;
 #pragma unroll
           for (int c = 0; c < 4; ++c) px_st16(tS + 16 * c, zero);
-          tmem_st_wait();
+          if (!finish(0)) break;
         }
-        if ((k0 < kPxPage || (k1 && k1 < kPxPage)) && x == (who & 1 ? 0 : 1)) {
-          // a page ends inside the tile: what lies behind its keys may be anything, and zero times that must be zero
-          const int st = tile & 1;
-          ok = mbar_wait_warp(&v_full[st], (uint32_t)((tile >> 1) & 1), abort_flag);
-          if (!ok) break;
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            const int n = p ? k1 : k0;
-            uint8_t* page = sV + st * TILE + p * NH * PAGE_BYTES;
-            if (n > 0) {
-#pragma unroll
-              for (int h = 0; h < NH; ++h)
-                for (int i = n * 8 + r; i < kPxPage * 8; i += 128) *reinterpret_cast<uint4*>(page + h * PAGE_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
-            }
-          }
-          fence_async_smem();
-        }
+        if (!finish(1)) break;
         begun = true;
         ++mine;
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[b]);
       }
       if (ok && begun) {
         ok = mbar_wait_warp(&pv_done[2 * x + ((mine - 1) & 1)], (uint32_t)(((mine - 1) >> 1) & 1), abort_flag);
@@ -630,11 +680,16 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
   if (threadIdx.x == 0 && s_abort) raise_fault(a.fault, a.layer, FS_WAIT_TIMEOUT);
 }
 
-// Joins the fragments of a row's heads: grid (n_kv, M), a thread for four values of a head (heads next to each other).
-template <int HEAD>
+// Joins the fragments of a row's heads: grid (n_kv, M, HEAD / 32), 256 threads.  One round trip brings the maxima and sums of all
+// fragments, a warp for a head; the outputs follow, a thread for four values of a head and every `sets`-th fragment.
+constexpr int kPxMaxCtas = 160;
+
+template <int HEAD, bool Q8>
 __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixArgs a) {
   extern __shared__ int s_line[];
-  const int kvh = blockIdx.x, m = blockIdx.y, G = a.n_q / a.n_kv;
+  __shared__ float s_w[kPxMaxCtas * 16], s_inv[16];
+  __shared__ float4 s_o[256];
+  const int kvh = blockIdx.x, m = blockIdx.y, G = a.n_q / a.n_kv, tid = threadIdx.x, lane = tid & 31;
   // lengths and tables are older than the launch in front, which started behind what wrote them
   bool bad;
   const int n = px_keys(a, m, bad);
@@ -649,42 +704,65 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixArgs a) {
     n_f = line.cta_of(hi - 1) - c + 1;
     id = kvh * a.n_units + unit + c;
   }
+  const int items = G * 8, sets = 256 / items, set = tid / items, h = tid % G, c = blockIdx.z * 8 + tid % items / G;
+  const float4* part = a.part + (((long)id * 2 + x) * (HEAD / 4) + c) * 128 + lane0 + h;
+  const float2* ml = a.ml + ((long)id * 2 + x) * 128 + lane0;
   pdl_wait();
   pdl_launch();
-  bool again = false;
-  for (int i = threadIdx.x; i < G * (HEAD / 4); i += blockDim.x) {
-    const int h = i % G, c = i / G;
-    const float2* ml = a.ml + ((long)id * 2 + x) * 128 + lane0 + h;
-    const float4* part = a.part + (((long)id * 2 + x) * (HEAD / 4) + c) * 128 + lane0 + h;
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int f = 0; f < n_f; ++f) top = fmaxf(top, __ldcg(ml + (long)f * 256).x);
-    float den = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int f = 0; f < n_f; ++f) {                                             // ascending order, fixed
-      const float2 q = __ldcg(ml + (long)f * 256);
-      if (q.x > -INFINITY) {
-        const float4 v = __ldcg(part + (long)f * 2 * (HEAD / 4) * 128);
-        const float w = px_ex2(q.x - top);
-        den = fmaf(w, q.y, den);
-        o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
-      }
+  for (int g = tid >> 5; g < G; g += 8) {
+    float2 q[kPxMaxCtas / 32];
+    float top = -INFINITY, den = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPxMaxCtas / 32; ++i) {
+      q[i] = lane + 32 * i < n_f ? __ldcg(ml + (long)(lane + 32 * i) * 256 + g) : make_float2(-INFINITY, 0.f);
+      top = fmaxf(top, q[i].x);
     }
-    const float inv = bad ? __int_as_float(0x7fc00000) : n > 0 ? 1.f / den : 0.f;
+    top = warp_max(top);
+#pragma unroll
+    for (int i = 0; i < kPxMaxCtas / 32; ++i) {
+      const float w = q[i].x > -INFINITY ? px_ex2(q[i].x - top) : 0.f;
+      den += w > 0.f || q[i].y != q[i].y ? w * q[i].y : 0.f;                    // a NaN stays one, whatever its weight
+      s_w[(lane + 32 * i) * 16 + g] = w;
+    }
+    den = warp_sum(den);
+    if (lane == 0) s_inv[g] = 1.f / den;
+  }
+  __syncthreads();
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (set < sets) {
+    constexpr int AHEAD = 8;                                                    // fragments in flight
+    for (int f0 = set; f0 < n_f; f0 += AHEAD * sets) {                          // ascending order, fixed
+      float4 v[AHEAD];
+      float w[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int f = f0 + i * sets;
+        w[i] = f < n_f ? s_w[f * 16 + h] : 0.f;
+        v[i] = w[i] != 0.f ? __ldcg(part + (long)f * 2 * (HEAD / 4) * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) { o.x = fmaf(w[i], v[i].x, o.x); o.y = fmaf(w[i], v[i].y, o.y); o.z = fmaf(w[i], v[i].z, o.z); o.w = fmaf(w[i], v[i].w, o.w); }
+    }
+  }
+  s_o[tid] = o;
+  __syncthreads();
+  bool again = false;
+  if (tid < items) {
+    for (int i = 1; i < sets; ++i) { const float4 v = s_o[tid + i * items]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w; }
+    const float inv = bad ? __int_as_float(0x7fc00000) : n > 0 ? s_inv[h] : 0.f;
     const __nv_bfloat162 b0 = __floats2bfloat162_rn(o.x * inv, o.y * inv), b1 = __floats2bfloat162_rn(o.z * inv, o.w * inv);
     *reinterpret_cast<uint2*>(a.out + ((long)m * a.n_q + kvh * G + h) * HEAD + c * 4) =
         make_uint2(*reinterpret_cast<const uint32_t*>(&b0), *reinterpret_cast<const uint32_t*>(&b1));
-    again |= !(fabsf((o.x + o.y) + (o.z + o.w)) * inv < INFINITY);
+    again = !(fabsf((o.x + o.y) + (o.z + o.w)) * inv < INFINITY);
   }
   // a key or value that is not finite, maybe another row's: this row's own say what its output is
   if (__syncthreads_or(again && n > 0)) {
-    for (int h = threadIdx.x >> 5; h < G; h += blockDim.x >> 5) {
-      float o[HEAD / 32];
-      px_row<HEAD, false>(a, m, kvh * G + h, n, o);
+    for (int g = tid >> 5; g < G; g += 8) {
+      float r[HEAD / 32];
+      px_row<HEAD, Q8>(a, m, kvh * G + g, n, r);
 #pragma unroll
       for (int i = 0; i < HEAD / 32; ++i)
-        a.out[((long)m * a.n_q + kvh * G + h) * HEAD + (threadIdx.x & 31) * (HEAD / 32) + i] = __float2bfloat16_rn(o[i]);
+        if (lane * (HEAD / 32) / 32 == (int)blockIdx.z) a.out[((long)m * a.n_q + kvh * G + g) * HEAD + lane * (HEAD / 32) + i] = __float2bfloat16_rn(r[i]);
     }
   }
 }
@@ -711,7 +789,7 @@ static int prefix_go(const PrefixArgs& a, cudaStream_t st) {
   }
   const cudaError_t e = launch(prefix_attn_kernel<HEAD>, dim3(a.n_cta), dim3(kPxThreads), (size_t)px_smem(HEAD, a.n_units, a.M), st, mk, mv, a);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch(prefix_join_kernel<HEAD>, dim3(a.n_kv, a.M), dim3(256), (size_t)(2 * a.M + a.n_units + 2) * 4, st, a);
+  return (int)launch(prefix_join_kernel<HEAD, false>, dim3(a.n_kv, a.M, HEAD / 32), dim3(256), (size_t)PxLine::words(a.M, a.n_units) * 4, st, a);
 }
 
 extern "C" {
@@ -727,7 +805,7 @@ int bl_prefix_attention(const float* q, const void* k_cache, const void* v_cache
                         cudaStream_t st) {
   BL_REQUIRE(head == 128 || head == 64, BL_ERR_SHAPE);
   BL_REQUIRE(n_kv >= 1 && n_q >= 1 && n_q % n_kv == 0 && n_q / n_kv <= 16, BL_ERR_SHAPE);
-  BL_REQUIRE(M >= 1 && M <= kPxMaxRows && n_units >= 1 && n_units <= M && n_cta >= 1 && n_slots >= 1 && max_pages >= 1 && n_pages >= 1, BL_ERR_SHAPE);
+  BL_REQUIRE(M >= 1 && M <= kPxMaxRows && n_units >= 1 && n_units <= M && n_cta >= 1 && n_cta <= kPxMaxCtas && n_slots >= 1 && max_pages >= 1 && n_pages >= 1, BL_ERR_SHAPE);
   BL_REQUIRE((long)n_pages * n_kv * kPxPage <= 0x7fffffffL && (long)(max_pages + 2) * M * n_kv <= 0x7fffffffL, BL_ERR_LIMIT);
   BL_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)work) & 15) == 0, BL_ERR_ALIGN);
   PrefixArgs a{q, (const uint8_t*)k_cache, (const uint8_t*)v_cache, row_pos, row_seq, block_table, n_slots, max_pages, n_pages, n_q, n_kv, M,

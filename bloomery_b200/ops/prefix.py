@@ -50,8 +50,8 @@ class PrefixPlan:
         self.rows = sum(group_rows)
         self.max_prefix = max(prefix_len)
         self.device = torch.device(device)
-        if self.rows > 1024:
-            raise ValueError("at most 1024 rows")
+        if self.rows > 512:
+            raise ValueError("at most 512 rows")
         # units: rows of a group that read all of their keys together, as many as two tiles of 128 (row, head) pairs of a key
         # head hold
         G = n_q // n_kv
@@ -63,7 +63,7 @@ class PrefixPlan:
             first += n
         self.n_units = len(units)
         self.meta = torch.tensor(rows + units, dtype=torch.int32).to(self.device)
-        self.n_cta = sm_count(self.device) if self.device.type == "cuda" else 1
+        self.n_cta = min(160, sm_count(self.device)) if self.device.type == "cuda" else 1
         fn = cuda().bl_prefix_work_bytes
         fn.restype = ctypes.c_long
         self.work = torch.empty(fn(head, n_kv, self.n_units, self.n_cta), dtype=torch.uint8, device=self.device)
