@@ -91,23 +91,6 @@ __device__ __forceinline__ void px_row(const PrefixArgs& a, int m, int h, int n,
   for (int i = 0; i < N; ++i) o[i] /= l;
 }
 
-// q8_0 caches.  grid (n_q, M), a warp
-template <int HEAD>
-__global__ void __launch_bounds__(32) prefix_rows_kernel(const PrefixArgs a) {
-  const int h = blockIdx.x, m = blockIdx.y;
-  pdl_wait();
-  pdl_launch();
-  bool bad;
-  const int n = px_keys(a, m, bad);
-  if (bad && threadIdx.x == 0) raise_fault(a.fault, a.layer, FS_KEY_COUNT);
-  float o[HEAD / 32];
-#pragma unroll
-  for (int i = 0; i < HEAD / 32; ++i) o[i] = bad ? __int_as_float(0x7fc00000) : 0.f;
-  if (n > 0) px_row<HEAD, true>(a, m, h, n, o);
-#pragma unroll
-  for (int i = 0; i < HEAD / 32; ++i) a.out[((long)m * a.n_q + h) * HEAD + threadIdx.x * (HEAD / 32) + i] = __float2bfloat16_rn(o[i]);
-}
-
 // ---- the line of work ---------------------------------------------------------------------------------------
 // Per KV head the tiles of all units (S), CTA c of n takes tiles c T / n .. (c + 1) T / n - 1 of the T = n_kv S.  A fragment is what
 // a stretch shares with a (KV head, unit); fragments' numbers (index + CTA) grow by one from each to the next within a unit and
@@ -264,36 +247,85 @@ __device__ __forceinline__ void px_st16(uint32_t taddr, const uint32_t (&r)[16])
                "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 
-constexpr int kPxThreads = 384;                          // of warps 8 to 11 two work; all four give registers to the softmax
 constexpr int kPxHalf = 128 * 128;                      // 16 KB: 128 rows of 64 f16 values, one swizzle atom wide
 constexpr int px_tile(int head) { return head / 64 * kPxHalf; }
-constexpr int px_smem(int head, int n_units, int M) { return 6 * px_tile(head) + 1024 + PxLine::words(M, n_units) * 4; }
+// f16 caches: two stages of keys and of values.  q8_0: one each, and two of the rows as they are in the cache.
+constexpr int px_stages(bool q8) { return q8 ? 1 : 2; }
+constexpr int px_raw(int head) { return kPxPage * (head / 32 * 34); }             // a page of q8_0 rows of one head: a multiple of 16
+constexpr int px_smem(int head, bool q8, int n_units, int M) {
+  return (2 + 2 * px_stages(q8)) * px_tile(head) + (q8 ? 8 * px_raw(head) : 0) + 1024 + PxLine::words(M, n_units) * 4;
+}
+// q8_0 caches have four more warps, which expand the rows
+constexpr int px_threads(bool q8) { return q8 ? 512 : 384; }
 
-// 3 x 168 registers a lane at the launch = 104 + 200 + 200
-__device__ __forceinline__ void px_give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 104;"); }
-__device__ __forceinline__ void px_take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 200;"); }
-
+// Registers a lane: 3 x 168 at the launch = 104 + 200 + 200, with the expanding warps 4 x 128 = 72 + 88 + 176 + 176.
+template <bool Q8> __device__ __forceinline__ void px_give_registers() {
+  if constexpr (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+}
+template <bool Q8> __device__ __forceinline__ void px_take_registers() {
+  if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+  else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+}
+__device__ __forceinline__ void px_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+// Four q8_0 codes times their scale as f16: a code is made the low byte of 1024 + 128 + code, which is exact.
+__device__ __forceinline__ void px_codes(uint32_t c, __half2 d, uint32_t& lo, uint32_t& hi) {
+  c ^= 0x80808080u;
+  const uint32_t a = __byte_perm(c, 0x64646464u, 0x4140), b = __byte_perm(c, 0x64646464u, 0x4342);
+  const __half2 bias = __float2half2_rn(1152.f);
+  const __half2 x = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&a), bias), d), y = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&b), bias), d);
+  lo = *reinterpret_cast<const uint32_t*>(&x);
+  hi = *reinterpret_cast<const uint32_t*>(&y);
+}
+// A q8_0 row in shared memory to f16 at `dst`: 16-byte chunks swizzled by the row, blocks of 64 values `pitch` bytes apart.
 template <int HEAD>
-__global__ void __launch_bounds__(kPxThreads, 1)
+__device__ __forceinline__ void px_expand(const uint8_t* row, uint8_t* dst, int pitch, int swizzle) {
+  const __half* scales = reinterpret_cast<const __half*>(row);
+  const uint8_t* codes = row + HEAD / 16;
+#pragma unroll
+  for (int c = 0; c < HEAD / 8; ++c) {                          // eight values
+    const __half2 d = __half2half2(scales[c >> 2]);
+    uint32_t w0, w1;
+    if constexpr (HEAD == 128) {                                // rows of 136 bytes, of 68 otherwise
+      const uint2 w = *reinterpret_cast<const uint2*>(codes + 8 * c);
+      w0 = w.x; w1 = w.y;
+    } else {
+      w0 = *reinterpret_cast<const uint32_t*>(codes + 8 * c);
+      w1 = *reinterpret_cast<const uint32_t*>(codes + 8 * c + 4);
+    }
+    uint4 o;
+    px_codes(w0, d, o.x, o.y);
+    px_codes(w1, d, o.z, o.w);
+    *reinterpret_cast<uint4*>(dst + (c >> 3) * pitch + (((c & 7) ^ swizzle) << 4)) = o;
+  }
+}
+
+template <int HEAD, bool Q8>
+__global__ void __launch_bounds__(px_threads(Q8), 1)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const PrefixArgs a) {
-  constexpr int NH = HEAD / 64, TILE = px_tile(HEAD), PAGE_BYTES = kPxPage * 128;
+  constexpr int NH = HEAD / 64, TILE = px_tile(HEAD), PAGE_BYTES = kPxPage * 128, ST = px_stages(Q8), RAW = px_raw(HEAD);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[4], p_full[8], pv_done[4], frag_start;
+  __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[4], p_full[8], pv_done[4], frag_start, raw_full[4], raw_empty[4];
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort, s_bad[8];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sQ = smem;                // [2 tiles][NH][128 rows][128 bytes]
-  uint8_t* sK = sQ + 2 * TILE;       // [2 stages][NH][128 keys][128 bytes]
-  uint8_t* sV = sK + 2 * TILE;       // [2 stages][2 pages][NH][64 keys][128 bytes]
+  uint8_t* sK = sQ + 2 * TILE;       // [ST stages][NH][128 keys][128 bytes]
+  uint8_t* sV = sK + ST * TILE;      // [ST stages][2 pages][NH][64 keys][128 bytes]
+  uint8_t* sRaw = sV + ST * TILE;    // q8_0: [2 stages][keys, values][2 pages][64 rows]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.n_q / a.n_kv, rows_tile = 128 / G, inv_G = 65536 / G + 1;     // i * inv_G >> 16 is i / G for i < 128
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 4); mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 2); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 2);
+      mbar_init(&q_full[i], 4); mbar_init(&k_full[i], Q8 ? 4 : 1); mbar_init(&k_empty[i], 2); mbar_init(&v_full[i], Q8 ? 4 : 1); mbar_init(&v_empty[i], 2);
     }
     for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&pv_done[i], 1); mbar_init(&p_full[i], 4); mbar_init(&p_full[4 + i], 4); }
     mbar_init(&frag_start, 2);
+    for (int i = 0; Q8 && i < 4; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -305,7 +337,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
   pdl_launch();
   PxLine line;
   tc_fence_before();
-  line.build(a, reinterpret_cast<int*>(sV + 2 * TILE), blockIdx.x == 0);
+  line.build(a, reinterpret_cast<int*>(sRaw + (Q8 ? 8 * RAW : 0)), blockIdx.x == 0);
   tc_fence_after();
   line.start(blockIdx.x);
   const uint32_t tmem_base = s_tmem_base;
@@ -314,8 +346,44 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
   PxFrag f;
   PxWalk w;
 
-  if (warp >= 8) {
-    px_give_registers();
+  if (Q8 && warp >= 12) {
+    // ---- q8_0 rows to f16: a thread for a row of the tile
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    const int key = threadIdx.x - 384;
+    int tile = 0;
+    bool ok = true;
+    while (ok && line.next(f)) {
+      w.start(line, f.unit, 2 * f.t_lo);
+      for (int t = 0; ok && t < f.n_t; ++t, ++tile) {
+        int o0, c0, k0, o1, c1, k1;
+        w.tile(f.t_lo + t, o0, c0, k0, o1, c1, k1);
+        const int slot = tile & 1, p = key / kPxPage, row = key % kPxPage;
+        const uint32_t par = (uint32_t)((tile >> 1) & 1), par1 = (uint32_t)(tile & 1);
+#pragma unroll 1
+        for (int kv = 0; ok && kv < 2; ++kv) {
+          uint64_t* const empty = kv ? &v_empty[0] : &k_empty[0];
+          ok = mbar_wait_warp(&raw_full[2 * kv + slot], par, abort_flag) && mbar_wait_warp(empty, par1 ^ 1, abort_flag);
+          if (!ok) break;
+          const uint8_t* src = sRaw + ((slot * 2 + kv) * 2 + p) * RAW + row * (RAW / kPxPage);
+          uint8_t* dst = kv ? sV + p * NH * PAGE_BYTES + row * 128 : sK + key * 128;
+          const int pitch = kv ? PAGE_BYTES : kPxHalf, n = p ? k1 : k0;
+          if (row < n) {
+            px_expand<HEAD>(src, dst, pitch, row & 7);
+          } else if (kv && n > 0) {                               // behind a sequence's end: zero, whatever lies there
+#pragma unroll
+            for (int c = 0; c < HEAD / 8; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * pitch + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(kv ? &v_full[0] : &k_full[0]);
+            mbar_arrive(&raw_empty[2 * kv + slot]);
+          }
+        }
+      }
+    }
+  } else if (warp >= 8) {
+    px_give_registers<Q8>();
     if (warp == 8) {
       // ---- producer: all lanes walk, lane 0 waits and copies
       int tile = 0;
@@ -350,24 +418,29 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
           }
           const int p0 = __shfl_sync(0xffffffffu, ids, 2 * t & 31), p1 = __shfl_sync(0xffffffffu, ids, (2 * t + 1) & 31);
           const int n_p = min(2, w.total - 2 * (f.t_lo + t));
-          const int st = tile & 1;
+          const int st = tile & 1;                              // both rings have two stages
           const uint32_t par = (uint32_t)((tile >> 1) & 1);
           if (lane == 0) {
-            ok = mbar_wait(&k_empty[st], par ^ 1, abort_flag);
-            if (ok) {
-              // behind this wait the softmax of four fragments ago is over: the flag may be used again
-              if (t == 0 || bad) s_bad[nf & 7] = bad;
-              mbar_expect_tx(&k_full[st], n_p * NH * PAGE_BYTES);
-              for (int p = 0; p < n_p; ++p)
-                for (int h = 0; h < NH; ++h)
-                  tma_load_2d(sK + st * TILE + h * kPxHalf + p * PAGE_BYTES, &tma_k, h * 64, ((p ? p1 : p0) * a.n_kv + f.kvh) * kPxPage, &k_full[st]);
-              ok = mbar_wait(&v_empty[st], par ^ 1, abort_flag);
-            }
-            if (ok) {
-              mbar_expect_tx(&v_full[st], n_p * NH * PAGE_BYTES);
-              for (int p = 0; p < n_p; ++p)
-                for (int h = 0; h < NH; ++h)
-                  tma_load_2d(sV + st * TILE + (p * NH + h) * PAGE_BYTES, &tma_v, h * 64, ((p ? p1 : p0) * a.n_kv + f.kvh) * kPxPage, &v_full[st]);
+#pragma unroll
+            for (int kv = 0; ok && kv < 2; ++kv) {
+              if constexpr (Q8) ok = mbar_wait(&raw_empty[2 * kv + st], par ^ 1, abort_flag);
+              else ok = kv ? mbar_wait(&v_empty[st], par ^ 1, abort_flag) : mbar_wait(&k_empty[st], par ^ 1, abort_flag);
+              if (!ok) break;
+              // behind the first of these waits the softmax of six fragments ago is over: the flag may be used again
+              if (kv == 0 && (t == 0 || bad)) s_bad[nf & 7] = bad;
+              uint64_t* const full = Q8 ? &raw_full[2 * kv + st] : kv ? &v_full[st] : &k_full[st];
+              mbar_expect_tx(full, n_p * (Q8 ? RAW : NH * PAGE_BYTES));
+              for (int p = 0; p < n_p; ++p) {
+                const int block = (p ? p1 : p0) * a.n_kv + f.kvh;
+                if constexpr (Q8) {
+                  px_bulk(sRaw + ((st * 2 + kv) * 2 + p) * RAW, (kv ? a.v : a.k) + (long)block * RAW, RAW, full);
+                } else {
+                  for (int h = 0; h < NH; ++h) {
+                    uint8_t* dst = kv ? sV + st * TILE + (p * NH + h) * PAGE_BYTES : sK + st * TILE + h * kPxHalf + p * PAGE_BYTES;
+                    tma_load_2d(dst, kv ? &tma_v : &tma_k, h * 64, block * kPxPage, full);
+                  }
+                }
+              }
             }
           }
           ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
@@ -394,8 +467,8 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
         tile += n_t;
         // S = Q K^T of tile t into score buffer b
         auto first_product = [&](int t, int b) {
-          const int st = (tile0 + t) & 1;
-          ok = ok && mbar_wait_warp(&k_full[st], (uint32_t)(((tile0 + t) >> 1) & 1), abort_flag);
+          const int st = (tile0 + t) % ST;
+          ok = ok && mbar_wait_warp(&k_full[st], (uint32_t)(((tile0 + t) / ST) & 1), abort_flag);
           if (!ok) return;
           tc_fence_after();
 #pragma unroll
@@ -412,9 +485,9 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
         };
         // O += P V of tile t out of buffer b, the halves as their probabilities arrive
         auto second_product = [&](int t, int b, uint32_t old) {
-          const int st = (tile0 + t) & 1, half = 2 * x + (n_o & 1);
+          const int st = (tile0 + t) % ST, half = 2 * x + (n_o & 1);
           const uint32_t par = (uint32_t)((n_o >> 1) & 1);
-          ok = ok && mbar_wait_warp(&v_full[st], (uint32_t)(((tile0 + t) >> 1) & 1), abort_flag) && mbar_wait_warp(&p_full[half], par, abort_flag);
+          ok = ok && mbar_wait_warp(&v_full[st], (uint32_t)(((tile0 + t) / ST) & 1), abort_flag) && mbar_wait_warp(&p_full[half], par, abort_flag);
           if (!ok) return;
           tc_fence_after();
           const uint32_t tP = uS + b * 128;
@@ -433,8 +506,8 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
         };
         // a tile that this tile of rows takes no part in
         auto pass = [&](int t) {
-          const int st = (tile0 + t) & 1;
-          const uint32_t par = (uint32_t)(((tile0 + t) >> 1) & 1);
+          const int st = (tile0 + t) % ST;
+          const uint32_t par = (uint32_t)(((tile0 + t) / ST) & 1);
           ok = ok && mbar_wait_warp(&k_full[st], par, abort_flag);
           if (ok && lane == 0) mbar_arrive(&k_empty[st]);
           ok = ok && mbar_wait_warp(&v_full[st], par, abort_flag);
@@ -474,7 +547,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
       }
     }
   } else {
-    px_take_registers();
+    px_take_registers<Q8>();
     // ---- softmax: a thread per query row ------------------------------------------------------------------
     const int x = warp >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;                          // row of the tile
@@ -547,7 +620,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
         // and zero times that must be zero: the first tile of rows that takes part clears it in the value tile.
         auto finish = [&](int p) {
           const int n = p ? k1 : k0;
-          if (n > 0 && n < kPxPage && x == (who & 1 ? 0 : 1)) {
+          if (!Q8 && n > 0 && n < kPxPage && x == (who & 1 ? 0 : 1)) {
             const int st = tile & 1;
             ok = mbar_wait_warp(&v_full[st], (uint32_t)((tile >> 1) & 1), abort_flag);
             if (!ok) return false;
@@ -771,25 +844,28 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixArgs a) {
 
 using namespace bl;
 
-template <int HEAD>
+template <int HEAD, bool Q8>
 static int prefix_go(const PrefixArgs& a, cudaStream_t st) {
-  CUtensorMap mk, mv;
-  const cuuint64_t dims[2] = {(cuuint64_t)HEAD, (cuuint64_t)a.n_pages * a.n_kv * kPxPage};
-  const cuuint64_t strides[1] = {(cuuint64_t)HEAD * 2};
-  const cuuint32_t box[2] = {64, kPxPage};
-  int rc = make_map_any(&mk, a.k, 2, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc) return rc;
-  rc = make_map_any(&mv, a.v, 2, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc) return rc;
+  CUtensorMap mk = {}, mv = {};
+  if (!Q8) {
+    const cuuint64_t dims[2] = {(cuuint64_t)HEAD, (cuuint64_t)a.n_pages * a.n_kv * kPxPage};
+    const cuuint64_t strides[1] = {(cuuint64_t)HEAD * 2};
+    const cuuint32_t box[2] = {64, kPxPage};
+    int rc = make_map_any(&mk, a.k, 2, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+    rc = make_map_any(&mv, a.v, 2, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
   static PerDevice limit;
   if (limit.due()) {
-    const cudaError_t e = cudaFuncSetAttribute(prefix_attn_kernel<HEAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, px_smem(HEAD, kPxMaxRows, kPxMaxRows));
+    const cudaError_t e = cudaFuncSetAttribute(prefix_attn_kernel<HEAD, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               px_smem(HEAD, Q8, kPxMaxRows, kPxMaxRows));
     if (e != cudaSuccess) return (int)e;
     limit.mark();
   }
-  const cudaError_t e = launch(prefix_attn_kernel<HEAD>, dim3(a.n_cta), dim3(kPxThreads), (size_t)px_smem(HEAD, a.n_units, a.M), st, mk, mv, a);
+  const cudaError_t e = launch(prefix_attn_kernel<HEAD, Q8>, dim3(a.n_cta), dim3(px_threads(Q8)), (size_t)px_smem(HEAD, Q8, a.n_units, a.M), st, mk, mv, a);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch(prefix_join_kernel<HEAD, false>, dim3(a.n_kv, a.M, HEAD / 32), dim3(256), (size_t)PxLine::words(a.M, a.n_units) * 4, st, a);
+  return (int)launch(prefix_join_kernel<HEAD, Q8>, dim3(a.n_kv, a.M, HEAD / 32), dim3(256), (size_t)PxLine::words(a.M, a.n_units) * 4, st, a);
 }
 
 extern "C" {
@@ -812,12 +888,8 @@ int bl_prefix_attention(const float* q, const void* k_cache, const void* v_cache
                meta, (__nv_bfloat16*)out, fault, layer, meta + (long)M * kPxMeta, n_units, n_cta};
   a.part = (float4*)work;
   a.ml = (float2*)((uint8_t*)work + ((long)n_kv * n_units + n_cta) * 256 * head * 4);
-  const dim3 grid(n_q, M);
-  if (kv_q8) {
-    if (head == 128) return (int)launch(prefix_rows_kernel<128>, grid, dim3(32), 0, st, a);
-    return (int)launch(prefix_rows_kernel<64>, grid, dim3(32), 0, st, a);
-  }
-  return head == 128 ? prefix_go<128>(a, st) : prefix_go<64>(a, st);
+  if (kv_q8) return head == 128 ? prefix_go<128, true>(a, st) : prefix_go<64, true>(a, st);
+  return head == 128 ? prefix_go<128, false>(a, st) : prefix_go<64, false>(a, st);
 }
 
 }  // extern "C"
