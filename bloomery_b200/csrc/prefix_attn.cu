@@ -42,6 +42,7 @@ struct PrefixArgs {
   unsigned* fault; int layer;
   const int* units;               // [n_units][first row, rows, shared positions, first row of the group, rows of the group]
   int n_units, n_cta;
+  int4* sched;                    // [M] tiles of a KV head; running sums of the row's unit; keys: of this call, for the joining launch
   float4* part; float2* ml;       // [fragment][tile][HEAD / 4][128], [fragment][tile][128]
 };
 constexpr int kPxMeta = 5, kPxUnit = 5;
@@ -95,7 +96,12 @@ __device__ __forceinline__ void px_row(const PrefixArgs& a, int m, int h, int n,
 // Per KV head the tiles of all units (S), CTA c of n takes tiles c T / n .. (c + 1) T / n - 1 of the T = n_kv S.  A fragment is what
 // a stretch shares with a (KV head, unit); fragments' numbers (index + CTA) grow by one from each to the next within a unit and
 // by one at least between units, so they name places in the scratch.  All CTAs and the joining launch work the line out alike.
-struct PxFrag { int unit, kvh, t_lo, n_t, id; };
+struct PxFrag {
+  int unit, kvh, t_lo, n_t, id;
+  int row0, rows, shared, total;  // rows of the unit; its pages, shared and in all
+  int row;                        // whose own pages it starts in
+  int pad[2];
+};
 
 struct PxLine {
   int* keys;                      // [M] keys of a row
@@ -103,7 +109,7 @@ struct PxLine {
   int* tiles;                     // [n_units + 1] running sum of the units' tiles
   int* seq;                       // [M]
   int* units;                     // [n_units][kPxUnit]
-  int n_units, n_kv, S, T, n_cta, cta, g, end;
+  int n_units, S, g, end, cta;
 
   __device__ __forceinline__ static int find(const int* cum, int n, int at) {      // the last i with cum[i] <= at
     int lo = 0, hi = n;
@@ -123,18 +129,20 @@ struct PxLine {
     if (lane == 0) cum[0] = 0;
   }
   __host__ __device__ static constexpr int words(int M, int n_units) { return 3 * M + 1 + n_units + 1 + n_units * kPxUnit; }
-  // whole block; `mem` holds words(M, n_units)
-  __device__ __forceinline__ void build(const PrefixArgs& a, int* mem, bool raise) {
+  // Whole block; `mem` holds words(M, n_units).  The first fragment is worked out once for all warps: a look-up costs each of them
+  // some hundred instructions that are met for the first time, at a dozen clocks each.
+  __device__ __forceinline__ void build(const PrefixArgs& a, int* mem, int4* s_first) {
     keys = mem; pages = keys + a.M; tiles = pages + a.M + 1; seq = tiles + a.n_units + 1; units = seq + a.M;
-    n_units = a.n_units; n_kv = a.n_kv;
+    n_units = a.n_units;
+    cta = blockIdx.x;
     for (int i = threadIdx.x; i < n_units * kPxUnit; i += blockDim.x) units[i] = a.units[i];
     for (int m = threadIdx.x; m < a.M; m += blockDim.x) {
-      const int shared = a.meta[m * kPxMeta + 2];
+      const int shared = a.meta[m * kPxMeta + 2], sq = a.row_seq[m];
       bool bad;
       const int n = px_keys(a, m, bad);
-      if (bad && raise) raise_fault(a.fault, a.layer, FS_KEY_COUNT);
+      if (bad && blockIdx.x == 0) raise_fault(a.fault, a.layer, FS_KEY_COUNT);
       keys[m] = n;
-      seq[m] = a.row_seq[m];
+      seq[m] = sq;
       pages[m + 1] = max(0, n - shared + kPxPage - 1) / kPxPage;
     }
     __syncthreads();
@@ -149,48 +157,64 @@ struct PxLine {
       }
       __syncwarp();
       running(tiles, n_units);
+      __syncwarp();
+      if (threadIdx.x == 0) {
+        S = tiles[n_units];
+        const unsigned T = (unsigned)(a.n_kv * S), n = min((unsigned)a.n_cta, T);  // a tile each at least: a unit's CTAs follow each other
+        g = (unsigned)cta < n ? (int)((unsigned)cta * T / n) : 0;
+        end = (unsigned)cta < n ? (int)((unsigned)(cta + 1) * T / n) : 0;
+        PxFrag f = {};
+        const int some = next(f);
+        const int4* from = reinterpret_cast<const int4*>(&f);
+        s_first[0] = make_int4(S, g, end, some);
+        s_first[1] = from[0]; s_first[2] = from[1]; s_first[3] = from[2];
+      }
     }
     __syncthreads();
-    S = tiles[n_units];
-    T = n_kv * S;
-    n_cta = min(a.n_cta, T);                                    // a tile each at least, so that a unit's CTAs follow each other
+    const int4 h = s_first[0];
+    S = h.x; g = h.y; end = h.z;
+    // for the launch that joins the fragments
+    if (blockIdx.x == 0)
+      for (int m = threadIdx.x; m < a.M; m += blockDim.x) {
+        const int u = a.meta[m * kPxMeta + 3];
+        a.sched[m] = make_int4(S, tiles[u], tiles[u + 1], keys[m]);
+      }
   }
-  __device__ __forceinline__ void start(int c) {
-    cta = c;
-    g = c < n_cta ? (int)((long)c * T / n_cta) : 0;
-    end = c < n_cta ? (int)((long)(c + 1) * T / n_cta) : 0;
+  __device__ __forceinline__ bool first(const int4* s_first, PxFrag& f) const {
+    int4* to = reinterpret_cast<int4*>(&f);
+    to[0] = s_first[1]; to[1] = s_first[2]; to[2] = s_first[3];
+    return s_first[0].w != 0;
   }
   __device__ __forceinline__ bool next(PxFrag& f) {
     if (g >= end) return false;
-    f.kvh = g / S;
+    f.kvh = (int)((unsigned)g / (unsigned)S);
     const int rem = g - f.kvh * S;
     f.unit = find(tiles, n_units, rem);
     f.t_lo = rem - tiles[f.unit];
     f.n_t = min(tiles[f.unit + 1] - rem, end - g);
     f.id = f.kvh * n_units + f.unit + cta;
     g += f.n_t;
+    const int* unit = units + f.unit * kPxUnit;
+    f.row0 = unit[0]; f.rows = unit[1]; f.shared = unit[2] / kPxPage;
+    f.total = f.shared + pages[f.row0 + f.rows] - pages[f.row0];
+    f.row = f.row0;
+    if (2 * f.t_lo > f.shared) f.row = f.row0 + find(pages + f.row0, f.rows, pages[f.row0] + 2 * f.t_lo - f.shared);
     return true;
   }
-  __device__ __forceinline__ int cta_of(int at) const { return (int)(((long)(at + 1) * n_cta - 1) / T); }
 };
 
 // The pages of a unit in order: the shared ones, then every row's own.  A tile is two of them.
 struct PxWalk {
   const int* keys; const int* pages;
   int row0, rows, shared, total, row;                           // shared, total: pages
-  __device__ __forceinline__ void start(const PxLine& line, int u, int page) {
-    const int* unit = line.units + u * kPxUnit;
+  __device__ __forceinline__ void start(const PxLine& line, const PxFrag& f) {
     keys = line.keys; pages = line.pages;
-    row0 = unit[0]; rows = unit[1]; shared = unit[2] / kPxPage;
-    total = shared + pages[row0 + rows] - pages[row0];
-    row = row0;
-    if (page > shared) row = row0 + PxLine::find(pages + row0, rows, pages[row0] + page - shared);
+    row0 = f.row0; rows = f.rows; shared = f.shared; total = f.total; row = f.row;
   }
   // Both pages of a tile at once; for shared pages, most of a long walk, nothing is looked up.
   __device__ __forceinline__ void tile(int t, int& o0, int& c0, int& n0, int& o1, int& c1, int& n1) {
-    if (2 * t + 2 <= shared) {
-      o0 = o1 = -1; c0 = 2 * t; c1 = 2 * t + 1; n0 = n1 = kPxPage;
-    } else {
+    o0 = o1 = -1; c0 = 2 * t; c1 = 2 * t + 1; n0 = n1 = kPxPage;
+    if (2 * t + 2 > shared) {
       page(2 * t, o0, c0, n0);
       page(2 * t + 1, o1, c1, n1);
     }
@@ -258,15 +282,6 @@ constexpr int px_smem(int head, bool q8, int n_units, int M) {
 // q8_0 caches have four more warps, which expand the rows
 constexpr int px_threads(bool q8) { return q8 ? 512 : 384; }
 
-// Registers a lane: 3 x 168 at the launch = 104 + 200 + 200, with the expanding warps 4 x 128 = 72 + 88 + 176 + 176.
-template <bool Q8> __device__ __forceinline__ void px_give_registers() {
-  if constexpr (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-}
-template <bool Q8> __device__ __forceinline__ void px_take_registers() {
-  if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-  else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-}
 __device__ __forceinline__ void px_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
@@ -303,6 +318,8 @@ __device__ __forceinline__ void px_expand(const uint8_t* row, uint8_t* dst, int 
   }
 }
 
+__device__ __forceinline__ void px_prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 template <int HEAD, bool Q8>
 __global__ void __launch_bounds__(px_threads(Q8), 1)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const PrefixArgs a) {
@@ -311,6 +328,8 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
   __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[4], p_full[8], pv_done[4], frag_start, raw_full[4], raw_empty[4];
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort, s_bad[8];
+  __shared__ int4 s_first[4];
+  __shared__ float s_scale[2][128];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sQ = smem;                // [2 tiles][NH][128 rows][128 bytes]
   uint8_t* sK = sQ + 2 * TILE;       // [ST stages][NH][128 keys][128 bytes]
@@ -333,13 +352,20 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // Ahead of the wait, for lines and address translations alone: a first touch of a page costs a processor the better part of a
+  // microsecond, and these would follow each other.
+  for (int i = threadIdx.x; i < a.M; i += blockDim.x) { px_prefetch(a.row_pos + i); px_prefetch(a.row_seq + i); px_prefetch(a.meta + i * kPxMeta); }
+  if (threadIdx.x < 32) { px_prefetch(a.units + min((int)threadIdx.x, a.n_units - 1) * kPxUnit); px_prefetch(a.table + threadIdx.x * 32); px_prefetch(a.part + threadIdx.x * 8); }
+  {
+    const long at = ((long)blockIdx.x * blockDim.x + threadIdx.x) * 32;
+    if (at < (long)a.M * a.n_q * HEAD) px_prefetch(a.q + at);
+  }
   pdl_wait();
   pdl_launch();
   PxLine line;
   tc_fence_before();
-  line.build(a, reinterpret_cast<int*>(sRaw + (Q8 ? 8 * RAW : 0)), blockIdx.x == 0);
+  line.build(a, reinterpret_cast<int*>(sRaw + (Q8 ? 8 * RAW : 0)), s_first);
   tc_fence_after();
-  line.start(blockIdx.x);
   const uint32_t tmem_base = s_tmem_base;
   volatile int* abort_flag = &s_abort;
   const uint32_t tS0 = tmem_base, tO0 = tmem_base + 256;        // score buffer b at column 128 b, output of tile x at 256 + HEAD x
@@ -348,12 +374,11 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
 
   if (Q8 && warp >= 12) {
     // ---- q8_0 rows to f16: a thread for a row of the tile
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     const int key = threadIdx.x - 384;
     int tile = 0;
     bool ok = true;
-    while (ok && line.next(f)) {
-      w.start(line, f.unit, 2 * f.t_lo);
+    for (bool more = line.first(s_first, f); ok && more; more = line.next(f)) {
+      w.start(line, f);
       for (int t = 0; ok && t < f.n_t; ++t, ++tile) {
         int o0, c0, k0, o1, c1, k1;
         w.tile(f.t_lo + t, o0, c0, k0, o1, c1, k1);
@@ -383,13 +408,13 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
       }
     }
   } else if (warp >= 8) {
-    px_give_registers<Q8>();
     if (warp == 8) {
       // ---- producer: all lanes walk, lane 0 waits and copies
       int tile = 0;
       bool ok = true;
-      for (int nf = 0; ok && line.next(f); ++nf) {
-        w.start(line, f.unit, 2 * f.t_lo);
+      int nf = 0;
+      for (bool more = line.first(s_first, f); ok && more; more = line.next(f), ++nf) {
+        w.start(line, f);
         const int* unit = line.units + f.unit * kPxUnit;
         int lead = -1;                                            // sequence of the first row of the group that has a table
         for (int i = 0; lead < 0 && i < unit[4]; i += 32) {
@@ -458,12 +483,10 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
       const uint32_t uS = (uint32_t)px_uniform((int)tS0), uO = uS + 256 + x * HEAD;
       int tile = 0, n_q = 0, n_s = 0, n_o = 0, n_f = 0;         // tiles through the rings; query tiles, first and second products; fragments
       bool ok = true;
-      for (int g = px_uniform(line.g), g_end = px_uniform(line.end); ok && g < g_end; ++n_f) {
-        line.next(f);
-        w.start(line, f.unit, 2 * f.t_lo);
+      for (int more = px_uniform(line.first(s_first, f)); ok && more; more = px_uniform(line.next(f)), ++n_f) {
+        w.start(line, f);
         const int n_x = px_uniform(w.rows > rows_tile ? 2 : 1), n_t = px_uniform(f.n_t), t_lo = px_uniform(f.t_lo), pages = px_uniform(w.total);
         const int shared = px_uniform(w.shared), tile0 = tile;
-        g += n_t;
         tile += n_t;
         // S = Q K^T of tile t into score buffer b
         auto first_product = [&](int t, int b) {
@@ -547,120 +570,109 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
       }
     }
   } else {
-    px_take_registers<Q8>();
     // ---- softmax: a thread per query row ------------------------------------------------------------------
     const int x = warp >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;                          // row of the tile
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint32_t tO = tO0 + x * HEAD + lane_base;
-    int tile = 0, mine = 0;                                     // tiles; jobs of this tile of rows
+    int tile = 0, mine = 0, nf = 0;                             // tiles; jobs of this tile of rows; fragments
     bool ok = true;
-    for (int nf = 0; ok && line.next(f); ++nf) {
-      w.start(line, f.unit, 2 * f.t_lo);
+    for (bool more = line.first(s_first, f); ok && more; more = line.next(f), ++nf) {
+      w.start(line, f);
       const int n_x = w.rows > rows_tile ? 2 : 1;
       const int live = max(0, min(rows_tile, w.rows - x * rows_tile)) * G;      // query rows of this tile
       const int my = r < live ? x * rows_tile + (r * inv_G >> 16) : -3;     // row of the unit
       const int n_keys = r < live ? w.keys[w.row0 + my] : 0;
       const bool busy = quarter * 32 < live;
-      float to_log2 = 0.f;
-      // queries to f16: four lanes a row, scaled by a power of two to a largest element in [512, 1024); all loads at once
+      // Queries to f16, scaled by a power of two a row to a largest element in [512, 1024): each warp takes every fourth row, four
+      // at a time.
       auto put_queries = [&]() {
-        if (busy) {
-          float4 v[4][HEAD / 16];
+        constexpr int N = HEAD / 32, AT_ONCE = 4;
+        const float* base = a.q + ((long)(w.row0 + x * rows_tile) * a.n_q + f.kvh * G) * HEAD + lane * N;
+        uint8_t* dst = sQ + x * TILE + (lane * N >> 6) * kPxHalf + ((lane * N * 2) & 15);
+        const int chunk = (lane * N & 63) >> 3;
+#pragma unroll 1
+        for (int i0 = quarter; i0 < live; i0 += 4 * AT_ONCE) {
+          float v[AT_ONCE][N];
 #pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            const int i = quarter * 32 + p * 8 + (lane >> 2), row = i * inv_G >> 16;
-            const float4* src = reinterpret_cast<const float4*>(a.q + ((long)(w.row0 + x * rows_tile + row) * a.n_q + f.kvh * G + i - row * G) * HEAD) + (lane & 3);
-#pragma unroll
-            for (int c = 0; c < HEAD / 16; ++c) v[p][c] = i < live ? __ldg(src + c * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-#pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            if (quarter * 32 + p * 8 >= live) break;
-            const int i = quarter * 32 + p * 8 + (lane >> 2);
-            float top = 0.f;
-#pragma unroll
-            for (int c = 0; c < HEAD / 16; ++c)
-              top = fmaxf(top, fmaxf(fmaxf(fabsf(v[p][c].x), fabsf(v[p][c].y)), fmaxf(fabsf(v[p][c].z), fabsf(v[p][c].w))));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = (int)(__float_as_uint(top) >> 23);    // top >= 0
-            const int se = e == 0 ? 127 : min(253, 263 - e);
-            const float scale = __uint_as_float((unsigned)se << 23);
-            const float back = kPxLog2e * __uint_as_float((unsigned)(254 - se) << 23);
-            const float given = __shfl_sync(0xffffffffu, back, (lane & 7) * 4);
-            if ((lane >> 3) == p) to_log2 = given;
-            uint8_t* dst = sQ + x * TILE + i * 128 + ((lane & 1) << 3);
-#pragma unroll
-            for (int c = 0; c < HEAD / 16; ++c) {
-              // values 4 (lane & 3) + 16 c ..: 8 bytes of 16-byte chunk 2 c + (lane & 3) / 2, swizzled within 64 values
-              const int chunk = 2 * c + ((lane >> 1) & 1);
-              *reinterpret_cast<uint2*>(dst + (chunk >> 3) * kPxHalf + (((chunk & 7) ^ (i & 7)) << 4)) =
-                  make_uint2(px_pack(v[p][c].x * scale, v[p][c].y * scale), px_pack(v[p][c].z * scale, v[p][c].w * scale));
+          for (int u = 0; u < AT_ONCE; ++u) {
+            const int i = i0 + 4 * u;
+            const float* src = base + (long)((i * inv_G >> 16) * (a.n_q - G) + i) * HEAD;
+            if constexpr (N == 4) {
+              const float4 q = i < live ? __ldg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+              v[u][0] = q.x; v[u][1] = q.y; v[u][2] = q.z; v[u][3] = q.w;
+            } else {
+              const float2 q = i < live ? __ldg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
+              v[u][0] = q.x; v[u][1] = q.y;
             }
           }
-          fence_async_smem();
+#pragma unroll
+          for (int u = 0; u < AT_ONCE; ++u) {
+            const int i = i0 + 4 * u;
+            float top = fabsf(v[u][0]);
+#pragma unroll
+            for (int j = 1; j < N; ++j) top = fmaxf(top, fabsf(v[u][j]));
+            const int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23);      // of non-negative floats: in order as integers
+            const int se = e == 0 ? 127 : min(253, 263 - e);
+            const float scale = __uint_as_float((unsigned)se << 23);
+            if (i < live) {
+              uint8_t* at = dst + i * 128 + ((chunk ^ (i & 7)) << 4);
+              const uint32_t lo = px_pack(v[u][0] * scale, v[u][1] * scale);
+              if constexpr (N == 4) *reinterpret_cast<uint2*>(at) = make_uint2(lo, px_pack(v[u][2] * scale, v[u][3] * scale));
+              else *reinterpret_cast<uint32_t*>(at) = lo;
+              if (lane == 0) s_scale[x][i] = kPxLog2e * __uint_as_float((unsigned)(254 - se) << 23);
+            }
+          }
         }
+        fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[x]);
       };
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f, to_log2 = 0.f;
       bool begun = false;
       for (int t = 0; t < f.n_t; ++t, ++tile) {
         int o0, c0, k0, o1, c1, k1;
         w.tile(f.t_lo + t, o0, c0, k0, o1, c1, k1);
         const unsigned who = px_tiles(o0, rows_tile, n_x) | px_tiles(o1, rows_tile, n_x);
         if (!(who >> x & 1)) continue;
-        const int b = n_x == 2 ? x : t & 1;
-        const uint32_t tS = tS0 + b * 128 + lane_base;
+        const uint32_t tS = tS0 + (n_x == 2 ? x : t & 1) * 128 + lane_base;
         // keys of either page that this thread's row attends to
         const int n0 = o0 == my ? k0 : o0 == -1 ? min(kPxPage, max(0, n_keys - kPxPage * c0)) : 0;
         const int n1 = o1 == my ? k1 : o1 == -1 ? min(kPxPage, max(0, n_keys - kPxPage * c1)) : 0;
-        // Half p of the probabilities is written.  Where a page ends inside the tile, what lies behind its keys may be anything,
-        // and zero times that must be zero: the first tile of rows that takes part clears it in the value tile.
-        auto finish = [&](int p) {
-          const int n = p ? k1 : k0;
-          if (!Q8 && n > 0 && n < kPxPage && x == (who & 1 ? 0 : 1)) {
-            const int st = tile & 1;
-            ok = mbar_wait_warp(&v_full[st], (uint32_t)((tile >> 1) & 1), abort_flag);
-            if (!ok) return false;
-            uint8_t* page = sV + st * TILE + p * NH * PAGE_BYTES;
-#pragma unroll
-            for (int h = 0; h < NH; ++h)
-              for (int i = n * 8 + r; i < kPxPage * 8; i += 128) *reinterpret_cast<uint4*>(page + h * PAGE_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
-            fence_async_smem();
-          }
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[4 * p + 2 * x + (mine & 1)]);
-          return true;
-        };
+        const bool some = __any_sync(0xffffffffu, n0 + n1 > 0), all = __all_sync(0xffffffffu, n0 + n1 == 2 * kPxPage);
         if (!begun) put_queries();
         ok = mbar_wait_warp(&s_full[2 * x + (mine & 1)], (uint32_t)((mine >> 1) & 1), abort_flag);
         if (!ok) break;
         tc_fence_after();
-        if (__any_sync(0xffffffffu, n0 + n1 > 0)) {
-          uint32_t v[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(tS + 32 * c, v[c]);
+        if (!begun) to_log2 = busy ? s_scale[x][r] : 0.f;       // written in front of what these scores waited for
+        // The scores are read twice, 32 at a time, in loops: 128 of them at once in straight code took 3,000 clocks the first time
+        // it was met, most of a short call's softmax.
+        auto scores = [&](int c, uint32_t (&v)[32]) {
+          tmem_ld32(tS + 32 * c, v);
           tmem_ld_wait();
-          if (__any_sync(0xffffffffu, n0 + n1 < 128)) {
+          if (!all) {
+            const int n = (c < 2 ? n0 : n1) - 32 * (c & 1);
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (32 * (c & 1) + i >= (c < 2 ? n0 : n1)) v[c][i] = 0xff800000u;      // -inf
+            for (int i = 0; i < 32; ++i)
+              if (i >= n) v[i] = 0xff800000u;                   // -inf
           }
+        };
+        float mb = 0.f, corr = 1.f;
+        if (some) {
           float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            scores(c, v);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2)
+            for (int i = 0; i < 32; i += 8)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) mx4[c] = fmaxf(fmaxf(mx4[c], __uint_as_float(v[c][i])), __uint_as_float(v[c][i + 1]));
+              for (int j = 0; j < 4; ++j) mx4[j] = fmaxf(fmaxf(mx4[j], __uint_as_float(v[i + j])), __uint_as_float(v[i + 4 + j]));
+          }
           float m_new = fmaxf(m, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
           if (m != -INFINITY && (m_new - m) * to_log2 <= kPxLazy) m_new = m;
-          const float mb = (m_new == -INFINITY) ? 0.f : m_new * to_log2;      // a row with no key yet keeps zeros
-          const float corr = (m == -INFINITY || m == m_new) ? 1.f : px_ex2(m * to_log2 - mb);
+          mb = (m_new == -INFINITY) ? 0.f : m_new * to_log2;    // a row with no key yet keeps zeros
+          corr = (m == -INFINITY || m == m_new) ? 1.f : px_ex2(m * to_log2 - mb);
           if (begun && __any_sync(0xffffffffu, corr != 1.0f)) {
             // the output is scaled in tensor memory, behind the tile's last product
             ok = mbar_wait_warp(&pv_done[2 * x + ((mine - 1) & 1)], (uint32_t)(((mine - 1) >> 1) & 1), abort_flag);
@@ -676,39 +688,53 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
               tmem_st32(tO + c * 32, o);
             }
           }
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
+          m = m_new;
+        }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+          if (some) {
+            uint32_t v[32];
+            scores(c, v);
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               uint32_t e0, e1;
               asm("{\n\t.reg .b64 rs, rk, rm, rr;\n\t"
                   "mov.b64 rs, {%2, %3};\n\tmov.b64 rk, {%4, %4};\n\tmov.b64 rm, {%5, %5};\n\t"
                   "fma.rn.f32x2 rr, rs, rk, rm;\n\tmov.b64 {%0, %1}, rr;\n\t}"
-                  : "=r"(e0), "=r"(e1) : "r"(v[c][i]), "r"(v[c][i + 1]), "f"(to_log2), "f"(-mb));
+                  : "=r"(e0), "=r"(e1) : "r"(v[i]), "r"(v[i + 1]), "f"(to_log2), "f"(-mb));
               const float p0 = px_ex2(__uint_as_float(e0)), p1 = px_ex2(__uint_as_float(e1));
               sum[i & 2] += p0; sum[(i & 2) + 1] += p1;
               pk[i >> 1] = px_pack(p0, p1);
             }
-            px_st16(tS + 16 * c, pk);
-            if (c == 1) {                                       // the first page's half of the second product may begin
-              if (!finish(0)) break;
-            }
+          } else {                                              // no row of this warp attends to these pages
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pk[i] = 0;
           }
-          if (!ok) break;
-          l = l * corr + ((sum[0] + sum[2]) + (sum[1] + sum[3]));
-          m = m_new;
-        } else {
-          // no row of this warp attends to these pages
-          uint32_t zero[16];
+          px_st16(tS + 16 * c, pk);
+          if (c & 1) {
+            // A page's half of the probabilities is written.  Where a sequence ends inside the page, what lies behind may be
+            // anything, and zero times that must be zero: the first tile of rows that takes part clears it.
+            const int p = c >> 1, n = p ? k1 : k0;
+            if (!Q8 && n > 0 && n < kPxPage && x == (who & 1 ? 0 : 1)) {
+              const int st = tile & 1;
+              ok = mbar_wait_warp(&v_full[st], (uint32_t)((tile >> 1) & 1), abort_flag);
+              if (!ok) break;
+              uint8_t* page = sV + st * TILE + p * NH * PAGE_BYTES;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) zero[i] = 0;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) px_st16(tS + 16 * c, zero);
-          if (!finish(0)) break;
+              for (int h = 0; h < NH; ++h)
+                for (int i = n * 8 + r; i < kPxPage * 8; i += 128) *reinterpret_cast<uint4*>(page + h * PAGE_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
+              fence_async_smem();
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[4 * p + 2 * x + (mine & 1)]);
+          }
         }
-        if (!finish(1)) break;
+        if (!ok) break;
+        l = l * corr + ((sum[0] + sum[2]) + (sum[1] + sum[3]));
         begun = true;
         ++mine;
       }
@@ -758,41 +784,55 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
 constexpr int kPxMaxCtas = 160;
 
 template <int HEAD, bool Q8>
-__global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixArgs a) {
-  extern __shared__ int s_line[];
+__global__ void __launch_bounds__(256, 4) prefix_join_kernel(const PrefixArgs a) {
   __shared__ float s_w[kPxMaxCtas * 16], s_inv[16];
   __shared__ float4 s_o[256];
   const int kvh = blockIdx.x, m = blockIdx.y, G = a.n_q / a.n_kv, tid = threadIdx.x, lane = tid & 31;
   // lengths and tables are older than the launch in front, which started behind what wrote them
   bool bad;
-  const int n = px_keys(a, m, bad);
+  px_keys(a, m, bad);
   const int* meta = a.meta + m * kPxMeta;
   const int unit = meta[3], x = meta[4] / 128, lane0 = meta[4] % 128;
-  PxLine line;
-  line.build(a, s_line, false);
-  int id = 0, n_f = 0;
-  if (n > 0) {
-    const int lo = kvh * line.S + line.tiles[unit], hi = kvh * line.S + line.tiles[unit + 1];
-    const int c = line.cta_of(lo);
-    n_f = line.cta_of(hi - 1) - c + 1;
-    id = kvh * a.n_units + unit + c;
-  }
   const int items = G * 8, sets = 256 / items, set = tid / items, h = tid % G, c = blockIdx.z * 8 + tid % items / G;
-  const float4* part = a.part + (((long)id * 2 + x) * (HEAD / 4) + c) * 128 + lane0 + h;
-  const float2* ml = a.ml + ((long)id * 2 + x) * 128 + lane0;
+  const float4* part = a.part + ((long)x * (HEAD / 4) + c) * 128 + lane0 + h;
+  const float2* ml = a.ml + (long)x * 128 + lane0;
+  int n_f = 0;
+  constexpr int AHEAD = 10, ROWS = kPxMaxCtas / 32;                             // fragments of a thread in flight; maxima of a lane
+  auto fetch = [&](int f0, float4 (&v)[AHEAD]) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int f = f0 + i * sets;
+      v[i] = set < sets && f < n_f ? __ldcg(part + (long)f * 2 * (HEAD / 4) * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  px_prefetch(a.sched + m);
+  if (tid == 0) px_prefetch(a.out + ((long)m * a.n_q + kvh * G) * HEAD);
   pdl_wait();
   pdl_launch();
+  const int4 sc = __ldcg(a.sched + m);                                          // tiles of a KV head, of the units before and up to this one; keys
+  const int n = sc.w;
+  if (n > 0) {
+    const unsigned T = (unsigned)(a.n_kv * sc.x), n_cta = min((unsigned)a.n_cta, T);
+    auto cta_of = [&](int at) { return (int)(((unsigned)(at + 1) * n_cta - 1) / T); };
+    const int c = cta_of(kvh * sc.x + sc.y);
+    n_f = cta_of(kvh * sc.x + sc.z - 1) - c + 1;
+    const long id = kvh * a.n_units + unit + c;
+    part += id * 2 * (HEAD / 4) * 128;
+    ml += id * 2 * 128;
+  }
+  float4 v[AHEAD];
+  fetch(set, v);
   for (int g = tid >> 5; g < G; g += 8) {
-    float2 q[kPxMaxCtas / 32];
+    float2 q[ROWS];
     float top = -INFINITY, den = 0.f;
 #pragma unroll
-    for (int i = 0; i < kPxMaxCtas / 32; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
       q[i] = lane + 32 * i < n_f ? __ldcg(ml + (long)(lane + 32 * i) * 256 + g) : make_float2(-INFINITY, 0.f);
       top = fmaxf(top, q[i].x);
     }
     top = warp_max(top);
 #pragma unroll
-    for (int i = 0; i < kPxMaxCtas / 32; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
       const float w = q[i].x > -INFINITY ? px_ex2(q[i].x - top) : 0.f;
       den += w > 0.f || q[i].y != q[i].y ? w * q[i].y : 0.f;                    // a NaN stays one, whatever its weight
       s_w[(lane + 32 * i) * 16 + g] = w;
@@ -802,19 +842,14 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixArgs a) {
   }
   __syncthreads();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (set < sets) {
-    constexpr int AHEAD = 8;                                                    // fragments in flight
-    for (int f0 = set; f0 < n_f; f0 += AHEAD * sets) {                          // ascending order, fixed
-      float4 v[AHEAD];
-      float w[AHEAD];
+  for (int f0 = set; f0 < n_f; f0 += AHEAD * sets) {                            // ascending order, fixed
+    if (f0 > set) fetch(f0, v);
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const int f = f0 + i * sets;
-        w[i] = f < n_f ? s_w[f * 16 + h] : 0.f;
-        v[i] = w[i] != 0.f ? __ldcg(part + (long)f * 2 * (HEAD / 4) * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) { o.x = fmaf(w[i], v[i].x, o.x); o.y = fmaf(w[i], v[i].y, o.y); o.z = fmaf(w[i], v[i].z, o.z); o.w = fmaf(w[i], v[i].w, o.w); }
+    for (int i = 0; i < AHEAD; ++i) {
+      const int f = f0 + i * sets;
+      const float w = f < n_f ? s_w[f * 16 + h] : 0.f;
+      // a fragment without keys of this row has no output: what lies there may be anything
+      if (w != 0.f) { o.x = fmaf(w, v[i].x, o.x); o.y = fmaf(w, v[i].y, o.y); o.z = fmaf(w, v[i].z, o.z); o.w = fmaf(w, v[i].w, o.w); }
     }
   }
   s_o[tid] = o;
@@ -865,14 +900,14 @@ static int prefix_go(const PrefixArgs& a, cudaStream_t st) {
   }
   const cudaError_t e = launch(prefix_attn_kernel<HEAD, Q8>, dim3(a.n_cta), dim3(px_threads(Q8)), (size_t)px_smem(HEAD, Q8, a.n_units, a.M), st, mk, mv, a);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch(prefix_join_kernel<HEAD, Q8>, dim3(a.n_kv, a.M, HEAD / 32), dim3(256), (size_t)PxLine::words(a.M, a.n_units) * 4, st, a);
+  return (int)launch(prefix_join_kernel<HEAD, Q8>, dim3(a.n_kv, a.M, HEAD / 32), dim3(256), 0, st, a);
 }
 
 extern "C" {
 
 // Bytes of scratch that bl_prefix_attention takes for these sizes (n_units units, n_cta processors).
 long bl_prefix_work_bytes(int head, int n_kv, int n_units, int n_cta) {
-  return ((long)n_kv * n_units + n_cta) * 256 * (head * 4 + 8);
+  return ((long)n_kv * n_units + n_cta) * 256 * (head * 4 + 8) + kPxMaxRows * 16;
 }
 
 int bl_prefix_attention(const float* q, const void* k_cache, const void* v_cache, const int* row_pos, const int* row_seq,
@@ -882,12 +917,13 @@ int bl_prefix_attention(const float* q, const void* k_cache, const void* v_cache
   BL_REQUIRE(head == 128 || head == 64, BL_ERR_SHAPE);
   BL_REQUIRE(n_kv >= 1 && n_q >= 1 && n_q % n_kv == 0 && n_q / n_kv <= 16, BL_ERR_SHAPE);
   BL_REQUIRE(M >= 1 && M <= kPxMaxRows && n_units >= 1 && n_units <= M && n_cta >= 1 && n_cta <= kPxMaxCtas && n_slots >= 1 && max_pages >= 1 && n_pages >= 1, BL_ERR_SHAPE);
-  BL_REQUIRE((long)n_pages * n_kv * kPxPage <= 0x7fffffffL && (long)(max_pages + 2) * M * n_kv <= 0x7fffffffL, BL_ERR_LIMIT);
+  BL_REQUIRE((long)n_pages * n_kv * kPxPage <= 0x7fffffffL && (long)(max_pages + 2) * M * n_kv <= 1L << 24, BL_ERR_LIMIT);
   BL_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)work) & 15) == 0, BL_ERR_ALIGN);
   PrefixArgs a{q, (const uint8_t*)k_cache, (const uint8_t*)v_cache, row_pos, row_seq, block_table, n_slots, max_pages, n_pages, n_q, n_kv, M,
                meta, (__nv_bfloat16*)out, fault, layer, meta + (long)M * kPxMeta, n_units, n_cta};
-  a.part = (float4*)work;
-  a.ml = (float2*)((uint8_t*)work + ((long)n_kv * n_units + n_cta) * 256 * head * 4);
+  a.sched = (int4*)work;
+  a.part = (float4*)((uint8_t*)work + kPxMaxRows * 16);
+  a.ml = (float2*)((uint8_t*)a.part + ((long)n_kv * n_units + n_cta) * 256 * head * 4);
   if (kv_q8) return head == 128 ? prefix_go<128, true>(a, st) : prefix_go<64, true>(a, st);
   return head == 128 ? prefix_go<128, false>(a, st) : prefix_go<64, false>(a, st);
 }
