@@ -398,9 +398,20 @@ long bl_beam_work_bytes(int V, int G, int B, int sms) {
   return R * 8 + R * n * 8 + R * n * B * 8 + R * B * 8 + (R + G) * 4;
 }
 
-int bl_beam_select(const float* logits, long stride, int V, int G, int B, const float* scores, const int* done, const int* lengths,
-                   int eos, float alpha, void* work, int sms, int* parent, int* token, float* out_scores, int* out_done,
-                   int* out_lengths, unsigned* fault, cudaStream_t st) {
+// Calls as one block of memory each: a host that makes one a step hands over a pointer instead of two dozen arguments.
+struct BeamSelectCall {
+  const float* logits; long stride; const float* scores; const int* done; const int* lengths; void* work;
+  int* parent; int* token; float* out_scores; int* out_done; int* out_lengths; unsigned* fault; cudaStream_t stream;
+  int V, G, B, eos, sms; float alpha;
+};
+struct BeamReorderCall {
+  void* k; void* v; long k_row, v_row; const int* table; int* table_out; const int* slots; const int* parent; const int* held;
+  unsigned* fault; cudaStream_t stream;
+  int n_layer, n_pages, n_kv, n_slots, max_pages, G, B, sms;
+};
+
+int bl_beam_select(const BeamSelectCall* call) {
+  const auto [logits, stride, scores, done, lengths, work, parent, token, out_scores, out_done, out_lengths, fault, st, V, G, B, eos, sms, alpha] = *call;
   BL_REQUIRE(V >= 1 && G >= 1 && B >= 1 && stride >= V && sms >= 1, BL_ERR_SHAPE);
   BL_REQUIRE(B <= kMaxBeams && (long)G * B <= 65535, BL_ERR_LIMIT);
   BL_REQUIRE(eos < V && (!done || eos >= 0) && (alpha == 0.f || lengths) && (!out_lengths || lengths), BL_ERR_SHAPE);
@@ -421,9 +432,8 @@ int bl_beam_select(const float* logits, long stride, int V, int G, int B, const 
   return (int)launch(beam_select_kernel<16>, grid, dim3(kBmThreads), 0, st, a);
 }
 
-int bl_beam_reorder(void* k, void* v, long k_row, long v_row, int n_layer, int n_pages, int n_kv, const int* table, int* table_out,
-                    int n_slots, int max_pages, const int* slots, const int* parent, const int* held, int G, int B, unsigned* fault,
-                    cudaStream_t st) {
+int bl_beam_reorder(const BeamReorderCall* call) {
+  const auto [k, v, k_row, v_row, table, table_out, slots, parent, held, fault, st, n_layer, n_pages, n_kv, n_slots, max_pages, G, B, sms] = *call;
   BL_REQUIRE(n_layer >= 1 && n_layer <= 65535 && n_pages >= 1 && n_kv >= 1 && G >= 1 && B >= 1 && n_slots >= 1 && max_pages >= 1,
              BL_ERR_SHAPE);
   BL_REQUIRE(B <= kMaxBeams, BL_ERR_LIMIT);

@@ -23,6 +23,8 @@
 // A value that is not finite would reach the masked rows of its tile as 0 x inf; rows whose output is not finite are summed again
 // key by key, over their own keys alone.
 // Every wait is bounded (1 s); on expiry the CTA raises the fault word, frees its TMEM and returns.
+#include <type_traits>
+
 #include "tc_common.cuh"
 
 namespace bl {
@@ -43,7 +45,11 @@ struct PrefixArgs {
   const int* units;               // [n_units][first row, rows, shared positions, first row of the group, rows of the group]
   int n_units, n_cta;
   int4* sched;                    // [M] tiles of a KV head; running sums of the row's unit; keys: of this call, for the joining launch
-  float4* part; float2* ml;       // [fragment][tile][HEAD / 4][128], [fragment][tile][128]
+  // [fragment][tiles of rows][outputs [HEAD / 4][pitch], then maxima and sums [pitch] of 8 bytes]: `slot` float4 a tile.  What lies
+  // close together needs few address translations.
+  float4* part;
+  int slot, slot_tiles, pitch;
+  long part_bytes;
 };
 constexpr int kPxMeta = 5, kPxUnit = 5;
 
@@ -320,8 +326,16 @@ __device__ __forceinline__ void px_expand(const uint8_t* row, uint8_t* dst, int 
 
 __device__ __forceinline__ void px_prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
+// a line of every 2 MB of the scratch
+__device__ __forceinline__ void px_touch_scratch(const PrefixArgs& a) {
+  for (long at = (long)threadIdx.x << 21; at < a.part_bytes; at += (long)blockDim.x << 21) px_prefetch(reinterpret_cast<const uint8_t*>(a.part) + at);
+  if (threadIdx.x < 32) px_prefetch(a.sched + threadIdx.x);
+}
+
 template <int HEAD, bool Q8>
-__global__ void __launch_bounds__(px_threads(Q8), 1)
+// Bounds of 512 threads in both forms: 128 registers a lane, so that blocks of the joining launch fit beside the 384 of f16 caches
+// and are there when these end (with 138 registers four beams behind 512 positions took 14.9 us a call instead of 12.5).
+__global__ void __launch_bounds__(512, 1)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const PrefixArgs a) {
   constexpr int NH = HEAD / 64, TILE = px_tile(HEAD), PAGE_BYTES = kPxPage * 128, ST = px_stages(Q8), RAW = px_raw(HEAD);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -355,7 +369,8 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
   // Ahead of the wait, for lines and address translations alone: a first touch of a page costs a processor the better part of a
   // microsecond, and these would follow each other.
   for (int i = threadIdx.x; i < a.M; i += blockDim.x) { px_prefetch(a.row_pos + i); px_prefetch(a.row_seq + i); px_prefetch(a.meta + i * kPxMeta); }
-  if (threadIdx.x < 32) { px_prefetch(a.units + min((int)threadIdx.x, a.n_units - 1) * kPxUnit); px_prefetch(a.table + threadIdx.x * 32); px_prefetch(a.part + threadIdx.x * 8); }
+  if (threadIdx.x < 32) { px_prefetch(a.units + min((int)threadIdx.x, a.n_units - 1) * kPxUnit); px_prefetch(a.table + threadIdx.x * 32); }
+  px_touch_scratch(a);
   {
     const long at = ((long)blockIdx.x * blockDim.x + threadIdx.x) * 32;
     if (at < (long)a.M * a.n_q * HEAD) px_prefetch(a.q + at);
@@ -585,14 +600,14 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
       const int n_keys = r < live ? w.keys[w.row0 + my] : 0;
       const bool busy = quarter * 32 < live;
       // Queries to f16, scaled by a power of two a row to a largest element in [512, 1024): each warp takes every fourth row, four
-      // at a time.
+      // or eight at a time.
       auto put_queries = [&]() {
-        constexpr int N = HEAD / 32, AT_ONCE = 4;
+        constexpr int N = HEAD / 32;
         const float* base = a.q + ((long)(w.row0 + x * rows_tile) * a.n_q + f.kvh * G) * HEAD + lane * N;
         uint8_t* dst = sQ + x * TILE + (lane * N >> 6) * kPxHalf + ((lane * N * 2) & 15);
         const int chunk = (lane * N & 63) >> 3;
-#pragma unroll 1
-        for (int i0 = quarter; i0 < live; i0 += 4 * AT_ONCE) {
+        auto some_rows = [&](int i0, auto at_once) {
+          constexpr int AT_ONCE = decltype(at_once)::value;
           float v[AT_ONCE][N];
 #pragma unroll
           for (int u = 0; u < AT_ONCE; ++u) {
@@ -623,6 +638,13 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
               if (lane == 0) s_scale[x][i] = kPxLog2e * __uint_as_float((unsigned)(254 - se) << 23);
             }
           }
+        };
+        if (live > 64) {
+#pragma unroll 1
+          for (int i0 = quarter; i0 < live; i0 += 32) some_rows(i0, std::integral_constant<int, 8>());
+        } else {
+#pragma unroll 1
+          for (int i0 = quarter; i0 < live; i0 += 16) some_rows(i0, std::integral_constant<int, 4>());
         }
         fence_async_smem();
         __syncwarp();
@@ -744,7 +766,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
       }
       if (!ok) break;
       if (busy) {
-        float4* part = a.part + ((long)f.id * 2 + x) * (HEAD / 4) * 128 + r;
+        float4* part = a.part + ((long)f.id * a.slot_tiles + x) * a.slot + r;
         if (begun && __any_sync(0xffffffffu, m != -INFINITY)) {
 #pragma unroll 1
           for (int c = 0; c < HEAD / 32; ++c) {
@@ -754,8 +776,8 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
             if (m != -INFINITY) {
 #pragma unroll
               for (int i = 0; i < 8; ++i)
-                __stcg(part + (c * 8 + i) * 128, make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                                             __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3])));
+                __stcg(part + (c * 8 + i) * a.pitch, make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                                 __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3])));
             }
           }
         }
@@ -763,7 +785,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
         // has no maximum, but a sum that tells
         const bool lost = l != l || (*(volatile int*)&s_bad[nf & 7] != 0 && m != -INFINITY);
         if (r < live)
-          __stcg(a.ml + ((long)f.id * 2 + x) * 128 + r,
+          __stcg(reinterpret_cast<float2*>(part - r + HEAD / 4 * a.pitch) + r,
                  lost ? make_float2(0.f, __int_as_float(0x7fc00000)) : make_float2(m == -INFINITY ? m : m * to_log2, l));
         tc_fence_before();
       }
@@ -793,41 +815,42 @@ __global__ void __launch_bounds__(256, 4) prefix_join_kernel(const PrefixArgs a)
   px_keys(a, m, bad);
   const int* meta = a.meta + m * kPxMeta;
   const int unit = meta[3], x = meta[4] / 128, lane0 = meta[4] % 128;
-  const int items = G * 8, sets = 256 / items, set = tid / items, h = tid % G, c = blockIdx.z * 8 + tid % items / G;
-  const float4* part = a.part + ((long)x * (HEAD / 4) + c) * 128 + lane0 + h;
-  const float2* ml = a.ml + (long)x * 128 + lane0;
-  int n_f = 0;
-  constexpr int AHEAD = 10, ROWS = kPxMaxCtas / 32;                             // fragments of a thread in flight; maxima of a lane
-  auto fetch = [&](int f0, float4 (&v)[AHEAD]) {
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int f = f0 + i * sets;
-      v[i] = set < sets && f < n_f ? __ldcg(part + (long)f * 2 * (HEAD / 4) * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-  };
-  px_prefetch(a.sched + m);
+  const int cols = HEAD / 4 / gridDim.z, items = G * cols;                      // float4 of a head, of the block: 256 at most
+  const int sets = 256 / items, set = tid / items, h = tid % G, c = blockIdx.z * cols + tid % items / G;
+  px_touch_scratch(a);
   if (tid == 0) px_prefetch(a.out + ((long)m * a.n_q + kvh * G) * HEAD);
   pdl_wait();
   pdl_launch();
-  const int4 sc = __ldcg(a.sched + m);                                          // tiles of a KV head, of the units before and up to this one; keys
+  const int4 sc = __ldcg(a.sched + m);                                          // pages of a KV head, of the units before and up to this one; keys
   const int n = sc.w;
+  int n_f = 0;
+  long id = 0;
   if (n > 0) {
     const unsigned T = (unsigned)(a.n_kv * sc.x), n_cta = min((unsigned)a.n_cta, T);
     auto cta_of = [&](int at) { return (int)(((unsigned)(at + 1) * n_cta - 1) / T); };
-    const int c = cta_of(kvh * sc.x + sc.y);
-    n_f = cta_of(kvh * sc.x + sc.z - 1) - c + 1;
-    const long id = kvh * a.n_units + unit + c;
-    part += id * 2 * (HEAD / 4) * 128;
-    ml += id * 2 * 128;
+    const int c0 = cta_of(kvh * sc.x + sc.y);
+    n_f = cta_of(kvh * sc.x + sc.z - 1) - c0 + 1;
+    id = kvh * a.n_units + unit + c0;
   }
+  const long step = (long)a.slot * a.slot_tiles;                                // float4 from a fragment to the next
+  const float4* part = a.part + id * step + x * a.slot + c * a.pitch + lane0 + h;
+  const float4* ml = a.part + id * step + x * a.slot + HEAD / 4 * a.pitch;
+  constexpr int AHEAD = 10, ROWS = kPxMaxCtas / 32;                             // fragments of a thread in flight; maxima of a lane
   float4 v[AHEAD];
-  fetch(set, v);
+  auto fetch = [&](int f0) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int f = f0 + i * sets;
+      v[i] = set < sets && f < n_f ? __ldcg(part + f * step) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  fetch(set);
   for (int g = tid >> 5; g < G; g += 8) {
     float2 q[ROWS];
     float top = -INFINITY, den = 0.f;
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      q[i] = lane + 32 * i < n_f ? __ldcg(ml + (long)(lane + 32 * i) * 256 + g) : make_float2(-INFINITY, 0.f);
+      q[i] = lane + 32 * i < n_f ? __ldcg(reinterpret_cast<const float2*>(ml + (lane + 32 * i) * step) + lane0 + g) : make_float2(-INFINITY, 0.f);
       top = fmaxf(top, q[i].x);
     }
     top = warp_max(top);
@@ -843,7 +866,7 @@ __global__ void __launch_bounds__(256, 4) prefix_join_kernel(const PrefixArgs a)
   __syncthreads();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int f0 = set; f0 < n_f; f0 += AHEAD * sets) {                            // ascending order, fixed
-    if (f0 > set) fetch(f0, v);
+    if (f0 > set) fetch(f0);
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int f = f0 + i * sets;
@@ -856,7 +879,7 @@ __global__ void __launch_bounds__(256, 4) prefix_join_kernel(const PrefixArgs a)
   __syncthreads();
   bool again = false;
   if (tid < items) {
-    for (int i = 1; i < sets; ++i) { const float4 v = s_o[tid + i * items]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w; }
+    for (int i = 1; i < sets; ++i) { const float4 u = s_o[tid + i * items]; o.x += u.x; o.y += u.y; o.z += u.z; o.w += u.w; }
     const float inv = bad ? __int_as_float(0x7fc00000) : n > 0 ? s_inv[h] : 0.f;
     const __nv_bfloat162 b0 = __floats2bfloat162_rn(o.x * inv, o.y * inv), b1 = __floats2bfloat162_rn(o.z * inv, o.w * inv);
     *reinterpret_cast<uint2*>(a.out + ((long)m * a.n_q + kvh * G + h) * HEAD + c * 4) =
@@ -870,7 +893,7 @@ __global__ void __launch_bounds__(256, 4) prefix_join_kernel(const PrefixArgs a)
       px_row<HEAD, Q8>(a, m, kvh * G + g, n, r);
 #pragma unroll
       for (int i = 0; i < HEAD / 32; ++i)
-        if (lane * (HEAD / 32) / 32 == (int)blockIdx.z) a.out[((long)m * a.n_q + kvh * G + g) * HEAD + lane * (HEAD / 32) + i] = __float2bfloat16_rn(r[i]);
+        if (lane * (HEAD / 32) / (4 * cols) == (int)blockIdx.z) a.out[((long)m * a.n_q + kvh * G + g) * HEAD + lane * (HEAD / 32) + i] = __float2bfloat16_rn(r[i]);
     }
   }
 }
@@ -900,31 +923,53 @@ static int prefix_go(const PrefixArgs& a, cudaStream_t st) {
   }
   const cudaError_t e = launch(prefix_attn_kernel<HEAD, Q8>, dim3(a.n_cta), dim3(px_threads(Q8)), (size_t)px_smem(HEAD, Q8, a.n_units, a.M), st, mk, mv, a);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch(prefix_join_kernel<HEAD, Q8>, dim3(a.n_kv, a.M, HEAD / 32), dim3(256), 0, st, a);
+  // few rows: a block for 32 values of a head, so that more of its fragments are in flight; many: as much of it as 256 threads hold
+  int z = HEAD / 32;
+  const int G = a.n_q / a.n_kv;
+  if (a.n_kv * a.M > a.n_cta) while (z > 1 && G * (HEAD / 4) / (z / 2) <= 256) z /= 2;
+  return (int)launch(prefix_join_kernel<HEAD, Q8>, dim3(a.n_kv, a.M, z), dim3(256), 0, st, a);
 }
 
 extern "C" {
 
-// Bytes of scratch that bl_prefix_attention takes for these sizes (n_units units, n_cta processors).
-long bl_prefix_work_bytes(int head, int n_kv, int n_units, int n_cta) {
-  return ((long)n_kv * n_units + n_cta) * 256 * (head * 4 + 8) + kPxMaxRows * 16;
+// Bytes of scratch that bl_prefix_attention takes for units of up to unit_rows rows (n_cta processors).
+static long prefix_slots(int head, int G, int n_kv, int n_units, int unit_rows, int n_cta, int& slot, int& tiles, int& pitch) {
+  const int per = 128 / G;
+  tiles = unit_rows > per ? 2 : 1;
+  pitch = ((unit_rows < per ? unit_rows : per) * G + 7) / 8 * 8;
+  slot = (head / 4 * pitch + pitch / 2);
+  return ((long)n_kv * n_units + n_cta) * tiles * slot * 16;
+}
+long bl_prefix_work_bytes(int head, int n_q, int n_kv, int n_units, int unit_rows, int n_cta) {
+  int slot, tiles, pitch;
+  return prefix_slots(head, n_q / n_kv, n_kv, n_units, unit_rows, n_cta, slot, tiles, pitch) + kPxMaxRows * 16;
 }
 
-int bl_prefix_attention(const float* q, const void* k_cache, const void* v_cache, const int* row_pos, const int* row_seq,
-                        const int* block_table, int n_slots, int max_pages, int n_pages, int head, int n_q, int n_kv, int M,
-                        const int* meta, int n_units, void* work, int kv_q8, void* out, int n_cta, unsigned* fault, int layer,
-                        cudaStream_t st) {
+// The call as one block of memory: a host that makes a call a layer hands over one pointer instead of two dozen arguments.
+struct PrefixCall {
+  const float* q; const void* k_cache; const void* v_cache; const int* row_pos; const int* row_seq; const int* block_table;
+  const int* meta; void* work; void* out; unsigned* fault; cudaStream_t stream;
+  int n_slots, max_pages, n_pages, head, n_q, n_kv, M, n_units, unit_rows, kv_q8, n_cta, layer;
+};
+
+int bl_prefix_attention(const PrefixCall* call) {
+  const PrefixCall& p = *call;
+  const int head = p.head, n_q = p.n_q, n_kv = p.n_kv, M = p.M, n_units = p.n_units, unit_rows = p.unit_rows, n_cta = p.n_cta;
+  const int max_pages = p.max_pages, n_pages = p.n_pages;
+  void* work = p.work;
   BL_REQUIRE(head == 128 || head == 64, BL_ERR_SHAPE);
   BL_REQUIRE(n_kv >= 1 && n_q >= 1 && n_q % n_kv == 0 && n_q / n_kv <= 16, BL_ERR_SHAPE);
-  BL_REQUIRE(M >= 1 && M <= kPxMaxRows && n_units >= 1 && n_units <= M && n_cta >= 1 && n_cta <= kPxMaxCtas && n_slots >= 1 && max_pages >= 1 && n_pages >= 1, BL_ERR_SHAPE);
+  BL_REQUIRE(M >= 1 && M <= kPxMaxRows && n_units >= 1 && n_units <= M && unit_rows >= 1 && unit_rows <= 2 * (128 / (n_q / n_kv)), BL_ERR_SHAPE);
+  BL_REQUIRE(n_cta >= 1 && n_cta <= kPxMaxCtas && p.n_slots >= 1 && max_pages >= 1 && n_pages >= 1, BL_ERR_SHAPE);
   BL_REQUIRE((long)n_pages * n_kv * kPxPage <= 0x7fffffffL && (long)(max_pages + 2) * M * n_kv <= 1L << 24, BL_ERR_LIMIT);
-  BL_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)work) & 15) == 0, BL_ERR_ALIGN);
-  PrefixArgs a{q, (const uint8_t*)k_cache, (const uint8_t*)v_cache, row_pos, row_seq, block_table, n_slots, max_pages, n_pages, n_q, n_kv, M,
-               meta, (__nv_bfloat16*)out, fault, layer, meta + (long)M * kPxMeta, n_units, n_cta};
+  BL_REQUIRE((((uintptr_t)p.q | (uintptr_t)p.k_cache | (uintptr_t)p.v_cache | (uintptr_t)p.out | (uintptr_t)work) & 15) == 0, BL_ERR_ALIGN);
+  PrefixArgs a{p.q, (const uint8_t*)p.k_cache, (const uint8_t*)p.v_cache, p.row_pos, p.row_seq, p.block_table, p.n_slots, max_pages, n_pages,
+               n_q, n_kv, M, p.meta, (__nv_bfloat16*)p.out, p.fault, p.layer, p.meta + (long)M * kPxMeta, n_units, n_cta};
+  const cudaStream_t st = p.stream;
   a.sched = (int4*)work;
   a.part = (float4*)((uint8_t*)work + kPxMaxRows * 16);
-  a.ml = (float2*)((uint8_t*)a.part + ((long)n_kv * n_units + n_cta) * 256 * head * 4);
-  if (kv_q8) return head == 128 ? prefix_go<128, true>(a, st) : prefix_go<64, true>(a, st);
+  a.part_bytes = prefix_slots(head, n_q / n_kv, n_kv, n_units, unit_rows, n_cta, a.slot, a.slot_tiles, a.pitch);
+  if (p.kv_q8) return head == 128 ? prefix_go<128, true>(a, st) : prefix_go<64, true>(a, st);
   return head == 128 ? prefix_go<128, false>(a, st) : prefix_go<64, false>(a, st);
 }
 

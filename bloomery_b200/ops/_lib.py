@@ -74,6 +74,11 @@ def stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def raw_stream(index: int) -> int:
+    """The handle of the current stream of device ``index``, without the object that :func:`stream` makes (a microsecond a call)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 I = ctypes.c_int
 L = ctypes.c_long
 F = ctypes.c_float

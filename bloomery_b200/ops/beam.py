@@ -2,30 +2,34 @@
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
 
 from ..runtime.kv import PAGE
-from ._lib import check, cuda
+from ._lib import check, cuda, raw_stream
 from .decode import sm_count
 
 MAX_BEAMS = 64
-_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
+_SELECT, _REORDER = struct.Struct("P1l11P5if"), struct.Struct("2P2l7P8i")        # BeamSelectCall, BeamReorderCall in the source
 _entries: dict = {}
 
 
-def _fn(name, *args):
+def _fn(name):
     fn = _entries.get(name)
     if fn is None:
-        fn = getattr(cuda(), name)
-        fn.argtypes = args
-        _entries[name] = fn
+        fn = _entries[name] = getattr(cuda(), name)
+        fn.argtypes = [ctypes.c_char_p]
     return fn
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return t.data_ptr() if t is not None else None
+def _same(name: str, t: torch.Tensor, dtype, n: int, index: int) -> int:
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous {dtype}, {n} values")
+    if t.get_device() != index:
+        raise ValueError(f"{name}: on another device than the rest")
+    return t.data_ptr()
 
 
 class BeamScratch:
@@ -37,17 +41,16 @@ class BeamScratch:
             raise ValueError(f"searches of 1 to {MAX_BEAMS} beams")
         self.groups, self.beams, self.vocab = groups, beams, vocab
         self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
         if groups * beams > 65535:
             raise ValueError("at most 65,535 beams in all")
         self.sms = sm_count(self.device) if self.device.type == "cuda" else 1
-        size = _fn("bl_beam_work_bytes", _I, _I, _I, _I)
-        size.restype = _L
+        self.index = self.device.index if self.device.type == "cuda" else -1      # as Tensor.get_device() says it
+        size = cuda().bl_beam_work_bytes
+        size.restype = ctypes.c_long
         self.work = torch.zeros(size(vocab, groups, beams, self.sms), dtype=torch.uint8, device=self.device)
-
-
-def _same(name: str, t: torch.Tensor, dtype, n: int) -> None:
-    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"{name}: contiguous {dtype}, {n} values")
+        self.work_ptr = self.work.data_ptr()
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, scratch: BeamScratch, parent: torch.Tensor, token: torch.Tensor,
@@ -63,26 +66,30 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, scratch: BeamScratch
     a logit of -inf are no candidates; where a search has too few, the last places get parent = their own index, token ``eos`` (0
     without one), score -inf and done.  A search with a NaN or +inf among its logits or scores gets NaN scores and raises
     ``fault``."""
-    G, B = scratch.groups, scratch.beams
+    G, B, V, index = scratch.groups, scratch.beams, scratch.vocab, scratch.index
     n = G * B
-    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.shape[0] != n or logits.shape[1] != scratch.vocab or \
-            (logits.stride(1) != 1 and scratch.vocab > 1):
-        raise ValueError(f"logits: fp32 [{n}, {scratch.vocab}], ids next to each other")
-    _same("scores", scores, torch.float32, n)
-    _same("out_scores", out_scores, torch.float32, n)
-    _same("parent", parent, torch.int32, n)
-    _same("token", token, torch.int32, n)
-    for name, t in (("done", done), ("lengths", lengths), ("out_done", out_done), ("out_lengths", out_lengths)):
-        if t is not None:
-            _same(name, t, torch.int32, n)
-    if eos >= scratch.vocab or (done is not None and eos < 0):
+    if logits.dtype is not torch.float32 or logits.shape != (n, V) or (logits.stride(1) != 1 and V > 1):
+        raise ValueError(f"logits: fp32 [{n}, {V}], ids next to each other")
+    if logits.get_device() != index:
+        raise ValueError("logits: on another device than the scratch")
+    i32 = torch.int32
+    at = (_same("scores", scores, torch.float32, n, index), _same("done", done, i32, n, index) if done is not None else 0,
+          _same("lengths", lengths, i32, n, index) if lengths is not None else 0, scratch.work_ptr,
+          _same("parent", parent, i32, n, index), _same("token", token, i32, n, index),
+          _same("out_scores", out_scores, torch.float32, n, index),
+          _same("out_done", out_done, i32, n, index) if out_done is not None else 0,
+          _same("out_lengths", out_lengths, i32, n, index) if out_lengths is not None else 0,
+          fault.data_ptr() if fault is not None else 0)
+    if eos >= V or (done is not None and eos < 0):
         raise ValueError("finished beams need the id of the end")
     if lengths is None and (alpha != 0.0 or out_lengths is not None):
         raise ValueError("a rank by length needs the lengths")
-    fn = _fn("bl_beam_select", _P, _L, _I, _I, _I, _P, _P, _P, _I, _F, _P, _I, _P, _P, _P, _P, _P, _P, _P)
-    check(fn(logits.data_ptr(), max(logits.stride(0), scratch.vocab), scratch.vocab, G, B, scores.data_ptr(), _ptr(done), _ptr(lengths), eos,
-             alpha, scratch.work.data_ptr(), scratch.sms, parent.data_ptr(), token.data_ptr(), out_scores.data_ptr(), _ptr(out_done),
-             _ptr(out_lengths), _ptr(fault), torch.cuda.current_stream(scratch.device).cuda_stream), "bl_beam_select")
+    if index < 0:
+        raise ValueError("the kernels need a CUDA device")
+    code = _fn("bl_beam_select")(_SELECT.pack(logits.data_ptr(), max(logits.stride(0), V), *at, raw_stream(index), V, G, B, max(eos, -1),
+                                              scratch.sms, alpha))
+    if code:
+        check(code, "bl_beam_select")
 
 
 def beam_reorder(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, table_out: torch.Tensor, slots: torch.Tensor,
@@ -96,18 +103,23 @@ def beam_reorder(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, table_ou
     over the page of a beam that has none and a copy of the positions in it.  The pages from the one being filled on must belong
     to one slot each.  A search whose parents, slots or positions are out of range stays as it is and raises ``fault``."""
     G, B = parent.shape
-    for name, t, n in (("slots", slots, G * B), ("parent", parent, G * B), ("held", held, G)):
-        _same(name, t, torch.int32, n)
-    if k.dim() != 5 or v.dim() != 5 or k.shape[:4] != v.shape[:4] or k.shape[3] != PAGE or not (k.is_contiguous() and v.is_contiguous()):
+    index = k.get_device()
+    at = (_same("slots", slots, torch.int32, G * B, index), _same("parent", parent, torch.int32, G * B, index),
+          _same("held", held, torch.int32, G, index), fault.data_ptr() if fault is not None else 0)
+    shape, v_shape, tables = k.shape, v.shape, table.shape
+    if len(shape) != 5 or len(v_shape) != 5 or shape[:4] != v_shape[:4] or shape[3] != PAGE or not (k.is_contiguous() and v.is_contiguous()):
         raise ValueError(f"pools: contiguous [layers, pages, heads, {PAGE}, row], alike but for the row")
     for t in (table, table_out):
-        if t.dtype != torch.int32 or t.dim() != 2 or not t.is_contiguous() or t.shape != table.shape:
+        if t.dtype is not torch.int32 or len(tables) != 2 or t.shape != tables or not t.is_contiguous() or t.get_device() != index:
             raise ValueError("tables: contiguous int32 [slots, pages]")
     if table.data_ptr() == table_out.data_ptr():
         raise ValueError("the new table is written while the old one is read: another tensor")
     if B > MAX_BEAMS:
         raise ValueError(f"at most {MAX_BEAMS} beams a search")
-    fn = _fn("bl_beam_reorder", _P, _P, _L, _L, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _I, _I, _P, _P)
-    check(fn(k.data_ptr(), v.data_ptr(), k.shape[4] * k.element_size(), v.shape[4] * v.element_size(), k.shape[0], k.shape[1],
-             k.shape[2], table.data_ptr(), table_out.data_ptr(), table.shape[0], table.shape[1], slots.data_ptr(), parent.data_ptr(),
-             held.data_ptr(), G, B, _ptr(fault), torch.cuda.current_stream(parent.device).cuda_stream), "bl_beam_reorder")
+    if index < 0 or v.get_device() != index:
+        raise ValueError("the kernels need the pools on one CUDA device")
+    code = _fn("bl_beam_reorder")(_REORDER.pack(k.data_ptr(), v.data_ptr(), shape[4] * k.element_size(), v_shape[4] * v.element_size(),
+                                                table.data_ptr(), table_out.data_ptr(), *at, raw_stream(index), shape[0], shape[1],
+                                                shape[2], tables[0], tables[1], G, B, sm_count(k.device)))
+    if code:
+        check(code, "bl_beam_reorder")

@@ -7,25 +7,17 @@ shared pages every row has keys of its own.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Sequence
 
 import torch
 
 from ..runtime.kv import PAGE
-from ._lib import check, cuda
+from ._lib import check, cuda, raw_stream
 from .decode import sm_count
 
 _entry = None
-
-
-def _fn():
-    global _entry
-    if _entry is None:
-        fn = cuda().bl_prefix_attention
-        P, I = ctypes.c_void_p, ctypes.c_int
-        fn.argtypes = [P, P, P, P, P, P, I, I, I, I, I, I, I, P, I, P, I, P, I, P, I, P]
-        _entry = fn
-    return _entry
+_CALL = struct.Struct("11P12i")                       # PrefixCall in the source
 
 
 class PrefixPlan:
@@ -50,6 +42,10 @@ class PrefixPlan:
         self.rows = sum(group_rows)
         self.max_prefix = max(prefix_len)
         self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.index = self.device.index if self.device.type == "cuda" else -1      # as Tensor.get_device() says it
+        self.q_shape, self.out_shape = (sum(group_rows), n_q, head), (sum(group_rows), n_q * head)
         if self.rows > 512:
             raise ValueError("at most 512 rows")
         # units: rows of a group that read all of their keys together, as many as two tiles of 128 (row, head) pairs of a key
@@ -61,12 +57,13 @@ class PrefixPlan:
             rows += [(first, n, p, len(units) + i // (2 * per), i % (2 * per) // per * 128 + i % per * G) for i in range(n)]
             units += [(first + i, min(2 * per, n - i), p, first, n) for i in range(0, n, 2 * per)]
             first += n
-        self.n_units = len(units)
+        self.n_units, self.unit_rows = len(units), max(u[1] for u in units)
         self.meta = torch.tensor(rows + units, dtype=torch.int32).to(self.device)
         self.n_cta = min(160, sm_count(self.device)) if self.device.type == "cuda" else 1
         fn = cuda().bl_prefix_work_bytes
         fn.restype = ctypes.c_long
-        self.work = torch.empty(fn(head, n_kv, self.n_units, self.n_cta), dtype=torch.uint8, device=self.device)
+        self.work = torch.empty(fn(head, n_q, n_kv, self.n_units, self.unit_rows, self.n_cta), dtype=torch.uint8, device=self.device)
+        self.meta_ptr, self.work_ptr = self.meta.data_ptr(), self.work.data_ptr()
 
 
 def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, row_pos: torch.Tensor, row_seq: torch.Tensor,
@@ -76,26 +73,39 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     0 .. row_pos of each row's sequence ``row_seq`` in the paged caches of one layer, f16 [pages, n_kv, 64, head] or q8_0 rows as
     uint8.  The first positions of a row come from the pages of its group's first live row.  Rows with a negative sequence get
     zeros; a row without keys, past its table or with a page that the pool does not have gets NaN and raises ``fault``."""
-    n_kv, head = plan.n_kv, plan.head
-    if q.dtype != torch.float32 or not q.is_contiguous() or q.shape != (plan.rows, plan.n_q, head):
-        raise ValueError(f"q: contiguous fp32 [{plan.rows}, {plan.n_q}, {head}]")
-    q8 = k_cache.dtype == torch.uint8
+    global _entry
+    rows, n_kv, head = plan.rows, plan.n_kv, plan.head
+    if q.dtype is not torch.float32 or q.shape != plan.q_shape or not q.is_contiguous():
+        raise ValueError(f"q: contiguous fp32 {list(plan.q_shape)}")
+    q8 = k_cache.dtype is torch.uint8
+    shape = k_cache.shape
     width = head // 32 * 34 if q8 else head
-    for c in (k_cache, v_cache):
-        if c.dtype != (torch.uint8 if q8 else torch.float16) or not c.is_contiguous() or c.dim() != 4 or c.shape[1:] != (n_kv, PAGE, width) \
-                or c.shape[0] != k_cache.shape[0]:
-            raise ValueError(f"caches: contiguous [pages, {n_kv}, {PAGE}, {width}], both f16 or both q8_0 bytes")
-    if out.dtype != torch.bfloat16 or not out.is_contiguous() or out.shape != (plan.rows, plan.n_q * head):
-        raise ValueError(f"out: contiguous bf16 [{plan.rows}, {plan.n_q * head}]")
+    if shape != v_cache.shape or len(shape) != 4 or shape[1] != n_kv or shape[2] != PAGE or shape[3] != width or \
+            (not q8 and k_cache.dtype is not torch.float16) or v_cache.dtype is not k_cache.dtype or \
+            not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError(f"caches: contiguous [pages, {n_kv}, {PAGE}, {width}], both f16 or both q8_0 bytes")
+    if out.dtype is not torch.bfloat16 or out.shape != plan.out_shape or not out.is_contiguous():
+        raise ValueError(f"out: contiguous bf16 {list(plan.out_shape)}")
     for t in (row_pos, row_seq):
-        if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < plan.rows:
-            raise ValueError(f"row_pos and row_seq: int32, {plan.rows} rows")
-    if block_table.dtype != torch.int32 or not block_table.is_contiguous() or block_table.dim() != 2:
+        if t.dtype is not torch.int32 or t.numel() < rows or not t.is_contiguous():
+            raise ValueError(f"row_pos and row_seq: int32, {rows} rows")
+    table = block_table.shape
+    if block_table.dtype is not torch.int32 or len(table) != 2 or not block_table.is_contiguous():
         raise ValueError("block_table: contiguous int32 [slots, pages]")
-    if plan.max_prefix > block_table.shape[1] * PAGE:
+    if plan.max_prefix > table[1] * PAGE:
         raise ValueError("the prefix is longer than a table row")
-    rc = _fn()(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), row_pos.data_ptr(), row_seq.data_ptr(), block_table.data_ptr(),
-               block_table.shape[0], block_table.shape[1], k_cache.shape[0], head, plan.n_q, n_kv, plan.rows, plan.meta.data_ptr(), plan.n_units, plan.work.data_ptr(),
-               1 if q8 else 0, out.data_ptr(), plan.n_cta, fault.data_ptr() if fault is not None else None, layer,
-               torch.cuda.current_stream(plan.device).cuda_stream)
-    check(rc, "bl_prefix_attention")
+    index = plan.index
+    for t in (q, k_cache, v_cache, row_pos, row_seq, block_table, out):
+        if t.get_device() != index:
+            raise ValueError("the tensors are on the plan's device")
+    if index < 0:
+        raise ValueError("the kernels need a CUDA device")
+    if _entry is None:
+        _entry = cuda().bl_prefix_attention
+        _entry.argtypes = [ctypes.c_char_p]
+    code = _entry(_CALL.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), row_pos.data_ptr(), row_seq.data_ptr(),
+                             block_table.data_ptr(), plan.meta_ptr, plan.work_ptr, out.data_ptr(),
+                             fault.data_ptr() if fault is not None else 0, raw_stream(index), table[0], table[1], shape[0], head,
+                             plan.n_q, n_kv, rows, plan.n_units, plan.unit_rows, q8, plan.n_cta, layer))
+    if code:
+        check(code, "bl_prefix_attention")
