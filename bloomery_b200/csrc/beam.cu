@@ -37,59 +37,78 @@ struct BeamArgs {
   unsigned* fault;
 };
 
-// The k best of a block's values, best first, ties to the lower id: store(rank, value, id) for each of the min(k, n) there are
-// (values of -inf are none).  A bound that k values at least reach comes from 8, 16, 32 or 64 groups of lanes, each of which
-// has a maximum: the smallest of them.  The few values from there on are listed and each counts the ones before it.  Data that
-// let more than the list through (an ascending row, say) are taken in k rounds instead.
-template <typename T, int E, typename Id, typename Store>
-__device__ __forceinline__ void block_best(const T (&v)[E], int k, T* s_value, int* s_id, T* s_group, int* s_n, Id id, Store store) {
-  const int tid = threadIdx.x, lane = tid & 31;
-  const T none = (T)-INFINITY;
-  T mine = none;
+// The order of values as integers; the two zeros are one.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ unsigned long long order_of(double v) {
+  const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+struct BestScratch {
+  __align__(16) unsigned long long key[kBmList + 1];
+  int id[kBmList];
+  double group[64];
+  int n;
+};
+
+// The smallest of the maxima of 8, 16, 32 or 64 groups of lanes, k at least: a bound that k of the block's values reach.  `mine`: the
+// largest value of this thread; -inf is none.
+template <typename T>
+__device__ __forceinline__ T block_bound(T mine, int k, BestScratch& s) {
+  const int tid = threadIdx.x, lane = tid & 31, lanes = k <= 8 ? 32 : k <= 16 ? 16 : k <= 32 ? 8 : 4, groups = kBmThreads / lanes;
+  T* group = reinterpret_cast<T*>(s.group);
 #pragma unroll
-  for (int i = 0; i < E; ++i) mine = v[i] > mine ? v[i] : mine;
-  const int lanes = k <= 8 ? 32 : k <= 16 ? 16 : k <= 32 ? 8 : 4;
-  T top = mine;
-  for (int o = lanes >> 1; o > 0; o >>= 1) { const T u = __shfl_xor_sync(0xffffffffu, top, o); top = u > top ? u : top; }
-  if ((lane & (lanes - 1)) == 0) s_group[tid / lanes] = top;
-  if (tid == 0) *s_n = 0;
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < lanes) { const T u = __shfl_xor_sync(0xffffffffu, mine, o); mine = u > mine ? u : mine; }
+  if ((lane & (lanes - 1)) == 0) group[tid / lanes] = mine;
+  if (tid == 0) s.n = 0;
   __syncthreads();
-  const int groups = kBmThreads / lanes;
-  T bound = s_group[lane % groups];
-  if (groups == 64) { const T u = s_group[lane + 32]; bound = u < bound ? u : bound; }
+  T bound = group[lane % groups];
+  if (groups == 64) { const T u = group[lane + 32]; bound = u < bound ? u : bound; }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) { const T u = __shfl_xor_sync(0xffffffffu, bound, o); bound = u < bound ? u : bound; }
-  if (mine >= bound && mine > none) {
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-      if (v[i] >= bound && v[i] > none) {
-        const int at = atomicAdd(s_n, 1);
-        if (at < kBmList) { s_value[at] = v[i]; s_id[at] = id(i); }
-      }
-  }
-  __syncthreads();
-  const int n = *s_n;
-  if (n <= kBmList) {
-    for (int e = tid; e < n; e += kBmThreads) {
-      const T value = s_value[e];
-      const int where = s_id[e];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += s_value[j] > value || (s_value[j] == value && s_id[j] < where);
-      if (rank < k) store(rank, value, where);
+  return bound;
+}
+
+// The listed candidates in order, s.n of them and no more than the list holds: store(rank, key, id) of the k best.  A candidate
+// counts the ones before it; where there are few, two or four threads share a candidate's count.
+template <bool IDS, typename Store>
+__device__ __forceinline__ void block_rank(int k, const BestScratch& s, Store store) {
+  const int tid = threadIdx.x, n = s.n, shift = n <= 64 ? 2 : n <= 128 ? 1 : 0;
+  for (int at = tid; (at & ~31) < n << shift; at += kBmThreads) {                // whole warps
+    const int e = at >> shift, part = at & ((1 << shift) - 1);
+    const bool there = e < n;
+    const unsigned long long key = there ? s.key[e] : 0;
+    const int id = IDS && there ? s.id[e] : 0;
+    int rank = 0;
+#pragma unroll 4
+    for (int j = part; j < n; j += 1 << shift) {
+      const unsigned long long u = s.key[j];
+      rank += (int)(u > key);
+      if (IDS) rank += (int)(u == key) & (int)(s.id[j] < id);
     }
-    __syncthreads();
-    return;
+    if (shift > 0) rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    if (shift > 1) rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    if (there && part == 0 && rank < k) store(rank, key, id);
   }
+}
+
+// The k best of the block's values by k rounds, for data that let more than the list through (an ascending row, say): next(last, last
+// id, best, id) gives a thread's best behind the last one taken.
+template <typename T, typename Next, typename Store>
+__device__ __forceinline__ void block_rounds(int k, BestScratch& s, Next next, Store store) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  const T none = (T)-INFINITY;
   T last = (T)INFINITY;
   int last_id = -1;
+  T* value = reinterpret_cast<T*>(s.group);
   for (int round = 0; round < k; ++round) {
     T best = none;
     int where = 0x7fffffff;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int w = id(i);
-      if ((v[i] < last || (v[i] == last && w > last_id)) && (v[i] > best || (v[i] == best && v[i] > none && w < where))) { best = v[i]; where = w; }
-    }
+    next(last, last_id, best, where);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const T u = __shfl_xor_sync(0xffffffffu, best, o);
@@ -97,17 +116,57 @@ __device__ __forceinline__ void block_best(const T (&v)[E], int k, T* s_value, i
       if (u > best || (u == best && w < where)) { best = u; where = w; }
     }
     __syncthreads();
-    if (lane == 0) { s_value[tid >> 5] = best; s_id[tid >> 5] = where; }
+    if (lane == 0) { value[tid >> 5] = best; s.id[tid >> 5] = where; }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kBmThreads / 32; ++w)
-      if (s_value[w] > best || (s_value[w] == best && s_id[w] < where)) { best = s_value[w]; where = s_id[w]; }
+      if (value[w] > best || (value[w] == best && s.id[w] < where)) { best = value[w]; where = s.id[w]; }
     if (best == none) break;
     if (tid == 0) store(round, best, where);
     last = best;
     last_id = where;
   }
+}
+
+// One of a block's best by value and id: for fp32 the id is the key's low half.
+__device__ __forceinline__ unsigned long long beam_key(float v, int id) { return (unsigned long long)order_of(v) << 32 | (unsigned)~id; }
+__device__ __forceinline__ BeamCell beam_cell(unsigned long long key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return BeamCell{__uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u), (int)~(uint32_t)key};
+}
+template <int E>
+__device__ __forceinline__ void next_of(const float (&v)[E], const int (&ids)[E], float last, int last_id, float& best, int& where) {
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    if ((v[i] < last || (v[i] == last && ids[i] > last_id)) && (v[i] > best || (v[i] == best && v[i] > -INFINITY && ids[i] < where))) { best = v[i]; where = ids[i]; }
+}
+// The k best of the cells [n] that blocks left in memory, E a thread.
+template <int E>
+__device__ __forceinline__ void merge_cells(const BeamCell* cells, int n, int k, BestScratch& s, BeamCell* best) {
+  float v[E], mine = -INFINITY;
+  int ids[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int e = threadIdx.x + i * kBmThreads;
+    const float2 q = e < n ? __ldcg(reinterpret_cast<const float2*>(cells + e)) : make_float2(-INFINITY, 0.f);
+    v[i] = q.x;
+    ids[i] = __float_as_int(q.y);
+    mine = fmaxf(mine, q.x);
+  }
+  const float bound = block_bound(mine, k, s);
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    if (v[i] >= bound && v[i] > -INFINITY) {
+      const int at = atomicAdd(&s.n, 1);
+      if (at < kBmList) s.key[at] = beam_key(v[i], ids[i]);
+    }
   __syncthreads();
+  auto store = [&](int rank, BeamCell c) { best[rank] = c; };
+  if (s.n <= kBmList) block_rank<false>(k, s, [&](int rank, unsigned long long key, int) { store(rank, beam_cell(key)); });
+  else block_rounds<float>(k, s, [&](float last, int last_id, float& b, int& w) { next_of<E>(v, ids, last, last_id, b, w); },
+                           [&](int rank, float value, int id) { store(rank, BeamCell{value, id}); });
+  const int had = min(k, s.n);
+  if ((int)threadIdx.x >= had && (int)threadIdx.x < k) best[threadIdx.x] = BeamCell{-INFINITY, 0x7fffffff};
 }
 
 // True in the block that arrives last of `n`: what the others wrote before they arrived is visible to it.
@@ -126,11 +185,46 @@ __device__ __forceinline__ bool block_last(int* ticket, int n, int* s_last) {
 
 // grid (n_chunks, G * B).  A block takes the sum of exponentials and the B best of a chunk; the last block of a row merges the
 // row's; the last row of a search ranks the B x B candidates that are left.
+// A search's places [B]: the best of the B x B candidates that its rows left, EB a thread.
+template <int EB, typename Rank>
+__device__ __forceinline__ void pick_places(int B, BestScratch& s, int* s_pick, Rank rank_of) {
+  double v[EB], mine = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < EB; ++i) {
+    const int e = threadIdx.x + i * kBmThreads;
+    v[i] = e < B * B ? rank_of(e) : (double)-INFINITY;
+    mine = v[i] > mine ? v[i] : mine;
+  }
+  const double bound = block_bound(mine, B, s);
+#pragma unroll
+  for (int i = 0; i < EB; ++i)
+    if (v[i] >= bound && v[i] > -INFINITY) {
+      const int at = atomicAdd(&s.n, 1);
+      if (at < kBmList) { s.key[at] = order_of(v[i]); s.id[at] = threadIdx.x + i * kBmThreads; }
+    }
+  __syncthreads();
+  if (s.n <= kBmList) {
+    block_rank<true>(B, s, [&](int rank, unsigned long long, int id) { s_pick[rank] = id; });
+  } else {
+    block_rounds<double>(B, s, [&](double last, int last_id, double& best, int& where) {
+#pragma unroll
+      for (int i = 0; i < EB; ++i) {
+        const int id = threadIdx.x + i * kBmThreads;
+        if ((v[i] < last || (v[i] == last && id > last_id)) && (v[i] > best || (v[i] == best && v[i] > -INFINITY && id < where))) { best = v[i]; where = id; }
+      }
+    }, [&](int rank, double, int id) { s_pick[rank] = id; });
+  }
+  __syncthreads();
+}
+
+// grid (n_chunks, G * B).  A block takes the sum of exponentials and the B best of a chunk; the last block of a row merges the
+// row's; the last row of a search ranks the B x B candidates that are left.  Steps that most calls need with one value a thread
+// have a form for that: code is fetched as it is first met, a dozen clocks an instruction.
 template <int E>
 __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamArgs a) {
-  __shared__ double s_value[kBmList], s_group[64], s_sum[8];
-  __shared__ double s_fac[kMaxBeams], s_lse[kMaxBeams];
-  __shared__ int s_id[kBmList], s_pick[kMaxBeams], s_n, s_last;
+  __shared__ BestScratch s;
+  __shared__ double s_fac[kMaxBeams], s_lse[kMaxBeams], s_sum[8];
+  __shared__ int s_pick[kMaxBeams], s_last;
   __shared__ float s_max[8], s_score[kMaxBeams];
   const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int B = a.B, V = a.V, g = r / B;
@@ -144,12 +238,12 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
     const float* x = a.logits + (long)r * a.stride;
     const int lo = c * a.chunk, hi = min(V, lo + a.chunk);
     const bool vec = ((uintptr_t)x & 15) == 0;
-    float m = -INFINITY, sum = 0.f;                       // of what this thread has seen
-    float v[E + 1];                                       // a tile's values, and one of the best so far
-    v[E] = -INFINITY;
-    int carried = 0;
+    BeamCell* out = a.cells + ((long)r * a.n_chunks + c) * B;
+    float m = -INFINITY, sum = 0.f, carried = -INFINITY;  // of what this thread has seen; one of the best so far
+    int carried_id = 0;
     for (int t0 = lo; t0 < hi; t0 += E * kBmThreads) {
       const int n = hi - t0;
+      float v[E];
       if (vec) {
 #pragma unroll
         for (int i = 0; i < E; i += 4) {
@@ -166,29 +260,52 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
 #pragma unroll
         for (int i = 0; i < E; ++i) v[i] = tid + i * kBmThreads < n ? __ldg(x + t0 + tid + i * kBmThreads) : -INFINITY;
       }
+      auto id_of = [&](int i) { return t0 + (vec ? (tid + (i >> 2) * kBmThreads) * 4 + (i & 3) : tid + i * kBmThreads); };
       float top = v[0];
 #pragma unroll
       for (int i = 1; i < E; ++i) top = fmaxf(top, v[i]);
-      top = fmaxf(top, m);
-      if (top > -INFINITY) {                              // NaN and +inf end up as a NaN of the sum
-        sum *= __expf(m - top);
+      const float seen = fmaxf(top, m);
+      if (seen > -INFINITY) {                             // NaN and +inf end up as a NaN of the sum
+        sum *= __expf(m - seen);
 #pragma unroll
-        for (int i = 0; i < E; ++i) sum += __expf(v[i] - top);
+        for (int i = 0; i < E; ++i) sum += __expf(v[i] - seen);
       } else {
 #pragma unroll
         for (int i = 0; i < E; ++i) sum += v[i] == -INFINITY ? 0.f : v[i];
       }
-      m = top;
-      BeamCell* out = a.cells + ((long)r * a.n_chunks + c) * B;
-      block_best<float, E + 1>(v, B, reinterpret_cast<float*>(s_value), s_id, reinterpret_cast<float*>(s_group), &s_n,
-          [&](int i) { return i == E ? carried : t0 + (vec ? (tid + i / 4 * kBmThreads) * 4 + i % 4 : tid + i * kBmThreads); },
-          [&](int rank, float value, int id) { out[rank] = BeamCell{value, id}; });
-      const int had = min(B, s_n);
+      m = seen;
+      const float bound = block_bound(fmaxf(top, carried), B, s);
+      uint32_t pass = 0;
+#pragma unroll
+      for (int i = 0; i < E; ++i) pass |= (uint32_t)(v[i] >= bound && v[i] > -INFINITY) << i;
+      while (pass) {                                      // few: read again, so that the registers need no index
+        const int id = id_of(__ffs(pass) - 1), at = atomicAdd(&s.n, 1);
+        pass &= pass - 1;
+        if (at < kBmList) s.key[at] = beam_key(__ldg(x + id), id);
+      }
+      if (carried >= bound && carried > -INFINITY) {
+        const int at = atomicAdd(&s.n, 1);
+        if (at < kBmList) s.key[at] = beam_key(carried, carried_id);
+      }
+      __syncthreads();
+      if (s.n <= kBmList) {
+        block_rank<false>(B, s, [&](int rank, unsigned long long key, int) { out[rank] = beam_cell(key); });
+      } else {
+        block_rounds<float>(B, s, [&](float last, int last_id, float& best, int& where) {
+          auto offer = [&](float u, int id) {
+            if ((u < last || (u == last && id > last_id)) && (u > best || (u == best && u > -INFINITY && id < where))) { best = u; where = id; }
+          };
+#pragma unroll
+          for (int i = 0; i < E; ++i) offer(v[i], id_of(i));
+          offer(carried, carried_id);
+        }, [&](int rank, float value, int id) { out[rank] = BeamCell{value, id}; });
+      }
+      const int had = min(B, s.n);
       if (tid >= had && tid < B) out[tid] = BeamCell{-INFINITY, 0x7fffffff};
       if (t0 + E * kBmThreads < hi) {                     // the best so far take part in the next tile's choice
         __syncthreads();
-        v[E] = -INFINITY;
-        if (tid < had) { v[E] = out[tid].value; carried = out[tid].id; }
+        carried = -INFINITY;
+        if (tid < had) { carried = out[tid].value; carried_id = out[tid].id; }
         __syncthreads();
       }
     }
@@ -207,20 +324,23 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
       a.sums[(long)r * a.n_chunks + c] = make_float2(all, (float)l);
     }
     if (!block_last(a.tickets + r, a.n_chunks, &s_last)) return;
-    // ---- the row: its log-sum and the best of its chunks' best
+    // ---- the row: the best of its chunks' best, and its log-sum
     const float2* sums = a.sums + (long)r * a.n_chunks;
-    float top = -INFINITY;
-    for (int i = tid; i < a.n_chunks; i += kBmThreads) top = fmaxf(top, __ldcg(sums + i).x);
+    const float2 first = tid < a.n_chunks ? __ldcg(sums + tid) : make_float2(-INFINITY, 0.f);
+    const BeamCell* cells = a.cells + (long)r * a.n_chunks * B;
+    const int n_cells = a.n_chunks * B;
+    if (n_cells <= kBmThreads) merge_cells<1>(cells, n_cells, B, s, a.best + (long)r * B);
+    else merge_cells<kBmMaxCells / kBmThreads>(cells, n_cells, B, s, a.best + (long)r * B);
+    float top = first.x;
+    for (int i = tid + kBmThreads; i < a.n_chunks; i += kBmThreads) top = fmaxf(top, __ldcg(sums + i).x);
     top = warp_max(top);
     if (lane == 0) s_max[warp] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 8; ++w) top = fmaxf(top, s_max[w]);
-    double l = 0.0;
-    for (int i = tid; i < a.n_chunks; i += kBmThreads) {
-      const float2 s = __ldcg(sums + i);
-      l += s.x > -INFINITY ? (double)s.y * exp((double)s.x - (double)top) : (double)s.y;
-    }
+    auto weighed = [&](float2 q) { return q.x > -INFINITY ? (double)q.y * (double)__expf(q.x - top) : (double)q.y; };
+    double l = weighed(first);
+    for (int i = tid + kBmThreads; i < a.n_chunks; i += kBmThreads) l += weighed(__ldcg(sums + i));
     l = warp_sum_d(l);
     if (lane == 0) s_sum[warp] = l;
     __syncthreads();
@@ -229,22 +349,6 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
       for (int w = 0; w < 8; ++w) total += s_sum[w];
       a.lse[r] = (double)top + log(total);                // -inf where every id is masked; NaN where a logit is not finite
     }
-    constexpr int EC = kBmMaxCells / kBmThreads;
-    const BeamCell* cells = a.cells + (long)r * a.n_chunks * B;
-    float w[EC];
-    int at[EC];
-#pragma unroll
-    for (int i = 0; i < EC; ++i) {
-      const int e = tid + i * kBmThreads;
-      w[i] = -INFINITY;
-      at[i] = 0x7fffffff;
-      if (e < a.n_chunks * B) { const float2 q = __ldcg(reinterpret_cast<const float2*>(cells + e)); w[i] = q.x; at[i] = __float_as_int(q.y); }
-    }
-    BeamCell* best = a.best + (long)r * B;
-    block_best<float, EC>(w, B, reinterpret_cast<float*>(s_value), s_id, reinterpret_cast<float*>(s_group), &s_n,
-                          [&](int i) { return at[i]; }, [&](int rank, float value, int id) { best[rank] = BeamCell{value, id}; });
-    const int had = min(B, s_n);
-    if (tid >= had && tid < B) best[tid] = BeamCell{-INFINITY, 0x7fffffff};
   }
   if (!block_last(a.tickets + a.G * B + g, B, &s_last)) return;
   // ---- the search
@@ -254,39 +358,36 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
     const int q = r0 + tid;
     const bool ended = a.done && a.done[q];
     const float sc = a.scores[q];
+    const double lse = __ldcg(a.lse + q);
     s_score[tid] = sc;
-    s_lse[tid] = sc == -INFINITY || ended ? 0.0 : __ldcg(a.lse + q);
+    s_lse[tid] = sc == -INFINITY || ended ? 0.0 : lse;
     bad = !(sc < INFINITY) || s_lse[tid] != s_lse[tid];
     s_fac[tid] = a.alpha != 0.f ? pow((double)max(1, a.lengths[q] + (ended ? 0 : 1)), -(double)a.alpha) : 1.0;
     s_pick[tid] = -1;
   }
   bad = __syncthreads_or(bad);
   auto cand = [&](int b, float value) { return (double)s_score[b] + ((double)value - s_lse[b]); };
-  constexpr int EB = kMaxBeams * kMaxBeams / kBmThreads;
-  double v[EB];
-#pragma unroll
-  for (int i = 0; i < EB; ++i) {
-    const int e = tid + i * kBmThreads;
-    v[i] = -INFINITY;
-    if (!bad && e < B * B) {
-      const int b = e / B, j = e % B;
-      const bool ended = a.done && a.done[r0 + b];
-      if (s_score[b] > -INFINITY) {
-        if (ended) v[i] = j == 0 ? (double)s_score[b] * s_fac[b] : -INFINITY;
-        else {
-          const float value = __ldcg(&a.best[(long)(r0 + b) * B + j].value);
-          if (value > -INFINITY) v[i] = cand(b, value) * s_fac[b];
-        }
-      }
-    }
-  }
   // within a beam the places are in order of logit and id, so that of equal ranks the lower place comes first
-  block_best<double, EB>(v, B, s_value, s_id, s_group, &s_n, [&](int i) { return tid + i * kBmThreads; },
-                         [&](int rank, double value, int id) { s_pick[rank] = id; });
+  auto rank_of = [&](int e) {
+    const int b = e / B, j = e - b * B;
+    const float value = __ldcg(&a.best[(long)(r0 + b) * B + j].value);           // read in any case: nothing waits for the tests
+    double rank = -INFINITY;
+    if (!bad && s_score[b] > -INFINITY) {
+      if (a.done && a.done[r0 + b]) rank = j == 0 ? (double)s_score[b] * s_fac[b] : -INFINITY;
+      else if (value > -INFINITY) rank = cand(b, value) * s_fac[b];
+    }
+    return rank;
+  };
+  if (B * B <= kBmThreads) pick_places<1>(B, s, s_pick, rank_of);
+  else pick_places<kMaxBeams * kMaxBeams / kBmThreads>(B, s, s_pick, rank_of);
   if (tid < B) {
     const int e = s_pick[tid], b = e < 0 ? tid : e / B, q = r0 + b;
     const bool ended = a.done && a.done[q];
-    const BeamCell cell = e < 0 || ended ? BeamCell{0.f, max(a.eos, 0)} : BeamCell{__ldcg(&a.best[(long)q * B + e % B].value), __ldcg(&a.best[(long)q * B + e % B].id)};
+    BeamCell cell{0.f, max(a.eos, 0)};
+    if (e >= 0 && !ended) {
+      const float2 got = __ldcg(reinterpret_cast<const float2*>(a.best + (long)q * B + (e - b * B)));
+      cell = BeamCell{got.x, __float_as_int(got.y)};
+    }
     a.parent[r0 + tid] = b;
     a.token[r0 + tid] = cell.id;
     a.out_scores[r0 + tid] = bad ? __int_as_float(0x7fc00000) : e < 0 ? -INFINITY : ended ? s_score[b] : (float)cand(b, cell.value);

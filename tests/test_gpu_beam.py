@@ -105,6 +105,25 @@ def test_ties_go_to_the_lowest_beam_and_id(B):
 
 
 @gpu
+@pytest.mark.parametrize("order", ["ascending", "descending", "one block", "zeros of both signs"])
+def test_orders_that_let_many_candidates_through(order):
+    """Rows whose blocks cannot tell their best from a few values, and zeros whose sign is no order."""
+    V, B = 30000, 7
+    row = torch.linspace(-3, 3, V, device=DEV)
+    if order == "descending":
+        row = row.flip(0)
+    elif order == "one block":
+        row = torch.full((V,), -INF, device=DEV)
+        row[8000:12000] = torch.linspace(-3, 3, 4000, device=DEV)
+    elif order == "zeros of both signs":
+        row = torch.where(torch.arange(V, device=DEV) % 3 == 0, -0.0, 0.0)
+    x = row.expand(B, -1).contiguous()
+    scores = torch.linspace(0, -0.5, B, device=DEV).view(1, B).contiguous()
+    scores[0, 3:] = 0
+    _check(_run(x, scores), _reference(x, scores))
+
+
+@gpu
 def test_logits_that_a_32_bit_sum_would_merge_keep_their_order():
     x = torch.full((2, 5000), -30.0, device=DEV)
     x[0, 4000], x[0, 7] = 1.0 + 2.0 ** -23, 1.0        # the larger one has the higher id
