@@ -220,7 +220,7 @@ __device__ __forceinline__ void pick_places(int B, BestScratch& s, int* s_pick, 
 // grid (n_chunks, G * B).  A block takes the sum of exponentials and the B best of a chunk; the last block of a row merges the
 // row's; the last row of a search ranks the B x B candidates that are left.  Steps that most calls need with one value a thread
 // have a form for that: code is fetched as it is first met, a dozen clocks an instruction.
-template <int E>
+template <int E, int NB>
 __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamArgs a) {
   __shared__ BestScratch s;
   __shared__ double s_fac[kMaxBeams], s_lse[kMaxBeams], s_sum[8];
@@ -239,49 +239,74 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
     const int lo = c * a.chunk, hi = min(V, lo + a.chunk);
     const bool vec = ((uintptr_t)x & 15) == 0;
     BeamCell* out = a.cells + ((long)r * a.n_chunks + c) * B;
-    float m = -INFINITY, sum = 0.f, carried = -INFINITY;  // of what this thread has seen; one of the best so far
-    int carried_id = 0;
-    for (int t0 = lo; t0 < hi; t0 += E * kBmThreads) {
-      const int n = hi - t0;
-      float v[E];
+    // values of batch b of a tile: this thread's, -inf behind the chunk's end
+    auto load = [&](int from, float (&v)[E]) {
+      const int n = hi - from;
       if (vec) {
 #pragma unroll
         for (int i = 0; i < E; i += 4) {
           const int e = (tid + i / 4 * kBmThreads) * 4;
           if (e + 4 <= n) {
-            const float4 q = __ldg(reinterpret_cast<const float4*>(x + t0 + e));
+            const float4 q = __ldg(reinterpret_cast<const float4*>(x + from + e));
             v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w;
           } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[i + j] = e + j < n ? __ldg(x + t0 + e + j) : -INFINITY;
+            for (int j = 0; j < 4; ++j) v[i + j] = e + j < n ? __ldg(x + from + e + j) : -INFINITY;
           }
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) v[i] = tid + i * kBmThreads < n ? __ldg(x + t0 + tid + i * kBmThreads) : -INFINITY;
+        for (int i = 0; i < E; ++i) v[i] = tid + i * kBmThreads < n ? __ldg(x + from + tid + i * kBmThreads) : -INFINITY;
       }
-      auto id_of = [&](int i) { return t0 + (vec ? (tid + (i >> 2) * kBmThreads) * 4 + (i & 3) : tid + i * kBmThreads); };
-      float top = v[0];
+    };
+    auto id_of = [&](int from, int i) { return from + (vec ? (tid + (i >> 2) * kBmThreads) * 4 + (i & 3) : tid + i * kBmThreads); };
+    float m = -INFINITY, sum = 0.f, carried = -INFINITY;  // of what this thread has seen; one of the best so far
+    int carried_id = 0;
+    for (int t0 = lo; t0 < hi; t0 += NB * E * kBmThreads) {
+      float v[E], tops[NB], mine = carried;
 #pragma unroll
-      for (int i = 1; i < E; ++i) top = fmaxf(top, v[i]);
-      const float seen = fmaxf(top, m);
-      if (seen > -INFINITY) {                             // NaN and +inf end up as a NaN of the sum
-        sum *= __expf(m - seen);
+      for (int b = 0; b < NB; ++b) {
+        load(t0 + b * E * kBmThreads, v);
+        float top = v[0];
 #pragma unroll
-        for (int i = 0; i < E; ++i) sum += __expf(v[i] - seen);
+        for (int i = 1; i < E; ++i) top = fmaxf(top, v[i]);
+        const float seen = fmaxf(top, m);
+        if (seen > -INFINITY) {                           // NaN and +inf end up as a NaN of the sum
+          sum *= __expf(m - seen);
+#pragma unroll
+          for (int i = 0; i < E; ++i) sum += __expf(v[i] - seen);
+        } else {
+#pragma unroll
+          for (int i = 0; i < E; ++i) sum += v[i] == -INFINITY ? 0.f : v[i];
+        }
+        m = seen;
+        tops[b] = top;
+        mine = fmaxf(mine, top);
+      }
+      const float bound = block_bound(mine, B, s);
+      // few pass: a batch that is no longer in registers is read again, and so are the values, so that registers need no index
+      auto list = [&](int from) {
+        uint32_t pass = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) pass |= (uint32_t)(v[i] >= bound && v[i] > -INFINITY) << i;
+        while (pass) {
+          const int id = id_of(from, __ffs(pass) - 1), at = atomicAdd(&s.n, 1);
+          pass &= pass - 1;
+          if (at < kBmList) s.key[at] = beam_key(__ldg(x + id), id);
+        }
+      };
+      if constexpr (NB == 1) {
+        list(t0);
       } else {
+        uint32_t want = 0;
 #pragma unroll
-        for (int i = 0; i < E; ++i) sum += v[i] == -INFINITY ? 0.f : v[i];
-      }
-      m = seen;
-      const float bound = block_bound(fmaxf(top, carried), B, s);
-      uint32_t pass = 0;
-#pragma unroll
-      for (int i = 0; i < E; ++i) pass |= (uint32_t)(v[i] >= bound && v[i] > -INFINITY) << i;
-      while (pass) {                                      // few: read again, so that the registers need no index
-        const int id = id_of(__ffs(pass) - 1), at = atomicAdd(&s.n, 1);
-        pass &= pass - 1;
-        if (at < kBmList) s.key[at] = beam_key(__ldg(x + id), id);
+        for (int b = 0; b < NB; ++b) want |= (uint32_t)(tops[b] >= bound && tops[b] > -INFINITY) << b;
+        while (want) {
+          const int from = t0 + (__ffs(want) - 1) * E * kBmThreads;
+          want &= want - 1;
+          load(from, v);
+          list(from);
+        }
       }
       if (carried >= bound && carried > -INFINITY) {
         const int at = atomicAdd(&s.n, 1);
@@ -295,14 +320,18 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
           auto offer = [&](float u, int id) {
             if ((u < last || (u == last && id > last_id)) && (u > best || (u == best && u > -INFINITY && id < where))) { best = u; where = id; }
           };
+#pragma unroll 1
+          for (int b = 0; b < NB; ++b) {
+            if (NB > 1) load(t0 + b * E * kBmThreads, v);
 #pragma unroll
-          for (int i = 0; i < E; ++i) offer(v[i], id_of(i));
+            for (int i = 0; i < E; ++i) offer(v[i], id_of(t0 + b * E * kBmThreads, i));
+          }
           offer(carried, carried_id);
         }, [&](int rank, float value, int id) { out[rank] = BeamCell{value, id}; });
       }
       const int had = min(B, s.n);
       if (tid >= had && tid < B) out[tid] = BeamCell{-INFINITY, 0x7fffffff};
-      if (t0 + E * kBmThreads < hi) {                     // the best so far take part in the next tile's choice
+      if (t0 + NB * E * kBmThreads < hi) {                // the best so far take part in the next tile's choice
         __syncthreads();
         carried = -INFINITY;
         if (tid < had) { carried = out[tid].value; carried_id = out[tid].id; }
@@ -409,11 +438,28 @@ struct ReorderArgs {
 
 constexpr int kBeamPage = 64;
 
-__device__ __forceinline__ void copy_bytes(uint8_t* dst, const uint8_t* src, int n) {
-  const int n16 = n >> 4;
-  for (int i = threadIdx.x; i < n16; i += blockDim.x) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
-  const int rest = (n & 15) >> 2;
-  if (threadIdx.x < rest) reinterpret_cast<uint32_t*>(dst + 16 * n16)[threadIdx.x] = reinterpret_cast<const uint32_t*>(src + 16 * n16)[threadIdx.x];
+// The first `n` bytes of every head's block of a page: all heads at once, eight loads of a thread in flight.
+__device__ __forceinline__ void copy_heads(uint8_t* dst, const uint8_t* src, int n, int pitch, int heads) {
+  constexpr int AHEAD = 8;
+  const unsigned words = (unsigned)n >> 4, total = words * heads;
+  for (unsigned i0 = threadIdx.x; i0 < total; i0 += AHEAD * blockDim.x) {
+    uint4 v[AHEAD];
+    unsigned at[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const unsigned i = i0 + u * blockDim.x, h = i / words;
+      at[u] = h * pitch + (i - h * words) * 16;
+      if (i < total) v[u] = *reinterpret_cast<const uint4*>(src + at[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (i0 + u * blockDim.x < total) *reinterpret_cast<uint4*>(dst + at[u]) = v[u];
+  }
+  const int rest = (n & 15) >> 2;                         // rows that are no multiple of 16 bytes (q8_0) may leave some words
+  for (int i = threadIdx.x; i < rest * heads; i += blockDim.x) {
+    const int at = i / rest * pitch + (n & ~15) + i % rest * 4;
+    *reinterpret_cast<uint32_t*>(dst + at) = *reinterpret_cast<const uint32_t*>(src + at);
+  }
 }
 
 // grid (G * B, layers), 256 threads
@@ -469,11 +515,9 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(const ReorderArgs a) 
   }
   if (source < 0) return;
   if (source >= a.n_pages || place < 0 || place >= a.n_pages) { if (tid == 0) raise_fault(a.fault, layer, FS_PAGE); return; }
-  for (int h = 0; h < a.n_kv; ++h) {
-    const long src = ((long)layer * a.n_pages + source) * a.n_kv + h, dst = ((long)layer * a.n_pages + place) * a.n_kv + h;
-    copy_bytes(a.k + dst * kBeamPage * a.k_row, a.k + src * kBeamPage * a.k_row, part * (int)a.k_row);
-    if (a.v_row) copy_bytes(a.v + dst * kBeamPage * a.v_row, a.v + src * kBeamPage * a.v_row, part * (int)a.v_row);
-  }
+  const long src = ((long)layer * a.n_pages + source) * a.n_kv * kBeamPage, dst = ((long)layer * a.n_pages + place) * a.n_kv * kBeamPage;
+  copy_heads(a.k + dst * a.k_row, a.k + src * a.k_row, part * (int)a.k_row, kBeamPage * (int)a.k_row, a.n_kv);
+  if (a.v_row) copy_heads(a.v + dst * a.v_row, a.v + src * a.v_row, part * (int)a.v_row, kBeamPage * (int)a.v_row, a.n_kv);
 }
 
 }  // namespace bl
@@ -483,8 +527,10 @@ using namespace bl;
 extern "C" {
 
 static void beam_chunks(int V, int rows, int B, int sms, int& tile, int& n, int& chunk) {
-  // 8,192 values a block cost less than 4,096 (the choice of the best is once a block) where both fill the processors
-  tile = (long)rows * ((V + 8191) / 8192) >= 2L * sms ? 8192 : 4096;
+  // The choice of the best is once a tile, so large tiles cost less where there are blocks enough: four of a processor's size are
+  // resident at a time.
+  auto blocks = [&](int size) { return (long)rows * ((V + size - 1) / size); };
+  tile = blocks(32768) >= 4L * sms ? 32768 : blocks(16384) >= 4L * sms ? 16384 : blocks(8192) >= 2L * sms ? 8192 : 4096;
   n = (V + tile - 1) / tile;
   if (n > kBmMaxCells / B) n = kBmMaxCells / B;
   chunk = ((V + n - 1) / n + 3) / 4 * 4;
@@ -529,8 +575,12 @@ int bl_beam_select(const BeamSelectCall* call) {
   a.tickets = (int*)w;
   a.parent = parent; a.token = token; a.out_scores = out_scores; a.out_done = out_done; a.out_lengths = out_lengths; a.fault = fault;
   const dim3 grid(a.n_chunks, (unsigned)R);
-  if (tile == 8192) return (int)launch(beam_select_kernel<32>, grid, dim3(kBmThreads), 0, st, a);
-  return (int)launch(beam_select_kernel<16>, grid, dim3(kBmThreads), 0, st, a);
+  switch (tile) {
+    case 32768: return (int)launch(beam_select_kernel<32, 4>, grid, dim3(kBmThreads), 0, st, a);
+    case 16384: return (int)launch(beam_select_kernel<32, 2>, grid, dim3(kBmThreads), 0, st, a);
+    case 8192: return (int)launch(beam_select_kernel<32, 1>, grid, dim3(kBmThreads), 0, st, a);
+    default: return (int)launch(beam_select_kernel<16, 1>, grid, dim3(kBmThreads), 0, st, a);
+  }
 }
 
 int bl_beam_reorder(const BeamReorderCall* call) {
@@ -539,6 +589,7 @@ int bl_beam_reorder(const BeamReorderCall* call) {
              BL_ERR_SHAPE);
   BL_REQUIRE(B <= kMaxBeams, BL_ERR_LIMIT);
   BL_REQUIRE(k_row >= 4 && v_row >= 0 && table != table_out, BL_ERR_SHAPE);
+  BL_REQUIRE((long)n_kv * kBeamPage * (k_row > v_row ? k_row : v_row) <= 0x7fffffffL, BL_ERR_LIMIT);
   BL_REQUIRE(k_row % 4 == 0 && v_row % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0, BL_ERR_ALIGN);
   ReorderArgs a{(uint8_t*)k, (uint8_t*)v, k_row, v_row, n_pages, n_kv, G, B, n_slots, max_pages, table, table_out, slots, parent, held, fault};
   return (int)launch(beam_reorder_kernel, dim3(G * B, n_layer), dim3(256), 0, st, a);
