@@ -332,10 +332,17 @@ __device__ __forceinline__ void px_touch_scratch(const PrefixArgs& a) {
   if (threadIdx.x < 32) px_prefetch(a.sched + threadIdx.x);
 }
 
-template <int HEAD, bool Q8>
-// Bounds of 512 threads in both forms: 128 registers a lane, so that blocks of the joining launch fit beside the 384 of f16 caches
-// and are there when these end (with 138 registers four beams behind 512 positions took 14.9 us a call instead of 12.5).
-__global__ void __launch_bounds__(512, 1)
+// LONG: for CTAs that go through several tiles.  The softmax's code is straight and holds a row's 128 scores (200 registers a lane, which
+// the other warps give up); the short form reads them twice in loops, because straight code that is met once costs more to fetch
+// than to run.  A job takes 4,900 clocks of a CTA with two tiles of rows in the long form and 6,000 in the short one; a call that
+// is one job a CTA spends 3,000 clocks on the long form's exponentials and 2,400 on the short one's.
+// Bounds of 512 threads for the short form, that is 128 registers a lane: blocks of the joining launch fit beside the 384 threads of f16
+// caches and are there when these end (with 138 registers four beams behind 512 positions took 14.9 us a call instead of 12.5).
+// Registers of the long form: 3 x 168 a lane at the launch = 104 + 200 + 200, with the expanding warps 4 x 128 = 72 + 88 + 176 + 176.
+constexpr int px_bound(bool q8, bool is_long) { return is_long ? px_threads(q8) : 512; }
+
+template <int HEAD, bool Q8, bool LONG>
+__global__ void __launch_bounds__(px_bound(Q8, LONG), 1)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const PrefixArgs a) {
   constexpr int NH = HEAD / 64, TILE = px_tile(HEAD), PAGE_BYTES = kPxPage * 128, ST = px_stages(Q8), RAW = px_raw(HEAD);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -389,6 +396,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
 
   if (Q8 && warp >= 12) {
     // ---- q8_0 rows to f16: a thread for a row of the tile
+    if constexpr (LONG) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     const int key = threadIdx.x - 384;
     int tile = 0;
     bool ok = true;
@@ -423,6 +431,10 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
       }
     }
   } else if (warp >= 8) {
+    if constexpr (LONG) {
+      if constexpr (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+      else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    }
     if (warp == 8) {
       // ---- producer: all lanes walk, lane 0 waits and copies
       int tile = 0;
@@ -585,6 +597,10 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
       }
     }
   } else {
+    if constexpr (LONG) {
+      if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+      else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    }
     // ---- softmax: a thread per query row ------------------------------------------------------------------
     const int x = warp >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;                          // row of the tile
@@ -667,38 +683,49 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
         if (!ok) break;
         tc_fence_after();
         if (!begun) to_log2 = busy ? s_scale[x][r] : 0.f;       // written in front of what these scores waited for
-        // The scores are read twice, 32 at a time, in loops: 128 of them at once in straight code took 3,000 clocks the first time
-        // it was met, most of a short call's softmax.
-        auto scores = [&](int c, uint32_t (&v)[32]) {
-          tmem_ld32(tS + 32 * c, v);
-          tmem_ld_wait();
-          if (!all) {
-            const int n = (c < 2 ? n0 : n1) - 32 * (c & 1);
+        // A page's half of the probabilities is written.  Where a sequence ends inside the page, what lies behind may be anything, and
+        // zero times that must be zero: the first tile of rows that takes part clears it.
+        auto finish = [&](int p) {
+          const int n = p ? k1 : k0;
+          if (!Q8 && n > 0 && n < kPxPage && x == (who & 1 ? 0 : 1)) {
+            const int st = tile & 1;
+            ok = mbar_wait_warp(&v_full[st], (uint32_t)((tile >> 1) & 1), abort_flag);
+            if (!ok) return;
+            uint8_t* page = sV + st * TILE + p * NH * PAGE_BYTES;
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i >= n) v[i] = 0xff800000u;                   // -inf
+            for (int h = 0; h < NH; ++h)
+              for (int i = n * 8 + r; i < kPxPage * 8; i += 128) *reinterpret_cast<uint4*>(page + h * PAGE_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
+            fence_async_smem();
           }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[4 * p + 2 * x + (mine & 1)]);
         };
-        float mb = 0.f, corr = 1.f;
-        if (some) {
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            scores(c, v);
+        auto mask = [&](int c, uint32_t (&v)[32]) {
+          const int n = (c < 2 ? n0 : n1) - 32 * (c & 1);
 #pragma unroll
-            for (int i = 0; i < 32; i += 8)
+          for (int i = 0; i < 32; ++i)
+            if (i >= n) v[i] = 0xff800000u;                     // -inf
+        };
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum[4] = {0.f, 0.f, 0.f, 0.f}, mb = 0.f, corr = 1.f;
+        auto widen = [&](const uint32_t (&v)[32]) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) mx4[j] = fmaxf(fmaxf(mx4[j], __uint_as_float(v[i + j])), __uint_as_float(v[i + 4 + j]));
-          }
+          for (int i = 0; i < 32; i += 8)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mx4[j] = fmaxf(fmaxf(mx4[j], __uint_as_float(v[i + j])), __uint_as_float(v[i + 4 + j]));
+        };
+        // the new maximum, and the output brought to it
+        auto settle = [&]() {
           float m_new = fmaxf(m, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
           if (m != -INFINITY && (m_new - m) * to_log2 <= kPxLazy) m_new = m;
           mb = (m_new == -INFINITY) ? 0.f : m_new * to_log2;    // a row with no key yet keeps zeros
           corr = (m == -INFINITY || m == m_new) ? 1.f : px_ex2(m * to_log2 - mb);
+          m = m_new;
           if (begun && __any_sync(0xffffffffu, corr != 1.0f)) {
-            // the output is scaled in tensor memory, behind the tile's last product
+            // scaled in tensor memory, behind the tile's last product
             ok = mbar_wait_warp(&pv_done[2 * x + ((mine - 1) & 1)], (uint32_t)(((mine - 1) >> 1) & 1), abort_flag);
-            if (!ok) break;
+            if (!ok) return;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < HEAD / 32; ++c) {
@@ -710,49 +737,70 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
               tmem_st32(tO + c * 32, o);
             }
           }
-          m = m_new;
-        }
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
-          if (some) {
-            uint32_t v[32];
-            scores(c, v);
+        };
+        auto powers = [&](const uint32_t (&v)[32], uint32_t (&pk)[16]) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              uint32_t e0, e1;
-              asm("{\n\t.reg .b64 rs, rk, rm, rr;\n\t"
-                  "mov.b64 rs, {%2, %3};\n\tmov.b64 rk, {%4, %4};\n\tmov.b64 rm, {%5, %5};\n\t"
-                  "fma.rn.f32x2 rr, rs, rk, rm;\n\tmov.b64 {%0, %1}, rr;\n\t}"
-                  : "=r"(e0), "=r"(e1) : "r"(v[i]), "r"(v[i + 1]), "f"(to_log2), "f"(-mb));
-              const float p0 = px_ex2(__uint_as_float(e0)), p1 = px_ex2(__uint_as_float(e1));
-              sum[i & 2] += p0; sum[(i & 2) + 1] += p1;
-              pk[i >> 1] = px_pack(p0, p1);
-            }
-          } else {                                              // no row of this warp attends to these pages
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pk[i] = 0;
+          for (int i = 0; i < 32; i += 2) {
+            uint32_t e0, e1;
+            asm("{\n\t.reg .b64 rs, rk, rm, rr;\n\t"
+                "mov.b64 rs, {%2, %3};\n\tmov.b64 rk, {%4, %4};\n\tmov.b64 rm, {%5, %5};\n\t"
+                "fma.rn.f32x2 rr, rs, rk, rm;\n\tmov.b64 {%0, %1}, rr;\n\t}"
+                : "=r"(e0), "=r"(e1) : "r"(v[i]), "r"(v[i + 1]), "f"(to_log2), "f"(-mb));
+            const float p0 = px_ex2(__uint_as_float(e0)), p1 = px_ex2(__uint_as_float(e1));
+            sum[i & 2] += p0; sum[(i & 2) + 1] += p1;
+            pk[i >> 1] = px_pack(p0, p1);
           }
-          px_st16(tS + 16 * c, pk);
-          if (c & 1) {
-            // A page's half of the probabilities is written.  Where a sequence ends inside the page, what lies behind may be
-            // anything, and zero times that must be zero: the first tile of rows that takes part clears it.
-            const int p = c >> 1, n = p ? k1 : k0;
-            if (!Q8 && n > 0 && n < kPxPage && x == (who & 1 ? 0 : 1)) {
-              const int st = tile & 1;
-              ok = mbar_wait_warp(&v_full[st], (uint32_t)((tile >> 1) & 1), abort_flag);
-              if (!ok) break;
-              uint8_t* page = sV + st * TILE + p * NH * PAGE_BYTES;
+        };
+        if (!some) {
+          // no row of this warp attends to these pages
+          uint32_t pk[16];
 #pragma unroll
-              for (int h = 0; h < NH; ++h)
-                for (int i = n * 8 + r; i < kPxPage * 8; i += 128) *reinterpret_cast<uint4*>(page + h * PAGE_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
-              fence_async_smem();
-            }
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[4 * p + 2 * x + (mine & 1)]);
+          for (int i = 0; i < 16; ++i) pk[i] = 0;
+#pragma unroll 1
+          for (int c = 0; ok && c < 4; ++c) {
+            px_st16(tS + 16 * c, pk);
+            if (c & 1) finish(c >> 1);
+          }
+        } else if constexpr (LONG) {
+          // all of a row's scores in registers, straight code
+          uint32_t v[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(tS + 32 * c, v[c]);
+          tmem_ld_wait();
+          if (!all) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mask(c, v[c]);
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) widen(v[c]);
+          settle();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
+            powers(v[c], pk);
+            px_st16(tS + 16 * c, pk);
+            if (ok && (c & 1)) finish(c >> 1);
+          }
+        } else {
+          // read twice, 32 at a time
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            tmem_ld32(tS + 32 * c, v);
+            tmem_ld_wait();
+            if (!all) mask(c, v);
+            widen(v);
+          }
+          settle();
+#pragma unroll 1
+          for (int c = 0; ok && c < 4; ++c) {
+            uint32_t v[32], pk[16];
+            tmem_ld32(tS + 32 * c, v);
+            tmem_ld_wait();
+            if (!all) mask(c, v);
+            powers(v, pk);
+            px_st16(tS + 16 * c, pk);
+            if (c & 1) finish(c >> 1);
           }
         }
         if (!ok) break;
@@ -902,7 +950,7 @@ __global__ void __launch_bounds__(256, 4) prefix_join_kernel(const PrefixArgs a)
 
 using namespace bl;
 
-template <int HEAD, bool Q8>
+template <int HEAD, bool Q8, bool LONG>
 static int prefix_go(const PrefixArgs& a, cudaStream_t st) {
   CUtensorMap mk = {}, mv = {};
   if (!Q8) {
@@ -916,12 +964,12 @@ static int prefix_go(const PrefixArgs& a, cudaStream_t st) {
   }
   static PerDevice limit;
   if (limit.due()) {
-    const cudaError_t e = cudaFuncSetAttribute(prefix_attn_kernel<HEAD, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    const cudaError_t e = cudaFuncSetAttribute(prefix_attn_kernel<HEAD, Q8, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                px_smem(HEAD, Q8, kPxMaxRows, kPxMaxRows));
     if (e != cudaSuccess) return (int)e;
     limit.mark();
   }
-  const cudaError_t e = launch(prefix_attn_kernel<HEAD, Q8>, dim3(a.n_cta), dim3(px_threads(Q8)), (size_t)px_smem(HEAD, Q8, a.n_units, a.M), st, mk, mv, a);
+  const cudaError_t e = launch(prefix_attn_kernel<HEAD, Q8, LONG>, dim3(a.n_cta), dim3(px_threads(Q8)), (size_t)px_smem(HEAD, Q8, a.n_units, a.M), st, mk, mv, a);
   if (e != cudaSuccess) return (int)e;
   // few rows: a block for 32 values of a head, so that more of its fragments are in flight; many: as much of it as 256 threads hold
   int z = HEAD / 32;
@@ -949,7 +997,7 @@ long bl_prefix_work_bytes(int head, int n_q, int n_kv, int n_units, int unit_row
 struct PrefixCall {
   const float* q; const void* k_cache; const void* v_cache; const int* row_pos; const int* row_seq; const int* block_table;
   const int* meta; void* work; void* out; unsigned* fault; cudaStream_t stream;
-  int n_slots, max_pages, n_pages, head, n_q, n_kv, M, n_units, unit_rows, kv_q8, n_cta, layer;
+  int n_slots, max_pages, n_pages, head, n_q, n_kv, M, n_units, unit_rows, kv_q8, n_cta, layer, shared_tiles;     // tiles of 128 shared keys of all units of a KV head
 };
 
 int bl_prefix_attention(const PrefixCall* call) {
@@ -969,8 +1017,17 @@ int bl_prefix_attention(const PrefixCall* call) {
   a.sched = (int4*)work;
   a.part = (float4*)((uint8_t*)work + kPxMaxRows * 16);
   a.part_bytes = prefix_slots(head, n_q / n_kv, n_kv, n_units, unit_rows, n_cta, a.slot, a.slot_tiles, a.pitch);
-  if (p.kv_q8) return head == 128 ? prefix_go<128, true>(a, st) : prefix_go<64, true>(a, st);
-  return head == 128 ? prefix_go<128, false>(a, st) : prefix_go<64, false>(a, st);
+  // four tiles of shared keys a CTA or more
+  const bool is_long = (long)n_kv * p.shared_tiles >= 4L * n_cta;
+  auto go = [&](auto head_, auto q8_) {
+    constexpr int HEAD = decltype(head_)::value;
+    constexpr bool Q8 = decltype(q8_)::value;
+    return is_long ? prefix_go<HEAD, Q8, true>(a, st) : prefix_go<HEAD, Q8, false>(a, st);
+  };
+  const std::integral_constant<int, 128> h128;
+  const std::integral_constant<int, 64> h64;
+  if (p.kv_q8) return head == 128 ? go(h128, std::true_type()) : go(h64, std::true_type());
+  return head == 128 ? go(h128, std::false_type()) : go(h64, std::false_type());
 }
 
 }  // extern "C"

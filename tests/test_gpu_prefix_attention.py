@@ -149,6 +149,16 @@ def test_many_rows_behind_a_long_prefix(n_q, n_kv, head, rows, prefix, tail, q8)
 
 @gpu
 @pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("n_q,n_kv,head,rows,prefix,tail", [(32, 4, 128, 64, 16448, 300), (8, 2, 64, 33, 39936, 70), (32, 4, 128, 5, 20480, 140),
+                                                            (48, 8, 128, 7, 16384, 1)])
+def test_prefixes_that_take_the_long_form(n_q, n_kv, head, rows, prefix, tail, q8):
+    """Four tiles of shared keys or more for every processor."""
+    c = Case([(prefix, [prefix + 1 + i * (tail - 1) // (rows - 1) for i in range(rows)]), (64, [70])], n_q, n_kv, head, q8, seed=rows)
+    c.check(c.run())
+
+
+@gpu
+@pytest.mark.parametrize("q8", [False, True])
 def test_tails_longer_than_the_prefix(q8):
     c = Case([(64, [3000, 70, 2500]), (128, [129, 1999])], 32, 4, 128, q8, seed=5)
     c.check(c.run())
