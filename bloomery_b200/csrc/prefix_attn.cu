@@ -4,21 +4,22 @@
 //   o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),   s_j = q . k_j,   m = max_j s_j
 // The keys are cut into fragments; each leaves its maximum, its sum and its unnormalised output, and a second launch joins them.
 //
-// f16 caches run on the 5th-generation tensor cores.  A unit is up to 256 stacked (row, head) pairs of one KV head, rows of one
-// group, in two tiles of 128: it reads the pages that its rows share and then the pages of each of its rows, all of them against
-// all of its query rows; for a page of one row the others' scores are masked.  (Multiplying rows that are masked costs no
-// time: a tile's products and exponentials take half of what its keys and values take to arrive.  With a fragment for each
-// row's own keys instead, 64 rows with 1 to 256 keys of their own behind 32,768 took 102 us: a fragment of two tiles costs as much
-// as eight more.)  Per 128 keys (two pages) and tile of rows, a job:
-//   S = Q K^T     tcgen05.mma kind::f16, M = N = 128, into one of two score buffers in tensor memory
+// Both kinds of cache run on the 5th-generation tensor cores.  A unit is up to 256 stacked (row, head) pairs of one KV head, rows
+// of one group, in two tiles of 128: it reads the pages that its rows share and then the pages of each of its rows, all of them
+// against all of its query rows; for a page of one row the others' scores are masked.  (Multiplying rows that are masked costs
+// little: a page's products take less than its keys and values take to arrive.  With a fragment for each row's own keys instead,
+// 64 rows with 1 to 256 keys of their own behind 32,768 took 102 us: a short fragment costs as much as eight pages more.)
+// Per page of 64 keys and tile of rows, a job:
+//   S = Q K^T     tcgen05.mma kind::f16, M = 128, N = 64, into one of the tile's two score buffers in tensor memory
 //   softmax       one thread per query row; the probabilities go back as f16 into the score columns they came from
 //   O += P V      P from tensor memory, V as it lies in the cache: rows of keys, the MN-major form of a B operand
-// Two tiles of rows take a score buffer each, and one's softmax runs under the other's products; a tile that is alone takes both
-// in turn.
-// The work of a call is one line of tiles, unit after unit; every CTA takes an equal stretch of it, whatever the lengths, and
+// Behind a job's second product the scores of the job after the next are multiplied, so that the softmax of a tile has scores to
+// go on with while the products of the last ones run.
+// The work of a call is one line of pages, unit after unit; every CTA takes an equal stretch of it, whatever the lengths, and
 // goes through the fragments that its stretch cuts.
 // Roles: warps 0..3 softmax of the first tile of rows, 4..7 of the second (warp id modulo 4 = TMEM lane quarter), warp 8 the TMA
-// producer (two-stage rings for keys and values, 128 KB in flight), warps 9 and 10 the MMA issuers of either tile; 9 owns the TMEM.
+// producer (four pages of keys and of values in flight), warps 9 and 10 the MMA issuers of either tile; 9 owns the TMEM.  q8_0 rows
+// are fetched as they are and expanded to f16 by four warps more.
 // Queries and probabilities are rounded to f16 (11 bits; queries scaled by a power of two a row): less than the output's 8 bits.
 // A value that is not finite would reach the masked rows of its tile as 0 x inf; rows whose output is not finite are summed again
 // key by key, over their own keys alone.
@@ -44,7 +45,7 @@ struct PrefixArgs {
   unsigned* fault; int layer;
   const int* units;               // [n_units][first row, rows, shared positions, first row of the group, rows of the group]
   int n_units, n_cta;
-  int4* sched;                    // [M] tiles of a KV head; running sums of the row's unit; keys: of this call, for the joining launch
+  int4* sched;                    // [M] pages of a KV head; running sums of the row's unit; keys: of this call, for the joining launch
   // [fragment][tiles of rows][outputs [HEAD / 4][pitch], then maxima and sums [pitch] of 8 bytes]: `slot` float4 a tile.  What lies
   // close together needs few address translations.
   float4* part;
@@ -99,20 +100,23 @@ __device__ __forceinline__ void px_row(const PrefixArgs& a, int m, int h, int n,
 }
 
 // ---- the line of work ---------------------------------------------------------------------------------------
-// Per KV head the tiles of all units (S), CTA c of n takes tiles c T / n .. (c + 1) T / n - 1 of the T = n_kv S.  A fragment is what
+// Per KV head the pages of all units (S), CTA c of n takes pages c T / n .. (c + 1) T / n - 1 of the T = n_kv S.  A fragment is what
 // a stretch shares with a (KV head, unit); fragments' numbers (index + CTA) grow by one from each to the next within a unit and
-// by one at least between units, so they name places in the scratch.  All CTAs and the joining launch work the line out alike.
+// by one at least between units, so they name places in the scratch.
+// CTAs that a line of T pages is cut for: a page each at least, so that a unit's CTAs follow each other
+__host__ __device__ __forceinline__ unsigned px_ctas(const PrefixArgs& a, unsigned T) { return T < (unsigned)a.n_cta ? T : (unsigned)a.n_cta; }
+
 struct PxFrag {
-  int unit, kvh, t_lo, n_t, id;
-  int row0, rows, shared, total;  // rows of the unit; its pages, shared and in all
+  int unit, kvh, lo, end, id;     // pages lo .. end - 1 of the unit
+  int row0, rows, shared;         // rows of the unit; its shared pages
   int row;                        // whose own pages it starts in
-  int pad[2];
+  int pad[3];
 };
 
 struct PxLine {
   int* keys;                      // [M] keys of a row
   int* pages;                     // [M + 1] running sum of the rows' own pages
-  int* tiles;                     // [n_units + 1] running sum of the units' tiles
+  int* cum;                       // [n_units + 1] running sum of the units' pages
   int* seq;                       // [M]
   int* units;                     // [n_units][kPxUnit]
   int n_units, S, g, end, cta;
@@ -138,7 +142,7 @@ struct PxLine {
   // Whole block; `mem` holds words(M, n_units).  The first fragment is worked out once for all warps: a look-up costs each of them
   // some hundred instructions that are met for the first time, at a dozen clocks each.
   __device__ __forceinline__ void build(const PrefixArgs& a, int* mem, int4* s_first) {
-    keys = mem; pages = keys + a.M; tiles = pages + a.M + 1; seq = tiles + a.n_units + 1; units = seq + a.M;
+    keys = mem; pages = keys + a.M; cum = pages + a.M + 1; seq = cum + a.n_units + 1; units = seq + a.M;
     n_units = a.n_units;
     cta = blockIdx.x;
     for (int i = threadIdx.x; i < n_units * kPxUnit; i += blockDim.x) units[i] = a.units[i];
@@ -159,14 +163,14 @@ struct PxLine {
         const int* unit = units + u * kPxUnit;
         int live = 0;                                           // a unit without a live row reads nothing
         for (int m = unit[0]; !live && m < unit[0] + unit[1]; ++m) live = keys[m];
-        tiles[u + 1] = live ? (unit[2] / kPxPage + pages[unit[0] + unit[1]] - pages[unit[0]] + 1) / 2 : 0;
+        cum[u + 1] = live ? unit[2] / kPxPage + pages[unit[0] + unit[1]] - pages[unit[0]] : 0;
       }
       __syncwarp();
-      running(tiles, n_units);
+      running(cum, n_units);
       __syncwarp();
       if (threadIdx.x == 0) {
-        S = tiles[n_units];
-        const unsigned T = (unsigned)(a.n_kv * S), n = min((unsigned)a.n_cta, T);  // a tile each at least: a unit's CTAs follow each other
+        S = cum[n_units];
+        const unsigned T = (unsigned)(a.n_kv * S), n = px_ctas(a, T);
         g = (unsigned)cta < n ? (int)((unsigned)cta * T / n) : 0;
         end = (unsigned)cta < n ? (int)((unsigned)(cta + 1) * T / n) : 0;
         PxFrag f = {};
@@ -183,7 +187,7 @@ struct PxLine {
     if (blockIdx.x == 0)
       for (int m = threadIdx.x; m < a.M; m += blockDim.x) {
         const int u = a.meta[m * kPxMeta + 3];
-        a.sched[m] = make_int4(S, tiles[u], tiles[u + 1], keys[m]);
+        a.sched[m] = make_int4(S, cum[u], cum[u + 1], keys[m]);
       }
   }
   __device__ __forceinline__ bool first(const int4* s_first, PxFrag& f) const {
@@ -195,47 +199,38 @@ struct PxLine {
     if (g >= end) return false;
     f.kvh = (int)((unsigned)g / (unsigned)S);
     const int rem = g - f.kvh * S;
-    f.unit = find(tiles, n_units, rem);
-    f.t_lo = rem - tiles[f.unit];
-    f.n_t = min(tiles[f.unit + 1] - rem, end - g);
+    f.unit = find(cum, n_units, rem);
+    f.lo = rem - cum[f.unit];
+    const int n = min(cum[f.unit + 1] - rem, end - g);
+    f.end = f.lo + n;
     f.id = f.kvh * n_units + f.unit + cta;
-    g += f.n_t;
+    g += n;
     const int* unit = units + f.unit * kPxUnit;
     f.row0 = unit[0]; f.rows = unit[1]; f.shared = unit[2] / kPxPage;
-    f.total = f.shared + pages[f.row0 + f.rows] - pages[f.row0];
     f.row = f.row0;
-    if (2 * f.t_lo > f.shared) f.row = f.row0 + find(pages + f.row0, f.rows, pages[f.row0] + 2 * f.t_lo - f.shared);
+    if (f.lo > f.shared) f.row = f.row0 + find(pages + f.row0, f.rows, pages[f.row0] + f.lo - f.shared);
     return true;
   }
 };
 
-// The pages of a unit in order: the shared ones, then every row's own.  A tile is two of them.
+// The pages of a unit in order: the shared ones, then every row's own.
 struct PxWalk {
   const int* keys; const int* pages;
-  int row0, rows, shared, total, row;                           // shared, total: pages
+  int row0, rows, shared, row;
   __device__ __forceinline__ void start(const PxLine& line, const PxFrag& f) {
     keys = line.keys; pages = line.pages;
-    row0 = f.row0; rows = f.rows; shared = f.shared; total = f.total; row = f.row;
+    row0 = f.row0; rows = f.rows; shared = f.shared; row = f.row;
   }
-  // Both pages of a tile at once; for shared pages, most of a long walk, nothing is looked up.
-  __device__ __forceinline__ void tile(int t, int& o0, int& c0, int& n0, int& o1, int& c1, int& n1) {
-    o0 = o1 = -1; c0 = 2 * t; c1 = 2 * t + 1; n0 = n1 = kPxPage;
-    if (2 * t + 2 > shared) {
-      page(2 * t, o0, c0, n0);
-      page(2 * t + 1, o1, c1, n1);
-    }
-  }
-  // owner: row of the unit, -1 all of them, -2 no page; col: page of the sequence; n: its keys.  Pages are asked for in order.
+  // owner: row of the unit, -1 all of them; col: page of the sequence; n: its keys.  Pages are asked for in order; for shared ones,
+  // most of a long walk, nothing is looked up.
   __device__ __forceinline__ void page(int p, int& owner, int& col, int& n) {
-    owner = -2; col = 0; n = 0;
-    if (p < shared) { owner = -1; col = p; n = kPxPage; }
-    else if (p < total) {
-      const int at = pages[row0] + p - shared;
-      while (pages[row + 1] <= at) ++row;
-      owner = row - row0;
-      col = shared + at - pages[row];
-      n = min(kPxPage, keys[row] - kPxPage * col);
-    }
+    owner = -1; col = p; n = kPxPage;
+    if (p < shared) return;
+    const int at = pages[row0] + p - shared;
+    while (pages[row + 1] <= at) ++row;
+    owner = row - row0;
+    col = shared + at - pages[row];
+    n = min(kPxPage, keys[row] - kPxPage * col);
   }
 };
 // The same value in a uniform register, which is where the tensor instructions take their operands from: what comes from memory
@@ -244,7 +239,7 @@ __device__ __forceinline__ int px_uniform(int v) { return (int)__reduce_or_sync(
 
 // tiles of rows that a page concerns, one bit each
 __device__ __forceinline__ unsigned px_tiles(int owner, int rows_tile, int n_x) {
-  return owner == -2 ? 0u : owner == -1 ? (n_x == 2 ? 3u : 1u) : owner < rows_tile ? 1u : 2u;
+  return owner == -1 ? (n_x == 2 ? 3u : 1u) : owner < rows_tile ? 1u : 2u;
 }
 
 // K-major tiles use umma_desc(); V as B operand in MN-major form: atoms of 64 values x 8 keys (1,024 bytes), 8-key groups one atom
@@ -279,11 +274,12 @@ __device__ __forceinline__ void px_st16(uint32_t taddr, const uint32_t (&r)[16])
 
 constexpr int kPxHalf = 128 * 128;                      // 16 KB: 128 rows of 64 f16 values, one swizzle atom wide
 constexpr int px_tile(int head) { return head / 64 * kPxHalf; }
-// f16 caches: two stages of keys and of values.  q8_0: one each, and two of the rows as they are in the cache.
-constexpr int px_stages(bool q8) { return q8 ? 1 : 2; }
+constexpr int px_page(int head) { return head / 64 * kPxPage * 128; }             // a page of one head as f16: [HEAD / 64][64 keys][128 bytes]
+// Pages of keys and of values in flight.  q8_0: four as they are in the cache, two expanded.
+constexpr int px_stages(bool q8) { return q8 ? 2 : 4; }
 constexpr int px_raw(int head) { return kPxPage * (head / 32 * 34); }             // a page of q8_0 rows of one head: a multiple of 16
 constexpr int px_smem(int head, bool q8, int n_units, int M) {
-  return (2 + 2 * px_stages(q8)) * px_tile(head) + (q8 ? 8 * px_raw(head) : 0) + 1024 + PxLine::words(M, n_units) * 4;
+  return 2 * px_tile(head) + 2 * px_stages(q8) * px_page(head) + (q8 ? 8 * px_raw(head) : 0) + 1024 + PxLine::words(M, n_units) * 4;
 }
 // q8_0 caches have four more warps, which expand the rows
 constexpr int px_threads(bool q8) { return q8 ? 512 : 384; }
@@ -332,40 +328,33 @@ __device__ __forceinline__ void px_touch_scratch(const PrefixArgs& a) {
   if (threadIdx.x < 32) px_prefetch(a.sched + threadIdx.x);
 }
 
-// LONG: for CTAs that go through several tiles.  The softmax's code is straight and holds a row's 128 scores (200 registers a lane, which
-// the other warps give up); the short form reads them twice in loops, because straight code that is met once costs more to fetch
-// than to run.  A job takes 4,900 clocks of a CTA with two tiles of rows in the long form and 6,000 in the short one; a call that
-// is one job a CTA spends 3,000 clocks on the long form's exponentials and 2,400 on the short one's.
-// Bounds of 512 threads for the short form, that is 128 registers a lane: blocks of the joining launch fit beside the 384 threads of f16
+// Bounds of 512 threads in both forms, that is 128 registers a lane: blocks of the joining launch fit beside the 384 threads of f16
 // caches and are there when these end (with 138 registers four beams behind 512 positions took 14.9 us a call instead of 12.5).
-// Registers of the long form: 3 x 168 a lane at the launch = 104 + 200 + 200, with the expanding warps 4 x 128 = 72 + 88 + 176 + 176.
-constexpr int px_bound(bool q8, bool is_long) { return is_long ? px_threads(q8) : 512; }
-
-template <int HEAD, bool Q8, bool LONG>
-__global__ void __launch_bounds__(px_bound(Q8, LONG), 1)
+template <int HEAD, bool Q8>
+__global__ void __launch_bounds__(512, 1)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const PrefixArgs a) {
-  constexpr int NH = HEAD / 64, TILE = px_tile(HEAD), PAGE_BYTES = kPxPage * 128, ST = px_stages(Q8), RAW = px_raw(HEAD);
+  constexpr int NH = HEAD / 64, TILE = px_tile(HEAD), PAGE = px_page(HEAD), ATOM = kPxPage * 128, ST = px_stages(Q8), RAW = px_raw(HEAD);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[4], p_full[8], pv_done[4], frag_start, raw_full[4], raw_empty[4];
+  __shared__ __align__(8) uint64_t q_full[2], k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[4], p_full[4], pv_done[4], raw_full[8], raw_empty[8];
   __shared__ uint32_t s_tmem_base;
-  __shared__ int s_abort, s_bad[8];
+  __shared__ int s_abort, s_bad[16];
   __shared__ int4 s_first[4];
   __shared__ float s_scale[2][128];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sQ = smem;                // [2 tiles][NH][128 rows][128 bytes]
-  uint8_t* sK = sQ + 2 * TILE;       // [ST stages][NH][128 keys][128 bytes]
-  uint8_t* sV = sK + ST * TILE;      // [ST stages][2 pages][NH][64 keys][128 bytes]
-  uint8_t* sRaw = sV + ST * TILE;    // q8_0: [2 stages][keys, values][2 pages][64 rows]
+  uint8_t* sK = sQ + 2 * TILE;       // [ST pages][NH][64 keys][128 bytes]
+  uint8_t* sV = sK + ST * PAGE;      // [ST pages][NH][64 keys][128 bytes]
+  uint8_t* sRaw = sV + ST * PAGE;    // q8_0: [4 pages][keys, values][64 rows]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.n_q / a.n_kv, rows_tile = 128 / G, inv_G = 65536 / G + 1;     // i * inv_G >> 16 is i / G for i < 128
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 4); mbar_init(&k_full[i], Q8 ? 4 : 1); mbar_init(&k_empty[i], 2); mbar_init(&v_full[i], Q8 ? 4 : 1); mbar_init(&v_empty[i], 2);
+    for (int i = 0; i < 2; ++i) mbar_init(&q_full[i], 4);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&k_full[i], Q8 ? 2 : 1); mbar_init(&k_empty[i], 2); mbar_init(&v_full[i], Q8 ? 2 : 1); mbar_init(&v_empty[i], 2);
+      mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&pv_done[i], 1);
     }
-    for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&pv_done[i], 1); mbar_init(&p_full[i], 4); mbar_init(&p_full[4 + i], 4); }
-    mbar_init(&frag_start, 2);
-    for (int i = 0; Q8 && i < 4; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
+    for (int i = 0; Q8 && i < 8; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 2); }
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -376,7 +365,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
   // Ahead of the wait, for lines and address translations alone: a first touch of a page costs a processor the better part of a
   // microsecond, and these would follow each other.
   for (int i = threadIdx.x; i < a.M; i += blockDim.x) { px_prefetch(a.row_pos + i); px_prefetch(a.row_seq + i); px_prefetch(a.meta + i * kPxMeta); }
-  if (threadIdx.x < 32) { px_prefetch(a.units + min((int)threadIdx.x, a.n_units - 1) * kPxUnit); px_prefetch(a.table + threadIdx.x * 32); }
+  if (threadIdx.x < 32) { px_prefetch(a.units + min((int)threadIdx.x, a.n_units - 1) * kPxUnit); px_prefetch(a.table + min((long)threadIdx.x * 32, (long)a.n_slots * a.max_pages - 1)); }
   px_touch_scratch(a);
   {
     const long at = ((long)blockIdx.x * blockDim.x + threadIdx.x) * 32;
@@ -390,223 +379,186 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
   tc_fence_after();
   const uint32_t tmem_base = s_tmem_base;
   volatile int* abort_flag = &s_abort;
-  const uint32_t tS0 = tmem_base, tO0 = tmem_base + 256;        // score buffer b at column 128 b, output of tile x at 256 + HEAD x
+  const uint32_t tS0 = tmem_base, tO0 = tmem_base + 256;        // score buffer b of tile x at column 128 x + 64 b, its output at 256 + HEAD x
   PxFrag f;
   PxWalk w;
 
   if (Q8 && warp >= 12) {
-    // ---- q8_0 rows to f16: a thread for a row of the tile
-    if constexpr (LONG) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    const int key = threadIdx.x - 384;
-    int tile = 0;
+    // ---- q8_0 rows to f16: two warps the keys, two the values, a thread for a row of the page
+    const int kv = (warp - 12) >> 1, row = threadIdx.x & 63;
+    uint64_t* const full = kv ? v_full : k_full;
+    uint64_t* const empty = kv ? v_empty : k_empty;
+    int page = 0;
     bool ok = true;
     for (bool more = line.first(s_first, f); ok && more; more = line.next(f)) {
       w.start(line, f);
-      for (int t = 0; ok && t < f.n_t; ++t, ++tile) {
-        int o0, c0, k0, o1, c1, k1;
-        w.tile(f.t_lo + t, o0, c0, k0, o1, c1, k1);
-        const int slot = tile & 1, p = key / kPxPage, row = key % kPxPage;
-        const uint32_t par = (uint32_t)((tile >> 1) & 1), par1 = (uint32_t)(tile & 1);
-#pragma unroll 1
-        for (int kv = 0; ok && kv < 2; ++kv) {
-          uint64_t* const empty = kv ? &v_empty[0] : &k_empty[0];
-          ok = mbar_wait_warp(&raw_full[2 * kv + slot], par, abort_flag) && mbar_wait_warp(empty, par1 ^ 1, abort_flag);
-          if (!ok) break;
-          const uint8_t* src = sRaw + ((slot * 2 + kv) * 2 + p) * RAW + row * (RAW / kPxPage);
-          uint8_t* dst = kv ? sV + p * NH * PAGE_BYTES + row * 128 : sK + key * 128;
-          const int pitch = kv ? PAGE_BYTES : kPxHalf, n = p ? k1 : k0;
-          if (row < n) {
-            px_expand<HEAD>(src, dst, pitch, row & 7);
-          } else if (kv && n > 0) {                               // behind a sequence's end: zero, whatever lies there
+      for (int p = f.lo; p < f.end; ++p, ++page) {
+        int owner, col, n;
+        w.page(p, owner, col, n);
+        const int slot = page & 3, st = page % ST;
+        ok = mbar_wait_warp(&raw_full[2 * slot + kv], (uint32_t)((page >> 2) & 1), abort_flag) &&
+             mbar_wait_warp(&empty[st], (uint32_t)((page / ST) & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        uint8_t* dst = (kv ? sV : sK) + st * PAGE + row * 128;
+        if (row < n) {
+          px_expand<HEAD>(sRaw + (slot * 2 + kv) * RAW + row * (RAW / kPxPage), dst, ATOM, row & 7);
+        } else {                                                // behind a sequence's end: zero, whatever lies there
 #pragma unroll
-            for (int c = 0; c < HEAD / 8; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * pitch + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(kv ? &v_full[0] : &k_full[0]);
-            mbar_arrive(&raw_empty[2 * kv + slot]);
-          }
+          for (int c = 0; c < HEAD / 8; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * ATOM + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&full[st]);
+          mbar_arrive(&raw_empty[2 * slot + kv]);
         }
       }
     }
-  } else if (warp >= 8) {
-    if constexpr (LONG) {
-      if constexpr (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-      else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    }
-    if (warp == 8) {
-      // ---- producer: all lanes walk, lane 0 waits and copies
-      int tile = 0;
-      bool ok = true;
-      int nf = 0;
-      for (bool more = line.first(s_first, f); ok && more; more = line.next(f), ++nf) {
-        w.start(line, f);
-        const int* unit = line.units + f.unit * kPxUnit;
-        int lead = -1;                                            // sequence of the first row of the group that has a table
-        for (int i = 0; lead < 0 && i < unit[4]; i += 32) {
-          const int mine = i + lane < unit[4] ? line.seq[unit[3] + i + lane] : -1;
-          const unsigned live = __ballot_sync(0xffffffffu, mine >= 0 && mine < a.n_slots);
-          if (live) lead = __shfl_sync(0xffffffffu, mine, __ffs(live) - 1);
-        }
-        int ids = 0;                                              // pages of the next 16 tiles, one a lane
-        bool bad = false;
-        for (int t = 0; ok && t < f.n_t; ++t, ++tile) {
-          if ((t & 15) == 0) {
-            PxWalk ahead = w;
-            int owner = -2, col = 0, n;
-            const int p = 2 * (f.t_lo + t) + lane;
-            if (p < ahead.shared) { owner = -1; col = p; }
-            else if (p < ahead.total && lane < 2 * (f.n_t - t)) {
-              ahead.row = w.row0 + PxLine::find(w.pages + w.row0, w.rows, w.pages[w.row0] + p - w.shared);
-              ahead.page(p, owner, col, n);
+  } else if (warp == 8) {
+    // ---- producer: the warp looks pages up 32 at a time, lane 0 waits and copies
+    int page = 0, nf = 0;
+    bool ok = true;
+    for (bool more = line.first(s_first, f); ok && more; more = line.next(f), ++nf) {
+      w.start(line, f);
+      const int* unit = line.units + f.unit * kPxUnit;
+      int lead = -1;                                            // sequence of the first row of the group that has a table
+      for (int i = 0; lead < 0 && i < unit[4]; i += 32) {
+        const int mine = i + lane < unit[4] ? line.seq[unit[3] + i + lane] : -1;
+        const unsigned live = __ballot_sync(0xffffffffu, mine >= 0 && mine < a.n_slots);
+        if (live) lead = __shfl_sync(0xffffffffu, mine, __ffs(live) - 1);
+      }
+      int ids = 0;
+      bool bad = false;
+      for (int p = f.lo; ok && p < f.end; ++p, ++page) {
+        const int i = (p - f.lo) & 31;
+        if (i == 0) {
+          const int mine = p + lane;
+          int seq = -1, col = mine;
+          if (mine < f.end) {
+            seq = lead;
+            if (mine >= w.shared) {
+              const int at = w.pages[w.row0] + mine - w.shared, row = w.row0 + PxLine::find(w.pages + w.row0, w.rows, at);
+              seq = line.seq[row];
+              col = w.shared + at - w.pages[row];
             }
-            const int seq = owner == -1 ? lead : owner >= 0 ? line.seq[w.row0 + owner] : -1;
-            ids = seq >= 0 ? a.table[(long)seq * a.max_pages + col] : 0;
-            const bool off = owner > -2 && lane < 2 * (f.n_t - t) && (ids < 0 || ids >= a.n_pages);
-            if (ids < 0 || ids >= a.n_pages) ids = 0;
-            if (off) raise_fault(a.fault, a.layer, FS_PAGE);
-            bad = bad || __any_sync(0xffffffffu, off);
           }
-          const int p0 = __shfl_sync(0xffffffffu, ids, 2 * t & 31), p1 = __shfl_sync(0xffffffffu, ids, (2 * t + 1) & 31);
-          const int n_p = min(2, w.total - 2 * (f.t_lo + t));
-          const int st = tile & 1;                              // both rings have two stages
-          const uint32_t par = (uint32_t)((tile >> 1) & 1);
-          if (lane == 0) {
+          ids = seq >= 0 ? a.table[(long)seq * a.max_pages + col] : 0;
+          const bool off = ids < 0 || ids >= a.n_pages;
+          if (off) { ids = 0; raise_fault(a.fault, a.layer, FS_PAGE); }
+          bad = bad || __any_sync(0xffffffffu, off);
+        }
+        const int block = __shfl_sync(0xffffffffu, ids, i) * a.n_kv + f.kvh, st = page & 3;
+        const uint32_t par = (uint32_t)((page >> 2) & 1);
+        if (lane == 0) {
 #pragma unroll
-            for (int kv = 0; ok && kv < 2; ++kv) {
-              if constexpr (Q8) ok = mbar_wait(&raw_empty[2 * kv + st], par ^ 1, abort_flag);
-              else ok = kv ? mbar_wait(&v_empty[st], par ^ 1, abort_flag) : mbar_wait(&k_empty[st], par ^ 1, abort_flag);
-              if (!ok) break;
-              // behind the first of these waits the softmax of six fragments ago is over: the flag may be used again
-              if (kv == 0 && (t == 0 || bad)) s_bad[nf & 7] = bad;
-              uint64_t* const full = Q8 ? &raw_full[2 * kv + st] : kv ? &v_full[st] : &k_full[st];
-              mbar_expect_tx(full, n_p * (Q8 ? RAW : NH * PAGE_BYTES));
-              for (int p = 0; p < n_p; ++p) {
-                const int block = (p ? p1 : p0) * a.n_kv + f.kvh;
-                if constexpr (Q8) {
-                  px_bulk(sRaw + ((st * 2 + kv) * 2 + p) * RAW, (kv ? a.v : a.k) + (long)block * RAW, RAW, full);
-                } else {
-                  for (int h = 0; h < NH; ++h) {
-                    uint8_t* dst = kv ? sV + st * TILE + (p * NH + h) * PAGE_BYTES : sK + st * TILE + h * kPxHalf + p * PAGE_BYTES;
-                    tma_load_2d(dst, kv ? &tma_v : &tma_k, h * 64, block * kPxPage, full);
-                  }
-                }
-              }
+          for (int kv = 0; ok && kv < 2; ++kv) {
+            if constexpr (Q8) ok = mbar_wait(&raw_empty[2 * st + kv], par ^ 1, abort_flag);
+            else ok = kv ? mbar_wait(&v_empty[st], par ^ 1, abort_flag) : mbar_wait(&k_empty[st], par ^ 1, abort_flag);
+            if (!ok) break;
+            // behind the first of these waits the softmax of a dozen pages ago is over: the flag may be used again
+            if (kv == 0 && (i == 0)) s_bad[nf & 15] = bad;
+            uint64_t* const full = Q8 ? &raw_full[2 * st + kv] : kv ? &v_full[st] : &k_full[st];
+            mbar_expect_tx(full, Q8 ? RAW : PAGE);
+            if constexpr (Q8) {
+              px_bulk(sRaw + (st * 2 + kv) * RAW, (kv ? a.v : a.k) + (long)block * RAW, RAW, full);
+            } else {
+#pragma unroll
+              for (int h = 0; h < NH; ++h) tma_load_2d((kv ? sV : sK) + st * PAGE + h * ATOM, kv ? &tma_v : &tma_k, h * 64, block * kPxPage, full);
             }
           }
-          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
         }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       }
-      if (*abort_flag) {
-        // copies of ours may still be landing: give them a bounded moment before the block's memory goes away
-        const unsigned long long t0 = globaltimer();
-        while (globaltimer() - t0 < 2000000ull) { }
-      }
-    } else if (warp <= 10) {
-      // ---- issuers: one for each tile of rows, so that neither's waits and look-ups hold the other's products up
-      const int x = px_uniform(warp - 9);
-      constexpr uint32_t idesc_s = px_idesc(128, 128, false), idesc_o = px_idesc(128, HEAD, true);
-      const uint32_t uS = (uint32_t)px_uniform((int)tS0), uO = uS + 256 + x * HEAD;
-      int tile = 0, n_q = 0, n_s = 0, n_o = 0, n_f = 0;         // tiles through the rings; query tiles, first and second products; fragments
-      bool ok = true;
-      for (int more = px_uniform(line.first(s_first, f)); ok && more; more = px_uniform(line.next(f)), ++n_f) {
-        w.start(line, f);
-        const int n_x = px_uniform(w.rows > rows_tile ? 2 : 1), n_t = px_uniform(f.n_t), t_lo = px_uniform(f.t_lo), pages = px_uniform(w.total);
-        const int shared = px_uniform(w.shared), tile0 = tile;
-        tile += n_t;
-        // S = Q K^T of tile t into score buffer b
-        auto first_product = [&](int t, int b) {
-          const int st = (tile0 + t) % ST;
-          ok = ok && mbar_wait_warp(&k_full[st], (uint32_t)(((tile0 + t) / ST) & 1), abort_flag);
+    }
+    if (*abort_flag) {
+      // copies of ours may still be landing: give them a bounded moment before the block's memory goes away
+      const unsigned long long t0 = globaltimer();
+      while (globaltimer() - t0 < 2000000ull) { }
+    }
+  } else if (warp == 9 || warp == 10) {
+    // ---- issuers: one for each tile of rows, so that neither's waits and look-ups hold the other's products up
+    const int x = px_uniform(warp - 9);
+    constexpr uint32_t idesc_s = px_idesc(128, kPxPage, false), idesc_o = px_idesc(128, HEAD, true);
+    const uint32_t uS = (uint32_t)px_uniform((int)tS0) + x * 128, uO = (uint32_t)px_uniform((int)tS0) + 256 + x * HEAD;
+    int page0 = 0, n_q = 0, n_s = 0, n_o = 0;                   // pages through the rings; query tiles, first and second products
+    bool ok = true;
+    for (int more = px_uniform(line.first(s_first, f)); ok && more; more = px_uniform(line.next(f))) {
+      w.start(line, f);
+      const int n_x = px_uniform(w.rows > rows_tile ? 2 : 1), n_p = px_uniform(f.end - f.lo), shared = px_uniform(w.shared - f.lo);
+      uint32_t own = 0;                                         // of the last 32 pages: whether this tile of rows takes part
+      bool asked = false;
+      uint32_t old = 0;
+      int t = 0;                                                // pages whose keys are done with
+      // S = Q K^T of the next pages: no further than their keys can have been fetched (the values of the pages between are still
+      // to be released here), and two of this tile's own ahead of its second products
+      auto first_products = [&](int at) {
+        while (ok && t < n_p && t < at + ST) {
+          bool part = n_x == 2 || x == 0;
+          if (t >= shared) {
+            PxWalk look = w;
+            int owner, col, n;
+            look.page(f.lo + t, owner, col, n);
+            w.row = look.row;
+            part = px_uniform((int)(px_tiles(owner, rows_tile, n_x) >> x & 1)) != 0;
+          }
+          if (part && n_s - n_o >= 2) return;
+          const int st = (page0 + t) % ST;
+          ok = mbar_wait_warp(&k_full[st], (uint32_t)(((page0 + t) / ST) & 1), abort_flag);
+          if (ok && part && !asked) ok = mbar_wait_warp(&q_full[x], (uint32_t)(n_q++ & 1), abort_flag);
           if (!ok) return;
+          own = (own & ~(1u << (t & 31))) | (uint32_t)part << (t & 31);
+          ++t;
+          if (!part) {
+            if (lane == 0) mbar_arrive(&k_empty[st]);
+            continue;
+          }
+          asked = true;
           tc_fence_after();
+          const uint32_t tS = uS + (n_s & 1) * 64;
 #pragma unroll
           for (int h = 0; h < NH; ++h) {
-            const uint64_t dq = umma_desc(smem_u32(sQ + x * TILE + h * kPxHalf)), dk = umma_desc(smem_u32(sK + st * TILE + h * kPxHalf));
+            const uint64_t dq = umma_desc(smem_u32(sQ + x * TILE + h * kPxHalf)), dk = umma_desc(smem_u32(sK + st * PAGE + h * ATOM));
 #pragma unroll
-            for (int k = 0; k < 4; ++k) umma_bf16(uS + b * 128, dq + (uint64_t)(k * 2), dk + (uint64_t)(k * 2), idesc_s, h + k > 0 ? 1u : 0u);
+            for (int k = 0; k < 4; ++k) umma_bf16(tS, dq + (uint64_t)(k * 2), dk + (uint64_t)(k * 2), idesc_s, h + k > 0 ? 1u : 0u);
           }
           // Two barriers, for every other job.  The softmax waits for its scores but not for every second product; when it comes
           // to a barrier, the job before the last is known to be complete (these scores were issued behind it), the last one is
           // not, and a wait by parity must not be two phases off.
           umma_commit(&s_full[2 * x + (n_s++ & 1)]);
           umma_commit(&k_empty[st]);
-        };
-        // O += P V of tile t out of buffer b, the halves as their probabilities arrive
-        auto second_product = [&](int t, int b, uint32_t old) {
-          const int st = (tile0 + t) % ST, half = 2 * x + (n_o & 1);
-          const uint32_t par = (uint32_t)((n_o >> 1) & 1);
-          ok = ok && mbar_wait_warp(&v_full[st], (uint32_t)(((tile0 + t) / ST) & 1), abort_flag) && mbar_wait_warp(&p_full[half], par, abort_flag);
-          if (!ok) return;
-          tc_fence_after();
-          const uint32_t tP = uS + b * 128;
-          const uint64_t dv = px_desc_v(smem_u32(sV + st * TILE)), dw = px_desc_v(smem_u32(sV + st * TILE + NH * PAGE_BYTES));
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16_ta(uO, tP + k * 8, dv + (uint64_t)(k * 128), idesc_o, k > 0 ? 1u : old);
-          ok = mbar_wait_warp(&p_full[4 + half], par, abort_flag);
-          if (!ok) return;
-          tc_fence_after();
-          if (2 * (t_lo + t) + 1 < pages) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) umma_bf16_ta(uO, tP + 32 + k * 8, dw + (uint64_t)(k * 128), idesc_o, 1u);
-          }
-          umma_commit(&pv_done[2 * x + (n_o++ & 1)]);
-          umma_commit(&v_empty[st]);
-        };
-        // a tile that this tile of rows takes no part in
-        auto pass = [&](int t) {
-          const int st = (tile0 + t) % ST;
-          const uint32_t par = (uint32_t)(((tile0 + t) / ST) & 1);
-          ok = ok && mbar_wait_warp(&k_full[st], par, abort_flag);
-          if (ok && lane == 0) mbar_arrive(&k_empty[st]);
-          ok = ok && mbar_wait_warp(&v_full[st], par, abort_flag);
-          if (ok && lane == 0) mbar_arrive(&v_empty[st]);
-        };
-        // both are through with what the last fragment left in the score buffers
-        if (lane == 0) mbar_arrive(&frag_start);
-        ok = mbar_wait_warp(&frag_start, (uint32_t)(n_f & 1), abort_flag);
-        if (n_x == 2) {
-          bool asked = false;
-          for (int t = 0; ok && t < n_t; ++t) {
-            bool part = true;
-            if (2 * (t_lo + t) + 2 > shared) {
-              int o0, o1, c0, c1, k0, k1;
-              w.tile(t_lo + t, o0, c0, k0, o1, c1, k1);
-              part = px_uniform((int)((px_tiles(o0, rows_tile, 2) | px_tiles(o1, rows_tile, 2)) >> x & 1)) != 0;
-            }
-            if (!part) { pass(t); continue; }
-            if (!asked) ok = mbar_wait_warp(&q_full[x], (uint32_t)(n_q & 1), abort_flag);
-            first_product(t, x);
-            second_product(t, x, asked);
-            n_q += !asked;
-            asked = true;
-          }
-        } else if (x == 0) {
-          // alone: both score buffers in turn, the scores of the tile after the next behind a tile's second product
-          ok = ok && mbar_wait_warp(&q_full[0], (uint32_t)(n_q++ & 1), abort_flag);
-          first_product(0, 0);
-          if (n_t > 1) first_product(1, 1);
-          for (int t = 0; ok && t < n_t; ++t) {
-            second_product(t, t & 1, t > 0);
-            if (t + 2 < n_t) first_product(t + 2, t & 1);
-          }
-        } else {
-          for (int t = 0; ok && t < n_t; ++t) pass(t);
         }
+      };
+      for (int at = 0; ok && at < n_p; ++at) {
+        first_products(at);
+        const int st = (page0 + at) % ST;
+        ok = ok && mbar_wait_warp(&v_full[st], (uint32_t)(((page0 + at) / ST) & 1), abort_flag);
+        if (!ok) break;
+        if (!(own >> (at & 31) & 1)) {
+          if (lane == 0) mbar_arrive(&v_empty[st]);
+          continue;
+        }
+        const int b = n_o & 1;
+        ok = mbar_wait_warp(&p_full[2 * x + b], (uint32_t)((n_o >> 1) & 1), abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t tP = uS + b * 64;
+        const uint64_t dv = px_desc_v(smem_u32(sV + st * PAGE));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_bf16_ta(uO, tP + k * 8, dv + (uint64_t)(k * 128), idesc_o, k > 0 ? 1u : old);
+        old = 1;
+        umma_commit(&pv_done[2 * x + b]);
+        umma_commit(&v_empty[st]);
+        ++n_o;
       }
+      page0 += n_p;
     }
-  } else {
-    if constexpr (LONG) {
-      if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-      else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    }
+  } else if (warp < 8) {
     // ---- softmax: a thread per query row ------------------------------------------------------------------
     const int x = warp >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;                          // row of the tile
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint32_t tO = tO0 + x * HEAD + lane_base;
-    int tile = 0, mine = 0, nf = 0;                             // tiles; jobs of this tile of rows; fragments
+    int page = 0, mine = 0, nf = 0;                             // pages; jobs of this tile of rows; fragments
     bool ok = true;
     for (bool more = line.first(s_first, f); ok && more; more = line.next(f), ++nf) {
       w.start(line, f);
@@ -668,142 +620,95 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
       };
       float m = -INFINITY, l = 0.f, to_log2 = 0.f;
       bool begun = false;
-      for (int t = 0; t < f.n_t; ++t, ++tile) {
-        int o0, c0, k0, o1, c1, k1;
-        w.tile(f.t_lo + t, o0, c0, k0, o1, c1, k1);
-        const unsigned who = px_tiles(o0, rows_tile, n_x) | px_tiles(o1, rows_tile, n_x);
+      for (int p = f.lo; p < f.end; ++p, ++page) {
+        int owner, col, held;
+        w.page(p, owner, col, held);
+        const unsigned who = px_tiles(owner, rows_tile, n_x);
         if (!(who >> x & 1)) continue;
-        const uint32_t tS = tS0 + (n_x == 2 ? x : t & 1) * 128 + lane_base;
-        // keys of either page that this thread's row attends to
-        const int n0 = o0 == my ? k0 : o0 == -1 ? min(kPxPage, max(0, n_keys - kPxPage * c0)) : 0;
-        const int n1 = o1 == my ? k1 : o1 == -1 ? min(kPxPage, max(0, n_keys - kPxPage * c1)) : 0;
-        const bool some = __any_sync(0xffffffffu, n0 + n1 > 0), all = __all_sync(0xffffffffu, n0 + n1 == 2 * kPxPage);
+        const int b = mine & 1;
+        const uint32_t tS = tS0 + x * 128 + b * 64 + lane_base;
+        // keys of the page that this thread's row attends to
+        const int n = owner == my ? held : owner == -1 ? min(kPxPage, max(0, n_keys - kPxPage * col)) : 0;
+        const bool some = __any_sync(0xffffffffu, n > 0), all = __all_sync(0xffffffffu, n == kPxPage);
         if (!begun) put_queries();
-        ok = mbar_wait_warp(&s_full[2 * x + (mine & 1)], (uint32_t)((mine >> 1) & 1), abort_flag);
+        ok = mbar_wait_warp(&s_full[2 * x + b], (uint32_t)((mine >> 1) & 1), abort_flag);
         if (!ok) break;
         tc_fence_after();
         if (!begun) to_log2 = busy ? s_scale[x][r] : 0.f;       // written in front of what these scores waited for
-        // A page's half of the probabilities is written.  Where a sequence ends inside the page, what lies behind may be anything, and
-        // zero times that must be zero: the first tile of rows that takes part clears it.
-        auto finish = [&](int p) {
-          const int n = p ? k1 : k0;
-          if (!Q8 && n > 0 && n < kPxPage && x == (who & 1 ? 0 : 1)) {
-            const int st = tile & 1;
-            ok = mbar_wait_warp(&v_full[st], (uint32_t)((tile >> 1) & 1), abort_flag);
-            if (!ok) return;
-            uint8_t* page = sV + st * TILE + p * NH * PAGE_BYTES;
-#pragma unroll
-            for (int h = 0; h < NH; ++h)
-              for (int i = n * 8 + r; i < kPxPage * 8; i += 128) *reinterpret_cast<uint4*>(page + h * PAGE_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
-            fence_async_smem();
-          }
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[4 * p + 2 * x + (mine & 1)]);
-        };
-        auto mask = [&](int c, uint32_t (&v)[32]) {
-          const int n = (c < 2 ? n0 : n1) - 32 * (c & 1);
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (i >= n) v[i] = 0xff800000u;                     // -inf
-        };
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum[4] = {0.f, 0.f, 0.f, 0.f}, mb = 0.f, corr = 1.f;
-        auto widen = [&](const uint32_t (&v)[32]) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 8)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mx4[j] = fmaxf(fmaxf(mx4[j], __uint_as_float(v[i + j])), __uint_as_float(v[i + 4 + j]));
-        };
-        // the new maximum, and the output brought to it
-        auto settle = [&]() {
-          float m_new = fmaxf(m, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
-          if (m != -INFINITY && (m_new - m) * to_log2 <= kPxLazy) m_new = m;
-          mb = (m_new == -INFINITY) ? 0.f : m_new * to_log2;    // a row with no key yet keeps zeros
-          corr = (m == -INFINITY || m == m_new) ? 1.f : px_ex2(m * to_log2 - mb);
-          m = m_new;
-          if (begun && __any_sync(0xffffffffu, corr != 1.0f)) {
-            // scaled in tensor memory, behind the tile's last product
-            ok = mbar_wait_warp(&pv_done[2 * x + ((mine - 1) & 1)], (uint32_t)(((mine - 1) >> 1) & 1), abort_flag);
-            if (!ok) return;
-            tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < HEAD / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(tO + c * 32, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-              tmem_st32(tO + c * 32, o);
-            }
-          }
-        };
-        auto powers = [&](const uint32_t (&v)[32], uint32_t (&pk)[16]) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            uint32_t e0, e1;
-            asm("{\n\t.reg .b64 rs, rk, rm, rr;\n\t"
-                "mov.b64 rs, {%2, %3};\n\tmov.b64 rk, {%4, %4};\n\tmov.b64 rm, {%5, %5};\n\t"
-                "fma.rn.f32x2 rr, rs, rk, rm;\n\tmov.b64 {%0, %1}, rr;\n\t}"
-                : "=r"(e0), "=r"(e1) : "r"(v[i]), "r"(v[i + 1]), "f"(to_log2), "f"(-mb));
-            const float p0 = px_ex2(__uint_as_float(e0)), p1 = px_ex2(__uint_as_float(e1));
-            sum[i & 2] += p0; sum[(i & 2) + 1] += p1;
-            pk[i >> 1] = px_pack(p0, p1);
-          }
-        };
-        if (!some) {
-          // no row of this warp attends to these pages
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pk[i] = 0;
-#pragma unroll 1
-          for (int c = 0; ok && c < 4; ++c) {
-            px_st16(tS + 16 * c, pk);
-            if (c & 1) finish(c >> 1);
-          }
-        } else if constexpr (LONG) {
-          // all of a row's scores in registers, straight code
-          uint32_t v[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(tS + 32 * c, v[c]);
+        uint32_t v[2][32];
+        float corr = 1.f, sum[4] = {0.f, 0.f, 0.f, 0.f};
+        if (some) {
+          tmem_ld32(tS, v[0]);
+          tmem_ld32(tS + 32, v[1]);
           tmem_ld_wait();
           if (!all) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) mask(c, v[c]);
+            for (int i = 0; i < 64; ++i)
+              if (i >= n) v[i >> 5][i & 31] = 0xff800000u;      // -inf
+          }
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top[j] = fmaxf(fmaxf(top[j], __uint_as_float(v[0][i + j])), __uint_as_float(v[1][i + j]));
+          float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+          if (m != -INFINITY && (m_new - m) * to_log2 <= kPxLazy) m_new = m;
+          const float mb = (m_new == -INFINITY) ? 0.f : m_new * to_log2;      // a row with no key yet keeps zeros
+          corr = (m == -INFINITY || m == m_new) ? 1.f : px_ex2(m * to_log2 - mb);
+          m = m_new;
+          if (begun && __any_sync(0xffffffffu, corr != 1.0f)) {
+            // the output is scaled in tensor memory, behind the tile's last product
+            ok = mbar_wait_warp(&pv_done[2 * x + (b ^ 1)], (uint32_t)(((mine - 1) >> 1) & 1), abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HEAD / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(tO + c * 16, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              px_st16(tO + c * 16, o);
+            }
           }
 #pragma unroll
-          for (int c = 0; c < 4; ++c) widen(v[c]);
-          settle();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             uint32_t pk[16];
-            powers(v[c], pk);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              uint32_t e0, e1;
+              asm("{\n\t.reg .b64 rs, rk, rm, rr;\n\t"
+                  "mov.b64 rs, {%2, %3};\n\tmov.b64 rk, {%4, %4};\n\tmov.b64 rm, {%5, %5};\n\t"
+                  "fma.rn.f32x2 rr, rs, rk, rm;\n\tmov.b64 {%0, %1}, rr;\n\t}"
+                  : "=r"(e0), "=r"(e1) : "r"(v[c][i]), "r"(v[c][i + 1]), "f"(to_log2), "f"(-mb));
+              const float p0 = px_ex2(__uint_as_float(e0)), p1 = px_ex2(__uint_as_float(e1));
+              sum[i & 2] += p0; sum[(i & 2) + 1] += p1;
+              pk[i >> 1] = px_pack(p0, p1);
+            }
             px_st16(tS + 16 * c, pk);
-            if (ok && (c & 1)) finish(c >> 1);
           }
-        } else {
-          // read twice, 32 at a time
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            tmem_ld32(tS + 32 * c, v);
-            tmem_ld_wait();
-            if (!all) mask(c, v);
-            widen(v);
-          }
-          settle();
-#pragma unroll 1
-          for (int c = 0; ok && c < 4; ++c) {
-            uint32_t v[32], pk[16];
-            tmem_ld32(tS + 32 * c, v);
-            tmem_ld_wait();
-            if (!all) mask(c, v);
-            powers(v, pk);
-            px_st16(tS + 16 * c, pk);
-            if (c & 1) finish(c >> 1);
-          }
+        } else {                                                // no row of this warp attends to this page
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pk[i] = 0;
+          px_st16(tS, pk);
+          px_st16(tS + 16, pk);
         }
-        if (!ok) break;
+        if (!Q8 && held < kPxPage) {
+          // A sequence ends inside the page: what lies behind may be anything, and zero times that must be zero.  The page is one
+          // row's, so its tile of rows alone reads it.
+          const int st = page & 3;
+          ok = mbar_wait_warp(&v_full[st], (uint32_t)((page >> 2) & 1), abort_flag);
+          if (!ok) break;
+#pragma unroll
+          for (int h = 0; h < NH; ++h)
+            for (int i = held * 8 + r; i < kPxPage * 8; i += 128) *reinterpret_cast<uint4*>(sV + st * PAGE + h * ATOM + i * 16) = make_uint4(0, 0, 0, 0);
+          fence_async_smem();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * x + b]);
         l = l * corr + ((sum[0] + sum[2]) + (sum[1] + sum[3]));
         begun = true;
         ++mine;
@@ -831,7 +736,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
         }
         // a fragment that met a page the pool does not have gives NaN to all that it serves; a row whose every score is NaN
         // has no maximum, but a sum that tells
-        const bool lost = l != l || (*(volatile int*)&s_bad[nf & 7] != 0 && m != -INFINITY);
+        const bool lost = l != l || (*(volatile int*)&s_bad[nf & 15] != 0 && m != -INFINITY);
         if (r < live)
           __stcg(reinterpret_cast<float2*>(part - r + HEAD / 4 * a.pitch) + r,
                  lost ? make_float2(0.f, __int_as_float(0x7fc00000)) : make_float2(m == -INFINITY ? m : m * to_log2, l));
@@ -874,7 +779,7 @@ __global__ void __launch_bounds__(256, 4) prefix_join_kernel(const PrefixArgs a)
   int n_f = 0;
   long id = 0;
   if (n > 0) {
-    const unsigned T = (unsigned)(a.n_kv * sc.x), n_cta = min((unsigned)a.n_cta, T);
+    const unsigned T = (unsigned)(a.n_kv * sc.x), n_cta = px_ctas(a, T);
     auto cta_of = [&](int at) { return (int)(((unsigned)(at + 1) * n_cta - 1) / T); };
     const int c0 = cta_of(kvh * sc.x + sc.y);
     n_f = cta_of(kvh * sc.x + sc.z - 1) - c0 + 1;
@@ -950,7 +855,7 @@ __global__ void __launch_bounds__(256, 4) prefix_join_kernel(const PrefixArgs a)
 
 using namespace bl;
 
-template <int HEAD, bool Q8, bool LONG>
+template <int HEAD, bool Q8>
 static int prefix_go(const PrefixArgs& a, cudaStream_t st) {
   CUtensorMap mk = {}, mv = {};
   if (!Q8) {
@@ -964,12 +869,12 @@ static int prefix_go(const PrefixArgs& a, cudaStream_t st) {
   }
   static PerDevice limit;
   if (limit.due()) {
-    const cudaError_t e = cudaFuncSetAttribute(prefix_attn_kernel<HEAD, Q8, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    const cudaError_t e = cudaFuncSetAttribute(prefix_attn_kernel<HEAD, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                px_smem(HEAD, Q8, kPxMaxRows, kPxMaxRows));
     if (e != cudaSuccess) return (int)e;
     limit.mark();
   }
-  const cudaError_t e = launch(prefix_attn_kernel<HEAD, Q8, LONG>, dim3(a.n_cta), dim3(px_threads(Q8)), (size_t)px_smem(HEAD, Q8, a.n_units, a.M), st, mk, mv, a);
+  const cudaError_t e = launch(prefix_attn_kernel<HEAD, Q8>, dim3(a.n_cta), dim3(px_threads(Q8)), (size_t)px_smem(HEAD, Q8, a.n_units, a.M), st, mk, mv, a);
   if (e != cudaSuccess) return (int)e;
   // few rows: a block for 32 values of a head, so that more of its fragments are in flight; many: as much of it as 256 threads hold
   int z = HEAD / 32;
@@ -997,7 +902,7 @@ long bl_prefix_work_bytes(int head, int n_q, int n_kv, int n_units, int unit_row
 struct PrefixCall {
   const float* q; const void* k_cache; const void* v_cache; const int* row_pos; const int* row_seq; const int* block_table;
   const int* meta; void* work; void* out; unsigned* fault; cudaStream_t stream;
-  int n_slots, max_pages, n_pages, head, n_q, n_kv, M, n_units, unit_rows, kv_q8, n_cta, layer, shared_tiles;     // tiles of 128 shared keys of all units of a KV head
+  int n_slots, max_pages, n_pages, head, n_q, n_kv, M, n_units, unit_rows, kv_q8, n_cta, layer;
 };
 
 int bl_prefix_attention(const PrefixCall* call) {
@@ -1017,17 +922,8 @@ int bl_prefix_attention(const PrefixCall* call) {
   a.sched = (int4*)work;
   a.part = (float4*)((uint8_t*)work + kPxMaxRows * 16);
   a.part_bytes = prefix_slots(head, n_q / n_kv, n_kv, n_units, unit_rows, n_cta, a.slot, a.slot_tiles, a.pitch);
-  // four tiles of shared keys a CTA or more
-  const bool is_long = (long)n_kv * p.shared_tiles >= 4L * n_cta;
-  auto go = [&](auto head_, auto q8_) {
-    constexpr int HEAD = decltype(head_)::value;
-    constexpr bool Q8 = decltype(q8_)::value;
-    return is_long ? prefix_go<HEAD, Q8, true>(a, st) : prefix_go<HEAD, Q8, false>(a, st);
-  };
-  const std::integral_constant<int, 128> h128;
-  const std::integral_constant<int, 64> h64;
-  if (p.kv_q8) return head == 128 ? go(h128, std::true_type()) : go(h64, std::true_type());
-  return head == 128 ? go(h128, std::false_type()) : go(h64, std::false_type());
+  if (p.kv_q8) return head == 128 ? prefix_go<128, true>(a, st) : prefix_go<64, true>(a, st);
+  return head == 128 ? prefix_go<128, false>(a, st) : prefix_go<64, false>(a, st);
 }
 
 }  // extern "C"

@@ -17,7 +17,7 @@ from ._lib import check, cuda, raw_stream
 from .decode import sm_count
 
 _entry = None
-_CALL = struct.Struct("11P13i")                       # PrefixCall in the source
+_CALL = struct.Struct("11P12i")                       # PrefixCall in the source
 
 
 class PrefixPlan:
@@ -58,7 +58,6 @@ class PrefixPlan:
             units += [(first + i, min(2 * per, n - i), p, first, n) for i in range(0, n, 2 * per)]
             first += n
         self.n_units, self.unit_rows = len(units), max(u[1] for u in units)
-        self.shared_tiles = sum((u[2] + 127) // 128 for u in units)
         self.meta = torch.tensor(rows + units, dtype=torch.int32).to(self.device)
         self.n_cta = min(160, sm_count(self.device)) if self.device.type == "cuda" else 1
         fn = cuda().bl_prefix_work_bytes
@@ -107,6 +106,6 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     code = _entry(_CALL.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), row_pos.data_ptr(), row_seq.data_ptr(),
                              block_table.data_ptr(), plan.meta_ptr, plan.work_ptr, out.data_ptr(),
                              fault.data_ptr() if fault is not None else 0, raw_stream(index), table[0], table[1], shape[0], head,
-                             plan.n_q, n_kv, rows, plan.n_units, plan.unit_rows, q8, plan.n_cta, layer, plan.shared_tiles))
+                             plan.n_q, n_kv, rows, plan.n_units, plan.unit_rows, q8, plan.n_cta, layer))
     if code:
         check(code, "bl_prefix_attention")
