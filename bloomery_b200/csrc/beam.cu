@@ -520,6 +520,32 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(const ReorderArgs a) 
   if (a.v_row) copy_heads(a.v + dst * a.v_row, a.v + src * a.v_row, part * (int)a.v_row, kBeamPage * (int)a.v_row, a.n_kv);
 }
 
+// ---- the next pass ------------------------------------------------------------------------------------------
+struct BeamAdvanceArgs {
+  int* tokens; int* row_pos; int* row_seq; int* held; int* hist; int* count;
+  const int* slots; const int* parent; const int* token; const int* done; const float* scores;
+  int G, B, cap;
+};
+
+// One block: the rows of the next pass, and the choice written down.  A finished or missing beam is a row without a sequence.
+__global__ void __launch_bounds__(256) beam_advance_kernel(const BeamAdvanceArgs a) {
+  pdl_wait();
+  pdl_launch();
+  const int R = a.G * a.B, step = *a.count;
+  for (int i = threadIdx.x; i < R; i += blockDim.x) {
+    a.tokens[i] = a.token[i];
+    a.row_pos[i] += 1;
+    a.row_seq[i] = a.done[i] || a.scores[i] == -INFINITY ? -1 : a.slots[i];
+    if (step < a.cap) {
+      a.hist[(long)step * 2 * R + i] = a.parent[i];
+      a.hist[((long)step * 2 + 1) * R + i] = a.token[i];
+    }
+  }
+  for (int g = threadIdx.x; g < a.G; g += blockDim.x) a.held[g] += 1;
+  __syncthreads();
+  if (threadIdx.x == 0) *a.count = step + 1;
+}
+
 }  // namespace bl
 
 using namespace bl;
@@ -593,6 +619,14 @@ int bl_beam_reorder(const BeamReorderCall* call) {
   BL_REQUIRE(k_row % 4 == 0 && v_row % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0, BL_ERR_ALIGN);
   ReorderArgs a{(uint8_t*)k, (uint8_t*)v, k_row, v_row, n_pages, n_kv, G, B, n_slots, max_pages, table, table_out, slots, parent, held, fault};
   return (int)launch(beam_reorder_kernel, dim3(G * B, n_layer), dim3(256), 0, st, a);
+}
+
+// tokens, row_pos, row_seq [G * B] of a pass; held [G]; hist [cap][2][G * B] parents and tokens of each step, count its number.
+int bl_beam_advance(int* tokens, int* row_pos, int* row_seq, int* held, int* hist, int cap, int* count, const int* slots, const int* parent,
+                    const int* token, const int* done, const float* scores, int G, int B, cudaStream_t st) {
+  BL_REQUIRE(G >= 1 && B >= 1 && cap >= 0 && (long)G * B <= 65535, BL_ERR_SHAPE);
+  BeamAdvanceArgs a{tokens, row_pos, row_seq, held, hist, count, slots, parent, token, done, scores, G, B, cap};
+  return (int)launch(beam_advance_kernel, dim3(1), dim3(256), 0, st, a);
 }
 
 }  // extern "C"

@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from ..runtime.kv import PAGE
-from ._lib import check, cuda, raw_stream
+from ._lib import I, check, cuda, p, raw_stream, stream
 from .decode import sm_count
 
 MAX_BEAMS = 64
@@ -123,3 +123,10 @@ def beam_reorder(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, table_ou
                                                 shape[2], tables[0], tables[1], G, B, sm_count(k.device)))
     if code:
         check(code, "bl_beam_reorder")
+
+
+def beam_advance(tokens, row_pos, row_seq, held, hist, count, slots, parent, token, done, scores, G: int, B: int) -> None:
+    """The rows of the next pass out of a choice: tokens, positions one further, sequences (-1 for finished and missing beams);
+    ``held`` [G] one more; ``hist`` int32 [cap, 2, G * B] takes the parents and tokens of step ``count``."""
+    check(cuda().bl_beam_advance(p(tokens), p(row_pos), p(row_seq), p(held), p(hist), I(hist.shape[0]), p(count), p(slots), p(parent),
+                                 p(token), p(done), p(scores), I(G), I(B), stream()), "bl_beam_advance")

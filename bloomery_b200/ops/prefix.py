@@ -27,20 +27,15 @@ class PrefixPlan:
     one plan follow each other on one stream."""
 
     def __init__(self, group_rows: Sequence[int], prefix_len: Sequence[int], n_q: int, n_kv: int, head: int, device):
-        if len(group_rows) != len(prefix_len) or not group_rows:
-            raise ValueError("a prefix length for every group, and one group at least")
-        if any(r < 1 for r in group_rows):
-            raise ValueError("a group has one row at least")
-        if any(n < 0 or n % PAGE for n in prefix_len):
-            raise ValueError(f"shared positions are whole pages of {PAGE}")
+        if not group_rows or any(r < 1 for r in group_rows):
+            raise ValueError("one group at least, and one row in each")
         if head not in (64, 128):
             raise ValueError(f"heads of 64 or 128 values, not {head}")
         if n_kv < 1 or n_q < 1 or n_q % n_kv or n_q // n_kv > 16:
             raise ValueError(f"{n_q} query heads over {n_kv} key heads: 1 to 16 each")
         self.n_q, self.n_kv, self.head = n_q, n_kv, head
-        self.group_rows, self.prefix_len = list(group_rows), list(prefix_len)
+        self.group_rows = list(group_rows)
         self.rows = sum(group_rows)
-        self.max_prefix = max(prefix_len)
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
@@ -48,22 +43,35 @@ class PrefixPlan:
         self.q_shape, self.out_shape = (sum(group_rows), n_q, head), (sum(group_rows), n_q * head)
         if self.rows > 512:
             raise ValueError("at most 512 rows")
-        # units: rows of a group that read all of their keys together, as many as two tiles of 128 (row, head) pairs of a key
-        # head hold
-        G = n_q // n_kv
-        per = 128 // G
-        rows, units, first = [], [], 0
-        for n, p in zip(group_rows, prefix_len):
-            rows += [(first, n, p, len(units) + i // (2 * per), i % (2 * per) // per * 128 + i % per * G) for i in range(n)]
-            units += [(first + i, min(2 * per, n - i), p, first, n) for i in range(0, n, 2 * per)]
-            first += n
-        self.n_units, self.unit_rows = len(units), max(u[1] for u in units)
-        self.meta = torch.tensor(rows + units, dtype=torch.int32).to(self.device)
+        rows = self._meta(prefix_len)
+        self.n_units, self.unit_rows = len(rows) - self.rows, max(u[1] for u in rows[self.rows:])
+        self.meta = torch.tensor(rows, dtype=torch.int32).to(self.device)
         self.n_cta = min(160, sm_count(self.device)) if self.device.type == "cuda" else 1
         fn = cuda().bl_prefix_work_bytes
         fn.restype = ctypes.c_long
         self.work = torch.empty(fn(head, n_q, n_kv, self.n_units, self.unit_rows, self.n_cta), dtype=torch.uint8, device=self.device)
         self.meta_ptr, self.work_ptr = self.meta.data_ptr(), self.work.data_ptr()
+
+    def _meta(self, prefix_len: Sequence[int]):
+        if len(prefix_len) != len(self.group_rows):
+            raise ValueError("a prefix length for every group")
+        if any(n < 0 or n % PAGE for n in prefix_len):
+            raise ValueError(f"shared positions are whole pages of {PAGE}")
+        self.prefix_len, self.max_prefix = list(prefix_len), max(prefix_len)
+        # units: rows of a group that read all of their keys together, as many as two tiles of 128 (row, head) pairs of a key
+        # head hold
+        G = self.n_q // self.n_kv
+        per = 128 // G
+        rows, units, first = [], [], 0
+        for n, p in zip(self.group_rows, prefix_len):
+            rows += [(first, n, p, len(units) + i // (2 * per), i % (2 * per) // per * 128 + i % per * G) for i in range(n)]
+            units += [(first + i, min(2 * per, n - i), p, first, n) for i in range(0, n, 2 * per)]
+            first += n
+        return rows + units
+
+    def set_prefix(self, prefix_len: Sequence[int]) -> None:
+        """Other shared positions for the same groups; graphs captured with the plan take them up."""
+        self.meta.copy_(torch.tensor(self._meta(prefix_len), dtype=torch.int32))
 
 
 def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, row_pos: torch.Tensor, row_seq: torch.Tensor,

@@ -26,6 +26,7 @@ import torch
 
 from ..ops import decode as K
 from ..ops import gemm as G
+from ..ops.prefix import prefix_attention
 
 TILE = 32
 BUCKETS = (16, 32, 64)
@@ -133,6 +134,7 @@ class BatchDecode:
         # the engine's own stream: its 8-row passes and prompts and these passes touch the same KV pages in order
         self._stream = getattr(engine, "_stream", None) or torch.cuda.Stream(device=dev)
         self._side = [torch.cuda.Stream(device=dev), torch.cuda.Stream(device=dev)]
+        self.prefix = None                      # a PrefixPlan: groups of rows read the positions that they share once for all
         from .timing import PromptTiming
         self.timing = PromptTiming()            # arm() it and call enqueue() eagerly for per-unit milliseconds of a pass
 
@@ -305,6 +307,10 @@ class BatchDecode:
         K.qk_norm_rope_append(self.qkv, w.f.get(b + "attn_q_norm.weight"), w.f.get(b + "attn_k_norm.weight"), e.inv_freq,
                               s.rms_eps, q_scale, s.head_dim, s.n_q, s.n_kv, M, self.row_pos, self.row_seq, kvp.table,
                               kvp.n_pages, kvp.k[il], kvp.v[il], self.q_out, e.fault, il, kv_q8=e.kv_q8); n += 1
+        if self.prefix is not None:
+            prefix_attention(self.q_out[:M], kvp.k[il], kvp.v[il], self.row_pos, self.row_seq, kvp.table, self.prefix,
+                             self.attn_bf[:M], e.fault, il)
+            return n + 2
         K.flash_decode_bf16(self.q_out, kvp.k[il], kvp.v[il], self.row_pos, self.row_seq, kvp.table, kvp.n_pages, s.head_dim,
                             s.n_q, s.n_kv, M, self.n_segs[M], e.slot_ctx, self.part_ml, self.part_acc, self.attn_bf, e.fault,
                             il, kv_q8=e.kv_q8); n += 2
