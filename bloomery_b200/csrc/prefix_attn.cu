@@ -45,12 +45,14 @@ struct PrefixArgs {
   unsigned* fault; int layer;
   const int* units;               // [n_units][first row, rows, shared positions, first row of the group, rows of the group]
   int n_units, n_cta;
-  int4* sched;                    // [M] pages of a KV head; running sums of the row's unit; keys: of this call, for the joining launch
+  int4* sched;                    // [M][pages of a KV head, of the units before, shared, keys; first own page, own pages, unit, place]: of this
+                                  // call, for the joining launch
   // [fragment][tiles of rows][outputs [HEAD / 4][pitch], then maxima and sums [pitch] of 8 bytes]: `slot` float4 a tile.  What lies
   // close together needs few address translations.
   float4* part;
   int slot, slot_tiles, pitch;
   long part_bytes;
+  int cols, items, sets, inv_items, inv_G;              // of the joining launch: see there
 };
 constexpr int kPxMeta = 5, kPxUnit = 5;
 
@@ -146,6 +148,12 @@ struct PxLine {
     n_units = a.n_units;
     cta = blockIdx.x;
     for (int i = threadIdx.x; i < n_units * kPxUnit; i += blockDim.x) units[i] = a.units[i];
+    const bool small = a.M <= 32;                               // then one warp has all in its registers
+    int unit[3] = {0, 0, 0}, own = 0, n_keys = 0;
+    if (small && (int)threadIdx.x < n_units) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) unit[i] = a.units[threadIdx.x * kPxUnit + i];
+    }
     for (int m = threadIdx.x; m < a.M; m += blockDim.x) {
       const int shared = a.meta[m * kPxMeta + 2], sq = a.row_seq[m];
       bool bad;
@@ -153,31 +161,80 @@ struct PxLine {
       if (bad && blockIdx.x == 0) raise_fault(a.fault, a.layer, FS_KEY_COUNT);
       keys[m] = n;
       seq[m] = sq;
-      pages[m + 1] = max(0, n - shared + kPxPage - 1) / kPxPage;
+      n_keys = n;
+      own = max(0, n - shared + kPxPage - 1) / kPxPage;
+      pages[m + 1] = own;
     }
-    __syncthreads();
-    if (threadIdx.x < 32) {
-      running(pages, a.M);
-      __syncwarp();
-      for (int u = threadIdx.x; u < n_units; u += 32) {
-        const int* unit = units + u * kPxUnit;
-        int live = 0;                                           // a unit without a live row reads nothing
-        for (int m = unit[0]; !live && m < unit[0] + unit[1]; ++m) live = keys[m];
-        cum[u + 1] = live ? unit[2] / kPxPage + pages[unit[0] + unit[1]] - pages[unit[0]] : 0;
-      }
-      __syncwarp();
-      running(cum, n_units);
-      __syncwarp();
-      if (threadIdx.x == 0) {
-        S = cum[n_units];
+    if (small) {
+      if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        auto scan = [&](int v) {
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += up; }
+          return v;
+        };
+        const int sum = scan(own);
+        const unsigned live = __ballot_sync(0xffffffffu, n_keys > 0);
+        const int upto = __shfl_sync(0xffffffffu, sum, (unit[0] + unit[1] - 1) & 31), prev = __shfl_sync(0xffffffffu, sum, (unit[0] - 1) & 31);
+        const int before = unit[0] ? prev : 0;
+        const unsigned mine = unit[1] >= 32 ? 0xffffffffu : (1u << unit[1]) - 1;
+        const int total = scan((live >> unit[0] & mine) != 0 ? unit[2] / kPxPage + upto - before : 0);
+        S = __shfl_sync(0xffffffffu, total, 31);
         const unsigned T = (unsigned)(a.n_kv * S), n = px_ctas(a, T);
         g = (unsigned)cta < n ? (int)((unsigned)cta * T / n) : 0;
         end = (unsigned)cta < n ? (int)((unsigned)(cta + 1) * T / n) : 0;
         PxFrag f = {};
-        const int some = next(f);
-        const int4* from = reinterpret_cast<const int4*>(&f);
-        s_first[0] = make_int4(S, g, end, some);
-        s_first[1] = from[0]; s_first[2] = from[1]; s_first[3] = from[2];
+        const bool some = g < end;
+        if (some) {
+          f.kvh = (int)((unsigned)g / (unsigned)S);
+          const int rem = g - f.kvh * S;
+          f.unit = __popc(__ballot_sync(0xffffffffu, total <= rem));            // units that end before
+          const int last = __shfl_sync(0xffffffffu, total, f.unit);
+          f.lo = rem - (f.unit ? __shfl_sync(0xffffffffu, total, f.unit - 1) : 0);
+          f.end = f.lo + min(last - rem, end - g);
+          f.id = f.kvh * n_units + f.unit + cta;
+          f.row0 = __shfl_sync(0xffffffffu, unit[0], f.unit);
+          f.rows = __shfl_sync(0xffffffffu, unit[1], f.unit);
+          f.shared = __shfl_sync(0xffffffffu, unit[2], f.unit) / kPxPage;
+          const int skip = f.lo - f.shared + __shfl_sync(0xffffffffu, before, f.unit);
+          f.row = f.lo > f.shared ? __popc(__ballot_sync(0xffffffffu, sum <= skip)) : f.row0;
+          g += f.end - f.lo;
+        }
+        if (lane < a.M) pages[lane + 1] = sum;
+        if (lane < n_units) cum[lane + 1] = total;
+        if (lane == 0) {
+          pages[0] = 0;
+          cum[0] = 0;
+          const int4* from = reinterpret_cast<const int4*>(&f);
+          s_first[0] = make_int4(S, g, end, some);
+          s_first[1] = from[0]; s_first[2] = from[1]; s_first[3] = from[2];
+        }
+      }
+    } else {
+      __syncthreads();
+      if (threadIdx.x < 32) {
+        running(pages, a.M);
+        __syncwarp();
+        for (int u = threadIdx.x; u < n_units; u += 32) {
+          const int* unit = units + u * kPxUnit;
+          int live = 0;                                           // a unit without a live row reads nothing
+          for (int m = unit[0]; !live && m < unit[0] + unit[1]; ++m) live = keys[m];
+          cum[u + 1] = live ? unit[2] / kPxPage + pages[unit[0] + unit[1]] - pages[unit[0]] : 0;
+        }
+        __syncwarp();
+        running(cum, n_units);
+        __syncwarp();
+        if (threadIdx.x == 0) {
+          S = cum[n_units];
+          const unsigned T = (unsigned)(a.n_kv * S), n = px_ctas(a, T);
+          g = (unsigned)cta < n ? (int)((unsigned)cta * T / n) : 0;
+          end = (unsigned)cta < n ? (int)((unsigned)(cta + 1) * T / n) : 0;
+          PxFrag f = {};
+          const int some = next(f);
+          const int4* from = reinterpret_cast<const int4*>(&f);
+          s_first[0] = make_int4(S, g, end, some);
+          s_first[1] = from[0]; s_first[2] = from[1]; s_first[3] = from[2];
+        }
       }
     }
     __syncthreads();
@@ -186,8 +243,9 @@ struct PxLine {
     // for the launch that joins the fragments
     if (blockIdx.x == 0)
       for (int m = threadIdx.x; m < a.M; m += blockDim.x) {
-        const int u = a.meta[m * kPxMeta + 3];
-        a.sched[m] = make_int4(S, cum[u], cum[u + 1], keys[m]);
+        const int u = a.meta[m * kPxMeta + 3], shared = units[u * kPxUnit + 2] / kPxPage;
+        a.sched[2 * m] = make_int4(S, cum[u], shared, keys[m]);
+        a.sched[2 * m + 1] = make_int4(shared + pages[m] - pages[units[u * kPxUnit]], pages[m + 1] - pages[m], u, a.meta[m * kPxMeta + 4]);
       }
   }
   __device__ __forceinline__ bool first(const int4* s_first, PxFrag& f) const {
@@ -325,7 +383,7 @@ __device__ __forceinline__ void px_prefetch(const void* p) { asm volatile("prefe
 // a line of every 2 MB of the scratch
 __device__ __forceinline__ void px_touch_scratch(const PrefixArgs& a) {
   for (long at = (long)threadIdx.x << 21; at < a.part_bytes; at += (long)blockDim.x << 21) px_prefetch(reinterpret_cast<const uint8_t*>(a.part) + at);
-  if (threadIdx.x < 32) px_prefetch(a.sched + threadIdx.x);
+  if (threadIdx.x < 32) px_prefetch(a.sched + 2 * threadIdx.x);
 }
 
 // Bounds of 512 threads in both forms, that is 128 registers a lane: blocks of the joining launch fit beside the 384 threads of f16
@@ -607,7 +665,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
             }
           }
         };
-        if (live > 64) {
+        if (live > 16) {
 #pragma unroll 1
           for (int i0 = quarter; i0 < live; i0 += 32) some_rows(i0, std::integral_constant<int, 8>());
         } else {
@@ -754,85 +812,89 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
   if (threadIdx.x == 0 && s_abort) raise_fault(a.fault, a.layer, FS_WAIT_TIMEOUT);
 }
 
-// Joins the fragments of a row's heads: grid (n_kv, M, HEAD / 32), 256 threads.  One round trip brings the maxima and sums of all
-// fragments, a warp for a head; the outputs follow, a thread for four values of a head and every `sets`-th fragment.
+// Joins the fragments of a row's heads: grid (n_kv, M, parts of the head), 256 threads.  A row has the fragments that cover its
+// shared pages and those that cover its own; other rows' are left out.  One round trip brings the maxima and sums, a warp for a
+// head, and the outputs, a thread for four values of a head and every `sets`-th fragment (of `cols` such columns, `items` in all).
 constexpr int kPxMaxCtas = 160;
 
 template <int HEAD, bool Q8>
 __global__ void __launch_bounds__(256, 4) prefix_join_kernel(const PrefixArgs a) {
-  __shared__ float s_w[kPxMaxCtas * 16], s_inv[16];
+  __shared__ float s_w[kPxMaxCtas][16], s_inv[16];
   __shared__ float4 s_o[256];
   const int kvh = blockIdx.x, m = blockIdx.y, G = a.n_q / a.n_kv, tid = threadIdx.x, lane = tid & 31;
-  // lengths and tables are older than the launch in front, which started behind what wrote them
+  const int set = tid * a.inv_items >> 16, item = tid - set * a.items, col = item * a.inv_G >> 16, h = item - col * G, c = blockIdx.z * a.cols + col;
+  // lengths are older than the launch in front, which started behind what wrote them
   bool bad;
   px_keys(a, m, bad);
-  const int* meta = a.meta + m * kPxMeta;
-  const int unit = meta[3], x = meta[4] / 128, lane0 = meta[4] % 128;
-  const int cols = HEAD / 4 / gridDim.z, items = G * cols;                      // float4 of a head, of the block: 256 at most
-  const int sets = 256 / items, set = tid / items, h = tid % G, c = blockIdx.z * cols + tid % items / G;
   px_touch_scratch(a);
   if (tid == 0) px_prefetch(a.out + ((long)m * a.n_q + kvh * G) * HEAD);
   pdl_wait();
   pdl_launch();
-  const int4 sc = __ldcg(a.sched + m);                                          // pages of a KV head, of the units before and up to this one; keys
-  const int n = sc.w;
-  int n_f = 0;
-  long id = 0;
+  const int4 s0 = __ldcg(a.sched + 2 * m), s1 = __ldcg(a.sched + 2 * m + 1);
+  const int n = s0.w, shared = s0.z, own = s1.x, n_own = s1.y, x = s1.w >> 7, lane0 = s1.w & 127;
+  int f1 = 0, n1 = 0, f2 = 0, n2 = 0;                           // first CTA and count: of the shared pages, of the row's own
   if (n > 0) {
-    const unsigned T = (unsigned)(a.n_kv * sc.x), n_cta = px_ctas(a, T);
-    auto cta_of = [&](int at) { return (int)(((unsigned)(at + 1) * n_cta - 1) / T); };
-    const int c0 = cta_of(kvh * sc.x + sc.y);
-    n_f = cta_of(kvh * sc.x + sc.z - 1) - c0 + 1;
-    id = kvh * a.n_units + unit + c0;
+    // four places on the line, a lane each
+    const unsigned T = (unsigned)(a.n_kv * s0.x), base = (unsigned)(kvh * s0.x + s0.y);
+    const unsigned at = base + (lane == 0 ? 0 : lane == 1 ? shared - 1 : lane == 2 ? own : own + n_own - 1);
+    const int cta = (int)(((at + 1) * px_ctas(a, T) - 1) / T);
+    const int c0 = __shfl_sync(0xffffffffu, cta, 0), c1 = __shfl_sync(0xffffffffu, cta, 1), c2 = __shfl_sync(0xffffffffu, cta, 2), c3 = __shfl_sync(0xffffffffu, cta, 3);
+    f1 = c0;
+    n1 = shared > 0 ? c1 - c0 + 1 : 0;
+    if (n_own > 0) {
+      f2 = c2 + (n1 > 0 && c2 == c1);                           // one fragment may hold both
+      n2 = c3 - f2 + 1;
+    }
   }
-  const long step = (long)a.slot * a.slot_tiles;                                // float4 from a fragment to the next
-  const float4* part = a.part + id * step + x * a.slot + c * a.pitch + lane0 + h;
-  const float4* ml = a.part + id * step + x * a.slot + HEAD / 4 * a.pitch;
-  constexpr int AHEAD = 10, ROWS = kPxMaxCtas / 32;                             // fragments of a thread in flight; maxima of a lane
+  const int n_f = n1 + n2, id0 = kvh * a.n_units + s1.z;
+  const int step = a.slot * a.slot_tiles;                       // float4 from a fragment to the next
+  auto at_of = [&](int f) { return (long)(id0 + (f < n1 ? f1 + f : f2 + f - n1)) * step; };
+  const float4* part = a.part + x * a.slot + c * a.pitch + lane0 + h;
+  const float2* ml = reinterpret_cast<const float2*>(a.part + x * a.slot + HEAD / 4 * a.pitch) + lane0;
+  constexpr int AHEAD = 8;                                      // fragments of a thread in flight
   float4 v[AHEAD];
   auto fetch = [&](int f0) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      const int f = f0 + i * sets;
-      v[i] = set < sets && f < n_f ? __ldcg(part + f * step) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const int f = f0 + i * a.sets;
+      if (f < n_f && set < a.sets) v[i] = __ldcg(part + at_of(f));
     }
   };
   fetch(set);
   for (int g = tid >> 5; g < G; g += 8) {
-    float2 q[ROWS];
     float top = -INFINITY, den = 0.f;
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      q[i] = lane + 32 * i < n_f ? __ldcg(reinterpret_cast<const float2*>(ml + (lane + 32 * i) * step) + lane0 + g) : make_float2(-INFINITY, 0.f);
-      top = fmaxf(top, q[i].x);
-    }
+    auto load = [&](int i) { return i < n_f ? __ldcg(ml + at_of(i) * 2 + g) : make_float2(-INFINITY, 0.f); };
+    const float2 first = load(lane);                            // most rows have no more than 32
+    top = first.x;
+    for (int i = lane + 32; i - lane < n_f; i += 32) top = fmaxf(top, load(i).x);
     top = warp_max(top);
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const float w = q[i].x > -INFINITY ? px_ex2(q[i].x - top) : 0.f;
-      den += w > 0.f || q[i].y != q[i].y ? w * q[i].y : 0.f;                    // a NaN stays one, whatever its weight
-      s_w[(lane + 32 * i) * 16 + g] = w;
+    for (int i = lane; i - lane < n_f; i += 32) {
+      const float2 q = i == lane ? first : load(i);
+      const float w = q.x > -INFINITY ? px_ex2(q.x - top) : 0.f;
+      den += w > 0.f || q.y != q.y ? w * q.y : 0.f;             // a NaN stays one, whatever its weight
+      s_w[i][g] = w;
     }
     den = warp_sum(den);
     if (lane == 0) s_inv[g] = 1.f / den;
   }
   __syncthreads();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int f0 = set; f0 < n_f; f0 += AHEAD * sets) {                            // ascending order, fixed
-    if (f0 > set) fetch(f0);
+  if (set < a.sets)
+    for (int f0 = set; f0 < n_f; f0 += AHEAD * a.sets) {        // ascending order, fixed
+      if (f0 > set) fetch(f0);
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int f = f0 + i * sets;
-      const float w = f < n_f ? s_w[f * 16 + h] : 0.f;
-      // a fragment without keys of this row has no output: what lies there may be anything
-      if (w != 0.f) { o.x = fmaf(w, v[i].x, o.x); o.y = fmaf(w, v[i].y, o.y); o.z = fmaf(w, v[i].z, o.z); o.w = fmaf(w, v[i].w, o.w); }
+      for (int i = 0; i < AHEAD; ++i) {
+        const int f = f0 + i * a.sets;
+        const float w = f < n_f ? s_w[f][h] : 0.f;
+        // a fragment without keys of this row (it ended inside the prefix) has no output: what lies there may be anything
+        if (w != 0.f) { o.x = fmaf(w, v[i].x, o.x); o.y = fmaf(w, v[i].y, o.y); o.z = fmaf(w, v[i].z, o.z); o.w = fmaf(w, v[i].w, o.w); }
+      }
     }
-  }
   s_o[tid] = o;
   __syncthreads();
   bool again = false;
-  if (tid < items) {
-    for (int i = 1; i < sets; ++i) { const float4 u = s_o[tid + i * items]; o.x += u.x; o.y += u.y; o.z += u.z; o.w += u.w; }
+  if (tid < a.items) {
+    for (int i = 1; i < a.sets; ++i) { const float4 u = s_o[tid + i * a.items]; o.x += u.x; o.y += u.y; o.z += u.z; o.w += u.w; }
     const float inv = bad ? __int_as_float(0x7fc00000) : n > 0 ? s_inv[h] : 0.f;
     const __nv_bfloat162 b0 = __floats2bfloat162_rn(o.x * inv, o.y * inv), b1 = __floats2bfloat162_rn(o.z * inv, o.w * inv);
     *reinterpret_cast<uint2*>(a.out + ((long)m * a.n_q + kvh * G + h) * HEAD + c * 4) =
@@ -846,7 +908,7 @@ __global__ void __launch_bounds__(256, 4) prefix_join_kernel(const PrefixArgs a)
       px_row<HEAD, Q8>(a, m, kvh * G + g, n, r);
 #pragma unroll
       for (int i = 0; i < HEAD / 32; ++i)
-        if (lane * (HEAD / 32) / (4 * cols) == (int)blockIdx.z) a.out[((long)m * a.n_q + kvh * G + g) * HEAD + lane * (HEAD / 32) + i] = __float2bfloat16_rn(r[i]);
+        if (lane * (HEAD / 32) / (4 * a.cols) == (int)blockIdx.z) a.out[((long)m * a.n_q + kvh * G + g) * HEAD + lane * (HEAD / 32) + i] = __float2bfloat16_rn(r[i]);
     }
   }
 }
@@ -856,7 +918,17 @@ __global__ void __launch_bounds__(256, 4) prefix_join_kernel(const PrefixArgs a)
 using namespace bl;
 
 template <int HEAD, bool Q8>
-static int prefix_go(const PrefixArgs& a, cudaStream_t st) {
+static int prefix_go(PrefixArgs a, cudaStream_t st) {
+  // The joining launch.  Few rows: a block for 32 values of a head, so that more of its fragments are in flight; many: as much of it
+  // as 256 threads hold.
+  int z = HEAD / 32;
+  const int G = a.n_q / a.n_kv;
+  if (a.n_kv * a.M > a.n_cta) while (z > 1 && G * (HEAD / 4) / (z / 2) <= 256) z /= 2;
+  a.cols = HEAD / 4 / z;
+  a.items = G * a.cols;
+  a.sets = 256 / a.items;
+  a.inv_items = 65536 / a.items + 1;                            // exact for the 256 threads: items and G divide them by 256 at most
+  a.inv_G = 65536 / G + 1;
   CUtensorMap mk = {}, mv = {};
   if (!Q8) {
     const cuuint64_t dims[2] = {(cuuint64_t)HEAD, (cuuint64_t)a.n_pages * a.n_kv * kPxPage};
@@ -876,10 +948,6 @@ static int prefix_go(const PrefixArgs& a, cudaStream_t st) {
   }
   const cudaError_t e = launch(prefix_attn_kernel<HEAD, Q8>, dim3(a.n_cta), dim3(px_threads(Q8)), (size_t)px_smem(HEAD, Q8, a.n_units, a.M), st, mk, mv, a);
   if (e != cudaSuccess) return (int)e;
-  // few rows: a block for 32 values of a head, so that more of its fragments are in flight; many: as much of it as 256 threads hold
-  int z = HEAD / 32;
-  const int G = a.n_q / a.n_kv;
-  if (a.n_kv * a.M > a.n_cta) while (z > 1 && G * (HEAD / 4) / (z / 2) <= 256) z /= 2;
   return (int)launch(prefix_join_kernel<HEAD, Q8>, dim3(a.n_kv, a.M, z), dim3(256), 0, st, a);
 }
 
@@ -895,7 +963,7 @@ static long prefix_slots(int head, int G, int n_kv, int n_units, int unit_rows, 
 }
 long bl_prefix_work_bytes(int head, int n_q, int n_kv, int n_units, int unit_rows, int n_cta) {
   int slot, tiles, pitch;
-  return prefix_slots(head, n_q / n_kv, n_kv, n_units, unit_rows, n_cta, slot, tiles, pitch) + kPxMaxRows * 16;
+  return prefix_slots(head, n_q / n_kv, n_kv, n_units, unit_rows, n_cta, slot, tiles, pitch) + kPxMaxRows * 32;
 }
 
 // The call as one block of memory: a host that makes a call a layer hands over one pointer instead of two dozen arguments.
@@ -920,7 +988,7 @@ int bl_prefix_attention(const PrefixCall* call) {
                n_q, n_kv, M, p.meta, (__nv_bfloat16*)p.out, p.fault, p.layer, p.meta + (long)M * kPxMeta, n_units, n_cta};
   const cudaStream_t st = p.stream;
   a.sched = (int4*)work;
-  a.part = (float4*)((uint8_t*)work + kPxMaxRows * 16);
+  a.part = (float4*)((uint8_t*)work + kPxMaxRows * 32);
   a.part_bytes = prefix_slots(head, n_q / n_kv, n_kv, n_units, unit_rows, n_cta, a.slot, a.slot_tiles, a.pitch);
   if (p.kv_q8) return head == 128 ? prefix_go<128, true>(a, st) : prefix_go<64, true>(a, st);
   return head == 128 ? prefix_go<128, false>(a, st) : prefix_go<64, false>(a, st);
