@@ -647,27 +647,35 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
               v[u][0] = q.x; v[u][1] = q.y;
             }
           }
+          // no branches, so that the rows' chains of steps run side by side; rows behind the last are zeros
+          unsigned top[AT_ONCE];
 #pragma unroll
           for (int u = 0; u < AT_ONCE; ++u) {
-            const int i = i0 + 4 * u;
-            float top = fabsf(v[u][0]);
+            float most = fabsf(v[u][0]);
 #pragma unroll
-            for (int j = 1; j < N; ++j) top = fmaxf(top, fabsf(v[u][j]));
-            const int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23);      // of non-negative floats: in order as integers
-            const int se = e == 0 ? 127 : min(253, 263 - e);
+            for (int j = 1; j < N; ++j) most = fmaxf(most, fabsf(v[u][j]));
+            top[u] = __reduce_max_sync(0xffffffffu, __float_as_uint(most));     // of non-negative floats: in order as integers
+          }
+#pragma unroll
+          for (int u = 0; u < AT_ONCE; ++u) {
+            const int i = i0 + 4 * u, e = (int)(top[u] >> 23), se = e == 0 ? 127 : min(253, 263 - e);
             const float scale = __uint_as_float((unsigned)se << 23);
-            if (i < live) {
-              uint8_t* at = dst + i * 128 + ((chunk ^ (i & 7)) << 4);
-              const uint32_t lo = px_pack(v[u][0] * scale, v[u][1] * scale);
-              if constexpr (N == 4) *reinterpret_cast<uint2*>(at) = make_uint2(lo, px_pack(v[u][2] * scale, v[u][3] * scale));
-              else *reinterpret_cast<uint32_t*>(at) = lo;
-              if (lane == 0) s_scale[x][i] = kPxLog2e * __uint_as_float((unsigned)(254 - se) << 23);
-            }
+            uint8_t* at = dst + i * 128 + ((chunk ^ (i & 7)) << 4);
+            const uint32_t lo = px_pack(v[u][0] * scale, v[u][1] * scale);
+            if constexpr (N == 4) *reinterpret_cast<uint2*>(at) = make_uint2(lo, px_pack(v[u][2] * scale, v[u][3] * scale));
+            else *reinterpret_cast<uint32_t*>(at) = lo;
+            if (lane == u) s_scale[x][i] = kPxLog2e * __uint_as_float((unsigned)(254 - se) << 23);
           }
         };
         if (live > 16) {
+          // the CTAs of a unit read the same rows: they begin at different ones
+          const int n_it = (live + 31) >> 5;
+          int it = (int)((unsigned)blockIdx.x % (unsigned)n_it);
 #pragma unroll 1
-          for (int i0 = quarter; i0 < live; i0 += 32) some_rows(i0, std::integral_constant<int, 8>());
+          for (int k = 0; k < n_it; ++k) {
+            some_rows(quarter + 32 * it, std::integral_constant<int, 8>());
+            it = it + 1 == n_it ? 0 : it + 1;
+          }
         } else {
 #pragma unroll 1
           for (int i0 = quarter; i0 < live; i0 += 16) some_rows(i0, std::integral_constant<int, 4>());
