@@ -18,7 +18,7 @@ constexpr int kMaxBeams = 64;
 
 constexpr int kBmThreads = 256;
 constexpr int kBmList = 512;                              // survivors that are ranked side by side
-constexpr int kBmMaxCells = 4096;                         // chunks of a row x beams: what one block merges
+constexpr int kBmMaxCells = kBmThreads;                   // chunks of a row x beams: merged with one a thread
 
 struct BeamCell { float value; int id; };
 
@@ -47,30 +47,78 @@ __device__ __forceinline__ unsigned long long order_of(double v) {
   return u >> 63 ? ~u : u | 1ull << 63;
 }
 
+__device__ __forceinline__ float value_of(uint32_t u) { return __uint_as_float(u >> 31 ? u & 0x7fffffffu : ~u); }
+__device__ __forceinline__ double value_of(unsigned long long u) { return __longlong_as_double((long long)(u >> 63 ? u & ~(1ull << 63) : ~u)); }
+
 struct BestScratch {
   __align__(16) unsigned long long key[kBmList + 1];
   int id[kBmList];
-  double group[64];
+  double group[128], bound;
+  int part[kBmThreads / 32];
   int n;
 };
 
-// The smallest of the maxima of 8, 16, 32 or 64 groups of lanes, k at least: a bound that k of the block's values reach.  `mine`: the
-// largest value of this thread; -inf is none.
+// A bound that k of the block's values reach: the k-th largest of the maxima of 32 groups of lanes, of 128 for more than 32.
+// `mine`: the largest value of this thread; -inf is none.
 template <typename T>
 __device__ __forceinline__ T block_bound(T mine, int k, BestScratch& s) {
-  const int tid = threadIdx.x, lane = tid & 31, lanes = k <= 8 ? 32 : k <= 16 ? 16 : k <= 32 ? 8 : 4, groups = kBmThreads / lanes;
+  const int tid = threadIdx.x, lane = tid & 31, lanes = k <= 32 ? 8 : 2;
   T* group = reinterpret_cast<T*>(s.group);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
+  for (int o = 4; o > 0; o >>= 1)
     if (o < lanes) { const T u = __shfl_xor_sync(0xffffffffu, mine, o); mine = u > mine ? u : mine; }
   if ((lane & (lanes - 1)) == 0) group[tid / lanes] = mine;
   if (tid == 0) s.n = 0;
   __syncthreads();
-  T bound = group[lane % groups];
-  if (groups == 64) { const T u = group[lane + 32]; bound = u < bound ? u : bound; }
+  if (k <= 32) {
+    const T bound = group[lane];
+    int before = 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) { const T u = __shfl_xor_sync(0xffffffffu, bound, o); bound = u < bound ? u : bound; }
-  return bound;
+    for (int j = 0; j < 32; ++j) { const T u = group[j]; before += (int)(u > bound) + ((int)(u == bound) & (int)(j < lane)); }
+    const unsigned at = __ballot_sync(0xffffffffu, before == k - 1);             // one lane's: the groups are in an order
+    return __shfl_sync(0xffffffffu, bound, __ffs(at) - 1);
+  }
+  if (tid < 128) {
+    const T bound = group[tid];
+    int before = 0;
+#pragma unroll 8
+    for (int j = 0; j < 128; ++j) { const T u = group[j]; before += (int)(u > bound) + ((int)(u == bound) & (int)(j < tid)); }
+    if (before == k - 1) s.bound = (double)bound;
+  }
+  __syncthreads();
+  return (T)s.bound;
+}
+
+// list(bound) lists the values that reach the bound.  Where these are more than the list holds (cells of 64 beams, each row's in
+// order, make a weak bound), the bound is narrowed by halving the values above it, until it leaves at least k and at most a list.
+// Behind it s.n says how many reached the bound; still too many only where that many are equal.
+template <typename T, typename Count, typename List>
+__device__ __forceinline__ void block_list(T bound, int k, BestScratch& s, Count count, List list) {
+  list(bound);
+  __syncthreads();
+  if (s.n <= kBmList) return;
+  auto lo = order_of(bound);
+  decltype(lo) hi = ~(decltype(lo))0;
+#pragma unroll 1
+  for (int step = 0; step < 64 && hi - lo > 1; ++step) {
+    const decltype(lo) mid = lo + (hi - lo) / 2;
+    const int mine = __reduce_add_sync(0xffffffffu, count(value_of(mid)));
+    if ((threadIdx.x & 31) == 0) s.part[threadIdx.x >> 5] = mine;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < kBmThreads / 32; ++w) all += s.part[w];
+    __syncthreads();
+    if (all > kBmList) lo = mid;
+    else if (all < k) hi = mid;
+    else {
+      if (threadIdx.x == 0) s.n = 0;
+      __syncthreads();
+      list(value_of(mid));
+      __syncthreads();
+      return;
+    }
+  }
 }
 
 // The listed candidates in order, s.n of them and no more than the list holds: store(rank, key, id) of the k best.  A candidate
@@ -131,42 +179,19 @@ __device__ __forceinline__ void block_rounds(int k, BestScratch& s, Next next, S
 // One of a block's best by value and id: for fp32 the id is the key's low half.
 __device__ __forceinline__ unsigned long long beam_key(float v, int id) { return (unsigned long long)order_of(v) << 32 | (unsigned)~id; }
 __device__ __forceinline__ BeamCell beam_cell(unsigned long long key) {
-  const uint32_t u = (uint32_t)(key >> 32);
-  return BeamCell{__uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u), (int)~(uint32_t)key};
+  return BeamCell{value_of((uint32_t)(key >> 32)), (int)~(uint32_t)key};
 }
-template <int E>
-__device__ __forceinline__ void next_of(const float (&v)[E], const int (&ids)[E], float last, int last_id, float& best, int& where) {
-#pragma unroll
-  for (int i = 0; i < E; ++i)
-    if ((v[i] < last || (v[i] == last && ids[i] > last_id)) && (v[i] > best || (v[i] == best && v[i] > -INFINITY && ids[i] < where))) { best = v[i]; where = ids[i]; }
-}
-// The k best of the cells [n] that blocks left in memory, E a thread.
-template <int E>
+
+// The k best of n cells that blocks left in memory, at most one a thread.
 __device__ __forceinline__ void merge_cells(const BeamCell* cells, int n, int k, BestScratch& s, BeamCell* best) {
-  float v[E], mine = -INFINITY;
-  int ids[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const int e = threadIdx.x + i * kBmThreads;
-    const float2 q = e < n ? __ldcg(reinterpret_cast<const float2*>(cells + e)) : make_float2(-INFINITY, 0.f);
-    v[i] = q.x;
-    ids[i] = __float_as_int(q.y);
-    mine = fmaxf(mine, q.x);
-  }
-  const float bound = block_bound(mine, k, s);
-#pragma unroll
-  for (int i = 0; i < E; ++i)
-    if (v[i] >= bound && v[i] > -INFINITY) {
-      const int at = atomicAdd(&s.n, 1);
-      if (at < kBmList) s.key[at] = beam_key(v[i], ids[i]);
-    }
+  const int tid = threadIdx.x;
+  const float2 q = tid < n ? __ldcg(reinterpret_cast<const float2*>(cells + tid)) : make_float2(-INFINITY, 0.f);
+  const float bound = block_bound(q.x, k, s);
+  if (q.x >= bound && q.x > -INFINITY) s.key[atomicAdd(&s.n, 1)] = beam_key(q.x, __float_as_int(q.y));
   __syncthreads();
-  auto store = [&](int rank, BeamCell c) { best[rank] = c; };
-  if (s.n <= kBmList) block_rank<false>(k, s, [&](int rank, unsigned long long key, int) { store(rank, beam_cell(key)); });
-  else block_rounds<float>(k, s, [&](float last, int last_id, float& b, int& w) { next_of<E>(v, ids, last, last_id, b, w); },
-                           [&](int rank, float value, int id) { store(rank, BeamCell{value, id}); });
+  block_rank<false>(k, s, [&](int rank, unsigned long long key, int) { best[rank] = beam_cell(key); });
   const int had = min(k, s.n);
-  if ((int)threadIdx.x >= had && (int)threadIdx.x < k) best[threadIdx.x] = BeamCell{-INFINITY, 0x7fffffff};
+  if (tid >= had && tid < k) best[tid] = BeamCell{-INFINITY, 0x7fffffff};
 }
 
 // True in the block that arrives last of `n`: what the others wrote before they arrived is visible to it.
@@ -183,8 +208,6 @@ __device__ __forceinline__ bool block_last(int* ticket, int n, int* s_last) {
   return last;
 }
 
-// grid (n_chunks, G * B).  A block takes the sum of exponentials and the B best of a chunk; the last block of a row merges the
-// row's; the last row of a search ranks the B x B candidates that are left.
 // A search's places [B]: the best of the B x B candidates that its rows left, EB a thread.
 template <int EB, typename Rank>
 __device__ __forceinline__ void pick_places(int B, BestScratch& s, int* s_pick, Rank rank_of) {
@@ -195,14 +218,19 @@ __device__ __forceinline__ void pick_places(int B, BestScratch& s, int* s_pick, 
     v[i] = e < B * B ? rank_of(e) : (double)-INFINITY;
     mine = v[i] > mine ? v[i] : mine;
   }
-  const double bound = block_bound(mine, B, s);
+  block_list(block_bound(mine, B, s), B, s, [&](double bound) {
+    int n = 0;
 #pragma unroll
-  for (int i = 0; i < EB; ++i)
-    if (v[i] >= bound && v[i] > -INFINITY) {
-      const int at = atomicAdd(&s.n, 1);
-      if (at < kBmList) { s.key[at] = order_of(v[i]); s.id[at] = threadIdx.x + i * kBmThreads; }
-    }
-  __syncthreads();
+    for (int i = 0; i < EB; ++i) n += (int)(v[i] >= bound) & (int)(v[i] > -INFINITY);
+    return n;
+  }, [&](double bound) {
+#pragma unroll
+    for (int i = 0; i < EB; ++i)
+      if (v[i] >= bound && v[i] > -INFINITY) {
+        const int at = atomicAdd(&s.n, 1);
+        if (at < kBmList) { s.key[at] = order_of(v[i]); s.id[at] = threadIdx.x + i * kBmThreads; }
+      }
+  });
   if (s.n <= kBmList) {
     block_rank<true>(B, s, [&](int rank, unsigned long long, int id) { s_pick[rank] = id; });
   } else {
@@ -266,6 +294,8 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
       float v[E], tops[NB], mine = carried;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
+        tops[b] = -INFINITY;
+        if (NB > 1 && t0 + b * E * kBmThreads >= hi) continue;
         load(t0 + b * E * kBmThreads, v);
         float top = v[0];
 #pragma unroll
@@ -283,36 +313,45 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
         tops[b] = top;
         mine = fmaxf(mine, top);
       }
-      const float bound = block_bound(mine, B, s);
       // few pass: a batch that is no longer in registers is read again, and so are the values, so that registers need no index
-      auto list = [&](int from) {
-        uint32_t pass = 0;
+      block_list(block_bound(mine, B, s), B, s, [&](float bound) {
+        int n = (int)(carried >= bound) & (int)(carried > -INFINITY);
+#pragma unroll 1
+        for (int b = 0; b < NB; ++b) {
+          load(t0 + b * E * kBmThreads, v);
 #pragma unroll
-        for (int i = 0; i < E; ++i) pass |= (uint32_t)(v[i] >= bound && v[i] > -INFINITY) << i;
-        while (pass) {
-          const int id = id_of(from, __ffs(pass) - 1), at = atomicAdd(&s.n, 1);
-          pass &= pass - 1;
-          if (at < kBmList) s.key[at] = beam_key(__ldg(x + id), id);
+          for (int i = 0; i < E; ++i) n += (int)(v[i] >= bound) & (int)(v[i] > -INFINITY);
         }
-      };
-      if constexpr (NB == 1) {
-        list(t0);
-      } else {
-        uint32_t want = 0;
+        return n;
+      }, [&](float bound) {
+        auto batch = [&](int from) {
+          uint32_t pass = 0;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) want |= (uint32_t)(tops[b] >= bound && tops[b] > -INFINITY) << b;
-        while (want) {
-          const int from = t0 + (__ffs(want) - 1) * E * kBmThreads;
-          want &= want - 1;
-          load(from, v);
-          list(from);
+          for (int i = 0; i < E; ++i) pass |= (uint32_t)(v[i] >= bound && v[i] > -INFINITY) << i;
+          while (pass) {
+            const int id = id_of(from, __ffs(pass) - 1), at = atomicAdd(&s.n, 1);
+            pass &= pass - 1;
+            if (at < kBmList) s.key[at] = beam_key(__ldg(x + id), id);
+          }
+        };
+        if constexpr (NB == 1) {
+          batch(t0);
+        } else {
+          uint32_t want = 0;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) want |= (uint32_t)(tops[b] >= bound && tops[b] > -INFINITY) << b;
+          while (want) {
+            const int from = t0 + (__ffs(want) - 1) * E * kBmThreads;
+            want &= want - 1;
+            load(from, v);
+            batch(from);
+          }
         }
-      }
-      if (carried >= bound && carried > -INFINITY) {
-        const int at = atomicAdd(&s.n, 1);
-        if (at < kBmList) s.key[at] = beam_key(carried, carried_id);
-      }
-      __syncthreads();
+        if (carried >= bound && carried > -INFINITY) {
+          const int at = atomicAdd(&s.n, 1);
+          if (at < kBmList) s.key[at] = beam_key(carried, carried_id);
+        }
+      });
       if (s.n <= kBmList) {
         block_rank<false>(B, s, [&](int rank, unsigned long long key, int) { out[rank] = beam_cell(key); });
       } else {
@@ -322,7 +361,7 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
           };
 #pragma unroll 1
           for (int b = 0; b < NB; ++b) {
-            if (NB > 1) load(t0 + b * E * kBmThreads, v);
+            load(t0 + b * E * kBmThreads, v);
 #pragma unroll
             for (int i = 0; i < E; ++i) offer(v[i], id_of(t0 + b * E * kBmThreads, i));
           }
@@ -357,20 +396,14 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
     const float2* sums = a.sums + (long)r * a.n_chunks;
     const float2 first = tid < a.n_chunks ? __ldcg(sums + tid) : make_float2(-INFINITY, 0.f);
     const BeamCell* cells = a.cells + (long)r * a.n_chunks * B;
-    const int n_cells = a.n_chunks * B;
-    if (n_cells <= kBmThreads) merge_cells<1>(cells, n_cells, B, s, a.best + (long)r * B);
-    else merge_cells<kBmMaxCells / kBmThreads>(cells, n_cells, B, s, a.best + (long)r * B);
-    float top = first.x;
-    for (int i = tid + kBmThreads; i < a.n_chunks; i += kBmThreads) top = fmaxf(top, __ldcg(sums + i).x);
-    top = warp_max(top);
+    merge_cells(cells, a.n_chunks * B, B, s, a.best + (long)r * B);
+    float top = warp_max(first.x);
     if (lane == 0) s_max[warp] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 8; ++w) top = fmaxf(top, s_max[w]);
     auto weighed = [&](float2 q) { return q.x > -INFINITY ? (double)q.y * (double)__expf(q.x - top) : (double)q.y; };
-    double l = weighed(first);
-    for (int i = tid + kBmThreads; i < a.n_chunks; i += kBmThreads) l += weighed(__ldcg(sums + i));
-    l = warp_sum_d(l);
+    const double l = warp_sum_d(weighed(first));
     if (lane == 0) s_sum[warp] = l;
     __syncthreads();
     if (tid == 0) {
@@ -552,21 +585,20 @@ using namespace bl;
 
 extern "C" {
 
-static void beam_chunks(int V, int rows, int B, int sms, int& tile, int& n, int& chunk) {
-  // The choice of the best is once a tile, so large tiles cost less where there are blocks enough: four of a processor's size are
-  // resident at a time.
-  auto blocks = [&](int size) { return (long)rows * ((V + size - 1) / size); };
-  tile = blocks(32768) >= 4L * sms ? 32768 : blocks(16384) >= 4L * sms ? 16384 : blocks(8192) >= 2L * sms ? 8192 : 4096;
-  n = (V + tile - 1) / tile;
-  if (n > kBmMaxCells / B) n = kBmMaxCells / B;
-  chunk = ((V + n - 1) / n + 3) / 4 * 4;
-  n = (V + chunk - 1) / chunk;
+// Chunks of a row: as many as one wave of four blocks a processor holds, of 4,096 values or more, and no more than a block merges
+// with one cell a thread.  Device time of 148 processors at 151,936 ids, us: 4 rows of 4 beams, 16 chunks 13.1, 38 (the rule)
+// 11.3; 64 rows of 8, 4 chunks 23.9, 9 (the rule) 22.7, 10 (a second wave) 23.7, 16 27.9; 256 rows of 16, 1 chunk 55.8, 2 (the
+// rule) 50.1, 3 56.2; 64 rows of 64, 2 chunks 61.3, 4 (the rule, 256 cells) 54.9, 9 (the wave's) 61.6.
+int bl_beam_chunks(int V, int rows, int B, int sms) {
+  const int most = (V + 4095) / 4096, wave = 4 * sms / rows, cells = kBmMaxCells / B;
+  int n = most < wave ? most : wave;
+  if (n > cells) n = cells;
+  return n > 1 ? n : 1;
 }
+static int beam_chunk(int V, int n) { return ((V + n - 1) / n + 3) / 4 * 4; }
 
 // Bytes of scratch that bl_beam_select takes; zeroed once.
-long bl_beam_work_bytes(int V, int G, int B, int sms) {
-  int tile, n, chunk;
-  beam_chunks(V, G * B, B, sms, tile, n, chunk);
+long bl_beam_work_bytes(int G, int B, int n) {
   const long R = (long)G * B;
   return R * 8 + R * n * 8 + R * n * B * 8 + R * B * 8 + (R + G) * 4;
 }
@@ -575,7 +607,7 @@ long bl_beam_work_bytes(int V, int G, int B, int sms) {
 struct BeamSelectCall {
   const float* logits; long stride; const float* scores; const int* done; const int* lengths; void* work;
   int* parent; int* token; float* out_scores; int* out_done; int* out_lengths; unsigned* fault; cudaStream_t stream;
-  int V, G, B, eos, sms; float alpha;
+  int V, G, B, eos, chunks; float alpha;                    // chunks: as bl_beam_chunks says
 };
 struct BeamReorderCall {
   void* k; void* v; long k_row, v_row; const int* table; int* table_out; const int* slots; const int* parent; const int* held;
@@ -584,14 +616,14 @@ struct BeamReorderCall {
 };
 
 int bl_beam_select(const BeamSelectCall* call) {
-  const auto [logits, stride, scores, done, lengths, work, parent, token, out_scores, out_done, out_lengths, fault, st, V, G, B, eos, sms, alpha] = *call;
-  BL_REQUIRE(V >= 1 && G >= 1 && B >= 1 && stride >= V && sms >= 1, BL_ERR_SHAPE);
-  BL_REQUIRE(B <= kMaxBeams && (long)G * B <= 65535, BL_ERR_LIMIT);
+  const auto [logits, stride, scores, done, lengths, work, parent, token, out_scores, out_done, out_lengths, fault, st, V, G, B, eos, chunks, alpha] = *call;
+  BL_REQUIRE(V >= 1 && G >= 1 && B >= 1 && stride >= V && chunks >= 1 && chunks <= V, BL_ERR_SHAPE);
+  BL_REQUIRE(B <= kMaxBeams && (long)G * B <= 65535 && (long)chunks * B <= kBmMaxCells, BL_ERR_LIMIT);
   BL_REQUIRE(eos < V && (!done || eos >= 0) && (alpha == 0.f || lengths) && (!out_lengths || lengths), BL_ERR_SHAPE);
   BL_REQUIRE(((uintptr_t)logits & 3) == 0 && ((uintptr_t)work & 7) == 0, BL_ERR_ALIGN);
   BeamArgs a{logits, stride, V, G, B, scores, done, lengths, eos, alpha};
-  int tile;
-  beam_chunks(V, G * B, B, sms, tile, a.n_chunks, a.chunk);
+  a.chunk = beam_chunk(V, chunks);
+  a.n_chunks = (V + a.chunk - 1) / a.chunk;
   const long R = (long)G * B;
   uint8_t* w = (uint8_t*)work;
   a.lse = (double*)w; w += R * 8;
@@ -601,12 +633,10 @@ int bl_beam_select(const BeamSelectCall* call) {
   a.tickets = (int*)w;
   a.parent = parent; a.token = token; a.out_scores = out_scores; a.out_done = out_done; a.out_lengths = out_lengths; a.fault = fault;
   const dim3 grid(a.n_chunks, (unsigned)R);
-  switch (tile) {
-    case 32768: return (int)launch(beam_select_kernel<32, 4>, grid, dim3(kBmThreads), 0, st, a);
-    case 16384: return (int)launch(beam_select_kernel<32, 2>, grid, dim3(kBmThreads), 0, st, a);
-    case 8192: return (int)launch(beam_select_kernel<32, 1>, grid, dim3(kBmThreads), 0, st, a);
-    default: return (int)launch(beam_select_kernel<16, 1>, grid, dim3(kBmThreads), 0, st, a);
-  }
+  if (a.chunk <= 4096) return (int)launch(beam_select_kernel<16, 1>, grid, dim3(kBmThreads), 0, st, a);
+  if (a.chunk <= 8192) return (int)launch(beam_select_kernel<16, 2>, grid, dim3(kBmThreads), 0, st, a);
+  if (a.chunk <= 16384) return (int)launch(beam_select_kernel<32, 2>, grid, dim3(kBmThreads), 0, st, a);
+  return (int)launch(beam_select_kernel<32, 4>, grid, dim3(kBmThreads), 0, st, a);
 }
 
 int bl_beam_reorder(const BeamReorderCall* call) {

@@ -45,11 +45,12 @@ class BeamScratch:
             self.device = torch.device("cuda", torch.cuda.current_device())
         if groups * beams > 65535:
             raise ValueError("at most 65,535 beams in all")
-        self.sms = sm_count(self.device) if self.device.type == "cuda" else 1
+        sms = sm_count(self.device) if self.device.type == "cuda" else 1
+        self.chunks = cuda().bl_beam_chunks(I(vocab), I(groups * beams), I(beams), I(sms))
         self.index = self.device.index if self.device.type == "cuda" else -1      # as Tensor.get_device() says it
         size = cuda().bl_beam_work_bytes
         size.restype = ctypes.c_long
-        self.work = torch.zeros(size(vocab, groups, beams, self.sms), dtype=torch.uint8, device=self.device)
+        self.work = torch.zeros(size(groups, beams, self.chunks), dtype=torch.uint8, device=self.device)
         self.work_ptr = self.work.data_ptr()
 
 
@@ -87,7 +88,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, scratch: BeamScratch
     if index < 0:
         raise ValueError("the kernels need a CUDA device")
     code = _fn("bl_beam_select")(_SELECT.pack(logits.data_ptr(), max(logits.stride(0), V), *at, raw_stream(index), V, G, B, max(eos, -1),
-                                              scratch.sms, alpha))
+                                              scratch.chunks, alpha))
     if code:
         check(code, "bl_beam_select")
 
