@@ -612,7 +612,7 @@ struct BeamSelectCall {
 struct BeamReorderCall {
   void* k; void* v; long k_row, v_row; const int* table; int* table_out; const int* slots; const int* parent; const int* held;
   unsigned* fault; cudaStream_t stream;
-  int n_layer, n_pages, n_kv, n_slots, max_pages, G, B, sms;
+  int n_layer, n_pages, n_kv, n_slots, max_pages, G, B;
 };
 
 int bl_beam_select(const BeamSelectCall* call) {
@@ -640,7 +640,7 @@ int bl_beam_select(const BeamSelectCall* call) {
 }
 
 int bl_beam_reorder(const BeamReorderCall* call) {
-  const auto [k, v, k_row, v_row, table, table_out, slots, parent, held, fault, st, n_layer, n_pages, n_kv, n_slots, max_pages, G, B, sms] = *call;
+  const auto [k, v, k_row, v_row, table, table_out, slots, parent, held, fault, st, n_layer, n_pages, n_kv, n_slots, max_pages, G, B] = *call;
   BL_REQUIRE(n_layer >= 1 && n_layer <= 65535 && n_pages >= 1 && n_kv >= 1 && G >= 1 && B >= 1 && n_slots >= 1 && max_pages >= 1,
              BL_ERR_SHAPE);
   BL_REQUIRE(B <= kMaxBeams, BL_ERR_LIMIT);

@@ -12,7 +12,7 @@ from ._lib import I, check, cuda, p, raw_stream, stream
 from .decode import sm_count
 
 MAX_BEAMS = 64
-_SELECT, _REORDER = struct.Struct("P1l11P5if"), struct.Struct("2P2l7P8i")        # BeamSelectCall, BeamReorderCall in the source
+_SELECT, _REORDER = struct.Struct("P1l11P5if"), struct.Struct("2P2l7P7i4x")      # BeamSelectCall, BeamReorderCall in the source
 _entries: dict = {}
 
 
@@ -121,7 +121,7 @@ def beam_reorder(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, table_ou
         raise ValueError("the kernels need the pools on one CUDA device")
     code = _fn("bl_beam_reorder")(_REORDER.pack(k.data_ptr(), v.data_ptr(), shape[4] * k.element_size(), v_shape[4] * v.element_size(),
                                                 table.data_ptr(), table_out.data_ptr(), *at, raw_stream(index), shape[0], shape[1],
-                                                shape[2], tables[0], tables[1], G, B, sm_count(k.device)))
+                                                shape[2], tables[0], tables[1], G, B))
     if code:
         check(code, "bl_beam_reorder")
 
