@@ -10,6 +10,8 @@
 // the page being filled (part = held % 64 positions) a parent's first child goes on; each further child takes the page of a beam
 // that has no child -- there are as many of these -- and a copy of the positions held.  What is read is never written, so all
 // copies run at once.  Pages behind belong to the slot.
+#include <cfloat>
+
 #include "common.cuh"
 
 namespace bl {
@@ -176,6 +178,24 @@ __device__ __forceinline__ void block_rounds(int k, BestScratch& s, Next next, S
   }
 }
 
+// 2^x; what is less than 2^-126 counts as nothing beside a sum of 1 or more, which saves the instructions that keep it.
+__device__ __forceinline__ float bm_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kBmLog2e = 1.4426950408889634f;
+// sum[2] += e^(v - top) of two values, additions and products of both at once
+__device__ __forceinline__ void bm_add2(float2& sum, float a, float b, float top) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, t, c;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 t, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
+      "add.rn.f32x2 x, x, t;\n\tmul.rn.f32x2 x, x, c;\n\tmov.b64 {%0, %1}, x;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a), "f"(b), "f"(-top), "f"(kBmLog2e));
+  d.x = bm_ex2(d.x);
+  d.y = bm_ex2(d.y);
+  asm("{\n\t.reg .b64 s, x;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 x, {%2, %3};\n\tadd.rn.f32x2 s, s, x;\n\tmov.b64 {%0, %1}, s;\n\t}"
+      : "+f"(sum.x), "+f"(sum.y) : "f"(d.x), "f"(d.y));
+}
+
 // One of a block's best by value and id: for fp32 the id is the key's low half.
 __device__ __forceinline__ unsigned long long beam_key(float v, int id) { return (unsigned long long)order_of(v) << 32 | (unsigned)~id; }
 __device__ __forceinline__ BeamCell beam_cell(unsigned long long key) {
@@ -266,11 +286,16 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
     const float* x = a.logits + (long)r * a.stride;
     const int lo = c * a.chunk, hi = min(V, lo + a.chunk);
     const bool vec = ((uintptr_t)x & 15) == 0;
-    BeamCell* out = a.cells + ((long)r * a.n_chunks + c) * B;
     // values of batch b of a tile: this thread's, -inf behind the chunk's end
     auto load = [&](int from, float (&v)[E]) {
       const int n = hi - from;
-      if (vec) {
+      if (vec && n >= E * kBmThreads) {
+#pragma unroll
+        for (int i = 0; i < E; i += 4) {
+          const float4 q = __ldg(reinterpret_cast<const float4*>(x + from + (tid + i / 4 * kBmThreads) * 4));
+          v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w;
+        }
+      } else if (vec) {
 #pragma unroll
         for (int i = 0; i < E; i += 4) {
           const int e = (tid + i / 4 * kBmThreads) * 4;
@@ -297,14 +322,15 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
         tops[b] = -INFINITY;
         if (NB > 1 && t0 + b * E * kBmThreads >= hi) continue;
         load(t0 + b * E * kBmThreads, v);
-        float top = v[0];
+        float top = fmaxf(v[0], v[1]);
 #pragma unroll
-        for (int i = 1; i < E; ++i) top = fmaxf(top, v[i]);
+        for (int i = 2; i < E; i += 2) top = fmaxf(top, fmaxf(v[i], v[i + 1]));
         const float seen = fmaxf(top, m);
         if (seen > -INFINITY) {                           // NaN and +inf end up as a NaN of the sum
-          sum *= __expf(m - seen);
+          float2 more = make_float2(sum * bm_ex2((m - seen) * kBmLog2e), 0.f);
 #pragma unroll
-          for (int i = 0; i < E; ++i) sum += __expf(v[i] - seen);
+          for (int i = 0; i < E; i += 2) bm_add2(more, v[i], v[i + 1], seen);
+          sum = more.x + more.y;
         } else {
 #pragma unroll
           for (int i = 0; i < E; ++i) sum += v[i] == -INFINITY ? 0.f : v[i];
@@ -325,9 +351,10 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
         return n;
       }, [&](float bound) {
         auto batch = [&](int from) {
+          const float least = fmaxf(bound, -FLT_MAX);     // an id with a logit of -inf is none
           uint32_t pass = 0;
 #pragma unroll
-          for (int i = 0; i < E; ++i) pass |= (uint32_t)(v[i] >= bound && v[i] > -INFINITY) << i;
+          for (int i = 0; i < E; ++i) pass |= v[i] >= least ? 1u << i : 0u;
           while (pass) {
             const int id = id_of(from, __ffs(pass) - 1), at = atomicAdd(&s.n, 1);
             pass &= pass - 1;
@@ -352,6 +379,7 @@ __global__ void __launch_bounds__(kBmThreads, 4) beam_select_kernel(const BeamAr
           if (at < kBmList) s.key[at] = beam_key(carried, carried_id);
         }
       });
+      BeamCell* out = a.cells + ((long)r * a.n_chunks + c) * B;
       if (s.n <= kBmList) {
         block_rank<false>(B, s, [&](int rank, unsigned long long key, int) { out[rank] = beam_cell(key); });
       } else {

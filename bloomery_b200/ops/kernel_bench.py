@@ -5,7 +5,8 @@ CUDA events.
     python -m bloomery_b200.ops.kernel_bench NAME [replays] [context] [--no-staged] [--rows M]
 
 NAME: chain (the six launches of a layer in order) | qkv | attn | o | router | gateup | down | rope | flash |
-flash_mma | gemm | gemmpair | gemmdist | pflash | prope | mplan | qgu | qdown | qo | qq | bgu | bdown | pgu | pdown | mla | sampler | sampler_split | gap.  ``--no-staged`` runs the register-streaming kernels
+flash_mma | gemm | gemmpair | gemmdist | pflash | prope | mplan | qgu | qdown | qo | qq | bgu | bdown | pgu | pdown | mla | sampler | sampler_split |
+prefix | bselect | breorder | gap.  ``--no-staged`` runs the register-streaming kernels
 instead of the shared-memory staged ones; ``--form exact`` / ``--form fine`` picks how the weights of qgu / qdown are expanded.
 It is also the small workload the ncu summaries under ``profiles/``
 were captured on.
@@ -129,6 +130,33 @@ def main(argv=None) -> int:
         extra = dict(G=G, pq=(torch.randn(n_q, ctx, hd, device=dev) * 0.3).bfloat16(), pk=(torch.randn(n_kv, tp, hd, device=dev)).bfloat16(),
                      pv=(torch.randn(n_kv, hd, tp, device=dev)).bfloat16(), po=torch.zeros(ctx, n_q * hd, device=dev, dtype=torch.bfloat16),
                      gst=torch.zeros(1, dtype=torch.int32, device=dev))
+    if which == "prefix":
+        # decode attention of M rows behind `ctx` shared positions, each with 1 to 256 of its own
+        from bloomery_b200.ops import prefix as PX
+        own, shared = [1 + 255 * i // max(1, M - 1) for i in range(M)], ctx // 64
+        first, lists = shared, []
+        for n in own:
+            lists.append(list(range(shared)) + list(range(first, first + (n + 63) // 64)) + [0] * (4 - (n + 63) // 64))
+            first += (n + 63) // 64
+        extra = dict(PX=PX, xk=torch.randn(first, n_kv, 64, hd, device=dev).half(), xv=torch.randn(first, n_kv, 64, hd, device=dev).half(),
+                     xt=torch.tensor(lists, dtype=torch.int32, device=dev), xp=torch.tensor([shared * 64 + n - 1 for n in own], dtype=torch.int32, device=dev),
+                     xs=torch.arange(M, dtype=torch.int32, device=dev), xqh=torch.randn(M, n_q, hd, device=dev) / math.sqrt(hd),
+                     xo=torch.zeros(M, n_q * hd, dtype=torch.bfloat16, device=dev), plan=PX.PrefixPlan([M], [shared * 64], n_q, n_kv, hd, dev))
+    if which == "bselect":
+        # the next beams of 8 searches of 8 over 151,936 ids
+        from bloomery_b200.ops import beam as BM
+        extra = dict(BM=BM, blog=[torch.randn(64, 151936, device=dev) for _ in range(NL)], bsc=torch.randn(8, 8, device=dev),
+                     bws=BM.BeamScratch(8, 8, 151936, dev), bp=torch.zeros(8, 8, dtype=torch.int32, device=dev),
+                     bt=torch.zeros(8, 8, dtype=torch.int32, device=dev), bo=torch.zeros(8, 8, device=dev))
+    if which == "breorder":
+        # states of 8 searches of 8 with 40 positions in the last page, in pools of 48 layers: half of the beams are copied
+        from bloomery_b200.ops import beam as BM
+        extra = dict(BM=BM, ck=torch.zeros(48, 160, n_kv, 64, hd, dtype=torch.float16, device=dev),
+                     cv=torch.zeros(48, 160, n_kv, 64, hd, dtype=torch.float16, device=dev),
+                     ct=torch.arange(128, dtype=torch.int32, device=dev).view(64, 2).contiguous(), co=torch.zeros(64, 2, dtype=torch.int32, device=dev),
+                     cs=torch.arange(64, dtype=torch.int32, device=dev).view(8, 8).contiguous(),
+                     cp=(torch.arange(8, dtype=torch.int32, device=dev) // 2).repeat(8, 1).contiguous(),
+                     ch=torch.full((8,), 104, dtype=torch.int32, device=dev))
     if which == "prope":
         # prompt RMSNorm + RoPE + KV append of `ctx` rows
         from bloomery_b200.ops import gemm as G
@@ -228,7 +256,7 @@ def main(argv=None) -> int:
         (K.down_staged if staged else K.down_combine)(actq, actds, ids, wts, None, l["d"], E, TOPK, M, x, None, x, fault, 0)
 
     def chain():
-        for l in layers:
+        for i, l in enumerate(layers):
             if which in ("chain", "chain2", "qkv"): K.gemv([l["q"], l["k"], l["v"]], M, qkv, x=x, gain=gain, fault=fault)
             if which in ("chain", "chain2", "attn", "attn_cluster"): attn(l)
             if which in ("chain", "chain2", "o"): K.gemv([l["o"]], M, x, xq=xq, xds=xds, resid=x, fault=fault)
@@ -247,6 +275,9 @@ def main(argv=None) -> int:
             if which in ("flash", "flash_mma"): K.flash_decode(fq, kc, vc, fpos, fseq, table, n_pages, hd, n_q, n_kv, 1, n_seg, ctx, pml, pacc, None, xq, xds, fault, 0)
             if which == "gemm": X["G"].gemm_bf16(X["A"], X["B"], X["tt"], out_bf16=X["C"], status=X["gst"])
             if which == "pflash": X["G"].flash_prefill(X["pq"], X["pk"], X["pv"], X["po"], 0, X["gst"])
+            if which == "prefix": X["PX"].prefix_attention(X["xqh"], X["xk"], X["xv"], X["xp"], X["xs"], X["xt"], X["plan"], X["xo"], fault)
+            if which == "bselect": X["BM"].beam_select(X["blog"][i], X["bsc"], X["bws"], X["bp"], X["bt"], X["bo"], fault=fault)
+            if which == "breorder": X["BM"].beam_reorder(X["ck"], X["cv"], X["ct"], X["co"], X["cs"], X["cp"], X["ch"], fault)
             if which == "prope": X["G"].qk_norm_rope_append_prefill(X["rqkv"], r_g, r_g, r_inv, 1e-6, 1.0 / math.sqrt(hd), hd, n_q, n_kv, ctx, X["rpos"], X["rseq"], table, n_pages, kc, vc, X["rqb"], fault, 0)
             if which == "mplan": X["G"].moe_plan(X["mids"], X["mwts"], E, X["mtt"], X["mpos_of"], X["mdst"], X["mscale"])
             if which == "qo": X["G"].qgemm(X["xo"], l["o"], X["tt"], out_f32=X["oo"], status=X["gst"])
