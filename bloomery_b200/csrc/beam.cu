@@ -146,8 +146,7 @@ __device__ __forceinline__ void block_rank(int k, const BestScratch& s, Store st
   }
 }
 
-// The k best of the block's values by k rounds, for data that let more than the list through (an ascending row, say): next(last, last
-// id, best, id) gives a thread's best behind the last one taken.
+// The k best of the block's values by k rounds, where more than the list holds are equal: next(last, last id, best, id) gives a thread's best behind the last one taken.
 template <typename T, typename Next, typename Store>
 __device__ __forceinline__ void block_rounds(int k, BestScratch& s, Next next, Store store) {
   const int tid = threadIdx.x, lane = tid & 31;
@@ -614,9 +613,9 @@ using namespace bl;
 extern "C" {
 
 // Chunks of a row: as many as one wave of four blocks a processor holds, of 4,096 values or more, and no more than a block merges
-// with one cell a thread.  Device time of 148 processors at 151,936 ids, us: 4 rows of 4 beams, 16 chunks 13.1, 38 (the rule)
-// 11.3; 64 rows of 8, 4 chunks 23.9, 9 (the rule) 22.7, 10 (a second wave) 23.7, 16 27.9; 256 rows of 16, 1 chunk 55.8, 2 (the
-// rule) 50.1, 3 56.2; 64 rows of 64, 2 chunks 61.3, 4 (the rule, 256 cells) 54.9, 9 (the wave's) 61.6.
+// with one cell a thread.  Device time on 148 processors at 151,936 ids, us: 4 rows of 4 beams, 16 chunks 12.2, 38 (the rule)
+// 10.3; 64 rows of 8, 4 chunks 21.5, 9 (the rule) 20.4, 10 (a second wave) 22.4, 16 24.5; 256 rows of 16, 1 chunk 48.9, 2 (the
+// rule) 44.5, 3 49.4; 64 rows of 64, 2 chunks 51.4, 4 (the rule, 256 cells) 45.5.
 int bl_beam_chunks(int V, int rows, int B, int sms) {
   const int most = (V + 4095) / 4096, wave = 4 * sms / rows, cells = kBmMaxCells / B;
   int n = most < wave ? most : wave;
@@ -661,9 +660,10 @@ int bl_beam_select(const BeamSelectCall* call) {
   a.tickets = (int*)w;
   a.parent = parent; a.token = token; a.out_scores = out_scores; a.out_done = out_done; a.out_lengths = out_lengths; a.fault = fault;
   const dim3 grid(a.n_chunks, (unsigned)R);
+  // A short chunk whole in registers, 4 rows of 151,936 in 38 chunks: 10.3 us, 11.2 as a part of the largest tile.  In two batches, 128
+  // rows of 32,000 in 4 chunks: 15.0 us against 15.7.
   if (a.chunk <= 4096) return (int)launch(beam_select_kernel<16, 1>, grid, dim3(kBmThreads), 0, st, a);
   if (a.chunk <= 8192) return (int)launch(beam_select_kernel<16, 2>, grid, dim3(kBmThreads), 0, st, a);
-  if (a.chunk <= 16384) return (int)launch(beam_select_kernel<32, 2>, grid, dim3(kBmThreads), 0, st, a);
   return (int)launch(beam_select_kernel<32, 4>, grid, dim3(kBmThreads), 0, st, a);
 }
 

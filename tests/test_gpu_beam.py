@@ -124,6 +124,21 @@ def test_orders_that_let_many_candidates_through(order):
 
 
 @gpu
+@pytest.mark.parametrize("G,B,V,stride", [(1, 4, 40000, 40000), (8, 8, 151936, 151936), (2, 64, 151936, 151936), (2, 40, 50001, 50003), (16, 16, 32768, 32769)])
+@pytest.mark.parametrize("equal", [False, True])
+def test_large_logits_that_sit_in_a_few_lanes(G, B, V, stride, equal):
+    """Every 1,024 ids eight of large logits: the same few threads hold all of the best, so that the maxima of the others say little.
+    Equal ones among them are more than a list holds."""
+    x = _logits(G * B, V, seed=V, stride=stride)
+    x.clamp_(max=8.0)
+    for j in range(8):
+        part = x[:, j::1024]
+        part.copy_(torch.full_like(part, 12.0) if equal else 12 + part.abs())
+    scores = -2 * torch.rand(G, B, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV)
+    _check(_run(x, scores), _reference(x, scores))
+
+
+@gpu
 def test_logits_that_a_32_bit_sum_would_merge_keep_their_order():
     x = torch.full((2, 5000), -30.0, device=DEV)
     x[0, 4000], x[0, 7] = 1.0 + 2.0 ** -23, 1.0        # the larger one has the higher id
