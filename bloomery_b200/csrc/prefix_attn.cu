@@ -23,6 +23,11 @@
 // Queries and probabilities are rounded to f16 (11 bits; queries scaled by a power of two a row): less than the output's 8 bits.
 // A value that is not finite would reach the masked rows of its tile as 0 x inf; rows whose output is not finite are summed again
 // key by key, over their own keys alone.
+// Device time of both launches in a graph (32 heads over 4 of 128 values): 4 rows behind 512 shared positions 10.5 us, 8 behind 2,048
+// 13.0, 21 behind 4,096 23.0, 24 rows of q8_0 behind three prefixes 29.6, 64 behind 32,768 62.7.  A short call is a chain of
+// latencies: launch, lengths and schedule, queries, a page, its softmax, the join.  A long one is bound by the softmax of a job, one
+// row a thread, and by the turns of the two tiles: about 1,200 clocks a job, the tensor pipe 32 % busy, 1.5 TB/s from memory; its
+// joining launch reads 19 MB of fragments in 8 us.
 // Every wait is bounded (1 s); on expiry the CTA raises the fault word, frees its TMEM and returns.
 #include <type_traits>
 
@@ -148,7 +153,9 @@ struct PxLine {
     n_units = a.n_units;
     cta = blockIdx.x;
     for (int i = threadIdx.x; i < n_units * kPxUnit; i += blockDim.x) units[i] = a.units[i];
-    const bool small = a.M <= 32;                               // then one warp has all in its registers
+    // One warp has up to 32 rows in its registers (4 rows behind 512 positions 10.5 us a call, 11.1 by way of shared memory; 24 q8_0
+    // rows 29.6 and 30.0).
+    const bool small = a.M <= 32;
     int unit[3] = {0, 0, 0}, own = 0, n_keys = 0;
     if (small && (int)threadIdx.x < n_units) {
 #pragma unroll
@@ -927,8 +934,9 @@ using namespace bl;
 
 template <int HEAD, bool Q8>
 static int prefix_go(PrefixArgs a, cudaStream_t st) {
-  // The joining launch.  Few rows: a block for 32 values of a head, so that more of its fragments are in flight; many: as much of it
-  // as 256 threads hold.
+  // The joining launch.  Few rows: a block for 32 values of a head, so that more of its fragments are in flight (8 rows behind 2,048
+  // positions 13.0 us a call, 15.2 with whole heads; 24 q8_0 rows 29.6 and 32.4); many: as much of it as 256 threads hold (100 rows
+  // 26.5 us, 32.6 in parts; 512 rows behind 1,024 positions 84.8 and 116.5).
   int z = HEAD / 32;
   const int G = a.n_q / a.n_kv;
   if (a.n_kv * a.M > a.n_cta) while (z > 1 && G * (HEAD / 4) / (z / 2) <= 256) z /= 2;
