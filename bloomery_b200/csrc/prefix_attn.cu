@@ -632,46 +632,47 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
       const int my = r < live ? x * rows_tile + (r * inv_G >> 16) : -3;     // row of the unit
       const int n_keys = r < live ? w.keys[w.row0 + my] : 0;
       const bool busy = quarter * 32 < live;
-      // Queries to f16, scaled by a power of two a row to a largest element in [512, 1024): each warp takes every fourth row, four
-      // or eight at a time.
+      // Queries to f16, scaled by a power of two a row to a largest element in [512, 1024).  Eight lanes have a row, so that a warp's
+      // steps serve four rows: a fragment goes through this code once or a few times, and most of its time is fetching it.
       auto put_queries = [&]() {
-        constexpr int N = HEAD / 32;
-        const float* base = a.q + ((long)(w.row0 + x * rows_tile) * a.n_q + f.kvh * G) * HEAD + lane * N;
-        uint8_t* dst = sQ + x * TILE + (lane * N >> 6) * kPxHalf + ((lane * N * 2) & 15);
-        const int chunk = (lane * N & 63) >> 3;
+        constexpr int N = HEAD / 32;                            // 16 bytes of a lane's, 128 bytes of its row apart
+        const int l = lane & 7;
+        const float* base = a.q + ((long)(w.row0 + x * rows_tile) * a.n_q + f.kvh * G) * HEAD + l * 4;
+        uint8_t* dst = sQ + x * TILE + (l & 1) * 8;
         auto some_rows = [&](int i0, auto at_once) {
           constexpr int AT_ONCE = decltype(at_once)::value;
-          float v[AT_ONCE][N];
+          float4 v[AT_ONCE][N];
 #pragma unroll
           for (int u = 0; u < AT_ONCE; ++u) {
             const int i = i0 + 4 * u;
             const float* src = base + (long)((i * inv_G >> 16) * (a.n_q - G) + i) * HEAD;
-            if constexpr (N == 4) {
-              const float4 q = i < live ? __ldg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
-              v[u][0] = q.x; v[u][1] = q.y; v[u][2] = q.z; v[u][3] = q.w;
-            } else {
-              const float2 q = i < live ? __ldg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
-              v[u][0] = q.x; v[u][1] = q.y;
-            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[u][j] = i < live ? __ldg(reinterpret_cast<const float4*>(src + j * 32)) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
           // no branches, so that the rows' chains of steps run side by side; rows behind the last are zeros
           unsigned top[AT_ONCE];
 #pragma unroll
           for (int u = 0; u < AT_ONCE; ++u) {
-            float most = fabsf(v[u][0]);
+            float most = 0.f;
 #pragma unroll
-            for (int j = 1; j < N; ++j) most = fmaxf(most, fabsf(v[u][j]));
-            top[u] = __reduce_max_sync(0xffffffffu, __float_as_uint(most));     // of non-negative floats: in order as integers
+            for (int j = 0; j < N; ++j)
+              most = fmaxf(fmaxf(most, fmaxf(fabsf(v[u][j].x), fabsf(v[u][j].y))), fmaxf(fabsf(v[u][j].z), fabsf(v[u][j].w)));
+            top[u] = __float_as_uint(most);                     // of non-negative floats: in order as integers
           }
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1)
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) top[u] = max(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
 #pragma unroll
           for (int u = 0; u < AT_ONCE; ++u) {
             const int i = i0 + 4 * u, e = (int)(top[u] >> 23), se = e == 0 ? 127 : min(253, 263 - e);
             const float scale = __uint_as_float((unsigned)se << 23);
-            uint8_t* at = dst + i * 128 + ((chunk ^ (i & 7)) << 4);
-            const uint32_t lo = px_pack(v[u][0] * scale, v[u][1] * scale);
-            if constexpr (N == 4) *reinterpret_cast<uint2*>(at) = make_uint2(lo, px_pack(v[u][2] * scale, v[u][3] * scale));
-            else *reinterpret_cast<uint32_t*>(at) = lo;
-            if (lane == u) s_scale[x][i] = kPxLog2e * __uint_as_float((unsigned)(254 - se) << 23);
+            uint8_t* at = dst + i * 128;
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+              *reinterpret_cast<uint2*>(at + (j >> 1) * kPxHalf + ((((j & 1) * 4 + (l >> 1)) ^ (i & 7)) << 4)) =
+                  make_uint2(px_pack(v[u][j].x * scale, v[u][j].y * scale), px_pack(v[u][j].z * scale, v[u][j].w * scale));
+            if (l == 0) s_scale[x][i] = kPxLog2e * __uint_as_float((unsigned)(254 - se) << 23);
           }
         };
         if (live > 16) {
@@ -680,12 +681,11 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
           int it = (int)((unsigned)blockIdx.x % (unsigned)n_it);
 #pragma unroll 1
           for (int k = 0; k < n_it; ++k) {
-            some_rows(quarter + 32 * it, std::integral_constant<int, 8>());
+            some_rows(8 * quarter + 32 * it + (lane >> 3), std::integral_constant<int, 2>());
             it = it + 1 == n_it ? 0 : it + 1;
           }
-        } else {
-#pragma unroll 1
-          for (int i0 = quarter; i0 < live; i0 += 16) some_rows(i0, std::integral_constant<int, 4>());
+        } else if (4 * quarter < live) {
+          some_rows(4 * quarter + (lane >> 3), std::integral_constant<int, 1>());
         }
         fence_async_smem();
         __syncwarp();
