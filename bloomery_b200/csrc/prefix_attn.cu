@@ -23,10 +23,10 @@
 // Queries and probabilities are rounded to f16 (11 bits; queries scaled by a power of two a row): less than the output's 8 bits.
 // A value that is not finite would reach the masked rows of its tile as 0 x inf; rows whose output is not finite are summed again
 // key by key, over their own keys alone.
-// Device time of both launches in a graph (32 heads over 4 of 128 values): 4 rows behind 512 shared positions 10.5 us, 8 behind 2,048
-// 13.0, 21 behind 4,096 23.0, 24 rows of q8_0 behind three prefixes 29.6, 64 behind 32,768 62.7.  A short call is a chain of
+// Device time of both launches in a graph (32 heads over 4 of 128 values): 4 rows behind 512 shared positions 10.0 us, 8 behind 2,048
+// 12.6, 21 behind 4,096 22.5, 24 rows of q8_0 behind three prefixes 29.8, 64 behind 32,768 61.3.  A short call is a chain of
 // latencies: launch, lengths and schedule, queries, a page, its softmax, the join.  A long one is bound by the softmax of a job, one
-// row a thread, and by the turns of the two tiles: about 1,200 clocks a job, the tensor pipe 32 % busy, 1.5 TB/s from memory; its
+// row a thread, and by the turns of the two tiles: about 1,200 clocks a job, the tensor pipe 32 % busy; its
 // joining launch reads 19 MB of fragments in 8 us.
 // Every wait is bounded (1 s); on expiry the CTA raises the fault word, frees its TMEM and returns.
 #include <type_traits>
