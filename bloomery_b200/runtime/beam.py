@@ -108,7 +108,7 @@ class BeamSearch:
         try:
             return self._search([list(map(int, p)) for p in prompts], n_new)
         finally:
-            kv.protect.difference_update(self.slots)
+            kv.pinned.difference_update(self.slots)
             for slot in self.slots:
                 e.reset(slot)
             kv.dirty = True                              # the tables were rewritten on the card
@@ -117,7 +117,7 @@ class BeamSearch:
 
     def _search(self, prompts: List[List[int]], n_new: int) -> List[List[Hypothesis]]:
         e, kv, bd, B, G, R = self.e, self.e.kv, self.bd, self.B, self.G, self.R
-        kv.protect.update(self.slots)
+        kv.pinned.update(self.slots)                     # from here on: a prompt's passes protect its own slot alone
         shared = []
         for g, prompt in enumerate(prompts):
             own = self.slots[g * B:(g + 1) * B]

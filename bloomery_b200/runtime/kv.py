@@ -49,7 +49,8 @@ class KvPool:
         # is copied to pinned host memory and its pages are reused; it comes back the next time it is needed
         # (the reference backs such pages with host memory in place: crates/gpu/src/room/mod.rs ``Backing::Spill``)
         self.spilled: Dict[int, tuple] = {}
-        self.protect: set = set()
+        self.protect: set = set()       # slots of the current pass: every pass names its own
+        self.pinned: set = set()        # slots that stay on the card from pass to pass, until their owner lets go
         self.stamp = [0] * n_slots
         self.clock = 0
         self.n_spills = 0
@@ -69,7 +70,7 @@ class KvPool:
         self.stamp[slot] = self.clock
 
     def _spill_one(self) -> bool:
-        victims = [s for s in range(self.n_slots) if self.pages[s] and s not in self.protect
+        victims = [s for s in range(self.n_slots) if self.pages[s] and s not in self.protect and s not in self.pinned
                    and all(self.refs[p] == 1 for p in self.pages[s])]
         if not victims or not self.allow_spill or self.n_pages * PAGE < self.floor_positions:
             return False

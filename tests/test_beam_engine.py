@@ -1,0 +1,100 @@
+"""What a beam search does to the engine around it, without a card: pages, their protection, and the order of streams.  The engine
+is a page pool with the bookkeeping of :class:`DecodeEngine`; the launches of a search are left out."""
+import contextlib
+import threading
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from bloomery_b200.runtime import beam
+from bloomery_b200.runtime.beam import BeamSearch
+from bloomery_b200.runtime.kv import PAGE, KvPool, OutOfPages
+
+
+class Reached(Exception):
+    """The launches of the first step would come next."""
+
+
+class FakeStream:
+    def __init__(self, name, log):
+        self.name, self.log = name, log
+
+    def wait_stream(self, other):
+        self.log.append((self.name, "waits for", other.name))
+
+
+class FakeEngine:
+    def __init__(self, n_pages, n_slots, max_pages, log):
+        self.kv = KvPool(1, 1, 4, n_pages, n_slots, max_pages, "cpu")
+        self.n_slots, self.slot_ctx, self.device = n_slots, max_pages * PAGE, "cpu"
+        self._lock, self.log = threading.Lock(), log
+
+    def reset(self, slot):
+        self.kv.truncate(slot, 0)
+
+    def prefill(self, slot, tokens):
+        with self._lock:
+            for i in range(0, len(tokens), 8):             # the 8-row pass: set_rows
+                self.kv.protect = {slot}
+                for pos in range(i, min(i + 8, len(tokens))):
+                    self.kv.ensure(slot, pos + 1)
+                    self.kv.own(slot, pos)
+
+
+@pytest.fixture
+def make(monkeypatch):
+    log = []
+    caller, current = FakeStream("caller", log), []
+    current.append(caller)
+
+    @contextlib.contextmanager
+    def stream(s):
+        current.append(s)
+        try:
+            yield
+        finally:
+            current.pop()
+
+    monkeypatch.setattr(torch.cuda, "stream", stream)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: current[-1])
+
+    def build(n_pages, n_slots, max_pages, beams, groups, first_slot=0):
+        e = FakeEngine(n_pages, n_slots, max_pages, log)
+        s = object.__new__(BeamSearch)
+        s.e, s.B, s.G, s.max_new, s.alpha, s.eos = e, beams, groups, 128, 0.0, -1
+        s.R = s.M = beams * groups
+        s.slots = list(range(first_slot, first_slot + s.R))
+        s.bd = SimpleNamespace(_stream=FakeStream("steps", log))
+
+        def first_step(shared):
+            log.append((current[-1].name, "first step", None))
+            assert all(e.kv.pages[x] for x in s.slots), "a beam without pages"
+            raise Reached
+        s.plan = SimpleNamespace(set_prefix=first_step)
+        for name in ("snapshot", "sync_table"):
+            def traced(*a, _f=getattr(e.kv, name), _n=name, **kw):
+                log.append((current[-1].name, _n, a[0] if a else None))
+                return _f(*a, **kw)
+            monkeypatch.setattr(e.kv, name, traced)
+        return s, e, log
+    return build
+
+
+def test_a_later_prompt_does_not_take_an_earlier_ones_pages(make):
+    """Nine pages; two searches of two beams whose prompts end in their first page, three pages a beam.  A prompt's passes
+    protect its own slot alone."""
+    s, e, log = make(9, 6, 4, beams=2, groups=2)
+    with pytest.raises(OutOfPages):
+        s.search([[1] * 21, [2] * 21], 110)
+    assert not e.kv.spilled and e.kv.n_spills == 0 and ("steps", "first step", None) not in log
+    assert e.kv.free_pages() == 9 and not e.kv.pinned
+
+
+def test_an_idle_sequence_makes_room_and_beams_keep_theirs(make):
+    s, e, log = make(9, 6, 4, beams=2, groups=2, first_slot=1)
+    e.prefill(0, [7] * 70)                                 # two pages that nobody needs now
+    with pytest.raises(Reached):
+        s.search([[1] * 21, [2] * 21], 80)                 # two pages a beam
+    assert set(e.kv.spilled) == {0} and e.kv.n_spills == 1
+    assert e.kv.free_pages() == 9 and not e.kv.pinned
