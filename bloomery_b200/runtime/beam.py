@@ -108,29 +108,35 @@ class BeamSearch:
         try:
             return self._search([list(map(int, p)) for p in prompts], n_new)
         finally:
-            kv.pinned.difference_update(self.slots)
-            for slot in self.slots:
-                e.reset(slot)
-            kv.dirty = True                              # the tables were rewritten on the card
-            with torch.cuda.stream(self.bd._stream):
+            with e._lock:
+                # whoever gets these pages, and the table, next does so behind the steps
+                torch.cuda.current_stream(e.device).wait_stream(self.bd._stream)
+                kv.pinned.difference_update(self.slots)
+                for slot in self.slots:
+                    e.reset(slot)
+                kv.dirty = True                          # the tables were rewritten on the card
                 kv.sync_table()
 
     def _search(self, prompts: List[List[int]], n_new: int) -> List[List[Hypothesis]]:
         e, kv, bd, B, G, R = self.e, self.e.kv, self.bd, self.B, self.G, self.R
-        kv.pinned.update(self.slots)                     # from here on: a prompt's passes protect its own slot alone
         shared = []
         for g, prompt in enumerate(prompts):
             own = self.slots[g * B:(g + 1) * B]
-            for slot in own:
-                e.reset(slot)
+            with e._lock:
+                kv.pinned.update(own)                    # from here on: a prompt's passes protect its own slot alone
+                for slot in own:
+                    e.reset(slot)
             n = len(prompt) - 1                          # the last id is the first pass's
             if n:
                 e.prefill(own[0], prompt[:n])
-            for slot in own[1:]:
-                kv.share_prefix(own[0], slot, n)
-            for slot in own:
-                kv.ensure(slot, len(prompt) + n_new)     # pages behind the shared ones belong to a beam each
+            with e._lock:
+                for slot in own[1:]:
+                    kv.share_prefix(own[0], slot, n)
+                for slot in own:
+                    kv.ensure(slot, len(prompt) + n_new)     # pages behind the shared ones belong to a beam each
             shared.append(n // PAGE * PAGE if B > 1 else 0)
+        # sequences that made room for the beams are copied out on this stream: the steps write their pages behind that
+        bd._stream.wait_stream(torch.cuda.current_stream(e.device))
         with e._lock, torch.cuda.stream(bd._stream):
             self.plan.set_prefix(shared + [0] * (self.M > R))
             kv.sync_table()

@@ -98,3 +98,30 @@ def test_an_idle_sequence_makes_room_and_beams_keep_theirs(make):
         s.search([[1] * 21, [2] * 21], 80)                 # two pages a beam
     assert set(e.kv.spilled) == {0} and e.kv.n_spills == 1
     assert e.kv.free_pages() == 9 and not e.kv.pinned
+
+
+def test_steps_wait_for_what_made_room_and_the_caller_for_the_steps(make):
+    """The copy of a sequence that makes room runs on the caller's stream: the steps that write its pages come behind it, and
+    the caller's next work, the table first, behind the steps."""
+    s, e, log = make(9, 6, 4, beams=2, groups=2, first_slot=1)
+    e.prefill(0, [7] * 70)
+    e.kv.protect = {5}                                     # as after a pass over another slot
+    with pytest.raises(Reached):
+        s.search([[1], [2]], 100)                          # two pages a beam, no prompt pass that the host waits for
+    spill, step = log.index(("caller", "snapshot", 0)), log.index(("steps", "first step", None))
+    assert ("steps", "waits for", "caller") in log[spill:step]
+    behind = log.index(("caller", "waits for", "steps"), step)
+    assert log.index(("caller", "sync_table", None), step) > behind
+    assert ("steps", "sync_table", None) not in log[step:]
+
+
+def test_pages_change_hands_under_the_engines_lock(make, monkeypatch):
+    s, e, log = make(9, 6, 4, beams=2, groups=2)
+    for name in ("ensure", "share_prefix", "truncate"):
+        def held(*a, _f=getattr(e.kv, name), _n=name, **kw):
+            assert e._lock.locked(), _n
+            return _f(*a, **kw)
+        monkeypatch.setattr(e.kv, name, held)
+    with pytest.raises(Reached):
+        s.search([[1] * 70, [2] * 5], 20)
+    assert not e._lock.locked()
