@@ -38,7 +38,10 @@ class BeamSearch:
 
     def __init__(self, engine, beams: int, groups: int = 1, eos: Optional[int] = None, alpha: float = 0.0, max_new: int = 512,
                  first_slot: int = 0):
+        from .engine import DecodeEngine
         s = engine.spec
+        if type(engine) is not DecodeEngine:             # their experts are elsewhere, or on several cards
+            raise NotImplementedError("beam search runs on a whole model on one card; tiered and sharded engines keep their own passes")
         if s.mla:
             raise NotImplementedError("beam search runs on grouped-query attention")
         if not 1 <= beams <= MAX_BEAMS or groups < 1 or beams * groups > BUCKETS[-1]:

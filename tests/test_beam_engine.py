@@ -125,3 +125,14 @@ def test_pages_change_hands_under_the_engines_lock(make, monkeypatch):
     with pytest.raises(Reached):
         s.search([[1] * 70, [2] * 5], 20)
     assert not e._lock.locked()
+
+
+def test_engines_whose_experts_are_elsewhere_are_refused():
+    """The batched pass would hand host stacks, or a rank's share of them, to the kernels."""
+    from bloomery_b200.parallel.sharded import ShardedEngine
+    from bloomery_b200.runtime.tiered import TieredEngine
+    for kind in (TieredEngine, ShardedEngine):
+        e = object.__new__(kind)
+        e.spec, e.n_slots = SimpleNamespace(mla=False, eos_id=2), 8
+        with pytest.raises(NotImplementedError):
+            BeamSearch(e, 4)
