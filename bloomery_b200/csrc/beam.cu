@@ -652,6 +652,18 @@ int bl_beam_select(const BeamSelectCall* call) {
   BL_REQUIRE(B <= kMaxBeams && (long)G * B <= 65535 && (long)chunks * B <= kBmMaxCells, BL_ERR_LIMIT);
   BL_REQUIRE(eos < V && (!done || eos >= 0) && (alpha == 0.f || lengths) && (!out_lengths || lengths), BL_ERR_SHAPE);
   BL_REQUIRE(((uintptr_t)logits & 3) == 0 && ((uintptr_t)work & 7) == 0, BL_ERR_ALIGN);
+  // Outputs lie apart from what is read.  Blocks of a search that has been written may still be to start: one that found another
+  // flag in `done` than its row had would take a ticket that nobody counts, and every later call with this scratch would be off.
+  const void* const out[5] = {parent, token, out_scores, out_done, out_lengths};
+  const void* const in[4] = {scores, done, lengths, logits};
+  const size_t cell = (size_t)G * B * 4, rows = (((size_t)G * B - 1) * stride + V) * 4;
+  auto apart = [](const void* p, size_t n, const void* q, size_t m) {
+    return !p || !q || (uintptr_t)p + n <= (uintptr_t)q || (uintptr_t)q + m <= (uintptr_t)p;
+  };
+  for (int i = 0; i < 5; ++i) {
+    for (int j = 0; j < 4; ++j) BL_REQUIRE(apart(out[i], cell, in[j], j == 3 ? rows : cell), BL_ERR_SHAPE);
+    for (int j = 0; j < i; ++j) BL_REQUIRE(apart(out[i], cell, out[j], cell), BL_ERR_SHAPE);
+  }
   BeamArgs a{logits, stride, V, G, B, scores, done, lengths, eos, alpha};
   a.chunk = beam_chunk(V, chunks);
   a.n_chunks = (V + a.chunk - 1) / a.chunk;

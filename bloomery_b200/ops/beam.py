@@ -66,7 +66,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, scratch: BeamScratch
     counted.  ``out_done`` / ``out_lengths``: the same of the next beams.  Ties go to the lower beam, then to the lower id.  Ids with
     a logit of -inf are no candidates; where a search has too few, the last places get parent = their own index, token ``eos`` (0
     without one), score -inf and done.  A search with a NaN or +inf among its logits or scores gets NaN scores and raises
-    ``fault``."""
+    ``fault``.  The outputs are tensors of their own: blocks that start late still read the inputs when the first places of a
+    search are written."""
     G, B, V, index = scratch.groups, scratch.beams, scratch.vocab, scratch.index
     n = G * B
     if logits.dtype is not torch.float32 or logits.shape != (n, V) or (logits.stride(1) != 1 and V > 1):
@@ -81,6 +82,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, scratch: BeamScratch
           _same("out_done", out_done, i32, n, index) if out_done is not None else 0,
           _same("out_lengths", out_lengths, i32, n, index) if out_lengths is not None else 0,
           fault.data_ptr() if fault is not None else 0)
+    if any(t and t in at[4:9] for t in at[:3]):
+        raise ValueError("the next beams are written while the old ones are read: other tensors")
     if eos >= V or (done is not None and eos < 0):
         raise ValueError("finished beams need the id of the end")
     if lengths is None and (alpha != 0.0 or out_lengths is not None):

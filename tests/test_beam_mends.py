@@ -1,0 +1,50 @@
+"""Calls of the beam operators that were taken although no kernel can serve them, without a card."""
+import ctypes
+
+import pytest
+import torch
+
+from bloomery_b200.ops import beam
+from bloomery_b200.ops._lib import cuda
+
+SHAPE = -2
+A = 0x1000000        # an aligned address nothing reads
+
+
+def _cells(dtype=torch.int32):
+    return torch.zeros(2, 3, dtype=dtype)
+
+
+def _select(**kw):
+    a = dict(logits=torch.zeros(6, 10), scores=_cells(torch.float32), scratch=beam.BeamScratch(2, 3, 10, "cpu"), parent=_cells(),
+             token=_cells(), out_scores=_cells(torch.float32), done=_cells(), lengths=_cells(), out_done=_cells(), out_lengths=_cells(),
+             eos=1)
+    a.update(kw)
+    beam.beam_select(**a)
+
+
+def test_a_choice_in_place_is_refused():
+    with pytest.raises(ValueError, match="CUDA device"):
+        _select()                                          # everything else is in order
+    x, i = _cells(torch.float32), _cells()
+    for kw in (dict(scores=x, out_scores=x), dict(done=i, out_done=i), dict(lengths=i, out_lengths=i), dict(done=i, out_lengths=i),
+               dict(done=i, parent=i)):
+        with pytest.raises(ValueError, match="other tensors"):
+            _select(**kw)
+
+
+@pytest.mark.parametrize("out", ["parent", "token", "out_scores", "out_done", "out_lengths"])
+@pytest.mark.parametrize("over", ["scores", "done", "lengths", "logits", "parent"])
+@pytest.mark.parametrize("off", [-28, 0, 28])
+def test_outputs_over_what_is_read_are_refused_before_the_launch(out, over, off):
+    """Two searches of four: 32 bytes a tensor; the logits are 28,000 bytes before their last row."""
+    if out == over:
+        return
+    names = ["logits", "scores", "done", "lengths", "work", "parent", "token", "out_scores", "out_done", "out_lengths"]
+    call = dict(logits=A, stride=1000, scores=0, done=0, lengths=0, work=0, parent=0, token=0, out_scores=0, out_done=0, out_lengths=0,
+                fault=0, stream=0, V=1000, G=2, B=4, eos=5, chunks=1, alpha=0.5)
+    call |= {n: A + (i << 16) for i, n in enumerate(names)}
+    call[out] = call[over] + (31000 if over == "logits" else 0) + off
+    fn = cuda().bl_beam_select
+    fn.argtypes = [ctypes.c_char_p]
+    assert fn(beam._SELECT.pack(*call.values())) == SHAPE
