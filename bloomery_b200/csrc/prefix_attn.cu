@@ -61,6 +61,10 @@ struct PrefixArgs {
 };
 constexpr int kPxMeta = 5, kPxUnit = 5;
 
+// Shared pages of a unit or a row, out of their positions: of a prefix longer than a table row, as far as the row goes.  (A plan's
+// lengths are written on the card behind the call that a graph replays; a row has no keys behind its table row.)
+__device__ __forceinline__ int px_shared(const PrefixArgs& a, int positions) { return min(positions / kPxPage, a.max_pages); }
+
 // Keys of row m: 0 for a dead row and for one that cannot be served.
 __device__ __forceinline__ int px_keys(const PrefixArgs& a, int m, bool& bad) {
   const int seq = a.row_seq[m], n = a.row_pos[m] + 1;
@@ -125,7 +129,7 @@ struct PxLine {
   int* pages;                     // [M + 1] running sum of the rows' own pages
   int* cum;                       // [n_units + 1] running sum of the units' pages
   int* seq;                       // [M]
-  int* units;                     // [n_units][kPxUnit]
+  int* units;                     // [n_units][kPxUnit], shared pages in place of positions
   int n_units, S, g, end, cta;
 
   __device__ __forceinline__ static int find(const int* cum, int n, int at) {      // the last i with cum[i] <= at
@@ -152,7 +156,7 @@ struct PxLine {
     keys = mem; pages = keys + a.M; cum = pages + a.M + 1; seq = cum + a.n_units + 1; units = seq + a.M;
     n_units = a.n_units;
     cta = blockIdx.x;
-    for (int i = threadIdx.x; i < n_units * kPxUnit; i += blockDim.x) units[i] = a.units[i];
+    for (int i = threadIdx.x; i < n_units * kPxUnit; i += blockDim.x) units[i] = i % kPxUnit == 2 ? px_shared(a, a.units[i]) : a.units[i];
     // One warp has up to 32 rows in its registers (4 rows behind 512 positions 10.5 us a call, 11.1 by way of shared memory; 24 q8_0
     // rows 29.6 and 30.0).
     const bool small = a.M <= 32;
@@ -160,16 +164,17 @@ struct PxLine {
     if (small && (int)threadIdx.x < n_units) {
 #pragma unroll
       for (int i = 0; i < 3; ++i) unit[i] = a.units[threadIdx.x * kPxUnit + i];
+      unit[2] = px_shared(a, unit[2]);
     }
     for (int m = threadIdx.x; m < a.M; m += blockDim.x) {
-      const int shared = a.meta[m * kPxMeta + 2], sq = a.row_seq[m];
+      const int shared = px_shared(a, a.meta[m * kPxMeta + 2]), sq = a.row_seq[m];
       bool bad;
       const int n = px_keys(a, m, bad);
       if (bad && blockIdx.x == 0) raise_fault(a.fault, a.layer, FS_KEY_COUNT);
       keys[m] = n;
       seq[m] = sq;
       n_keys = n;
-      own = max(0, n - shared + kPxPage - 1) / kPxPage;
+      own = max(0, n - shared * kPxPage + kPxPage - 1) / kPxPage;
       pages[m + 1] = own;
     }
     if (small) {
@@ -185,7 +190,7 @@ struct PxLine {
         const int upto = __shfl_sync(0xffffffffu, sum, (unit[0] + unit[1] - 1) & 31), prev = __shfl_sync(0xffffffffu, sum, (unit[0] - 1) & 31);
         const int before = unit[0] ? prev : 0;
         const unsigned mine = unit[1] >= 32 ? 0xffffffffu : (1u << unit[1]) - 1;
-        const int total = scan((live >> unit[0] & mine) != 0 ? unit[2] / kPxPage + upto - before : 0);
+        const int total = scan((live >> unit[0] & mine) != 0 ? unit[2] + upto - before : 0);
         S = __shfl_sync(0xffffffffu, total, 31);
         const unsigned T = (unsigned)(a.n_kv * S), n = px_ctas(a, T);
         g = (unsigned)cta < n ? (int)((unsigned)cta * T / n) : 0;
@@ -202,7 +207,7 @@ struct PxLine {
           f.id = f.kvh * n_units + f.unit + cta;
           f.row0 = __shfl_sync(0xffffffffu, unit[0], f.unit);
           f.rows = __shfl_sync(0xffffffffu, unit[1], f.unit);
-          f.shared = __shfl_sync(0xffffffffu, unit[2], f.unit) / kPxPage;
+          f.shared = __shfl_sync(0xffffffffu, unit[2], f.unit);
           const int skip = f.lo - f.shared + __shfl_sync(0xffffffffu, before, f.unit);
           f.row = f.lo > f.shared ? __popc(__ballot_sync(0xffffffffu, sum <= skip)) : f.row0;
           g += f.end - f.lo;
@@ -226,7 +231,7 @@ struct PxLine {
           const int* unit = units + u * kPxUnit;
           int live = 0;                                           // a unit without a live row reads nothing
           for (int m = unit[0]; !live && m < unit[0] + unit[1]; ++m) live = keys[m];
-          cum[u + 1] = live ? unit[2] / kPxPage + pages[unit[0] + unit[1]] - pages[unit[0]] : 0;
+          cum[u + 1] = live ? unit[2] + pages[unit[0] + unit[1]] - pages[unit[0]] : 0;
         }
         __syncwarp();
         running(cum, n_units);
@@ -250,7 +255,7 @@ struct PxLine {
     // for the launch that joins the fragments
     if (blockIdx.x == 0)
       for (int m = threadIdx.x; m < a.M; m += blockDim.x) {
-        const int u = a.meta[m * kPxMeta + 3], shared = units[u * kPxUnit + 2] / kPxPage;
+        const int u = a.meta[m * kPxMeta + 3], shared = units[u * kPxUnit + 2];
         a.sched[2 * m] = make_int4(S, cum[u], shared, keys[m]);
         a.sched[2 * m + 1] = make_int4(shared + pages[m] - pages[units[u * kPxUnit]], pages[m + 1] - pages[m], u, a.meta[m * kPxMeta + 4]);
       }
@@ -271,7 +276,7 @@ struct PxLine {
     f.id = f.kvh * n_units + f.unit + cta;
     g += n;
     const int* unit = units + f.unit * kPxUnit;
-    f.row0 = unit[0]; f.rows = unit[1]; f.shared = unit[2] / kPxPage;
+    f.row0 = unit[0]; f.rows = unit[1]; f.shared = unit[2];
     f.row = f.row0;
     if (f.lo > f.shared) f.row = f.row0 + find(pages + f.row0, f.rows, pages[f.row0] + f.lo - f.shared);
     return true;

@@ -43,6 +43,7 @@ class PrefixPlan:
         self.q_shape, self.out_shape = (sum(group_rows), n_q, head), (sum(group_rows), n_q * head)
         if self.rows > 512:
             raise ValueError("at most 512 rows")
+        self.max_pages = None                             # of the narrowest table that a call of the plan came with
         rows = self._meta(prefix_len)
         self.n_units, self.unit_rows = len(rows) - self.rows, max(u[1] for u in rows[self.rows:])
         self.meta = torch.tensor(rows, dtype=torch.int32).to(self.device)
@@ -57,6 +58,8 @@ class PrefixPlan:
             raise ValueError("a prefix length for every group")
         if any(n < 0 or n % PAGE for n in prefix_len):
             raise ValueError(f"shared positions are whole pages of {PAGE}")
+        if self.max_pages is not None and max(prefix_len) > self.max_pages * PAGE:
+            raise ValueError(f"the prefix is longer than a table row of {self.max_pages} pages")
         self.prefix_len, self.max_prefix = list(prefix_len), max(prefix_len)
         # units: rows of a group that read all of their keys together, as many as two tiles of 128 (row, head) pairs of a key
         # head hold
@@ -70,7 +73,8 @@ class PrefixPlan:
         return rows + units
 
     def set_prefix(self, prefix_len: Sequence[int]) -> None:
-        """Other shared positions for the same groups; graphs captured with the plan take them up."""
+        """Other shared positions for the same groups, within the table rows that the plan was called with; graphs captured with
+        the plan take them up."""
         self.meta.copy_(torch.tensor(self._meta(prefix_len), dtype=torch.int32))
 
 
@@ -102,6 +106,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError("block_table: contiguous int32 [slots, pages]")
     if plan.max_prefix > table[1] * PAGE:
         raise ValueError("the prefix is longer than a table row")
+    if plan.max_pages is None or table[1] < plan.max_pages:
+        plan.max_pages = table[1]                        # a graph captured with this call goes on with this table
     index = plan.index
     for t in (q, k_cache, v_cache, row_pos, row_seq, block_table, out):
         if t.get_device() != index:

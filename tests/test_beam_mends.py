@@ -48,3 +48,21 @@ def test_outputs_over_what_is_read_are_refused_before_the_launch(out, over, off)
     fn = cuda().bl_beam_select
     fn.argtypes = [ctypes.c_char_p]
     assert fn(beam._SELECT.pack(*call.values())) == SHAPE
+
+
+def test_a_plan_takes_no_prefix_that_its_tables_cannot_hold():
+    """A replayed graph checks nothing: the lengths that it will find are checked where they are set."""
+    from bloomery_b200.ops.prefix import PrefixPlan, prefix_attention
+    plan = PrefixPlan([2], [64], 4, 2, 64, "cpu")
+    plan.set_prefix([640])                                 # no call so far
+    plan.set_prefix([64])
+    cache = torch.zeros(3, 2, 64, 64, dtype=torch.float16)
+    rows = torch.zeros(2, dtype=torch.int32)
+    for pages in (9, 4, 6):
+        with pytest.raises(ValueError, match="CUDA device"):
+            prefix_attention(torch.zeros(2, 4, 64), cache, cache, rows, rows, torch.zeros(2, pages, dtype=torch.int32), plan,
+                             torch.zeros(2, 256, dtype=torch.bfloat16))
+    plan.set_prefix([256])
+    with pytest.raises(ValueError, match="longer than a table row of 4"):
+        plan.set_prefix([320])
+    assert plan.prefix_len == [256] and plan.meta[0, 2] == 256
