@@ -558,6 +558,7 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(const ReorderArgs a) 
   const int* own = a.table + (long)slot * a.max_pages;
   const int* from = own;
   int place = -1, source = -1;                            // the page being filled, and what is copied into it
+  bool copies = false, lost = false;                      // takes another page over; a page that the pools do not have
   if (bad) {                                              // nobody moves
     if (tid == 0) raise_fault(a.fault, layer, FS_BEAM);
   } else {
@@ -566,19 +567,22 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(const ReorderArgs a) 
       const unsigned long long more = s_more[0] | (unsigned long long)s_more[1] << 32;
       unsigned long long bare = s_bare[0] | (unsigned long long)s_bare[1] << 32;
       place = from[col];
-      if (more >> i & 1) {
+      copies = more >> i & 1;
+      if (copies) {
         for (int n = __popcll(more & ((1ull << i) - 1)); n > 0; --n) bare &= bare - 1;
         source = place;
         place = a.table[(long)a.slots[r0 + __ffsll((long long)bare) - 1] * a.max_pages + col];
       }
+      // a beam that goes on in its own slot changes nothing here, pages or not (a place without a beam)
+      lost = (copies || s_parent[i] != i) && (place < 0 || place >= a.n_pages || (copies && (source < 0 || source >= a.n_pages)));
+      if (lost && tid == 0) raise_fault(a.fault, layer, FS_PAGE);
     }
   }
-  if (layer == 0) {
+  if (layer == 0) {                                       // a child whose history is not there keeps its slot's row
     int* to = a.table_out + (long)slot * a.max_pages;
-    for (int c = tid; c < a.max_pages; c += 256) to[c] = !bad && c < col ? from[c] : place >= 0 && c == col ? place : own[c];
+    for (int c = tid; c < a.max_pages; c += 256) to[c] = bad || lost || c > col ? own[c] : c < col ? from[c] : part ? place : own[c];
   }
-  if (source < 0) return;
-  if (source >= a.n_pages || place < 0 || place >= a.n_pages) { if (tid == 0) raise_fault(a.fault, layer, FS_PAGE); return; }
+  if (!copies || lost) return;
   const long src = ((long)layer * a.n_pages + source) * a.n_kv * kBeamPage, dst = ((long)layer * a.n_pages + place) * a.n_kv * kBeamPage;
   copy_heads(a.k + dst * a.k_row, a.k + src * a.k_row, part * (int)a.k_row, kBeamPage * (int)a.k_row, a.n_kv);
   if (a.v_row) copy_heads(a.v + dst * a.v_row, a.v + src * a.v_row, part * (int)a.v_row, kBeamPage * (int)a.v_row, a.n_kv);

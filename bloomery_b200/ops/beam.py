@@ -105,7 +105,8 @@ def beam_reorder(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, table_ou
     values).  ``table_out``, another table than ``table``, gets the rows of these slots: full pages are the parent's, pages behind the
     one being filled stay the slot's.  In the page being filled a parent's first child goes on; each further child takes
     over the page of a beam that has none and a copy of the positions in it.  The pages from the one being filled on must belong
-    to one slot each.  A search whose parents, slots or positions are out of range stays as it is and raises ``fault``."""
+    to one slot each.  A search whose parents, slots or positions are out of range stays as it is and raises ``fault``;
+    so does a child whose page being filled, its parent's or the one it takes over, is none of the pools'."""
     G, B = parent.shape
     index = k.get_device()
     at = (_same("slots", slots, torch.int32, G * B, index), _same("parent", parent, torch.int32, G * B, index),
