@@ -75,7 +75,10 @@ def stream() -> ctypes.c_void_p:
 
 
 def raw_stream(index: int) -> int:
-    """The handle of the current stream of device ``index``, without the object that :func:`stream` makes (a microsecond a call)."""
+    """The handle of the current stream of device ``index``, without the object that :func:`stream` makes (a microsecond a call).
+    Launches go to the current device: tensors of another one are refused, its default stream has the same handle."""
+    if torch._C._cuda_getDevice() != index:
+        raise ValueError(f"the tensors are on cuda:{index}, which is not the current device")
     return torch._C._cuda_getCurrentRawStream(index)
 
 

@@ -66,3 +66,34 @@ def test_a_plan_takes_no_prefix_that_its_tables_cannot_hold():
     with pytest.raises(ValueError, match="longer than a table row of 4"):
         plan.set_prefix([320])
     assert plan.prefix_len == [256] and plan.meta[0, 2] == 256
+
+
+def test_launches_for_another_device_than_the_current_one_are_refused(monkeypatch):
+    from bloomery_b200.ops import prefix
+    from bloomery_b200.ops._lib import raw_stream
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 40 + index, raising=False)
+    assert raw_stream(0) == 40
+    with pytest.raises(ValueError, match="not the current device"):
+        raw_stream(1)
+
+    # the calls take their stream from there: tensors that say they are on the second card
+    class Far(torch.Tensor):
+        def get_device(self):
+            return 1
+
+    def far(*shape, dtype=torch.int32):
+        return torch.zeros(*shape, dtype=dtype).as_subclass(Far)
+    scratch = beam.BeamScratch(2, 3, 10, "cpu")
+    scratch.index = 1
+    with pytest.raises(ValueError, match="not the current device"):
+        beam.beam_select(far(6, 10, dtype=torch.float32), far(2, 3, dtype=torch.float32), scratch, far(2, 3), far(2, 3),
+                         far(2, 3, dtype=torch.float32))
+    with pytest.raises(ValueError, match="not the current device"):
+        beam.beam_reorder(far(1, 4, 1, 64, 8), far(1, 4, 1, 64, 8), far(2, 4), far(2, 4), far(2), far(1, 2), far(1))
+    plan = prefix.PrefixPlan([2], [64], 4, 2, 64, "cpu")
+    plan.index = 1
+    cache = far(3, 2, 64, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="not the current device"):
+        prefix.prefix_attention(far(2, 4, 64, dtype=torch.float32), cache, cache, far(2), far(2), far(2, 4), plan,
+                                far(2, 256, dtype=torch.bfloat16))
