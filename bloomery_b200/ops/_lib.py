@@ -82,6 +82,15 @@ def raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def fault_ptr(fault: Optional[torch.Tensor], index: int) -> int:
+    """The address of a fault word, 0 for none: one int32 on device ``index``."""
+    if fault is None:
+        return 0
+    if fault.dtype is not torch.int32 or fault.numel() < 1 or fault.get_device() != index:
+        raise ValueError("fault: an int32 on the device of the rest")
+    return fault.data_ptr()
+
+
 I = ctypes.c_int
 L = ctypes.c_long
 F = ctypes.c_float

@@ -13,7 +13,7 @@ from typing import Optional, Sequence
 import torch
 
 from ..runtime.kv import PAGE
-from ._lib import check, cuda, raw_stream
+from ._lib import check, cuda, fault_ptr, raw_stream
 from .decode import sm_count
 
 _entry = None
@@ -112,6 +112,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     for t in (q, k_cache, v_cache, row_pos, row_seq, block_table, out):
         if t.get_device() != index:
             raise ValueError("the tensors are on the plan's device")
+    fault_at = fault_ptr(fault, index)
     if index < 0:
         raise ValueError("the kernels need a CUDA device")
     if _entry is None:
@@ -119,7 +120,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         _entry.argtypes = [ctypes.c_char_p]
     code = _entry(_CALL.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), row_pos.data_ptr(), row_seq.data_ptr(),
                              block_table.data_ptr(), plan.meta_ptr, plan.work_ptr, out.data_ptr(),
-                             fault.data_ptr() if fault is not None else 0, raw_stream(index), table[0], table[1], shape[0], head,
+                             fault_at, raw_stream(index), table[0], table[1], shape[0], head,
                              plan.n_q, n_kv, rows, plan.n_units, plan.unit_rows, q8, plan.n_cta, layer))
     if code:
         check(code, "bl_prefix_attention")

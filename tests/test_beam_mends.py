@@ -97,3 +97,24 @@ def test_launches_for_another_device_than_the_current_one_are_refused(monkeypatc
     with pytest.raises(ValueError, match="not the current device"):
         prefix.prefix_attention(far(2, 4, 64, dtype=torch.float32), cache, cache, far(2), far(2), far(2, 4), plan,
                                 far(2, 256, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("fault", [torch.zeros(1, dtype=torch.int64), torch.zeros(0, dtype=torch.int32), torch.zeros(1),
+                                   torch.zeros(1, dtype=torch.int32, device="meta")])
+def test_a_fault_word_is_an_int32_on_the_device_of_the_rest(fault):
+    from bloomery_b200.ops.prefix import PrefixPlan, prefix_attention
+    if fault.device.type == "meta":                        # a tensor of some other device
+        fault = fault.as_subclass(type("Far", (torch.Tensor,), {"get_device": lambda self: 0}))
+    cache, rows = torch.zeros(3, 2, 64, 64, dtype=torch.float16), torch.zeros(2, dtype=torch.int32)
+    calls = [
+        lambda f: _select(fault=f),
+        lambda f: beam.beam_reorder(torch.zeros(1, 4, 1, 64, 8), torch.zeros(1, 4, 1, 64, 8), torch.zeros(2, 4, dtype=torch.int32),
+                                    torch.zeros(2, 4, dtype=torch.int32), rows, rows.view(1, 2), rows[:1], f),
+        lambda f: prefix_attention(torch.zeros(2, 4, 64), cache, cache, rows, rows, torch.zeros(2, 4, dtype=torch.int32),
+                                   PrefixPlan([2], [64], 4, 2, 64, "cpu"), torch.zeros(2, 256, dtype=torch.bfloat16), f),
+    ]
+    for call in calls:
+        with pytest.raises(ValueError, match="CUDA device"):
+            call(torch.zeros(1, dtype=torch.int32))        # everything else is in order
+        with pytest.raises(ValueError, match="fault"):
+            call(fault)
