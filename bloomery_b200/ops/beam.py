@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from ..runtime.kv import PAGE
-from ._lib import I, check, cuda, fault_ptr, p, raw_stream, stream
+from ._lib import I, check, cuda, fault_ptr, p, raw_stream
 from .decode import sm_count
 
 MAX_BEAMS = 64
@@ -133,5 +133,20 @@ def beam_reorder(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, table_ou
 def beam_advance(tokens, row_pos, row_seq, held, hist, count, slots, parent, token, done, scores, G: int, B: int) -> None:
     """The rows of the next pass out of a choice: tokens, positions one further, sequences (-1 for finished and missing beams);
     ``held`` [G] one more; ``hist`` int32 [cap, 2, G * B] takes the parents and tokens of step ``count``."""
+    index, n, i32 = tokens.get_device(), G * B, torch.int32
+    if G < 1 or B < 1 or n > 65535:
+        raise ValueError("1 to 65,535 beams in all")
+    for name, t in (("tokens", tokens), ("row_pos", row_pos), ("row_seq", row_seq)):
+        if t.dtype is not i32 or t.dim() != 1 or t.numel() < n or not t.is_contiguous() or t.get_device() != index:
+            raise ValueError(f"{name}: contiguous int32, {n} rows at least, on one device")
+    if hist.dim() != 3 or tuple(hist.shape[1:]) != (2, n):
+        raise ValueError(f"hist: int32 [steps, 2, {n}]")
+    _same("hist", hist, i32, hist.shape[0] * 2 * n, index)
+    for name, t, size in (("held", held, G), ("count", count, 1), ("slots", slots, n), ("parent", parent, n), ("token", token, n),
+                          ("done", done, n)):
+        _same(name, t, i32, size, index)
+    _same("scores", scores, torch.float32, n, index)
+    if index < 0:
+        raise ValueError("the kernels need a CUDA device")
     check(cuda().bl_beam_advance(p(tokens), p(row_pos), p(row_seq), p(held), p(hist), I(hist.shape[0]), p(count), p(slots), p(parent),
-                                 p(token), p(done), p(scores), I(G), I(B), stream()), "bl_beam_advance")
+                                 p(token), p(done), p(scores), I(G), I(B), ctypes.c_void_p(raw_stream(index))), "bl_beam_advance")

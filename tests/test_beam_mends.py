@@ -118,3 +118,28 @@ def test_a_fault_word_is_an_int32_on_the_device_of_the_rest(fault):
             call(torch.zeros(1, dtype=torch.int32))        # everything else is in order
         with pytest.raises(ValueError, match="fault"):
             call(fault)
+
+
+def _advance(**kw):
+    G, B, i32 = 2, 3, dict(dtype=torch.int32)
+    a = dict(tokens=torch.zeros(16, **i32), row_pos=torch.zeros(16, **i32), row_seq=torch.zeros(16, **i32), held=torch.zeros(G, **i32),
+             hist=torch.zeros(8, 2, G * B, **i32), count=torch.zeros(1, **i32), slots=torch.zeros(G * B, **i32),
+             parent=torch.zeros(G * B, **i32), token=torch.zeros(G * B, **i32), done=torch.zeros(G, B, **i32), scores=torch.zeros(G, B),
+             G=G, B=B)
+    a.update(kw)
+    beam.beam_advance(**a)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(tokens=torch.zeros(5, dtype=torch.int32)), dict(row_pos=torch.zeros(16, dtype=torch.int64)),
+    dict(row_seq=torch.zeros(32, dtype=torch.int32)[::2]), dict(held=torch.zeros(3, dtype=torch.int32)),
+    dict(hist=torch.zeros(8, 2, 5, dtype=torch.int32)), dict(hist=torch.zeros(8, 12, dtype=torch.int32)), dict(hist=torch.zeros(8, 2, 6)),
+    dict(count=torch.zeros(0, dtype=torch.int32)), dict(slots=torch.zeros(5, dtype=torch.int32)),
+    dict(parent=torch.zeros(6, dtype=torch.int64)), dict(token=torch.zeros(6)), dict(done=torch.zeros(2, 3, dtype=torch.bool)),
+    dict(scores=torch.zeros(2, 3, dtype=torch.float64)), dict(G=0), dict(B=0)])
+def test_arguments_of_the_bookkeeping_are_checked(kw):
+    with pytest.raises(ValueError, match="CUDA device"):
+        _advance()                                         # everything else is in order
+    with pytest.raises(ValueError) as e:
+        _advance(**kw)
+    assert "CUDA device" not in str(e.value)
