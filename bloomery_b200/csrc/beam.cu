@@ -17,6 +17,7 @@
 namespace bl {
 
 constexpr int kMaxBeams = 64;
+constexpr float kMaxAlpha = 16.f;                         // length^alpha, and a score times it, in range of 64 bits for any length of 32
 
 constexpr int kBmThreads = 256;
 constexpr int kBmList = 512;                              // survivors that are ranked side by side
@@ -654,6 +655,7 @@ int bl_beam_select(const BeamSelectCall* call) {
   const auto [logits, stride, scores, done, lengths, work, parent, token, out_scores, out_done, out_lengths, fault, st, V, G, B, eos, chunks, alpha] = *call;
   BL_REQUIRE(V >= 1 && G >= 1 && B >= 1 && stride >= V && chunks >= 1 && chunks <= V, BL_ERR_SHAPE);
   BL_REQUIRE(B <= kMaxBeams && (long)G * B <= 65535 && (long)chunks * B <= kBmMaxCells, BL_ERR_LIMIT);
+  BL_REQUIRE(alpha >= -kMaxAlpha && alpha <= kMaxAlpha, BL_ERR_SHAPE);           // ranks without an order otherwise: NaN, or all zero
   BL_REQUIRE(eos < V && (!done || eos >= 0) && (alpha == 0.f || lengths) && (!out_lengths || lengths), BL_ERR_SHAPE);
   BL_REQUIRE(((uintptr_t)logits & 3) == 0 && ((uintptr_t)work & 7) == 0, BL_ERR_ALIGN);
   // Outputs lie apart from what is read.  Blocks of a search that has been written may still be to start: one that found another

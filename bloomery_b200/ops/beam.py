@@ -12,6 +12,7 @@ from ._lib import I, check, cuda, fault_ptr, p, raw_stream
 from .decode import sm_count
 
 MAX_BEAMS = 64
+MAX_ALPHA = 16              # length ** alpha and a score times it stay in range of 64 bits for any length of 32
 _SELECT, _REORDER = struct.Struct("P1l11P5if"), struct.Struct("2P2l7P7i4x")      # BeamSelectCall, BeamReorderCall in the source
 _entries: dict = {}
 
@@ -62,8 +63,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, scratch: BeamScratch
 
     ``logits`` fp32 [groups * beams, vocab] (rows may be strided), ``scores`` fp32 [groups, beams]; a score of -inf is no beam (the
     first step has one beam a search) and its logits are not read.  ``done`` int32: a finished beam continues as itself, with
-    token ``eos``.  ``lengths`` int32: tokens of each beam; candidates are ranked by score / length ** alpha, the new token
-    counted.  ``out_done`` / ``out_lengths``: the same of the next beams.  Ties go to the lower beam, then to the lower id.  Ids with
+    token ``eos``.  ``lengths`` int32: tokens of each beam; candidates are ranked by score / length ** alpha (``alpha`` of -16 to 16), the new
+    token counted.  ``out_done`` / ``out_lengths``: the same of the next beams.  Ties go to the lower beam, then to the lower id.  Ids with
     a logit of -inf are no candidates; where a search has too few, the last places get parent = their own index, token ``eos`` (0
     without one), score -inf and done.  A search with a NaN or +inf among its logits or scores gets NaN scores and raises
     ``fault``.  The outputs are tensors of their own: blocks that start late still read the inputs when the first places of a
@@ -86,6 +87,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, scratch: BeamScratch
         raise ValueError("the next beams are written while the old ones are read: other tensors")
     if eos >= V or (done is not None and eos < 0):
         raise ValueError("finished beams need the id of the end")
+    if not -MAX_ALPHA <= alpha <= MAX_ALPHA:
+        raise ValueError(f"alpha: -{MAX_ALPHA} to {MAX_ALPHA}")
     if lengths is None and (alpha != 0.0 or out_lengths is not None):
         raise ValueError("a rank by length needs the lengths")
     if index < 0:

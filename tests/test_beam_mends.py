@@ -143,3 +143,18 @@ def test_arguments_of_the_bookkeeping_are_checked(kw):
     with pytest.raises(ValueError) as e:
         _advance(**kw)
     assert "CUDA device" not in str(e.value)
+
+
+@pytest.mark.parametrize("alpha", [float("nan"), float("inf"), float("-inf"), 17.0, -17.0])
+def test_an_exponent_that_leaves_no_order_is_refused(alpha):
+    """Ranks of NaN found no candidate at all, an infinite exponent made all of them equal."""
+    with pytest.raises(ValueError, match="CUDA device"):
+        _select(alpha=16.0)
+    with pytest.raises(ValueError, match="alpha"):
+        _select(alpha=alpha)
+    call = dict(logits=A, stride=1000, scores=A + 0x10000, done=0, lengths=A + 0x20000, work=A + 0x30000, parent=A + 0x40000,
+                token=A + 0x50000, out_scores=A + 0x60000, out_done=0, out_lengths=0, fault=0, stream=0, V=1000, G=2, B=4, eos=-1,
+                chunks=1, alpha=alpha)
+    fn = cuda().bl_beam_select
+    fn.argtypes = [ctypes.c_char_p]
+    assert fn(beam._SELECT.pack(*call.values())) == SHAPE
