@@ -35,3 +35,34 @@ def test_a_prefix_longer_than_a_table_row_ends_with_the_row(rows, q8):
         torch.cuda.synchronize()
         assert torch.equal(out, first)
     assert int(c.fault) == -1
+
+
+@gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("n_q,n_kv,head", [(32, 4, 128), (8, 2, 64)])
+@pytest.mark.parametrize("gap", [5.0, 12.0, 14.5, 16.3])
+@pytest.mark.parametrize("first", [True, False])
+def test_what_lies_far_below_the_largest_score_keeps_its_bits(gap, first, n_q, n_kv, head, q8):
+    """One key takes nearly all of the weight and its value is zero: the output is the sum over all others, which score ``gap``
+    nats less, all the same.  The band is that of any other case: rounded probabilities are off by 2^-11 of themselves."""
+    c = Case([(512, [520])], n_q, n_kv, head, q8, seed=22)
+    ids = c.rows[0][1]
+    top, at = (ids[0], 3) if first else (ids[-1], 5)
+    G = n_q // n_kv
+    q = c.q[0].double().view(n_kv, G, head)
+    k0 = torch.linalg.pinv(q) @ torch.full((n_kv, G, 1), gap, dtype=torch.float64, device=DEV)     # q . k0 = gap for every head
+    for page in ids:
+        n = c.keys[page].shape[1]
+        c.keys[page].zero_()
+        c.k[page, :, :n] = 0
+    if q8:
+        from test_gpu_prefix_attention import _q8
+        d, codes = _q8(k0.squeeze(-1).float())
+        c.k[top, :, at] = torch.cat([d.view(torch.uint8), codes.view(torch.uint8)], -1)
+        c.keys[top][:, at] = codes.double() * d.double().repeat_interleave(32, -1)
+    else:
+        c.k[top, :, at] = k0.squeeze(-1).half()
+        c.keys[top][:, at] = k0.squeeze(-1).half().double()
+    c.v[top, :, at] = 0
+    c.values[top][:, at] = 0
+    c.check(c.run())
