@@ -372,14 +372,17 @@ __device__ __forceinline__ void px_codes(uint32_t c, __half2 d, uint32_t& lo, ui
   lo = *reinterpret_cast<const uint32_t*>(&x);
   hi = *reinterpret_cast<const uint32_t*>(&y);
 }
-// A q8_0 row in shared memory to f16 at `dst`: 16-byte chunks swizzled by the row, blocks of 64 values `pitch` bytes apart.
+// A q8_0 row in shared memory to f16 at `dst`: 16-byte chunks swizzled by the row, blocks of 64 values `pitch` bytes apart.  A
+// block whose values may pass f16's range becomes NaN, so that the rows it concerns are summed key by key: as an infinity it could
+// make a score of -inf, which nothing tells from a key without weight.
 template <int HEAD>
 __device__ __forceinline__ void px_expand(const uint8_t* row, uint8_t* dst, int pitch, int swizzle) {
   const __half* scales = reinterpret_cast<const __half*>(row);
   const uint8_t* codes = row + HEAD / 16;
 #pragma unroll
   for (int c = 0; c < HEAD / 8; ++c) {                          // eight values
-    const __half2 d = __half2half2(scales[c >> 2]);
+    const __half scale = scales[c >> 2];
+    const __half2 d = __half2half2(__hle(__habs(scale), __float2half_rn(65504.f / 128)) ? scale : __ushort_as_half(0x7fff));
     uint32_t w0, w1;
     if constexpr (HEAD == 128) {                                // rows of 136 bytes, of 68 otherwise
       const uint2 w = *reinterpret_cast<const uint2*>(codes + 8 * c);

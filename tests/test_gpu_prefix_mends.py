@@ -66,3 +66,32 @@ def test_what_lies_far_below_the_largest_score_keeps_its_bits(gap, first, n_q, n
     c.v[top, :, at] = 0
     c.values[top][:, at] = 0
     c.check(c.run())
+
+
+@gpu
+@pytest.mark.parametrize("n_q,n_kv,head", [(32, 4, 128), (8, 2, 64)])
+@pytest.mark.parametrize("at", [3, 130])                   # in the shared pages, in a row's own
+def test_q8_0_keys_past_the_range_of_f16(at, n_q, n_kv, head):
+    """-127 * 520 is no f16, the sum with 127 * 508 and 3 * 508 is 0: a key like all others, not one of weight 0.  Scores are exact
+    and equal, so that the output is the mean of the values, summed in 32 bits and rounded to 8."""
+    c = Case([(128, [140, 150])], n_q, n_kv, head, True, seed=23)
+    c.q.zero_()
+    c.q[:, :, [0, 32, 33]] = 1.0
+    for pages in (c.rows[0][1], c.rows[1][1]):
+        for page in pages:
+            c.keys[page].zero_()
+            c.k[page, :, :c.keys[page].shape[1]] = 0
+    page, i = c.rows[0][1][at // 64], at % 64
+    d = torch.zeros(n_kv, head // 32, dtype=torch.float16, device=DEV)
+    d[:, 0], d[:, 1] = 520.0, 508.0
+    codes = torch.zeros(n_kv, head, dtype=torch.int8, device=DEV)
+    codes[:, 0], codes[:, 32], codes[:, 33] = -127, 127, 3
+    c.k[page, :, i] = torch.cat([d.view(torch.uint8), codes.view(torch.uint8)], -1)
+    c.keys[page][:, i] = codes.double() * d.double().repeat_interleave(32, -1)
+    wide = torch.full((n_kv, head), 100, dtype=torch.int8, device=DEV)          # a value that is missed if the key is
+    c.v[page, :, i] = torch.cat([torch.ones_like(d).view(torch.uint8), wide.view(torch.uint8)], -1)
+    c.values[page][:, i] = 100.0
+    out = c.run()
+    want, _ = c.reference()
+    assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-4).all()
+    assert int(c.fault) == -1
