@@ -44,27 +44,35 @@ def test_a_prefix_longer_than_a_table_row_ends_with_the_row(rows, q8):
 @pytest.mark.parametrize("first", [True, False])
 def test_what_lies_far_below_the_largest_score_keeps_its_bits(gap, first, n_q, n_kv, head, q8):
     """One key takes nearly all of the weight and its value is zero: the output is the sum over all others, which score ``gap``
-    nats less, all the same.  The band is that of any other case: rounded probabilities are off by 2^-11 of themselves."""
-    c = Case([(512, [520])], n_q, n_kv, head, q8, seed=22)
-    ids = c.rows[0][1]
-    top, at = (ids[0], 3) if first else (ids[-1], 5)
+    nats less, all the same.  The band is that of any other case: rounded probabilities are off by 2^-11 of themselves.  No
+    value is negative, so that what all of the probabilities lose is not lost among values that cancel; there are groups enough
+    that a processor has most of a row's pages behind one maximum."""
+    from test_gpu_prefix_attention import _q8
+    c = Case([(512, [520])] * (40 * 4 // n_kv), n_q, n_kv, head, q8, seed=22)
     G = n_q // n_kv
-    q = c.q[0].double().view(n_kv, G, head)
-    k0 = torch.linalg.pinv(q) @ torch.full((n_kv, G, 1), gap, dtype=torch.float64, device=DEV)     # q . k0 = gap for every head
-    for page in ids:
-        n = c.keys[page].shape[1]
-        c.keys[page].zero_()
-        c.k[page, :, :n] = 0
-    if q8:
-        from test_gpu_prefix_attention import _q8
-        d, codes = _q8(k0.squeeze(-1).float())
-        c.k[top, :, at] = torch.cat([d.view(torch.uint8), codes.view(torch.uint8)], -1)
-        c.keys[top][:, at] = codes.double() * d.double().repeat_interleave(32, -1)
-    else:
-        c.k[top, :, at] = k0.squeeze(-1).half()
-        c.keys[top][:, at] = k0.squeeze(-1).half().double()
-    c.v[top, :, at] = 0
-    c.values[top][:, at] = 0
+    for r, (_, ids) in enumerate(c.rows):
+        top, at = (ids[0], 3) if first else (ids[-1], 5)
+        q = c.q[r].double().view(n_kv, G, head)
+        k0 = (torch.linalg.pinv(q) @ torch.full((n_kv, G, 1), gap, dtype=torch.float64, device=DEV)).squeeze(-1)   # q . k0 = gap
+        for page in ids:
+            n = c.keys[page].shape[1]
+            c.keys[page].zero_()
+            c.k[page, :, :n] = 0
+            c.values[page].abs_()
+            if q8:
+                codes = c.v[page, :, :n, head // 16:]
+                codes.copy_(codes.contiguous().view(torch.int8).abs().view(torch.uint8))
+            else:
+                c.v[page, :, :n].abs_()
+        if q8:
+            d, codes = _q8(k0.float())
+            c.k[top, :, at] = torch.cat([d.view(torch.uint8), codes.view(torch.uint8)], -1)
+            c.keys[top][:, at] = codes.double() * d.double().repeat_interleave(32, -1)
+        else:
+            c.k[top, :, at] = k0.half()
+            c.keys[top][:, at] = k0.half().double()
+        c.v[top, :, at] = 0
+        c.values[top][:, at] = 0
     c.check(c.run())
 
 
