@@ -436,6 +436,7 @@ class BatchDecode:
         h = self._params_np
         h[:2] = 0
         h[2] = -1
+        e.kv.protect = {r[0] for r in rows}             # slots of this pass never spill
         for i, (slot, tok, pos) in enumerate(rows):
             e.kv.ensure(slot, pos + 1)
             e.kv.own(slot, pos)

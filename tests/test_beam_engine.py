@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from bloomery_b200.runtime import beam
+from bloomery_b200.runtime.batch_decode import BatchDecode
 from bloomery_b200.runtime.beam import BeamSearch
 from bloomery_b200.runtime.kv import PAGE, KvPool, OutOfPages
 
@@ -136,3 +137,24 @@ def test_engines_whose_experts_are_elsewhere_are_refused():
         e.spec, e.n_slots = SimpleNamespace(mla=False, eos_id=2), 8
         with pytest.raises(NotImplementedError):
             BeamSearch(e, 4)
+
+
+def _batched(e):
+    bd = object.__new__(BatchDecode)
+    bd.e, bd._stream = e, FakeStream("steps", e.log)
+    bd.params, bd.params_host = torch.zeros(3, 16, dtype=torch.int32), torch.zeros(3, 16, dtype=torch.int32)
+    bd._params_np = bd.params_host.numpy()
+    e.slot_len = [0] * e.n_slots
+    return bd
+
+
+def test_rows_of_a_batched_pass_do_not_take_each_others_pages(make):
+    """Twelve sequences of a page each, a pool of twelve: the last row's second page has to come from nobody in the pass."""
+    _, e, _ = make(12, 12, 4, beams=2, groups=2)
+    bd = _batched(e)
+    bd.set_rows([(i, 1, 40) for i in range(12)])
+    with pytest.raises(OutOfPages):
+        bd.set_rows([(i, 1, 64 if i == 11 else 41) for i in range(12)])
+    assert not e.kv.spilled
+    bd.set_rows([(i, 1, 64 if i == 11 else 41) for i in range(3, 12)])      # three idle ones: the oldest makes room
+    assert set(e.kv.spilled) == {0}
