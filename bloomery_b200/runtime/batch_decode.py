@@ -443,6 +443,8 @@ class BatchDecode:
             h[0, i], h[1, i], h[2, i] = tok, pos, slot
             e.slot_len[slot] = max(e.slot_len[slot], pos + 1)
         e.kv.sync_table()
+        # the table, and what was copied to make room for these rows, is on the caller's stream
+        self._stream.wait_stream(torch.cuda.current_stream(e.device))
         with torch.cuda.stream(self._stream):
             self.params.copy_(self.params_host, non_blocking=True)
         return M

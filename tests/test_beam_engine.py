@@ -158,3 +158,13 @@ def test_rows_of_a_batched_pass_do_not_take_each_others_pages(make):
     assert not e.kv.spilled
     bd.set_rows([(i, 1, 64 if i == 11 else 41) for i in range(3, 12)])      # three idle ones: the oldest makes room
     assert set(e.kv.spilled) == {0}
+
+
+def test_a_batched_pass_waits_for_the_table_and_for_what_made_room(make):
+    _, e, log = make(12, 13, 4, beams=2, groups=2)
+    bd = _batched(e)
+    bd.set_rows([(i, 1, 40) for i in range(12)])
+    del log[:]
+    bd.set_rows([(12, 1, 0)])
+    spill, table = log.index(("caller", "snapshot", 0)), log.index(("caller", "sync_table", None))
+    assert spill < table < log.index(("steps", "waits for", "caller"))
