@@ -32,12 +32,18 @@ class Hypothesis:
 
 class BeamSearch:
     """Searches of ``beams`` beams, ``groups`` prompts at a time, in slots ``first_slot`` and on of a :class:`DecodeEngine` with
-    grouped-query attention.  ``eos``: the id that ends a sequence (-1: none does); candidates are ranked by score / length ** alpha."""
+    grouped-query attention.  ``eos``: the id that ends a sequence (-1: none does); candidates are ranked by score / length ** alpha.
+
+    ``shared_attention``: whether the prompt's pages are read once for all beams (:func:`prefix_attention`, queries and probabilities
+    of 11 bits) or by each beam as in every other batched pass (22 bits or more).  None, the default, shares
+    where there is something to share, and q8_0 caches in any case.  Device time of a layer's attention, shared / not (32 heads over
+    4 of 128): 16 beams with nothing shared and 20, 400, 2,000 positions of their own 12.7 / 8.0, 16.4 / 17.8, 29.3 / 25.2 us in f16 and
+    13.1 / 8.8, 17.4 / 19.7, 33.2 / 49.2 in q8_0; behind 512 shared ones 13.5 / 19.0, 16.6 / 20.7, 29.5 / 27.9 in f16."""
 
     CHECK = 16                      # steps between looks at whether every beam has ended
 
     def __init__(self, engine, beams: int, groups: int = 1, eos: Optional[int] = None, alpha: float = 0.0, max_new: int = 512,
-                 first_slot: int = 0):
+                 first_slot: int = 0, shared_attention: Optional[bool] = None):
         from .engine import DecodeEngine
         s = engine.spec
         if type(engine) is not DecodeEngine:             # their experts are elsewhere, or on several cards
@@ -55,8 +61,9 @@ class BeamSearch:
         dev = engine.device
         self.slots = list(range(first_slot, first_slot + R))
         self.bd = BatchDecode(engine, max_rows=M)
-        self.plan = PrefixPlan([beams] * groups + [M - R] * (M > R), [0] * (groups + (M > R)), s.n_q, s.n_kv, s.head_dim, dev)
-        self.bd.prefix = self.plan
+        self.shared_attention = shared_attention
+        self.plan = None if shared_attention is False else \
+            PrefixPlan([beams] * groups + [M - R] * (M > R), [0] * (groups + (M > R)), s.n_q, s.n_kv, s.head_dim, dev)
         self.scratch = BeamScratch(groups, beams, s.vocab, dev)
         i32 = dict(dtype=torch.int32, device=dev)
         self.slots_dev = torch.tensor(self.slots, **i32)
@@ -67,7 +74,7 @@ class BeamSearch:
         self.held = torch.zeros(groups, **i32)
         self.hist, self.count = torch.zeros(max_new, 2, R, **i32), torch.zeros(1, **i32)
         self.tables = [engine.kv.table, torch.empty_like(engine.kv.table)]
-        self.graphs: list = [None, None]
+        self.graphs: dict = {}                           # (step & 1, whether the attention is the shared one) -> graph
 
     # ---- one step -----------------------------------------------------------------------------------------------
     def _enqueue(self, par: int) -> None:
@@ -85,15 +92,16 @@ class BeamSearch:
                      self.token, self.done[nxt], self.scores[nxt], self.G, self.B)
 
     def _step(self, i: int) -> None:
-        """Step ``i`` on the current stream: the first two of this object run as launches, the next two are captured."""
+        """Step ``i`` on the current stream: the first two of either attention run as launches, the next two are captured."""
         par = i & 1
-        if self.graphs[par] is None and i >= 2 and self.e.use_graphs:
+        key = par, self.bd.prefix is not None
+        if key not in self.graphs and i >= 2 and self.e.use_graphs:
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g, stream=self.bd._stream):
                 self._enqueue(par)
-            self.graphs[par] = g
-        if self.graphs[par] is not None:
-            self.graphs[par].replay()
+            self.graphs[key] = g
+        if key in self.graphs:
+            self.graphs[key].replay()
         else:
             self._enqueue(par)
 
@@ -141,7 +149,12 @@ class BeamSearch:
         # sequences that made room for the beams are copied out on this stream: the steps write their pages behind that
         bd._stream.wait_stream(torch.cuda.current_stream(e.device))
         with e._lock, torch.cuda.stream(bd._stream):
-            self.plan.set_prefix(shared + [0] * (self.M > R))
+            share = self.shared_attention
+            if share is None:
+                share = e.kv_q8 or any(shared)
+            bd.prefix = self.plan if share else None
+            if share:
+                self.plan.set_prefix(shared + [0] * (self.M > R))
             kv.sync_table()
             self.tables[0] = kv.table
             self.tables[1].copy_(kv.table)
@@ -196,6 +209,7 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     ap.add_argument("--beams", type=int, default=4)
     ap.add_argument("--new", type=int, default=32)
     ap.add_argument("--alpha", type=float, default=0.0)
+    ap.add_argument("--separate", action="store_true", help="every beam reads the prompt's pages itself, with more bits of each probability")
     a = ap.parse_args(argv)
     from ..models.weights import Weights, open_model, synth_tensors
     from .engine import DecodeEngine
@@ -210,7 +224,7 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
         w = Weights.from_items(spec, synth_tensors(spec, "cpu", seed=0), "cpu").to("cuda:0")
     ids = tk.encode(a.prompt) if tk is not None else [1 + b for b in a.prompt.encode()]
     eng = DecodeEngine(w, n_slots=a.beams, slot_ctx=(len(ids) + a.new + PAGE) // PAGE * PAGE)
-    for h in BeamSearch(eng, a.beams, alpha=a.alpha, max_new=a.new).search([ids])[0]:
+    for h in BeamSearch(eng, a.beams, alpha=a.alpha, max_new=a.new, shared_attention=False if a.separate else None).search([ids])[0]:
         print(f"{h.rank:10.4f}  {tk.decode(h.tokens) if tk is not None else h.tokens}")
     return 0
 

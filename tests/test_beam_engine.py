@@ -7,7 +7,6 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from bloomery_b200.runtime import beam
 from bloomery_b200.runtime.batch_decode import BatchDecode
 from bloomery_b200.runtime.beam import BeamSearch
 from bloomery_b200.runtime.kv import PAGE, KvPool, OutOfPages
@@ -29,7 +28,7 @@ class FakeEngine:
     def __init__(self, n_pages, n_slots, max_pages, log):
         self.kv = KvPool(1, 1, 4, n_pages, n_slots, max_pages, "cpu")
         self.n_slots, self.slot_ctx, self.device = n_slots, max_pages * PAGE, "cpu"
-        self._lock, self.log = threading.Lock(), log
+        self._lock, self.log, self.kv_q8 = threading.Lock(), log, False
 
     def reset(self, slot):
         self.kv.truncate(slot, 0)
@@ -64,6 +63,7 @@ def make(monkeypatch):
         e = FakeEngine(n_pages, n_slots, max_pages, log)
         s = object.__new__(BeamSearch)
         s.e, s.B, s.G, s.max_new, s.alpha, s.eos = e, beams, groups, 128, 0.0, -1
+        s.shared_attention = True
         s.R = s.M = beams * groups
         s.slots = list(range(first_slot, first_slot + s.R))
         s.bd = SimpleNamespace(_stream=FakeStream("steps", log))
@@ -168,3 +168,19 @@ def test_a_batched_pass_waits_for_the_table_and_for_what_made_room(make):
     bd.set_rows([(12, 1, 0)])
     spill, table = log.index(("caller", "snapshot", 0)), log.index(("caller", "sync_table", None))
     assert spill < table < log.index(("steps", "waits for", "caller"))
+
+
+@pytest.mark.parametrize("asked,q8,lengths,shared", [
+    (None, False, [21, 9], False), (None, False, [64, 9], False), (None, False, [21, 65], True), (None, True, [21, 9], True),
+    (True, False, [21, 9], True), (False, False, [130, 130], False), (False, True, [130, 130], False)])
+def test_which_attention_a_search_takes(make, monkeypatch, asked, q8, lengths, shared):
+    s, e, log = make(16, 6, 4, beams=2, groups=2)
+    s.shared_attention, e.kv_q8 = asked, q8
+    if asked is False:
+        s.plan = None
+    zeros = torch.zeros
+    s.tables, s.scores, s.done, s.lengths = [None, zeros(1)], [zeros(2, 2)], [zeros(2, 2)], [zeros(2, 2)]
+    monkeypatch.setattr(e.kv, "sync_table", lambda: (_ for _ in ()).throw(Reached) if s.bd.prefix is None else None)
+    with pytest.raises(Reached):
+        s.search([[1] * n for n in lengths], 20)
+    assert (s.bd.prefix is s.plan and s.plan is not None) is shared
