@@ -74,18 +74,19 @@ def stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+_device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def raw_stream(index: int) -> int:
     """The handle of the current stream of device ``index``, without the object that :func:`stream` makes (a microsecond a call).
     Launches go to the current device: tensors of another one are refused, its default stream has the same handle."""
-    if torch._C._cuda_getDevice() != index:
+    if _device() != index:
         raise ValueError(f"the tensors are on cuda:{index}, which is not the current device")
-    return torch._C._cuda_getCurrentRawStream(index)
+    return _stream(index)
 
 
-def fault_ptr(fault: Optional[torch.Tensor], index: int) -> int:
-    """The address of a fault word, 0 for none: one int32 on device ``index``."""
-    if fault is None:
-        return 0
+def fault_ptr(fault: torch.Tensor, index: int) -> int:
+    """The address of a fault word: one int32 on device ``index``."""
     if fault.dtype is not torch.int32 or fault.numel() < 1 or fault.get_device() != index:
         raise ValueError("fault: an int32 on the device of the rest")
     return fault.data_ptr()

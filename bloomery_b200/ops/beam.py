@@ -82,8 +82,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, scratch: BeamScratch
           _same("out_scores", out_scores, torch.float32, n, index),
           _same("out_done", out_done, i32, n, index) if out_done is not None else 0,
           _same("out_lengths", out_lengths, i32, n, index) if out_lengths is not None else 0,
-          fault_ptr(fault, index))
-    if any(t and t in at[4:9] for t in at[:3]):
+          0 if fault is None else fault_ptr(fault, index))
+    old_scores, old_done, old_lengths = at[:3]
+    out = at[4:9]
+    if old_scores in out or (old_done and old_done in out) or (old_lengths and old_lengths in out):
         raise ValueError("the next beams are written while the old ones are read: other tensors")
     if eos >= V or (done is not None and eos < 0):
         raise ValueError("finished beams need the id of the end")
@@ -113,7 +115,7 @@ def beam_reorder(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, table_ou
     G, B = parent.shape
     index = k.get_device()
     at = (_same("slots", slots, torch.int32, G * B, index), _same("parent", parent, torch.int32, G * B, index),
-          _same("held", held, torch.int32, G, index), fault_ptr(fault, index))
+          _same("held", held, torch.int32, G, index), 0 if fault is None else fault_ptr(fault, index))
     shape, v_shape, tables = k.shape, v.shape, table.shape
     if len(shape) != 5 or len(v_shape) != 5 or shape[:4] != v_shape[:4] or shape[3] != PAGE or not (k.is_contiguous() and v.is_contiguous()):
         raise ValueError(f"pools: contiguous [layers, pages, heads, {PAGE}, row], alike but for the row")

@@ -1,8 +1,12 @@
-"""Decode attention of rows that share a prefix (``csrc/prefix_attn.cu``): the shared keys are read once for all rows.
+"""Decode attention of rows that share a prefix (``csrc/prefix_attn.cu``): the shared keys are read once for up to 256 (row, query
+head) pairs of a key head.
 
 A group is a run of consecutive rows of a pass whose sequences hold the same first positions in the same pages (beams of a
 prompt, answers to one question, chats behind one system prompt: :meth:`KvPool.share_prefix` maps such pages).  Behind the
-shared pages every row has keys of its own.
+shared pages every row has keys of its own.  ``BatchDecode.prefix`` takes a plan for its passes; beam search sets one.
+
+Queries, probabilities and expanded q8_0 rows are held in the 11 bits of f16, which the bf16 output hardly shows at scores of a few
+nats and by some percent where scores are in the hundreds; ``flash_decode_bf16`` keeps 22 bits or more.
 """
 from __future__ import annotations
 
@@ -43,7 +47,7 @@ class PrefixPlan:
         self.q_shape, self.out_shape = (sum(group_rows), n_q, head), (sum(group_rows), n_q * head)
         if self.rows > 512:
             raise ValueError("at most 512 rows")
-        self.max_pages = None                             # of the narrowest table that a call of the plan came with
+        self.max_pages = 1 << 24                          # of the narrowest table that a call of the plan came with
         rows = self._meta(prefix_len)
         self.n_units, self.unit_rows = len(rows) - self.rows, max(u[1] for u in rows[self.rows:])
         self.meta = torch.tensor(rows, dtype=torch.int32).to(self.device)
@@ -58,7 +62,7 @@ class PrefixPlan:
             raise ValueError("a prefix length for every group")
         if any(n < 0 or n % PAGE for n in prefix_len):
             raise ValueError(f"shared positions are whole pages of {PAGE}")
-        if self.max_pages is not None and max(prefix_len) > self.max_pages * PAGE:
+        if max(prefix_len) > self.max_pages * PAGE:
             raise ValueError(f"the prefix is longer than a table row of {self.max_pages} pages")
         self.prefix_len, self.max_prefix = list(prefix_len), max(prefix_len)
         # units: rows of a group that read all of their keys together, as many as two tiles of 128 (row, head) pairs of a key
@@ -98,21 +102,22 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError(f"caches: contiguous [pages, {n_kv}, {PAGE}, {width}], both f16 or both q8_0 bytes")
     if out.dtype is not torch.bfloat16 or out.shape != plan.out_shape or not out.is_contiguous():
         raise ValueError(f"out: contiguous bf16 {list(plan.out_shape)}")
-    for t in (row_pos, row_seq):
-        if t.dtype is not torch.int32 or t.numel() < rows or not t.is_contiguous():
-            raise ValueError(f"row_pos and row_seq: int32, {rows} rows")
+    i32 = torch.int32
+    if row_pos.dtype is not i32 or row_pos.numel() < rows or not row_pos.is_contiguous() or \
+            row_seq.dtype is not i32 or row_seq.numel() < rows or not row_seq.is_contiguous():
+        raise ValueError(f"row_pos and row_seq: int32, {rows} rows")
     table = block_table.shape
-    if block_table.dtype is not torch.int32 or len(table) != 2 or not block_table.is_contiguous():
+    if block_table.dtype is not i32 or len(table) != 2 or not block_table.is_contiguous():
         raise ValueError("block_table: contiguous int32 [slots, pages]")
     if plan.max_prefix > table[1] * PAGE:
         raise ValueError("the prefix is longer than a table row")
-    if plan.max_pages is None or table[1] < plan.max_pages:
+    if table[1] < plan.max_pages:
         plan.max_pages = table[1]                        # a graph captured with this call goes on with this table
     index = plan.index
-    for t in (q, k_cache, v_cache, row_pos, row_seq, block_table, out):
-        if t.get_device() != index:
-            raise ValueError("the tensors are on the plan's device")
-    fault_at = fault_ptr(fault, index)
+    if not (index == q.get_device() == k_cache.get_device() == v_cache.get_device() == row_pos.get_device() == row_seq.get_device()
+            == block_table.get_device() == out.get_device()):
+        raise ValueError("the tensors are on the plan's device")
+    fault_at = 0 if fault is None else fault_ptr(fault, index)
     if index < 0:
         raise ValueError("the kernels need a CUDA device")
     if _entry is None:

@@ -69,10 +69,10 @@ def test_a_plan_takes_no_prefix_that_its_tables_cannot_hold():
 
 
 def test_launches_for_another_device_than_the_current_one_are_refused(monkeypatch):
-    from bloomery_b200.ops import prefix
+    from bloomery_b200.ops import _lib, prefix
     from bloomery_b200.ops._lib import raw_stream
-    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
-    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 40 + index, raising=False)
+    monkeypatch.setattr(_lib, "_device", lambda: 0)
+    monkeypatch.setattr(_lib, "_stream", lambda index: 40 + index)
     assert raw_stream(0) == 40
     with pytest.raises(ValueError, match="not the current device"):
         raw_stream(1)
