@@ -372,17 +372,29 @@ __device__ __forceinline__ void px_codes(uint32_t c, __half2 d, uint32_t& lo, ui
   lo = *reinterpret_cast<const uint32_t*>(&x);
   hi = *reinterpret_cast<const uint32_t*>(&y);
 }
-// A q8_0 row in shared memory to f16 at `dst`: 16-byte chunks swizzled by the row, blocks of 64 values `pitch` bytes apart.  A
-// block whose values may pass f16's range becomes NaN, so that the rows it concerns are summed key by key: as an infinity it could
-// make a score of -inf, which nothing tells from a key without weight.
+// Whether a q8_0 row may hold a value past f16's range.  It becomes NaN then, so that the query rows it concerns are summed key by
+// key: as an infinity it could make a score of -inf, which nothing tells from a key without weight.
+template <int HEAD>
+__device__ __forceinline__ bool px_wide(const uint8_t* row) {
+  bool wide = false;
+#pragma unroll
+  for (int c = 0; c < HEAD / 64; ++c) wide |= !__hble2(__habs2(reinterpret_cast<const __half2*>(row)[c]), __float2half2_rn(65504.f / 128));
+  return wide;
+}
+// All values of a row at `dst` the same two: blocks of 64 values `pitch` bytes apart.
+template <int HEAD>
+__device__ __forceinline__ void px_fill(uint8_t* dst, int pitch, uint32_t v) {
+#pragma unroll
+  for (int c = 0; c < HEAD / 8; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * pitch + ((c & 7) << 4)) = make_uint4(v, v, v, v);
+}
+// A q8_0 row in shared memory to f16 at `dst`: 16-byte chunks swizzled by the row, blocks of 64 values `pitch` bytes apart.
 template <int HEAD>
 __device__ __forceinline__ void px_expand(const uint8_t* row, uint8_t* dst, int pitch, int swizzle) {
   const __half* scales = reinterpret_cast<const __half*>(row);
   const uint8_t* codes = row + HEAD / 16;
 #pragma unroll
   for (int c = 0; c < HEAD / 8; ++c) {                          // eight values
-    const __half scale = scales[c >> 2];
-    const __half2 d = __half2half2(__hle(__habs(scale), __float2half_rn(65504.f / 128)) ? scale : __ushort_as_half(0x7fff));
+    const __half2 d = __half2half2(scales[c >> 2]);
     uint32_t w0, w1;
     if constexpr (HEAD == 128) {                                // rows of 136 bytes, of 68 otherwise
       const uint2 w = *reinterpret_cast<const uint2*>(codes + 8 * c);
@@ -474,16 +486,15 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_const
         int owner, col, n;
         w.page(p, owner, col, n);
         const int slot = page & 3, st = page % ST;
-        ok = mbar_wait_warp(&raw_full[2 * slot + kv], (uint32_t)((page >> 2) & 1), abort_flag) &&
-             mbar_wait_warp(&empty[st], (uint32_t)((page / ST) & 1) ^ 1, abort_flag);
+        ok = mbar_wait_warp(&raw_full[2 * slot + kv], (uint32_t)((page >> 2) & 1), abort_flag);
+        if (!ok) break;
+        const uint8_t* raw = sRaw + (slot * 2 + kv) * RAW + row * (RAW / kPxPage);
+        const bool wide = px_wide<HEAD>(raw);                   // while the page before is multiplied
+        ok = mbar_wait_warp(&empty[st], (uint32_t)((page / ST) & 1) ^ 1, abort_flag);
         if (!ok) break;
         uint8_t* dst = (kv ? sV : sK) + st * PAGE + row * 128;
-        if (row < n) {
-          px_expand<HEAD>(sRaw + (slot * 2 + kv) * RAW + row * (RAW / kPxPage), dst, ATOM, row & 7);
-        } else {                                                // behind a sequence's end: zero, whatever lies there
-#pragma unroll
-          for (int c = 0; c < HEAD / 8; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * ATOM + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-        }
+        if (row < n && !wide) px_expand<HEAD>(raw, dst, ATOM, row & 7);
+        else px_fill<HEAD>(dst, ATOM, row < n ? 0x7fff7fffu : 0u);               // behind a sequence's end: zero, whatever lies there
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
