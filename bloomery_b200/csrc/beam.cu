@@ -267,8 +267,8 @@ __device__ __forceinline__ void pick_places(int B, BestScratch& s, int* s_pick, 
 
 // grid (n_chunks, G * B).  A block takes the sum of exponentials and the B best of a chunk; the last block of a row merges the
 // row's; the last row of a search ranks the B x B candidates that are left.  Logits are read once; the batches of a tile whose
-// values reach the bound are read again, out of L2.  Device time over 151,936 ids: 4 rows 11.0 us, 64 (39 MB) 20.7, 208 of
-// 16 searches (126 MB) with ranks by length 42.7: 3.0 TB/s.  Behind the last logit a call waits 10 to 12 us for what comes one after the other: bound,
+// values reach the bound are read again, out of L2.  Device time over 151,936 ids, logits not in L2: 4 rows 10.9 us, 64 (39 MB) 20.6,
+// 208 of 16 searches (126 MB) with ranks by length 42.2: 3.0 TB/s.  Behind the last logit a call waits 10 to 12 us for what comes one after the other: bound,
 // list and ranks of the last chunk, the row's merge and the search's, a few hundred clocks a barrier and a dozen for each
 // instruction that is fetched for the first time.
 template <int E, int NB>
@@ -622,9 +622,9 @@ using namespace bl;
 extern "C" {
 
 // Chunks of a row: as many as one wave of four blocks a processor holds, of 4,096 values or more, and no more than a block merges
-// with one cell a thread.  Device time on 148 processors at 151,936 ids, us: 4 rows of 4 beams, 16 chunks 12.2, 38 (the rule)
-// 10.3; 64 rows of 8, 4 chunks 21.5, 9 (the rule) 20.4, 10 (a second wave) 22.4, 16 24.5; 256 rows of 16, 1 chunk 48.9, 2 (the
-// rule) 44.5, 3 49.4; 64 rows of 64, 2 chunks 51.4, 4 (the rule, 256 cells) 45.5.
+// with one cell a thread.  Device time on 148 processors at 151,936 ids that are not in L2, us: 4 rows of 4 beams, 16 chunks 13.2, 38
+// (the rule) 10.9; 64 rows of 8, 4 chunks 21.8, 9 (the rule) 20.6, 10 (a second wave) 22.8, 16 25.8; 256 rows of 16, 1 chunk 48.5, 2
+// (the rule) 44.2, 3 49.1; 64 rows of 64, 2 chunks 57.2, 4 (the rule, 256 cells) 50.5.
 int bl_beam_chunks(int V, int rows, int B, int sms) {
   const int most = (V + 4095) / 4096, wave = 4 * sms / rows, cells = kBmMaxCells / B;
   int n = most < wave ? most : wave;
@@ -682,8 +682,8 @@ int bl_beam_select(const BeamSelectCall* call) {
   a.tickets = (int*)w;
   a.parent = parent; a.token = token; a.out_scores = out_scores; a.out_done = out_done; a.out_lengths = out_lengths; a.fault = fault;
   const dim3 grid(a.n_chunks, (unsigned)R);
-  // A short chunk whole in registers, 4 rows of 151,936 in 38 chunks: 10.3 us, 11.2 as a part of the largest tile.  In two batches, 128
-  // rows of 32,000 in 4 chunks: 15.0 us against 15.7.
+  // A short chunk whole in registers, 4 rows of 151,936 in 38 chunks: 10.9 us, 11.8 as a part of the largest tile.  In two batches, 128
+  // rows of 32,000 in 4 chunks: 16.1 us against 16.8.
   if (a.chunk <= 4096) return (int)launch(beam_select_kernel<16, 1>, grid, dim3(kBmThreads), 0, st, a);
   if (a.chunk <= 8192) return (int)launch(beam_select_kernel<16, 2>, grid, dim3(kBmThreads), 0, st, a);
   return (int)launch(beam_select_kernel<32, 4>, grid, dim3(kBmThreads), 0, st, a);

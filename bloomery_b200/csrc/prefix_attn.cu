@@ -6,9 +6,10 @@
 //
 // Both kinds of cache run on the 5th-generation tensor cores.  A unit is up to 256 stacked (row, head) pairs of one KV head, rows
 // of one group, in two tiles of 128: it reads the pages that its rows share and then the pages of each of its rows, all of them
-// against all of its query rows; for a page of one row the others' scores are masked.  (Multiplying rows that are masked costs
-// little: a page's products take less than its keys and values take to arrive.  With a fragment for each row's own keys instead,
-// 64 rows with 1 to 256 keys of their own behind 32,768 took 102 us: a short fragment costs as much as eight pages more.)
+// against all of its query rows; for a page of one row the others' scores are masked.  (A page of one row costs a whole job, of
+// whose 128 rows at most 16 count.  Where own pages are most of the line they bound the call: 21 rows with up to 1,100 own positions
+// behind 4,096 have 190 own pages a KV head beside 64 shared ones.  A fragment for each row's own keys cost more in the form
+// that was tried, as much as eight pages on top for a short one: 64 rows with 1 to 256 keys of their own behind 32,768, 102 us.)
 // Per page of 64 keys and tile of rows, a job:
 //   S = Q K^T     tcgen05.mma kind::f16, M = 128, N = 64, into one of the tile's two score buffers in tensor memory
 //   softmax       one thread per query row; the probabilities go back as f16 into the score columns they came from
@@ -20,14 +21,19 @@
 // Roles: warps 0..3 softmax of the first tile of rows, 4..7 of the second (warp id modulo 4 = TMEM lane quarter), warp 8 the TMA
 // producer (four pages of keys and of values in flight), warps 9 and 10 the MMA issuers of either tile; 9 owns the TMEM.  q8_0 rows
 // are fetched as they are and expanded to f16 by four warps more.
-// Queries and probabilities are rounded to f16 (11 bits; queries scaled by a power of two a row): less than the output's 8 bits.
+// Three roundings to the 11 bits of f16: queries (scaled by a power of two a row), probabilities (scaled by 2^7, see kPxShift) and the
+// expanded keys and values of q8_0 caches.  A probability's or a value's own rounding is less than the output's 8 bits.  A query's,
+// or a q8_0 key's, moves a score by some 2^-12 of the root of the sum of its terms' squares, and the probability by that much of
+// itself: the output's 0.2 % where that root is 8 nats, 1 % at 40, several percent in the hundreds; the ordinary batched pass keeps
+// 22 bits of queries and probabilities (flash_mma.cuh).  At scores of 1.4 standard deviations the error against 64 bits is 0.2 to 1.9 %
+// above that of sums in 32 bits, both 1.65e-3 to 1.69e-3, the output's rounding.
 // A value that is not finite would reach the masked rows of its tile as 0 x inf; rows whose output is not finite are summed again
 // key by key, over their own keys alone.
-// Device time of both launches in a graph (32 heads over 4 of 128 values): 4 rows behind 512 shared positions 10.0 us, 8 behind 2,048
-// 12.6, 21 behind 4,096 22.5, 24 rows of q8_0 behind three prefixes 29.8, 64 behind 32,768 61.3.  A short call is a chain of
-// latencies: launch, lengths and schedule, queries, a page, its softmax, the join.  A long one is bound by the softmax of a job, one
-// row a thread, and by the turns of the two tiles: about 1,200 clocks a job, the tensor pipe 32 % busy; its
-// joining launch reads 19 MB of fragments in 8 us.
+// Device time of both launches in a graph, inputs not in L2 (32 heads over 4 of 128 values): 4 rows behind 512 shared positions 10.3 us,
+// 8 behind 2,048 13.6, 21 behind 4,096 23.2, 24 rows of q8_0 behind three prefixes 30.4, 64 behind 32,768 62.1.  A short call is a
+// chain of latencies: launch, lengths and schedule, queries, a page, its softmax, the join.  A long one is bound by the softmax of a
+// job, one row a thread, and by the turns of the two tiles: about 1,200 clocks a job, the tensor pipe 33 % busy; its joining launch
+// reads 19 MB of fragments in 8 us.
 // Every wait is bounded (1 s); on expiry the CTA raises the fault word, frees its TMEM and returns.
 #include <type_traits>
 
@@ -162,8 +168,8 @@ struct PxLine {
     n_units = a.n_units;
     cta = blockIdx.x;
     for (int i = threadIdx.x; i < n_units * kPxUnit; i += blockDim.x) units[i] = i % kPxUnit == 2 ? px_shared(a, a.units[i]) : a.units[i];
-    // One warp has up to 32 rows in its registers (4 rows behind 512 positions 10.5 us a call, 11.1 by way of shared memory; 24 q8_0
-    // rows 29.6 and 30.0).
+    // One warp has up to 32 rows in its registers (4 rows behind 512 positions 10.3 us a call, 10.9 by way of shared memory; 24 q8_0
+    // rows 30.4 and 30.9).
     const bool small = a.M <= 32;
     int unit[3] = {0, 0, 0}, own = 0, n_keys = 0;
     if (small && (int)threadIdx.x < n_units) {
@@ -959,8 +965,8 @@ using namespace bl;
 template <int HEAD, bool Q8>
 static int prefix_go(PrefixArgs a, cudaStream_t st) {
   // The joining launch.  Few rows: a block for 32 values of a head, so that more of its fragments are in flight (8 rows behind 2,048
-  // positions 13.0 us a call, 15.2 with whole heads; 24 q8_0 rows 29.6 and 32.4); many: as much of it as 256 threads hold (100 rows
-  // 26.5 us, 32.6 in parts; 512 rows behind 1,024 positions 84.8 and 116.5).
+  // positions 13.6 us a call, 15.8 with whole heads; 24 q8_0 rows 30.4 and 33.1; 21 rows behind 4,096 23.2 and 22.7); many: as much
+  // of it as 256 threads hold (100 rows behind 1,024 with up to 64 of their own 23.2 us, 29.1 in parts; 512 such rows 57.7 and 89.6).
   int z = HEAD / 32;
   const int G = a.n_q / a.n_kv;
   if (a.n_kv * a.M > a.n_cta) while (z > 1 && G * (HEAD / 4) / (z / 2) <= 256) z /= 2;
