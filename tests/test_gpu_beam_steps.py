@@ -104,3 +104,10 @@ def test_captured_steps_take_up_other_prompts():
         eng.use_graphs = True
         assert got == want, lengths
     assert len(search.graphs) == 4
+
+
+@gpu
+def test_the_example_takes_either_attention(capsys):
+    from bloomery_b200.runtime.beam import main
+    assert main(["--beams", "3", "--new", "6", "--separate"]) == 0
+    assert len(capsys.readouterr().out.strip().splitlines()) == 3
