@@ -74,7 +74,8 @@ def stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-_device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# absent from builds of torch without CUDA, where nothing calls them
+_device, _stream = (getattr(torch._C, name, None) for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))
 
 
 def raw_stream(index: int) -> int:

@@ -35,10 +35,10 @@ class BeamSearch:
     grouped-query attention.  ``eos``: the id that ends a sequence (-1: none does); candidates are ranked by score / length ** alpha.
 
     ``shared_attention``: whether the prompt's pages are read once for all beams (:func:`prefix_attention`, queries and probabilities
-    of 11 bits) or by each beam as in every other batched pass (22 bits or more).  None, the default, shares
-    where there is something to share, and q8_0 caches in any case.  Device time of a layer's attention, shared / not (32 heads over
-    4 of 128): 16 beams with nothing shared and 20, 400, 2,000 positions of their own 12.7 / 8.0, 16.4 / 17.8, 29.3 / 25.2 us in f16 and
-    13.1 / 8.8, 17.4 / 19.7, 33.2 / 49.2 in q8_0; behind 512 shared ones 13.5 / 19.0, 16.6 / 20.7, 29.5 / 27.9 in f16."""
+    of 11 bits) or by each beam, as in every other batched pass (22 bits or more).  None, the default, shares where there is
+    something to share, and q8_0 caches in any case.  Device time of a layer's attention, shared / not, of 16 beams (32 heads over
+    4 of 128) with 20, 400 and 2,000 positions of their own: nothing shared 12.7 / 8.0, 16.4 / 17.8, 29.3 / 25.2 us in f16 and 13.1 /
+    8.8, 17.4 / 19.7, 33.2 / 49.2 in q8_0; behind 512 shared ones 13.5 / 19.0, 16.6 / 20.7, 29.5 / 27.9 in f16."""
 
     CHECK = 16                      # steps between looks at whether every beam has ended
 
