@@ -1,0 +1,135 @@
+// What the NVFP4 kernels share: the quantiser of a block of 16 values and the tcgen05 instructions of block-scaled four-bit
+// operands.
+//
+// A row of K values is K / 2 bytes of E2M1 codes (the even value in the low half), K / 16 E4M3 scales and one fp32 scale, padded
+// to 16 bytes: value = code * scale * row scale.  Weights of a checkpoint and quantised activations have the same layout.
+//
+// Quantising is exact: the scale of a block is the E4M3 value nearest to amax / (6 g), a code the E2M1 value nearest to x / d
+// with d = scale * g in fp32, ties to the even code, in the reals.  Quotients in fp32 decide all but the values next to a midpoint
+// m; there the sign of fma(-m, d, x) decides, which has one rounding and so the right sign.
+#pragma once
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+
+#include "tc_common.cuh"
+
+namespace bl {
+
+constexpr float FP4_ROW = 2688.0f;                    // 6 * 448: what a row's largest value becomes
+constexpr float FP4_LEAST = 7.888609052210118e-31f;   // 2^-100, the least row scale: keeps a row of zeros, and 1 / d, in range
+constexpr unsigned FP4_INF = 0x7f800000u;
+
+__host__ __device__ constexpr long fp4_row_bytes(int K) { return (K / 2 + K / 16 + 4 + 15) / 16 * 16; }
+
+// The scale of a row whose largest magnitude has these bits; NaN where that is none.
+__device__ __forceinline__ float fp4_row_scale(unsigned amax_bits) {
+  return amax_bits < FP4_INF ? fmaxf(__fdiv_rn(__uint_as_float(amax_bits), FP4_ROW), FP4_LEAST) : __uint_as_float(0x7fc00000u);
+}
+
+// E4M3 code nearest to amax / (6 g); its value in `s`
+__device__ __forceinline__ unsigned fp4_block_scale(float amax, float g, float& s) {
+  const float q = __fdiv_rn(amax, 6.0f * g);
+  unsigned c = __nv_cvt_float_to_fp8(fminf(q, 448.0f), __NV_SATFINITE, __NV_E4M3);
+  auto value = [](unsigned code) {                    // also of 0x7f, as the step above 448
+    const unsigned e = code >> 3, m = code & 7;
+    return (float)(e ? 8 + m : m) * __uint_as_float(((e ? e : 1u) + 117u) << 23);
+  };
+  s = value(c);
+  if (c < 0x7eu) {
+    const float up = value(c + 1), r = fmaf(-3.0f * (s + up), g, amax);       // 6 times the midpoint: seven bits
+    if (r > 0.0f || (r == 0.0f && (c & 1))) { ++c; s = up; }
+  }
+  if (c > 0u) {
+    const float down = value(c - 1), r = fmaf(-3.0f * (s + down), g, amax);
+    if (r < 0.0f || (r == 0.0f && (c & 1))) { --c; s = down; }
+  }
+  return c;
+}
+
+// Codes of eight values (value i in bits 4i ..), steps of d.  The quotients are off by less than 2^-21; where 2^-20 to either side gives
+// another code the midpoint is looked at itself.
+__device__ __forceinline__ uint32_t fp4_codes8(const float* x, float d, float lo, float hi) {
+  uint32_t a = 0, b = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(x[2 * i] * lo, x[2 * i + 1] * lo), __NV_E2M1, cudaRoundNearest) << (8 * i);
+    b |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(x[2 * i] * hi, x[2 * i + 1] * hi), __NV_E2M1, cudaRoundNearest) << (8 * i);
+  }
+  if (a != b) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const unsigned c = a >> (4 * i) & 7u;
+      if ((b >> (4 * i) & 7u) != c) {                 // one step above: c < 7
+        const float mid = c < 4 ? 0.5f * (float)c + 0.25f : c == 4 ? 2.5f : c == 5 ? 3.5f : 5.0f;
+        const float r = fmaf(-mid, d, fabsf(x[i]));
+        if (r > 0.0f || (r == 0.0f && (c & 1))) a += 1u << (4 * i);
+      }
+    }
+  }
+  return a;
+}
+
+// A block of 16 values of a row with scale g: its codes and the byte of its scale.  A row with anything that is not finite has NaN
+// for g and gets zeros: its products are NaN by the row scale alone.
+__device__ __forceinline__ uint2 fp4_block(const float* x, float g, unsigned& scale) {
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));
+  if (!(g > 0.0f)) { scale = 0; return make_uint2(0u, 0u); }
+  float s;
+  scale = fp4_block_scale(amax, g, s);
+  if (scale == 0u) return make_uint2(0u, 0u);
+  const float d = s * g, inv = __frcp_rn(d), lo = inv * (1.0f - 9.5367431640625e-7f), hi = inv * (1.0f + 9.5367431640625e-7f);
+  return make_uint2(fp4_codes8(x, d, lo, hi), fp4_codes8(x + 8, d, lo, hi));
+}
+
+// ---- instructions ---------------------------------------------------------------------------------------
+// kind::mxf4nvf4 instruction descriptor: D = f32, A = B = E2M1 (K-major), scales E4M3 without sign, M 128 x N, K 64
+__host__ __device__ constexpr uint32_t fp4_idesc(int n) {
+  return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+// The scales of 64 values of a row are one 32-bit cell of tensor memory: row r of an operand has its cell in lane r % 32 (the same in
+// all four quarters), column r / 32.  32 lanes x 16 bytes of shared memory become the four columns of 128 rows.
+__device__ __forceinline__ void fp4_scales_to_tmem(uint32_t taddr, uint32_t smem) {
+  const uint64_t desc = (uint64_t)((smem >> 4) & 0x3FFF) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;     // rows of 16 bytes, no swizzle
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xFFFFFFFF;\n\t"
+      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void umma_fp4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "elect.sync _|e, 0xFFFFFFFF;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
+}
+
+// Scales of 256 values (16 bytes) of up to 128 rows, as they lie in the rows, into the cells of four instructions: thread = lane, word
+// s of row 32 j + lane goes to word j of instruction s.  `groups`: groups of 32 rows there are.
+__device__ __forceinline__ void fp4_turn_scales(const uint4* raw, uint4* cells, int lane, int groups) {
+  uint4 r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = j < groups ? raw[32 * j + lane] : make_uint4(0u, 0u, 0u, 0u);
+  cells[lane] = make_uint4(r[0].x, r[1].x, r[2].x, r[3].x);
+  cells[32 + lane] = make_uint4(r[0].y, r[1].y, r[2].y, r[3].y);
+  cells[64 + lane] = make_uint4(r[0].z, r[1].z, r[2].z, r[3].z);
+  cells[96 + lane] = make_uint4(r[0].w, r[1].w, r[2].w, r[3].w);
+}
+
+// Maps of NVFP4 rows [groups][rows][row bytes]: codes in boxes of 256 values (zeros past the row's end) and scales of as many.
+inline int fp4_maps(CUtensorMap* codes, CUtensorMap* scales, const void* base, int K, long rows, long groups, int box_rows) {
+  const cuuint64_t rb = (cuuint64_t)fp4_row_bytes(K);
+  cuuint64_t dims[3] = {(cuuint64_t)K / 2, (cuuint64_t)rows, (cuuint64_t)groups};
+  cuuint64_t str[2] = {rb, rb * (cuuint64_t)rows};
+  cuuint32_t box[3] = {128, (cuuint32_t)box_rows, 1};
+  int rc = make_map_any(codes, base, 3, dims, str, box, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  dims[0] = (cuuint64_t)K / 16;
+  box[0] = 16;
+  return make_map_any(scales, (const uint8_t*)base + K / 2, 3, dims, str, box, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+}  // namespace bl

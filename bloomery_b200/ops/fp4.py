@@ -1,0 +1,161 @@
+"""NVFP4 activations and their products with NVFP4 weights (``csrc/fp4_rows.cu``, ``csrc/fp4_gemm.cu``, ``csrc/fp4_moe.cu``).
+
+A row of K values is K / 2 bytes of E2M1 codes, K / 16 E4M3 scales and one fp32 scale, padded to 16 bytes: the layout of resident
+NVFP4 weights.  :func:`fp4_rows` makes such rows of activations, :func:`fp4_gemm` multiplies them with NVFP4 weights on the four-bit
+tensor cores, :func:`fp4_moe` runs the routed experts of a few tokens in two launches.  ``BatchDecode`` and ``GemmPrefill`` take them
+for NVFP4 weights where ``BLOOMERY_FP4_NATIVE`` is on.
+"""
+from __future__ import annotations
+
+import ctypes
+import struct
+from typing import Optional
+
+import torch
+
+from ..formats.resident import resident_row_bytes
+from ._lib import check, cuda, raw_stream
+from .decode import QWeight, sm_count
+from .gemm import TileTable
+
+_ROWS, _GEMM = struct.Struct("6P2ld4i"), struct.Struct("12P3l6i")      # Fp4RowsCall, Fp4GemmCall in the sources
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_K = 32768                                             # values of a row that fp4_rows holds in registers
+_entries: dict = {}
+
+
+def _fn(name):
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(cuda(), name)
+        fn.argtypes = [ctypes.c_char_p]
+    return fn
+
+
+def _index(device) -> int:
+    """The device's number as ``Tensor.get_device`` says it."""
+    device = torch.device(device)
+    if device.type != "cuda":
+        return -1
+    return torch.cuda.current_device() if device.index is None else device.index
+
+
+class Fp4Rows:
+    """Buffer of ``rows`` NVFP4 rows of ``k`` values."""
+
+    def __init__(self, rows: int, k: int, device):
+        if rows < 1 or k < 64 or k % 64 or k > MAX_K:
+            raise ValueError(f"rows of 64 to {MAX_K} values, a multiple of 64")
+        self.rows, self.k = rows, k
+        self.data = torch.zeros(rows, resident_row_bytes("NVFP4", k), dtype=torch.uint8, device=device)
+        self.ptr, self.index = self.data.data_ptr(), self.data.get_device()
+
+    @property
+    def weight(self) -> QWeight:
+        """The rows as a resident NVFP4 matrix (what expands or dots one takes them too)."""
+        return QWeight(self.data, "NVFP4", self.k)
+
+
+def fp4_tile_rows(rows: int, groups: int = 1, gated: bool = False) -> int:
+    """Rows of a tile of :func:`fp4_gemm` for ``rows`` rows dealt to ``groups`` matrices; ``gated``: with a second matrix."""
+    per = -(-rows // groups)
+    return 32 if per <= 32 else 64 if per <= 64 else 128 if per <= 128 or gated else 256
+
+
+def fp4_tiles(rows: int, device) -> TileTable:
+    """The table of a product of ``rows`` rows with one matrix."""
+    return TileTable.dense(rows, device, fp4_tile_rows(rows), host=True)
+
+
+def fp4_rows(x: torch.Tensor, out: Fp4Rows, *, gain: Optional[torch.Tensor] = None, eps: float = 0.0,
+             tensor_scale: Optional[torch.Tensor] = None, pos_of: Optional[torch.Tensor] = None) -> None:
+    """NVFP4 rows of ``x`` [M, k] (bf16, f16 or fp32; rows may be strided) in the first M rows of ``out``.
+
+    A row's scale takes its largest magnitude to 6 x 448 (or is ``tensor_scale``, one fp32 on the device; larger values saturate), a
+    block's scale takes its own to 6; scales and codes are the nearest, ties go to the even code.  A row with a NaN or an
+    infinity becomes one whose products are all NaN.  ``gain`` fp32 [k] (fp32 rows): RMSNorm first.  ``pos_of`` int32 [M * copies]:
+    row m goes to the rows ``pos_of[m * copies + j]`` of ``out`` (none where that is negative or past the end), as ``moe_plan``
+    deals the slots of M tokens."""
+    kind = _TYPES.get(x.dtype)
+    index = out.index
+    if kind is None or x.dim() != 2 or x.shape[1] != out.k or x.stride(1) != 1:
+        raise ValueError(f"x: bf16, f16 or fp32 [rows, {out.k}], values next to each other")
+    M = x.shape[0]
+    copies, at = 1, 0
+    if pos_of is not None:
+        copies, rest = divmod(pos_of.numel(), M) if M else (0, 0)
+        if pos_of.dtype is not torch.int32 or not pos_of.is_contiguous() or rest or copies < 1 or pos_of.get_device() != index:
+            raise ValueError("pos_of: contiguous int32, as many places for every row, on the device of the rest")
+        at = pos_of.data_ptr()
+    elif M > out.rows:
+        raise ValueError(f"{M} rows into {out.rows}")
+    gain_at = scale_at = 0
+    if gain is not None:
+        if kind != 2 or gain.dtype is not torch.float32 or gain.numel() != out.k or not gain.is_contiguous() or gain.get_device() != index:
+            raise ValueError(f"gain: contiguous fp32 [{out.k}] beside fp32 rows, on the device of the rest")
+        gain_at = gain.data_ptr()
+    if tensor_scale is not None:
+        if tensor_scale.dtype is not torch.float32 or tensor_scale.numel() != 1 or tensor_scale.get_device() != index:
+            raise ValueError("tensor_scale: one fp32 on the device of the rest")
+        scale_at = tensor_scale.data_ptr()
+    if x.get_device() != index:
+        raise ValueError("x: on another device than the rows")
+    if index < 0:
+        raise ValueError("the kernels need a CUDA device")
+    if M == 0:
+        return
+    ldx = x.stride(0) if M > 1 else out.k
+    code = _fn("bl_fp4_rows")(_ROWS.pack(x.data_ptr(), gain_at, scale_at, at, out.ptr, raw_stream(index), ldx, out.rows, eps, kind, M, out.k,
+                                         copies))
+    if code:
+        check(code, "bl_fp4_rows")
+
+
+class Fp4Work:
+    """Partial sums and tickets of products that split their depth: one per stream that runs them."""
+
+    def __init__(self, device):
+        pass
+
+
+def _matrix(name: str, w: QWeight, k: int, index: int) -> int:
+    if w.qtype != "NVFP4" or w.k != k or not w.data.is_contiguous() or w.data.get_device() != index:
+        raise ValueError(f"{name}: contiguous NVFP4 rows of {k} values on the device of the rest")
+    return w.data.data_ptr()
+
+
+def fp4_gemm(X: Fp4Rows, W: QWeight, tiles: TileTable, *, out_f32: Optional[torch.Tensor] = None,
+             out_bf16: Optional[torch.Tensor] = None, W2: Optional[QWeight] = None, dst_row=None, row_scale=None, resid=None,
+             status: Optional[torch.Tensor] = None, work: Optional[Fp4Work] = None) -> None:
+    """C = X @ W[g].T per token tile, codes by codes on tcgen05 ``kind::mxf4nvf4`` with fp32 sums: ``X`` NVFP4 rows, W (and W2)
+    resident NVFP4 matrices [N, bytes] or stacks [G, N, bytes]; tiles of 32, 64 or 128 rows, without W2 of 256 too
+    (:func:`fp4_tile_rows`).  With W2 the output is silu(X W^T) * (X W2^T).  Epilogue options as :func:`gemm.qgemm`.  Block scales are
+    taken without their sign, which no checkpoint sets (:func:`fp4_supports`)."""
+    index, k = X.index, X.k
+    wp = _matrix("W", W, k, index)
+    shape = W.data.shape
+    G, N = (shape[0] if len(shape) == 3 else 1), shape[-2]
+    w2p = 0
+    if W2 is not None:
+        w2p = _matrix("W2", W2, k, index)
+        if W2.data.shape != shape:
+            raise ValueError("W and W2 are alike")
+    f32 = out_f32 is not None
+    out = out_f32 if f32 else out_bf16
+    if (out_f32 is None) == (out_bf16 is None) or out.dtype is not (torch.float32 if f32 else torch.bfloat16) or out.dim() != 2 or \
+            out.shape[1] != N or (out.stride(1) != 1 and N > 1) or out.get_device() != index:
+        raise ValueError(f"one output, fp32 or bf16 [rows, {N}], on the device of the rest")
+    rp = ldr = 0
+    if resid is not None:
+        if resid.dtype is not torch.float32 or resid.shape != out.shape or (resid.stride(1) != 1 and N > 1) or resid.get_device() != index:
+            raise ValueError("resid: fp32, shaped like the output")
+        rp, ldr = resid.data_ptr(), resid.stride(0)
+    if index < 0:
+        raise ValueError("the kernels need a CUDA device")
+    code = _fn("bl_fp4_gemm")(_GEMM.pack(
+        X.ptr, wp, w2p, tiles.mtiles.data_ptr(), tiles.n_mtiles.data_ptr(), out.data_ptr() if f32 else 0, 0 if f32 else out.data_ptr(),
+        0 if dst_row is None else dst_row.data_ptr(), 0 if row_scale is None else row_scale.data_ptr(), rp,
+        0 if status is None else status.data_ptr(), raw_stream(index), X.rows, out.stride(0), ldr, G, N, k,
+        tiles.fixed or tiles.max_mtiles, tiles.tile_rows, sm_count()))
+    if code:
+        check(code, "bl_fp4_gemm")
