@@ -83,6 +83,58 @@ __device__ __forceinline__ uint2 fp4_block(const float* x, float g, unsigned& sc
   return make_uint2(fp4_codes8(x, d, lo, hi), fp4_codes8(x + 8, d, lo, hi));
 }
 
+// ---- pieces of a row --------------------------------------------------------------------------------------
+__device__ __forceinline__ void fp4_load16(const void* x, int type, long at, float* v) {       // type: 0 bf16, 1 f16, 2 fp32
+  if (type == 2) {
+    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float4 f = p[i]; v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w; }
+  } else {
+    const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + at);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 u = p[i];
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (type == 0) {
+          v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+          v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+          v[8 * i + 2 * j] = f.x;
+          v[8 * i + 2 * j + 1] = f.y;
+        }
+      }
+    }
+  }
+}
+// v * r * gain
+__device__ __forceinline__ void fp4_scale16(float* v, float r, const float* gain) {
+  const float4* g4 = reinterpret_cast<const float4*>(gain);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 g = g4[i];
+    v[4 * i] = v[4 * i] * r * g.x; v[4 * i + 1] = v[4 * i + 1] * r * g.y;
+    v[4 * i + 2] = v[4 * i + 2] * r * g.z; v[4 * i + 3] = v[4 * i + 3] * r * g.w;
+  }
+}
+// The largest magnitude as bits: a NaN is above everything.
+__device__ __forceinline__ unsigned fp4_top16(const float* v) {
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  return top;
+}
+// Block `at` of a row of K values with scale g
+__device__ __forceinline__ void fp4_store_block(uint8_t* row, int K, int at, const float* v, float g) {
+  unsigned scale;
+  const uint2 codes = fp4_block(v, g, scale);
+  *reinterpret_cast<uint2*>(row + 8 * at) = codes;
+  row[K / 2 + at] = (uint8_t)scale;
+  if (at == 0) *reinterpret_cast<float*>(row + K / 2 + K / 16) = g;
+}
+
 // ---- instructions ---------------------------------------------------------------------------------------
 // kind::mxf4nvf4 instruction descriptor: D = f32, A = B = E2M1 (K-major), scales E4M3 without sign, M 128 x N, K 64
 __host__ __device__ constexpr uint32_t fp4_idesc(int n) {

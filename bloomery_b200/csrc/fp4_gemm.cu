@@ -9,17 +9,14 @@
 //   * "dual" mode runs gate and up in one main loop; the epilogue writes silu(gate) * up;
 //   * the epilogue scatters and scales like the other GEMMs (dst_row / row_scale / resid).
 // Every wait is bounded; on expiry the CTA raises status word 1, leaves its loops, frees its TMEM and returns.
-#include "fp4_common.cuh"
+#include "fp4_pipe.cuh"
 
 namespace bl {
-
-constexpr int F4_THREADS = 256;             // warp 0 TMA, 1 MMA + TMEM, 2..5 epilogue, 6 and 7 scales
-constexpr int F4_MAX_STAGES = 8;
 
 struct F4Tile { int group, row0, row_end, pad; };
 
 struct F4Args {
-  int N, K, tiles_w;
+  int N, K, tiles_w, tile_rows;
   const F4Tile* tiles;
   const int* n_tiles;
   int max_tiles;
@@ -37,156 +34,49 @@ struct F4Args {
   unsigned* status;
 };
 
-// What a stage holds, in bytes from its start, and what it has in tensor memory, in columns
-template <bool DUAL, int BN>
-struct F4Shape {
-  static constexpr int MATS = DUAL ? 2 : 1;
-  static constexpr int BOX = BN < 64 ? BN : 64;                    // token rows of a box
-  static constexpr int B = MATS * 16384, RA = B + BN * 128, RB = RA + MATS * 2048, TA = RB + BN * 16, TB = TA + MATS * 2048;
-  static constexpr int B_CELLS = BN > 128 ? 8 : 4;                 // columns of an instruction's token scales
-  static constexpr int STAGE = (TB + 4 * 128 * B_CELLS + 1023) / 1024 * 1024;
-  static constexpr int STAGES = 222 * 1024 / STAGE > F4_MAX_STAGES ? F4_MAX_STAGES : 222 * 1024 / STAGE;
-  static constexpr int SCALE_COLS = 16 * MATS + 4 * B_CELLS;
-  static constexpr int ACCS = 2 * MATS * BN + STAGES * SCALE_COLS <= 512 ? 2 : 1;
-  static constexpr int SCALE0 = ACCS * MATS * BN;                  // first column of the scales
-  static constexpr size_t SMEM = (size_t)STAGES * STAGE + 1024;
-  static_assert(STAGES >= 2 && SCALE0 + STAGES * SCALE_COLS <= 512, "tensor memory");
+struct F4GemmTiles {
+  const F4Args& a;
+  int total, kblocks;
+  __device__ __forceinline__ int count() const { return total > (int)blockIdx.x ? (total - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0; }
+  __device__ __forceinline__ F4Work at(int i) const {
+    const int t = (int)blockIdx.x + i * (int)gridDim.x;
+    const F4Tile mt = a.tiles[t / a.tiles_w];
+    return F4Work{mt.group, t % a.tiles_w * 128, mt.row0, min(a.tile_rows, mt.row_end - mt.row0), 0, kblocks};
+  }
 };
 
 template <bool DUAL, int BN>
 __global__ void __launch_bounds__(F4_THREADS, 1)
-fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_xs,
-                const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_ws,
-                const __grid_constant__ CUtensorMap map_w2, const __grid_constant__ CUtensorMap map_ws2, const F4Args a) {
+fp4_gemm_kernel(const __grid_constant__ F4Maps map, const F4Args a) {
   using S = F4Shape<DUAL, BN>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full_bar[S::STAGES], cells_bar[S::STAGES], empty_bar[S::STAGES], acc_full[S::ACCS], acc_empty[S::ACCS];
-  __shared__ uint32_t s_tmem_base;
-  __shared__ int s_abort;
+  __shared__ __align__(8) F4Bars<S> bar;
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < S::STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&cells_bar[s], 2); mbar_init(&empty_bar[s], 1); }
-    for (int b = 0; b < S::ACCS; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 4); }
-    s_abort = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(512) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  f4_open<S>(bar);
   pdl_wait();
   pdl_launch();
-  const uint32_t tmem = s_tmem_base;
-  volatile int* abort_flag = &s_abort;
-  const int total = min(*a.n_tiles, a.max_tiles) * a.tiles_w, kblocks = (a.K + 255) / 256;
+  F4GemmTiles tiles{a, min(*a.n_tiles, a.max_tiles) * a.tiles_w, (a.K + 255) / 256};
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0, issued = 0; uint32_t phase = 0;
-      for (int t = blockIdx.x; t < total && !*abort_flag; t += gridDim.x) {
-        const F4Tile mt = a.tiles[t / a.tiles_w];
-        const int n0 = (t % a.tiles_w) * 128, boxes = (min(BN, mt.row_end - mt.row0) + S::BOX - 1) / S::BOX;
-        for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) break;
-          uint8_t* s = smem + (size_t)stage * S::STAGE;
-          mbar_expect_tx(&full_bar[stage], S::MATS * (16384 + 2048) + boxes * S::BOX * (128 + 16));
-          // rows past a matrix and values past a row arrive as zeros
-          tma_load_3d(s, &map_w, kb * 128, n0, mt.group, &full_bar[stage]);
-          tma_load_3d(s + S::RA, &map_ws, kb * 16, n0, mt.group, &full_bar[stage]);
-          if (DUAL) {
-            tma_load_3d(s + 16384, &map_w2, kb * 128, n0, mt.group, &full_bar[stage]);
-            tma_load_3d(s + S::RA + 2048, &map_ws2, kb * 16, n0, mt.group, &full_bar[stage]);
-          }
-          for (int b = 0; b < boxes; ++b) {
-            tma_load_3d(s + S::B + b * S::BOX * 128, &map_x, kb * 128, mt.row0 + b * S::BOX, 0, &full_bar[stage]);
-            tma_load_3d(s + S::RB + b * S::BOX * 16, &map_xs, kb * 16, mt.row0 + b * S::BOX, 0, &full_bar[stage]);
-          }
-          ++issued;
-          if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
-        }
-      }
-      if (*abort_flag) {
-        // copies of this thread may still be landing in shared memory: the CTA must not exit under them
-        unsigned long long t0 = globaltimer();
-        while (issued > 0 && globaltimer() - t0 < 2000000ull) {}
-      }
-    }
+    if (lane == 0) f4_produce<DUAL, S>(smem, bar, map, tiles, [] { return true; });
   } else if (warp == 1) {
-    int stage = 0; uint32_t phase = 0;
-    uint32_t ab = 0, aphase = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      const F4Tile mt = a.tiles[t / a.tiles_w];
-      const uint32_t idesc = fp4_idesc((min(BN, mt.row_end - mt.row0) + 31) / 32 * 32);
-      if (!mbar_wait_warp(&acc_empty[ab], aphase ^ 1, abort_flag)) break;
-      const uint32_t d0 = tmem + ab * (S::MATS * BN);
-      for (int kb = 0; kb < kblocks; ++kb) {
-        if (!mbar_wait_warp(&full_bar[stage], phase, abort_flag) || !mbar_wait_warp(&cells_bar[stage], phase, abort_flag)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t sm = smem_u32(smem + (size_t)stage * S::STAGE), sc = tmem + S::SCALE0 + stage * S::SCALE_COLS;
-        const uint32_t sb = sc + 16 * S::MATS;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-#pragma unroll
-          for (int m = 0; m < S::MATS; ++m) fp4_scales_to_tmem(sc + 16 * m + 4 * k, sm + S::TA + 2048 * m + 512 * k);
-#pragma unroll
-          for (int h = 0; h < S::B_CELLS / 4; ++h) fp4_scales_to_tmem(sb + S::B_CELLS * k + 4 * h, sm + S::TB + 2048 * h + 512 * k);
-        }
-        const uint64_t da = umma_desc(sm), db = umma_desc(sm + S::B);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {                              // 64 values are 32 bytes
-#pragma unroll
-          for (int m = 0; m < S::MATS; ++m)
-            umma_fp4(d0 + m * BN, da + (uint64_t)(m * 16384 / 16 + 2 * k), db + (uint64_t)(2 * k), idesc, sc + 16 * m + 4 * k,
-                     sb + S::B_CELLS * k, kb > 0 || k > 0 ? 1u : 0u);
-        }
-        umma_commit(&empty_bar[stage]);
-        if (kb == kblocks - 1) umma_commit(&acc_full[ab]);
-        if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
-      }
-      if (++ab == S::ACCS) { ab = 0; aphase ^= 1; }
-    }
+    f4_issue<DUAL, S>(smem, bar, tiles);
   } else if (warp >= 6) {
-    int stage = 0; uint32_t phase = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      const F4Tile mt = a.tiles[t / a.tiles_w];
-      const int groups = (min(BN, mt.row_end - mt.row0) + 31) / 32;
-      for (int kb = 0; kb < kblocks; ++kb) {
-        if (!mbar_wait_warp(&full_bar[stage], phase, abort_flag)) { ok = false; break; }
-        uint8_t* s = smem + (size_t)stage * S::STAGE;
-        if (warp == 6) {
-#pragma unroll
-          for (int m = 0; m < S::MATS; ++m)
-            fp4_turn_scales(reinterpret_cast<const uint4*>(s + S::RA + 2048 * m), reinterpret_cast<uint4*>(s + S::TA + 2048 * m), lane, 4);
-        } else {
-#pragma unroll
-          for (int h = 0; h < S::B_CELLS / 4; ++h)
-            fp4_turn_scales(reinterpret_cast<const uint4*>(s + S::RB + 2048 * h), reinterpret_cast<uint4*>(s + S::TB + 2048 * h), lane, groups - 4 * h);
-        }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&cells_bar[stage]);
-        if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
-      }
-    }
+    f4_turn<DUAL, S>(smem, bar, tiles);
   } else {
     const int q = warp & 3;                                        // TMEM lane quarter of this warp
     uint32_t ab = 0, aphase = 0;
-    for (int t = blockIdx.x; t < total; t += gridDim.x) {
-      const F4Tile mt = a.tiles[t / a.tiles_w];
-      const int n = (t % a.tiles_w) * 128 + q * 32 + lane, nt = min(BN, mt.row_end - mt.row0);   // weight row = output column
+    for (int i = 0; i < tiles.count(); ++i) {
+      const F4Work mt = tiles.at(i);
+      const int n = mt.n0 + q * 32 + lane, nt = mt.rows;             // weight row = output column
       const long scale_at = a.K / 2 + a.K / 16, wrow = (long)mt.group * a.group_bytes + (long)min(n, a.N - 1) * a.row_bytes + scale_at;
       const float ws = *reinterpret_cast<const float*>(a.w + wrow), ws2 = DUAL ? *reinterpret_cast<const float*>(a.w2 + wrow) : 0.0f;
       // a row's scale is a factor of every value: store_tokens applies it where there is a factor at all
       const TokenOut out{a.c_f32, a.c_bf16, (unsigned)a.ldc, DUAL ? a.row_scale : reinterpret_cast<const float*>(a.x), a.resid, (unsigned)a.ldr, a.N};
-      if (!mbar_wait_warp(&acc_full[ab], aphase, abort_flag)) break;
+      if (!mbar_wait_warp(&bar.acc_full[ab], aphase, &bar.abort)) break;
       tc_fence_after();
-      const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + ab * (S::MATS * BN);
+      const uint32_t tbase = bar.tmem + ((uint32_t)(q * 32) << 16) + ab * (S::MATS * BN);
 #pragma unroll 1
       for (int b = 0; b < nt; b += 32) {
         const int r = mt.row0 + b + lane;
@@ -218,18 +108,12 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[ab]);
+      if (lane == 0) mbar_arrive(&bar.acc_empty[ab]);
       if (++ab == S::ACCS) { ab = 0; aphase ^= 1; }
     }
   }
 
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
-  }
-  if (threadIdx.x == 0 && s_abort && a.status) atomicMax(a.status, 1u);
+  f4_close<S>(bar, a.status);
 }
 
 }  // namespace bl
@@ -248,11 +132,8 @@ namespace bl {
 template <bool DUAL, int BN>
 static int fp4_gemm_go(const Fp4GemmCall& c, const F4Args& a) {
   using S = F4Shape<DUAL, BN>;
-  CUtensorMap mx, mxs, mw, mws, mw2, mws2;
-  int rc = fp4_maps(&mx, &mxs, c.x, c.K, c.rows_x, 1, S::BOX);
-  if (!rc) rc = fp4_maps(&mw, &mws, c.w, c.K, c.N, c.n_groups, 128);
-  mw2 = mw; mws2 = mws;
-  if (!rc && DUAL) rc = fp4_maps(&mw2, &mws2, c.w2, c.K, c.N, c.n_groups, 128);
+  F4Maps m;
+  const int rc = f4_maps<DUAL, S>(&m, c.x, c.rows_x, c.w, c.w2, c.K, c.N, c.n_groups);
   if (rc) return rc;
   static PerDevice limit;
   if (limit.due()) {
@@ -260,8 +141,7 @@ static int fp4_gemm_go(const Fp4GemmCall& c, const F4Args& a) {
     limit.mark();
   }
   const long total = (long)c.max_tiles * a.tiles_w;
-  return (int)launch(fp4_gemm_kernel<DUAL, BN>, dim3((unsigned)(total < c.sms ? total : c.sms)), dim3(F4_THREADS), S::SMEM, c.stream, mx, mxs,
-                     mw, mws, mw2, mws2, a);
+  return (int)launch(fp4_gemm_kernel<DUAL, BN>, dim3((unsigned)(total < c.sms ? total : c.sms)), dim3(F4_THREADS), S::SMEM, c.stream, m, a);
 }
 
 }  // namespace bl
@@ -278,7 +158,7 @@ int bl_fp4_gemm(const Fp4GemmCall* c) {
   BL_REQUIRE(((uintptr_t)c->x & 15) == 0 && ((uintptr_t)c->w & 15) == 0 && ((uintptr_t)c->w2 & 15) == 0, BL_ERR_ALIGN);
   BL_REQUIRE((c->c_f32 != nullptr) != (c->c_bf16 != nullptr) && c->ldc < 1L << 30 && c->ldr < 1L << 30, BL_ERR_SHAPE);
   F4Args a{};
-  a.N = c->N; a.K = c->K; a.tiles_w = (c->N + 127) / 128;
+  a.N = c->N; a.K = c->K; a.tiles_w = (c->N + 127) / 128; a.tile_rows = c->tile_rows;
   a.tiles = (const F4Tile*)c->tiles; a.n_tiles = c->n_tiles; a.max_tiles = c->max_tiles;
   BL_REQUIRE((long)a.max_tiles * a.tiles_w < 1L << 31, BL_ERR_LIMIT);
   a.x = (const uint8_t*)c->x; a.w = (const uint8_t*)c->w; a.w2 = (const uint8_t*)c->w2;

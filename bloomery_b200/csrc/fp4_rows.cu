@@ -15,32 +15,6 @@ struct Fp4RowsArgs {
   const int* pos_of; int copies;          // row m goes to rows pos_of[m * copies + j]; null: to row m
 };
 
-__device__ __forceinline__ void fp4_load16(const Fp4RowsArgs& a, long at, float* v) {
-  if (a.type == 2) {
-    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.x) + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { const float4 f = p[i]; v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w; }
-  } else {
-    const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.x) + at);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 u = p[i];
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (a.type == 0) {
-          v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
-          v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-          v[8 * i + 2 * j] = f.x;
-          v[8 * i + 2 * j + 1] = f.y;
-        }
-      }
-    }
-  }
-}
-
 template <int NB>
 __global__ void __launch_bounds__(512) fp4_rows_kernel(const Fp4RowsArgs a) {
   __shared__ double s_sum[16];
@@ -52,7 +26,7 @@ __global__ void __launch_bounds__(512) fp4_rows_kernel(const Fp4RowsArgs a) {
   float v[NB][16];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
-    if (tid + b * nthr < blocks) fp4_load16(a, (long)m * a.ldx + 16 * (tid + b * nthr), v[b]);
+    if (tid + b * nthr < blocks) fp4_load16(a.x, a.type, (long)m * a.ldx + 16 * (tid + b * nthr), v[b]);
   if (a.gain) {
     double ss = 0.0;
 #pragma unroll
@@ -69,23 +43,12 @@ __global__ void __launch_bounds__(512) fp4_rows_kernel(const Fp4RowsArgs a) {
     const float r = (float)(1.0 / sqrt(all / (double)a.K + a.eps));
 #pragma unroll
     for (int b = 0; b < NB; ++b)
-      if (tid + b * nthr < blocks) {
-        const float4* g4 = reinterpret_cast<const float4*>(a.gain + 16 * (tid + b * nthr));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 g = g4[i];
-          v[b][4 * i] = v[b][4 * i] * r * g.x; v[b][4 * i + 1] = v[b][4 * i + 1] * r * g.y;
-          v[b][4 * i + 2] = v[b][4 * i + 2] * r * g.z; v[b][4 * i + 3] = v[b][4 * i + 3] * r * g.w;
-        }
-      }
+      if (tid + b * nthr < blocks) fp4_scale16(v[b], r, a.gain + 16 * (tid + b * nthr));
   }
-  unsigned top = 0;                                   // magnitudes as bits: a NaN is above everything
+  unsigned top = 0;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
-    if (tid + b * nthr < blocks) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[b][i]) & 0x7fffffffu);
-    }
+    if (tid + b * nthr < blocks) top = max(top, fp4_top16(v[b]));
   top = __reduce_max_sync(0xFFFFFFFFu, top);
   if (lane == 0) s_max[warp] = top;
   __syncthreads();

@@ -18,7 +18,7 @@ from ._lib import check, cuda, raw_stream
 from .decode import QWeight, sm_count
 from .gemm import TileTable
 
-_ROWS, _GEMM = struct.Struct("6P2ld4i"), struct.Struct("12P3l6i")      # Fp4RowsCall, Fp4GemmCall in the sources
+_ROWS, _GEMM, _MOE = struct.Struct("6P2ld4i"), struct.Struct("12P3l6i"), struct.Struct("13P3ld8i")      # Fp4RowsCall, Fp4GemmCall, Fp4MoeCall
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_K = 32768                                             # values of a row that fp4_rows holds in registers
 _entries: dict = {}
@@ -159,3 +159,65 @@ def fp4_gemm(X: Fp4Rows, W: QWeight, tiles: TileTable, *, out_f32: Optional[torc
         tiles.fixed or tiles.max_mtiles, tiles.tile_rows, sm_count()))
     if code:
         check(code, "bl_fp4_gemm")
+
+
+MOE_TOKENS, MOE_USED, MOE_EXPERTS, MOE_WIDTH = 64, 16, 512, 8192
+
+
+class Fp4MoeWork:
+    """Scratch of :func:`fp4_moe` for up to ``rows`` tokens of ``used`` experts each, of ``n_expert``, ``hidden`` and ``inter`` values wide:
+    one per stream that runs them.  After a call that raised its status word make another."""
+
+    def __init__(self, rows: int, used: int, hidden: int, inter: int, n_expert: int, device):
+        if not 1 <= rows <= MOE_TOKENS or not 1 <= used <= MOE_USED or not 1 <= n_expert <= MOE_EXPERTS:
+            raise ValueError(f"1 to {MOE_TOKENS} tokens, 1 to {MOE_USED} of up to {MOE_EXPERTS} experts each")
+        if any(n < 64 or n % 64 or n > MOE_WIDTH for n in (hidden, inter)):
+            raise ValueError(f"widths of 64 to {MOE_WIDTH}, multiples of 64")
+        self.rows, self.used, self.hidden, self.inter, self.n_expert = rows, used, hidden, inter, n_expert
+        size = cuda().bl_fp4_moe_work_bytes
+        size.restype = ctypes.c_long
+        self.data = torch.zeros(size(rows, used, n_expert, hidden, inter), dtype=torch.uint8, device=device)
+        self.ptr, self.index = self.data.data_ptr(), self.data.get_device()
+
+
+def fp4_moe(x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, gate: QWeight, up: QWeight, down: QWeight, work: Fp4MoeWork, *,
+            out_f32: Optional[torch.Tensor] = None, out_bf16: Optional[torch.Tensor] = None, gain: Optional[torch.Tensor] = None,
+            eps: float = 0.0, resid: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
+    """out[t] = resid[t] + sum_j wts[t, j] down_e(silu(gate_e(x_t)) * up_e(x_t)), e = ids[t, j], for 1 to 64 tokens in two launches:
+    tokens ``x`` [T, hidden] (fp32 or bf16; ``gain`` fp32: RMSNorm of fp32 rows first) and the products in between go through NVFP4 rows
+    as :func:`fp4_rows` makes them.  ``ids`` int32 and ``wts`` fp32 [T, used]; a slot whose id is not in 0 .. experts - 1 is another
+    tier's and adds nothing.  ``out`` may be ``resid`` and, in fp32, ``x``."""
+    T = x.shape[0] if x.dim() == 2 else 0
+    kind, index = _TYPES.get(x.dtype), work.index
+    H, I_, E, k = work.hidden, work.inter, work.n_expert, work.used
+    if kind not in (0, 2) or not 1 <= T <= work.rows or x.shape[1] != H or x.stride(1) != 1 or x.get_device() != index:
+        raise ValueError(f"x: fp32 or bf16 [1 to {work.rows}, {H}], values next to each other, on the scratch's device")
+    if ids.dtype is not torch.int32 or ids.numel() != T * k or not ids.is_contiguous() or ids.get_device() != index:
+        raise ValueError(f"ids: contiguous int32 [{T}, {k}] on the scratch's device")
+    if wts.dtype is not torch.float32 or wts.numel() != T * k or not wts.is_contiguous() or wts.get_device() != index:
+        raise ValueError(f"wts: contiguous fp32 [{T}, {k}] on the scratch's device")
+    at = [_matrix(n, w, d, index) for n, w, d in (("gate", gate, H), ("up", up, H), ("down", down, I_))]
+    if gate.data.shape[:-1] != (E, I_) or up.data.shape[:-1] != (E, I_) or down.data.shape[:-1] != (E, H):
+        raise ValueError(f"gate and up: stacks of {E} x {I_} rows, down of {E} x {H}")
+    f32 = out_f32 is not None
+    out = out_f32 if f32 else out_bf16
+    if (out_f32 is None) == (out_bf16 is None) or out.dtype is not (torch.float32 if f32 else torch.bfloat16) or out.shape != (T, H) or \
+            out.stride(1) != 1 or out.get_device() != index:
+        raise ValueError(f"one output, fp32 or bf16 [{T}, {H}], on the scratch's device")
+    rp = ldr = gain_at = 0
+    if resid is not None:
+        if resid.dtype is not torch.float32 or resid.shape != out.shape or resid.stride(1) != 1 or resid.get_device() != index:
+            raise ValueError("resid: fp32, shaped like the output")
+        rp, ldr = resid.data_ptr(), resid.stride(0)
+    if gain is not None:
+        if kind != 2 or gain.dtype is not torch.float32 or gain.numel() != H or not gain.is_contiguous() or gain.get_device() != index:
+            raise ValueError(f"gain: contiguous fp32 [{H}] beside fp32 rows")
+        gain_at = gain.data_ptr()
+    if index < 0:
+        raise ValueError("the kernels need a CUDA device")
+    ldx = x.stride(0) if T > 1 else H
+    code = _fn("bl_fp4_moe")(_MOE.pack(x.data_ptr(), gain_at, ids.data_ptr(), wts.data_ptr(), *at, work.ptr, rp, out.data_ptr() if f32 else 0,
+                                       0 if f32 else out.data_ptr(), 0 if status is None else status.data_ptr(), raw_stream(index), ldx, ldr,
+                                       out.stride(0), eps, kind, T, k, E, H, I_, work.rows, sm_count()))
+    if code:
+        check(code, "bl_fp4_moe")
