@@ -135,6 +135,9 @@ __device__ __forceinline__ void fp4_store_block(uint8_t* row, int K, int at, con
   if (at == 0) *reinterpret_cast<float*>(row + K / 2 + K / 16) = g;
 }
 
+// x / (1 + exp(-x)), a few units of 2^-23 off (a quotient whose denominator is past 2^126 is zero, where the value is below 2^-119)
+__device__ __forceinline__ float fp4_silu(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
+
 // ---- instructions ---------------------------------------------------------------------------------------
 // kind::mxf4nvf4 instruction descriptor: D = f32, A = B = E2M1 (K-major), scales E4M3 without sign, M 128 x N, K 64
 __host__ __device__ constexpr uint32_t fp4_idesc(int n) {
@@ -160,19 +163,20 @@ __device__ __forceinline__ void umma_fp4(uint32_t tmem_d, uint64_t adesc, uint64
 }
 
 // Scales of 256 values (16 bytes) of up to 128 rows, as they lie in the rows, into the cells of four instructions: thread = lane, word
-// s of row 32 j + lane goes to word j of instruction s.  `groups`: groups of 32 rows there are.
+// s of row 32 j + lane goes to word j of instruction s.  Rows lie PITCH times 16 bytes apart; `groups`: groups of 32 rows there are.
+template <int PITCH>
 __device__ __forceinline__ void fp4_turn_scales(const uint4* raw, uint4* cells, int lane, int groups) {
   uint4 r[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) r[j] = j < groups ? raw[32 * j + lane] : make_uint4(0u, 0u, 0u, 0u);
+  for (int j = 0; j < 4; ++j) r[j] = j < groups ? raw[(32 * j + lane) * PITCH] : make_uint4(0u, 0u, 0u, 0u);
   cells[lane] = make_uint4(r[0].x, r[1].x, r[2].x, r[3].x);
   cells[32 + lane] = make_uint4(r[0].y, r[1].y, r[2].y, r[3].y);
   cells[64 + lane] = make_uint4(r[0].z, r[1].z, r[2].z, r[3].z);
   cells[96 + lane] = make_uint4(r[0].w, r[1].w, r[2].w, r[3].w);
 }
 
-// Maps of NVFP4 rows [groups][rows][row bytes]: codes in boxes of 256 values (zeros past the row's end) and scales of as many.
-inline int fp4_maps(CUtensorMap* codes, CUtensorMap* scales, const void* base, int K, long rows, long groups, int box_rows) {
+// Maps of NVFP4 rows [groups][rows][row bytes]: codes in boxes of 256 values (zeros past the row's end), scales in boxes of 256 * span.
+inline int fp4_maps(CUtensorMap* codes, CUtensorMap* scales, const void* base, int K, long rows, long groups, int box_rows, int span) {
   const cuuint64_t rb = (cuuint64_t)fp4_row_bytes(K);
   cuuint64_t dims[3] = {(cuuint64_t)K / 2, (cuuint64_t)rows, (cuuint64_t)groups};
   cuuint64_t str[2] = {rb, rb * (cuuint64_t)rows};
@@ -180,7 +184,7 @@ inline int fp4_maps(CUtensorMap* codes, CUtensorMap* scales, const void* base, i
   int rc = make_map_any(codes, base, 3, dims, str, box, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
   dims[0] = (cuuint64_t)K / 16;
-  box[0] = 16;
+  box[0] = 16 * span;
   return make_map_any(scales, (const uint8_t*)base + K / 2, 3, dims, str, box, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 

@@ -13,6 +13,8 @@
 
 namespace bl {
 
+constexpr int F4_GEMM_ROOM = 190 * 1024, F4_GEMM_WARPS = 8;
+
 struct F4Tile { int group, row0, row_end, pad; };
 
 struct F4Args {
@@ -32,6 +34,7 @@ struct F4Args {
   const float* resid;
   long ldr;
   unsigned* status;
+  int wide;                 // rows of the output (and of resid) start at 16 bytes and hold whole 16 bytes
 };
 
 struct F4GemmTiles {
@@ -45,12 +48,88 @@ struct F4GemmTiles {
   }
 };
 
+// 16 tokens of the 32 columns from n0 on, `f` this lane's column of them (lane = column); rows below zero are none.
+// Wide: they are turned in shared memory, so that a lane stores 16 bytes of a token: a store of four bytes, or two, costs its warp some 19
+// clocks with the address of its token, 16 bytes cost them for four tokens, or eight.
+__device__ __forceinline__ void f4_store16(const F4Args& a, const float (&f)[16], const int* rows, int n0, uint8_t* stage, int lane) {
+  if (a.wide && a.c_bf16 && !a.resid) {
+    __nv_bfloat16* s = reinterpret_cast<__nv_bfloat16*>(stage);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s[32 * j + lane] = __float2bfloat16_rn(f[j]);
+    __syncwarp();
+    const int n = n0 + 8 * (lane & 3), none = n < a.N ? 0 : -1;
+    int row[2];
+    uint4 v[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      row[j] = rows[8 * j + (lane >> 2)] | none;
+      v[j] = *reinterpret_cast<const uint4*>(s + 32 * (8 * j + (lane >> 2)) + 8 * (lane & 3));
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (row[j] >= 0) *reinterpret_cast<uint4*>(a.c_bf16 + (unsigned long long)(unsigned)row[j] * (unsigned)a.ldc + n) = v[j];
+    __syncwarp();
+    return;
+  }
+  float* s = reinterpret_cast<float*>(stage);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) s[32 * j + lane] = f[j];
+  __syncwarp();
+  if (a.wide) {
+    const int n = n0 + 4 * (lane & 7), none = n < a.N ? 0 : -1;
+    int row[4];
+    float4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      row[j] = rows[4 * j + (lane >> 3)] | none;
+      v[j] = *reinterpret_cast<const float4*>(s + 32 * (4 * j + (lane >> 3)) + 4 * (lane & 7));
+    }
+    if (a.resid) {
+      float4 r[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        r[j] = row[j] >= 0 ? *reinterpret_cast<const float4*>(a.resid + (unsigned long long)(unsigned)row[j] * (unsigned)a.ldr + n)
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { v[j].x += r[j].x; v[j].y += r[j].y; v[j].z += r[j].z; v[j].w += r[j].w; }
+    }
+    if (a.c_f32) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (row[j] >= 0) *reinterpret_cast<float4*>(a.c_f32 + (unsigned long long)(unsigned)row[j] * (unsigned)a.ldc + n) = v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(v[j].x, v[j].y), hi = __floats2bfloat162_rn(v[j].z, v[j].w);
+        if (row[j] >= 0)
+          *reinterpret_cast<uint2*>(a.c_bf16 + (unsigned long long)(unsigned)row[j] * (unsigned)a.ldc + n) =
+              make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      }
+    }
+  } else {
+    const int n = n0 + lane;
+#pragma unroll 8
+    for (int j = 0; j < 16; ++j) {
+      const int row = rows[j];
+      float v = s[32 * j + lane];
+      if (row < 0 || n >= a.N) continue;
+      if (a.resid) v += a.resid[(unsigned long long)(unsigned)row * (unsigned)a.ldr + n];
+      if (a.c_f32) a.c_f32[(unsigned long long)(unsigned)row * (unsigned)a.ldc + n] = v;
+      else a.c_bf16[(unsigned long long)(unsigned)row * (unsigned)a.ldc + n] = __float2bfloat16_rn(v);
+    }
+  }
+  __syncwarp();
+}
+
 template <bool DUAL, int BN>
-__global__ void __launch_bounds__(F4_THREADS, 1)
+__global__ void __launch_bounds__(128 + 32 * F4_GEMM_WARPS, 1)
 fp4_gemm_kernel(const __grid_constant__ F4Maps map, const F4Args a) {
-  using S = F4Shape<DUAL, BN>;
+  using S = F4Shape<DUAL, BN, F4_GEMM_ROOM, F4_GEMM_WARPS>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) F4Bars<S> bar;
+  __shared__ __align__(16) int s_row[2][BN];
+  __shared__ __align__(16) float s_xs[2][BN], s_factor[2][DUAL ? BN : 1];
+  __shared__ __align__(16) uint8_t s_stage[F4_GEMM_WARPS][2048];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   f4_open<S>(bar);
@@ -62,49 +141,66 @@ fp4_gemm_kernel(const __grid_constant__ F4Maps map, const F4Args a) {
     if (lane == 0) f4_produce<DUAL, S>(smem, bar, map, tiles, [] { return true; });
   } else if (warp == 1) {
     f4_issue<DUAL, S>(smem, bar, tiles);
-  } else if (warp >= 6) {
+  } else if (warp < 4) {
     f4_turn<DUAL, S>(smem, bar, tiles);
   } else {
-    const int q = warp & 3;                                        // TMEM lane quarter of this warp
+    const int q = warp & 3, half = (warp - 4) >> 2, et = threadIdx.x - 128;          // TMEM lane quarter of this warp; 0 .. 255
+    const int n_tiles = tiles.count();
+    const long scale_at = a.K / 2 + a.K / 16;
+    // What a tile needs beside its products is asked for while the tile before is worked on, a token a thread, and laid down in shared
+    // memory behind it; the entry of the table a tile earlier.
+    struct Beside { int row; float xs, factor, ws, ws2; } nxt{};
+    auto open = [&](const F4Work& w) {
+      const int r = w.row0 + et;
+      nxt.row = -1;
+      if (et < w.rows) {
+        nxt.row = a.dst_row ? a.dst_row[r] : r;
+        nxt.xs = *reinterpret_cast<const float*>(a.x + (long)r * a.row_bytes + scale_at);
+        nxt.factor = a.row_scale ? a.row_scale[r] : 1.0f;
+      }
+      const long at = (long)w.group * a.group_bytes + (long)min(w.n0 + q * 32 + lane, a.N - 1) * a.row_bytes + scale_at;
+      nxt.ws = *reinterpret_cast<const float*>(a.w + at);
+      if (DUAL) nxt.ws2 = *reinterpret_cast<const float*>(a.w2 + at);
+    };
     uint32_t ab = 0, aphase = 0;
-    for (int i = 0; i < tiles.count(); ++i) {
-      const F4Work mt = tiles.at(i);
-      const int n = mt.n0 + q * 32 + lane, nt = mt.rows;             // weight row = output column
-      const long scale_at = a.K / 2 + a.K / 16, wrow = (long)mt.group * a.group_bytes + (long)min(n, a.N - 1) * a.row_bytes + scale_at;
-      const float ws = *reinterpret_cast<const float*>(a.w + wrow), ws2 = DUAL ? *reinterpret_cast<const float*>(a.w2 + wrow) : 0.0f;
-      // a row's scale is a factor of every value: store_tokens applies it where there is a factor at all
-      const TokenOut out{a.c_f32, a.c_bf16, (unsigned)a.ldc, DUAL ? a.row_scale : reinterpret_cast<const float*>(a.x), a.resid, (unsigned)a.ldr, a.N};
-      if (!mbar_wait_warp(&bar.acc_full[ab], aphase, &bar.abort)) break;
+    F4Work w{}, w1{}, w2{};                                        // this tile, the next one and the one behind it
+    if (n_tiles > 0) { w1 = tiles.at(0); open(w1); }
+    if (n_tiles > 1) w2 = tiles.at(1);
+    for (int i = 0; i < n_tiles; ++i) {
+      w = w1;
+      w1 = w2;
+      const float ws = nxt.ws, ws2 = nxt.ws2;
+      if (et < BN) {
+        s_row[i & 1][et] = nxt.row;
+        s_xs[i & 1][et] = DUAL ? nxt.xs : nxt.xs * nxt.factor;
+        if (DUAL) s_factor[i & 1][et] = nxt.factor;
+      }
+      if (i + 1 < n_tiles) open(w1);
+      if (i + 2 < n_tiles) w2 = tiles.at(i + 2);
+      if (!f4_all<F4_GEMM_WARPS>(mbar_wait_warp(&bar.acc_full[ab], aphase, &bar.abort))) break;
       tc_fence_after();
       const uint32_t tbase = bar.tmem + ((uint32_t)(q * 32) << 16) + ab * (S::MATS * BN);
 #pragma unroll 1
-      for (int b = 0; b < nt; b += 32) {
-        const int r = mt.row0 + b + lane;
-        int orow = -1;
-        float xs = 0.0f, factor = 1.0f;
-        if (b + lane < nt) {
-          orow = a.dst_row ? a.dst_row[r] : r;
-          xs = *reinterpret_cast<const float*>(a.x + (long)r * a.row_bytes + scale_at);
-          if (a.row_scale) factor = a.row_scale[r];
-        }
-#pragma unroll 1
-        for (int h = 0; h < 32 && b + h < nt; h += 16) {
-          uint32_t v[16], u[DUAL ? 16 : 1];
-          tmem_ld16(tbase + b + h, v);
-          if constexpr (DUAL) tmem_ld16(tbase + BN + b + h, u);
-          tmem_ld_wait();
-          float f[16];
+      for (int b = 16 * half; b < w.rows; b += 32) {               // the two warps of a quarter take 16 tokens each in turn
+        uint32_t v[16], u[DUAL ? 16 : 1];
+        tmem_ld16(tbase + b, v);
+        if constexpr (DUAL) tmem_ld16(tbase + BN + b, u);
+        tmem_ld_wait();
+        float f[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            f[i] = __uint_as_float(v[i]) * ws;
+        for (int j = 0; j < 16; j += 4) {
+          const float4 x4 = *reinterpret_cast<const float4*>(&s_xs[i & 1][b + j]);
+          const float x[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            f[j + c] = __uint_as_float(v[j + c]) * ws * x[c];
             if constexpr (DUAL) {
-              const float x = __shfl_sync(0xFFFFFFFFu, xs, h + i);
-              f[i] *= x;
-              f[i] = (f[i] / (1.0f + __expf(-f[i]))) * (__uint_as_float(u[i]) * ws2 * x);
+              f[j + c] = fp4_silu(f[j + c]) * (__uint_as_float(u[j + c]) * ws2 * x[c]);
+              if (a.row_scale) f[j + c] *= s_factor[i & 1][b + j + c];
             }
           }
-          store_tokens<16>(out, f, orow, DUAL ? factor : xs * factor, h, n);
         }
+        f4_store16(a, f, &s_row[i & 1][b], w.n0 + q * 32, s_stage[warp - 4], lane);
       }
       tc_fence_before();
       __syncwarp();
@@ -131,7 +227,7 @@ namespace bl {
 
 template <bool DUAL, int BN>
 static int fp4_gemm_go(const Fp4GemmCall& c, const F4Args& a) {
-  using S = F4Shape<DUAL, BN>;
+  using S = F4Shape<DUAL, BN, F4_GEMM_ROOM, F4_GEMM_WARPS>;
   F4Maps m;
   const int rc = f4_maps<DUAL, S>(&m, c.x, c.rows_x, c.w, c.w2, c.K, c.N, c.n_groups);
   if (rc) return rc;
@@ -141,7 +237,7 @@ static int fp4_gemm_go(const Fp4GemmCall& c, const F4Args& a) {
     limit.mark();
   }
   const long total = (long)c.max_tiles * a.tiles_w;
-  return (int)launch(fp4_gemm_kernel<DUAL, BN>, dim3((unsigned)(total < c.sms ? total : c.sms)), dim3(F4_THREADS), S::SMEM, c.stream, m, a);
+  return (int)launch(fp4_gemm_kernel<DUAL, BN>, dim3((unsigned)(total < c.sms ? total : c.sms)), dim3(S::THREADS), S::SMEM, c.stream, m, a);
 }
 
 }  // namespace bl
@@ -165,6 +261,9 @@ int bl_fp4_gemm(const Fp4GemmCall* c) {
   a.row_bytes = fp4_row_bytes(c->K); a.group_bytes = a.row_bytes * c->N;
   a.c_f32 = c->c_f32; a.c_bf16 = (__nv_bfloat16*)c->c_bf16; a.ldc = c->ldc;
   a.dst_row = c->dst_row; a.row_scale = c->row_scale; a.resid = c->resid; a.ldr = c->ldr; a.status = c->status;
+  const int es = c->c_f32 ? 4 : 2;
+  a.wide = (((uintptr_t)c->c_f32 | (uintptr_t)c->c_bf16 | (uintptr_t)c->resid) & 15) == 0 && c->ldc * es % 16 == 0 && (!c->resid || c->ldr % 4 == 0) &&
+           c->N % (c->c_f32 || c->resid ? 4 : 8) == 0;
   if (dual) {
     if (c->tile_rows == 32) return fp4_gemm_go<true, 32>(*c, a);
     if (c->tile_rows == 64) return fp4_gemm_go<true, 64>(*c, a);

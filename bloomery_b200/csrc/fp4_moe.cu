@@ -19,6 +19,7 @@
 namespace bl {
 
 constexpr int FM_TOKENS = 64, FM_SLOTS = 1024, FM_EXPERTS = 512, FM_WIDTH = 8192;
+constexpr int FM_ROOM = 206 * 1024, FM_THREADS = 256;
 
 struct FmArgs {
   const void* x; long ldx; int x_type;              // 0 bf16, 2 fp32
@@ -48,9 +49,9 @@ struct FmPlan {
 
 __device__ __forceinline__ void fm_plan(FmPlan& p, const FmArgs& a, int most) {
   const int tid = threadIdx.x, n = a.T * a.k;
-  for (int e = tid; e < a.E; e += F4_THREADS) p.count[e] = 0;
+  for (int e = tid; e < a.E; e += FM_THREADS) p.count[e] = 0;
   __syncthreads();
-  for (int s = tid; s < n; s += F4_THREADS) {
+  for (int s = tid; s < n; s += FM_THREADS) {
     const int e = a.ids[s];
     p.id[s] = (short)(e >= 0 && e < a.E ? e : -1);
   }
@@ -84,19 +85,9 @@ __device__ __forceinline__ void fm_plan(FmPlan& p, const FmArgs& a, int most) {
     }
   }
   __syncthreads();
-  for (int s = tid; s < n; s += F4_THREADS)
+  for (int s = tid; s < n; s += FM_THREADS)
     if (p.id[s] >= 0) p.slot[p.first[p.id[s]] + p.place[s]] = (short)s;
   __syncthreads();
-}
-
-__device__ __forceinline__ void fm_meet() { asm volatile("bar.sync 1, 128;" ::: "memory"); }     // the four epilogue warps
-
-// Whether all four had what they waited for: where one gave up none goes on to a meeting.
-__device__ __forceinline__ bool fm_all(bool ok) {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-               : "=r"(r) : "r"((uint32_t)ok) : "memory");
-  return r != 0;
 }
 
 struct FmUpTiles {
@@ -129,7 +120,7 @@ struct FmDownTiles {
 // A token's row in NVFP4, by the 128 threads of the epilogue warps.
 __device__ __forceinline__ void fm_token(const FmArgs& a, int t, double* s_sum, unsigned* s_max) {
   constexpr int NB = FM_WIDTH / 16 / 128;
-  const int et = threadIdx.x - 64, lane = et & 31, w = et >> 5, blocks = a.H / 16;
+  const int et = threadIdx.x - 128, lane = et & 31, w = et >> 5, blocks = a.H / 16;
   float v[NB][16];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -144,7 +135,7 @@ __device__ __forceinline__ void fm_token(const FmArgs& a, int t, double* s_sum, 
       }
     ss = warp_sum_d(ss);
     if (lane == 0) s_sum[w] = ss;
-    fm_meet();
+    f4_meet<4>();
     const float r = (float)(1.0 / sqrt((s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) / (double)a.H + a.eps));
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -156,7 +147,7 @@ __device__ __forceinline__ void fm_token(const FmArgs& a, int t, double* s_sum, 
     if (et + 128 * b < blocks) top = max(top, fp4_top16(v[b]));
   top = __reduce_max_sync(0xFFFFFFFFu, top);
   if (lane == 0) s_max[w] = top;
-  fm_meet();
+  f4_meet<4>();
   const float g = fp4_row_scale(max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3])));
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -165,7 +156,7 @@ __device__ __forceinline__ void fm_token(const FmArgs& a, int t, double* s_sum, 
 
 // Rows first .. first + rows - 1 of the activations in NVFP4, a warp a row.
 __device__ __forceinline__ void fm_rows(const FmArgs& a, int first, int rows) {
-  const int et = threadIdx.x - 64, lane = et & 31, blocks = a.I / 16;
+  const int et = threadIdx.x - 128, lane = et & 31, blocks = a.I / 16;
   for (int r = et >> 5; r < rows; r += 4) {
     const float* x = a.act + (long)(first + r) * a.I;
     uint8_t* out = a.aq + (first + r) * fp4_row_bytes(a.I);
@@ -199,8 +190,8 @@ __device__ __forceinline__ void fm_rows(const FmArgs& a, int first, int rows) {
 }
 
 template <int BN>
-__global__ void __launch_bounds__(F4_THREADS, 1) fp4_moe_up_kernel(const __grid_constant__ F4Maps map, const FmArgs a) {
-  using S = F4Shape<true, BN>;
+__global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_up_kernel(const __grid_constant__ F4Maps map, const FmArgs a) {
+  using S = F4Shape<true, BN, FM_ROOM, 4>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) F4Bars<S> bar;
   __shared__ FmPlan plan;
@@ -232,22 +223,22 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_moe_up_kernel(const __grid_
       });
   } else if (warp == 1) {
     f4_issue<true, S>(smem, bar, tiles);
-  } else if (warp >= 6) {
+  } else if (warp < 4) {
     f4_turn<true, S>(smem, bar, tiles);
   } else {
-    const int q = warp & 3, et = threadIdx.x - 64;
+    const int q = warp & 3, et = threadIdx.x - 128;
     for (;;) {
       if (et == 0) s_word = atomicAdd(a.claim, 1);
-      fm_meet();
+      f4_meet<4>();
       const int t = s_word;
       if (t >= a.T) break;
       fm_token(a, t, s_sum, s_max);
       __threadfence();
       asm volatile("fence.proxy.async;" ::: "memory");
-      fm_meet();
+      f4_meet<4>();
       if (et == 0) atomicAdd(a.claim + 1, 1);
     }
-    fm_meet();                                                       // s_word is read
+    f4_meet<4>();                                                       // s_word is read
     uint32_t ab = 0, aphase = 0;
     const int tiles_w = tiles.tiles_w;
     for (int i = 0; i < tiles.count(); ++i) {
@@ -256,7 +247,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_moe_up_kernel(const __grid_
       const int n = mt.n0 + q * 32 + lane;
       const long x_scale = a.H / 2 + a.H / 16, wrow = ((long)mt.group * a.I + min(n, a.I - 1)) * fp4_row_bytes(a.H) + x_scale;
       const float ws = *reinterpret_cast<const float*>(a.wg + wrow), ws2 = *reinterpret_cast<const float*>(a.wu + wrow);
-      if (!fm_all(mbar_wait_warp(&bar.acc_full[ab], aphase, &bar.abort))) break;
+      if (!f4_all<4>(mbar_wait_warp(&bar.acc_full[ab], aphase, &bar.abort))) break;
       tc_fence_after();
       const uint32_t tbase = bar.tmem + ((uint32_t)(q * 32) << 16) + ab * (2 * BN);
       for (int r0 = 0; r0 < e.rows; r0 += 4) {
@@ -281,7 +272,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_moe_up_kernel(const __grid_
       if (lane == 0) mbar_arrive(&bar.acc_empty[ab]);
       if (++ab == S::ACCS) { ab = 0; aphase ^= 1; }
       __threadfence();
-      fm_meet();
+      f4_meet<4>();
       if (et == 0) {
         int* ticket = a.claim + 2 + e.expert;
         const int last = atomicAdd(ticket, 1) == tiles_w - 1;
@@ -289,7 +280,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_moe_up_kernel(const __grid_
         __threadfence();
         s_word = last;
       }
-      fm_meet();
+      f4_meet<4>();
       if (s_word) fm_rows(a, e.first, e.rows);
     }
   }
@@ -298,7 +289,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_moe_up_kernel(const __grid_
 
 // 128 columns of the output from column n0 on: the slots of every token, in order.
 __device__ __forceinline__ void fm_combine(const FmArgs& a, const FmPlan& p, int n0) {
-  const int et = threadIdx.x - 64, lane = et & 31, n = n0 + 4 * lane;
+  const int et = threadIdx.x - 128, lane = et & 31, n = n0 + 4 * lane;
   if (n >= a.H) return;
   for (int t = et >> 5; t < a.T; t += 4) {
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -326,8 +317,8 @@ __device__ __forceinline__ void fm_combine(const FmArgs& a, const FmPlan& p, int
 }
 
 template <int BN>
-__global__ void __launch_bounds__(F4_THREADS, 1) fp4_moe_down_kernel(const __grid_constant__ F4Maps map, const FmArgs a) {
-  using S = F4Shape<false, BN>;
+__global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_down_kernel(const __grid_constant__ F4Maps map, const FmArgs a) {
+  using S = F4Shape<false, BN, FM_ROOM, 4>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) F4Bars<S> bar;
   __shared__ FmPlan plan;
@@ -343,10 +334,10 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_moe_down_kernel(const __gri
     if (lane == 0) f4_produce<false, S>(smem, bar, map, tiles, [] { pdl_wait(); pdl_launch(); return true; });
   } else if (warp == 1) {
     f4_issue<false, S>(smem, bar, tiles);
-  } else if (warp >= 6) {
+  } else if (warp < 4) {
     f4_turn<false, S>(smem, bar, tiles);
   } else {
-    const int q = warp & 3, et = threadIdx.x - 64, tiles_w = tiles.tiles_w;
+    const int q = warp & 3, et = threadIdx.x - 128, tiles_w = tiles.tiles_w;
     pdl_wait();
     if (blockIdx.x == 0 && et < 2) a.claim[et] = 0;                  // ready for the next call
     uint32_t ab = 0, aphase = 0;
@@ -355,7 +346,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_moe_down_kernel(const __gri
       const int n = mt.n0 + q * 32 + lane;
       const long a_scale = a.I / 2 + a.I / 16;
       const float ws = *reinterpret_cast<const float*>(a.wd + ((long)mt.group * a.H + min(n, a.H - 1)) * fp4_row_bytes(a.I) + a_scale);
-      if (!fm_all(mbar_wait_warp(&bar.acc_full[ab], aphase, &bar.abort))) break;
+      if (!f4_all<4>(mbar_wait_warp(&bar.acc_full[ab], aphase, &bar.abort))) break;
       tc_fence_after();
       const uint32_t tbase = bar.tmem + ((uint32_t)(q * 32) << 16) + ab * BN;
       for (int r0 = 0; r0 < mt.rows; r0 += 4) {
@@ -379,7 +370,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_moe_down_kernel(const __gri
       if (lane == 0) mbar_arrive(&bar.acc_empty[ab]);
       if (++ab == S::ACCS) { ab = 0; aphase ^= 1; }
       __threadfence();
-      fm_meet();
+      f4_meet<4>();
       if (et == 0) {
         int* ticket = a.claim + 2 + a.E + mt.n0 / 128;
         const int last = atomicAdd(ticket, 1) == plan.n_entries - 1;
@@ -387,7 +378,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_moe_down_kernel(const __gri
         __threadfence();
         s_word = last;
       }
-      fm_meet();
+      f4_meet<4>();
       if (s_word) fm_combine(a, plan, mt.n0);
     }
     if (plan.n_entries == 0)                                         // every slot is another tier's
@@ -425,8 +416,8 @@ struct FmWork {
 
 template <int BN>
 static int fp4_moe_go(const Fp4MoeCall& c, const FmArgs& a) {
-  using SU = F4Shape<true, BN>;
-  using SD = F4Shape<false, BN>;
+  using SU = F4Shape<true, BN, FM_ROOM, 4>;
+  using SD = F4Shape<false, BN, FM_ROOM, 4>;
   F4Maps up, down;
   int rc = f4_maps<true, SU>(&up, a.xq, a.T, a.wg, a.wu, a.H, a.I, a.E);
   if (!rc) rc = f4_maps<false, SD>(&down, a.aq, (long)a.T * a.k, a.wd, nullptr, a.I, a.H, a.E);
@@ -438,9 +429,9 @@ static int fp4_moe_go(const Fp4MoeCall& c, const FmArgs& a) {
     limit.mark();
   }
   const long hit = a.E < a.T * a.k ? a.E : a.T * a.k, n_up = hit * ((a.I + 127) / 128), n_down = hit * ((a.H + 127) / 128);
-  rc = (int)launch(fp4_moe_up_kernel<BN>, dim3((unsigned)(n_up < c.sms ? n_up : c.sms)), dim3(F4_THREADS), SU::SMEM, c.stream, up, a);
+  rc = (int)launch(fp4_moe_up_kernel<BN>, dim3((unsigned)(n_up < c.sms ? n_up : c.sms)), dim3(FM_THREADS), SU::SMEM, c.stream, up, a);
   if (rc) return rc;
-  return (int)launch(fp4_moe_down_kernel<BN>, dim3((unsigned)(n_down < c.sms ? n_down : c.sms)), dim3(F4_THREADS), SD::SMEM, c.stream, down, a);
+  return (int)launch(fp4_moe_down_kernel<BN>, dim3((unsigned)(n_down < c.sms ? n_down : c.sms)), dim3(FM_THREADS), SD::SMEM, c.stream, down, a);
 }
 
 }  // namespace bl

@@ -59,7 +59,7 @@ class Fp4Rows:
 def fp4_tile_rows(rows: int, groups: int = 1, gated: bool = False) -> int:
     """Rows of a tile of :func:`fp4_gemm` for ``rows`` rows dealt to ``groups`` matrices; ``gated``: with a second matrix."""
     per = -(-rows // groups)
-    return 32 if per <= 32 else 64 if per <= 64 else 128 if per <= 128 or gated else 256
+    return 32 if per <= 32 else 64 if per <= 64 else 128 if per <= (128 if groups == 1 else 1024) or gated else 256
 
 
 def fp4_tiles(rows: int, device) -> TileTable:
