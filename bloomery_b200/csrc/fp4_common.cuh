@@ -143,15 +143,6 @@ __device__ __forceinline__ float fp4_silu(float x) { return __fdividef(x, 1.0f +
 __host__ __device__ constexpr uint32_t fp4_idesc(int n) {
   return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-// The scales of 64 values of a row are one 32-bit cell of tensor memory: row r of an operand has its cell in lane r % 32 (the same in
-// all four quarters), column r / 32.  32 lanes x 16 bytes of shared memory become the four columns of 128 rows.
-__device__ __forceinline__ void fp4_scales_to_tmem(uint32_t taddr, uint32_t smem) {
-  const uint64_t desc = (uint64_t)((smem >> 4) & 0x3FFF) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;     // rows of 16 bytes, no swizzle
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t"
-      "elect.sync _|e, 0xFFFFFFFF;\n\t"
-      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc) : "memory");
-}
 __device__ __forceinline__ void umma_fp4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sa, uint32_t sb,
                                          uint32_t accumulate) {
   asm volatile(
@@ -162,20 +153,35 @@ __device__ __forceinline__ void umma_fp4(uint32_t tmem_d, uint64_t adesc, uint64
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
 }
 
-// Scales of 256 values (16 bytes) of up to 128 rows, as they lie in the rows, into the cells of four instructions: thread = lane, word
-// s of row 32 j + lane goes to word j of instruction s.  Rows lie PITCH times 16 bytes apart; `groups`: groups of 32 rows there are.
-template <int PITCH>
-__device__ __forceinline__ void fp4_turn_scales(const uint4* raw, uint4* cells, int lane, int groups) {
-  uint4 r[4];
+// The scales of 64 values of a row are one 32-bit cell of tensor memory: row r of an operand has its cell in lane r % 32, the same in all four
+// quarters, column r / 32.  Four warps, one for each quarter, take the 16 bytes of 256 values of each row out of its box in shared memory (SPAN
+// pieces of 16 bytes a row, swizzled so that eight rows lie in different banks) and store the cells of four instructions: word k of
+// row 32 j + lane goes to column k * COLUMNS + j.
+__device__ __forceinline__ void fp4_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+template <int SPAN>
+__device__ __forceinline__ uint4 fp4_raw(const uint8_t* box, int row, int at) {
+  const int turn = SPAN == 4 ? row >> 1 & 3 : row >> 2 & 1;
+  return *reinterpret_cast<const uint4*>(box + row * (16 * SPAN) + ((at ^ turn) << 4));
+}
+template <int SPAN, int COLUMNS>
+__device__ __forceinline__ void fp4_cells(uint32_t taddr, const uint8_t* box, int at, int lane, int groups) {
+  uint32_t c[4 * COLUMNS];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) r[j] = j < groups ? raw[(32 * j + lane) * PITCH] : make_uint4(0u, 0u, 0u, 0u);
-  cells[lane] = make_uint4(r[0].x, r[1].x, r[2].x, r[3].x);
-  cells[32 + lane] = make_uint4(r[0].y, r[1].y, r[2].y, r[3].y);
-  cells[64 + lane] = make_uint4(r[0].z, r[1].z, r[2].z, r[3].z);
-  cells[96 + lane] = make_uint4(r[0].w, r[1].w, r[2].w, r[3].w);
+  for (int j = 0; j < COLUMNS; ++j) {
+    const uint4 r = j < groups ? fp4_raw<SPAN>(box, 32 * j + lane, at) : make_uint4(0u, 0u, 0u, 0u);
+    c[j] = r.x; c[COLUMNS + j] = r.y; c[2 * COLUMNS + j] = r.z; c[3 * COLUMNS + j] = r.w;
+  }
+  if constexpr (COLUMNS == 8) tmem_st32(taddr, c);
+  else fp4_st16(taddr, c);
 }
 
-// Maps of NVFP4 rows [groups][rows][row bytes]: codes in boxes of 256 values (zeros past the row's end), scales in boxes of 256 * span.
+// Maps of NVFP4 rows [groups][rows][row bytes]: codes in boxes of 256 values (zeros past the row's end), scales in boxes of
+// 256 * span.
 inline int fp4_maps(CUtensorMap* codes, CUtensorMap* scales, const void* base, int K, long rows, long groups, int box_rows, int span) {
   const cuuint64_t rb = (cuuint64_t)fp4_row_bytes(K);
   cuuint64_t dims[3] = {(cuuint64_t)K / 2, (cuuint64_t)rows, (cuuint64_t)groups};
@@ -185,7 +191,8 @@ inline int fp4_maps(CUtensorMap* codes, CUtensorMap* scales, const void* base, i
   if (rc) return rc;
   dims[0] = (cuuint64_t)K / 16;
   box[0] = 16 * span;
-  return make_map_any(scales, (const uint8_t*)base + K / 2, 3, dims, str, box, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE);
+  return make_map_any(scales, (const uint8_t*)base + K / 2, 3, dims, str, box, CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                      span == 4 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
 }
 
 }  // namespace bl

@@ -1,11 +1,11 @@
 // Grouped product of NVFP4 rows with NVFP4 weights on tcgen05 (sm_100a): four-bit codes go to the tensor cores as they are.
 //   C[t, n] = xs[t] ws[n] sum_b sx[t, b] sw[n, b] sum_{k in block b} x[t, k] w[g][n, k]        blocks of 16 values
 //
-// The 128 weight rows of a tile are the M side of the MMA, its tokens the N side.  A TMA thread streams boxes of 256 values: 128
-// bytes of codes a row (128-byte swizzle) and 16 bytes of scales.  Two warps turn the scales of a stage into the cells that the
-// instruction reads (weights and activations keep the layout of their rows in memory, which the decode chain reads too), the
-// issuing warp copies them to tensor memory (tcgen05.cp) and issues four kind::mxf4nvf4 MMAs a stage, K = 64 each, which multiply codes,
-// apply both blocks' scales and add in fp32.  Four epilogue warps apply the two fp32 scales.
+// The weight rows of a tile are the M side of the MMA, its tokens the N side.  TMA threads stream boxes of 256 values: 128 bytes of
+// codes a row (128-byte swizzle) and, for several boxes at once, 16 bytes of scales.  Weights and activations keep the layout of their rows in
+// memory, which the decode chain reads too: four warps bring a stage's scales into the cells of tensor memory that the instruction reads
+// (tcgen05.st).  The issuing warp issues four kind::mxf4nvf4 MMAs a stage, K = 64 each, which multiply codes, apply both blocks' scales and
+// add in fp32.  Eight epilogue warps apply the two fp32 scales.
 //   * "dual" mode runs gate and up in one main loop; the epilogue writes silu(gate) * up;
 //   * the epilogue scatters and scales like the other GEMMs (dst_row / row_scale / resid).
 // Every wait is bounded; on expiry the CTA raises status word 1, leaves its loops, frees its TMEM and returns.
@@ -37,6 +37,7 @@ struct F4Args {
   int wide;                 // rows of the output (and of resid) start at 16 bytes and hold whole 16 bytes
 };
 
+template <int AR>
 struct F4GemmTiles {
   const F4Args& a;
   int total, kblocks;
@@ -44,20 +45,20 @@ struct F4GemmTiles {
   __device__ __forceinline__ F4Work at(int i) const {
     const int t = (int)blockIdx.x + i * (int)gridDim.x;
     const F4Tile mt = a.tiles[t / a.tiles_w];
-    return F4Work{mt.group, t % a.tiles_w * 128, mt.row0, min(a.tile_rows, mt.row_end - mt.row0), 0, kblocks};
+    return F4Work{mt.group, t % a.tiles_w * AR, mt.row0, min(a.tile_rows, mt.row_end - mt.row0), 0, kblocks};
   }
 };
 
-// 16 tokens of the 32 columns from n0 on, `f` this lane's column of them (lane = column); rows below zero are none.
+// 16 tokens of the 32 columns from n0 on (below `end`), `f` this lane's column of them (lane = column); rows below zero are none.
 // Wide: they are turned in shared memory, so that a lane stores 16 bytes of a token: a store of four bytes, or two, costs its warp some 19
 // clocks with the address of its token, 16 bytes cost them for four tokens, or eight.
-__device__ __forceinline__ void f4_store16(const F4Args& a, const float (&f)[16], const int* rows, int n0, uint8_t* stage, int lane) {
+__device__ __forceinline__ void f4_store16(const F4Args& a, const float (&f)[16], const int* rows, int n0, int end, uint8_t* stage, int lane) {
   if (a.wide && a.c_bf16 && !a.resid) {
     __nv_bfloat16* s = reinterpret_cast<__nv_bfloat16*>(stage);
 #pragma unroll
     for (int j = 0; j < 16; ++j) s[32 * j + lane] = __float2bfloat16_rn(f[j]);
     __syncwarp();
-    const int n = n0 + 8 * (lane & 3), none = n < a.N ? 0 : -1;
+    const int n = n0 + 8 * (lane & 3), none = n < end ? 0 : -1;
     int row[2];
     uint4 v[2];
 #pragma unroll
@@ -76,7 +77,7 @@ __device__ __forceinline__ void f4_store16(const F4Args& a, const float (&f)[16]
   for (int j = 0; j < 16; ++j) s[32 * j + lane] = f[j];
   __syncwarp();
   if (a.wide) {
-    const int n = n0 + 4 * (lane & 7), none = n < a.N ? 0 : -1;
+    const int n = n0 + 4 * (lane & 7), none = n < end ? 0 : -1;
     int row[4];
     float4 v[4];
 #pragma unroll
@@ -112,7 +113,7 @@ __device__ __forceinline__ void f4_store16(const F4Args& a, const float (&f)[16]
     for (int j = 0; j < 16; ++j) {
       const int row = rows[j];
       float v = s[32 * j + lane];
-      if (row < 0 || n >= a.N) continue;
+      if (row < 0 || n >= end) continue;
       if (a.resid) v += a.resid[(unsigned long long)(unsigned)row * (unsigned)a.ldr + n];
       if (a.c_f32) a.c_f32[(unsigned long long)(unsigned)row * (unsigned)a.ldc + n] = v;
       else a.c_bf16[(unsigned long long)(unsigned)row * (unsigned)a.ldc + n] = __float2bfloat16_rn(v);
@@ -121,10 +122,10 @@ __device__ __forceinline__ void f4_store16(const F4Args& a, const float (&f)[16]
   __syncwarp();
 }
 
-template <bool DUAL, int BN>
-__global__ void __launch_bounds__(128 + 32 * F4_GEMM_WARPS, 1)
+template <bool DUAL, int BN, int AR>
+__global__ void __launch_bounds__(F4_EPILOGUE + 32 * F4_GEMM_WARPS, 1)
 fp4_gemm_kernel(const __grid_constant__ F4Maps map, const F4Args a) {
-  using S = F4Shape<DUAL, BN, F4_GEMM_ROOM, F4_GEMM_WARPS>;
+  using S = F4Shape<DUAL, BN, F4_GEMM_ROOM, F4_GEMM_WARPS, AR>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) F4Bars<S> bar;
   __shared__ __align__(16) int s_row[2][BN];
@@ -132,19 +133,21 @@ fp4_gemm_kernel(const __grid_constant__ F4Maps map, const F4Args a) {
   __shared__ __align__(16) uint8_t s_stage[F4_GEMM_WARPS][2048];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  f4_open<S>(bar);
+  f4_open<S>(bar, map);
   pdl_wait();
   pdl_launch();
-  F4GemmTiles tiles{a, min(*a.n_tiles, a.max_tiles) * a.tiles_w, (a.K + 255) / 256};
+  F4GemmTiles<AR> tiles{a, min(*a.n_tiles, a.max_tiles) * a.tiles_w, (a.K + 255) / 256};
 
   if (warp == 0) {
-    if (lane == 0) f4_produce<DUAL, S>(smem, bar, map, tiles, [] { return true; });
+    if (lane == 0) f4_weights<S>(smem, bar, map, tiles);
+  } else if (warp == 6) {
+    if (lane == 0) f4_tokens<S>(smem, bar, map, tiles);
   } else if (warp == 1) {
-    f4_issue<DUAL, S>(smem, bar, tiles);
-  } else if (warp < 4) {
-    f4_turn<DUAL, S>(smem, bar, tiles);
+    f4_issue<S>(smem, bar, tiles);
+  } else if (warp < 6) {
+    f4_cells<S>(smem, bar, tiles);
   } else {
-    const int q = warp & 3, half = (warp - 4) >> 2, et = threadIdx.x - 128;          // TMEM lane quarter of this warp; 0 .. 255
+    const int q = warp & 3, half = (warp - 7) >> 2, et = threadIdx.x - F4_EPILOGUE;          // TMEM lane quarter of this warp; 0 .. 255
     const int n_tiles = tiles.count();
     const long scale_at = a.K / 2 + a.K / 16;
     // What a tile needs beside its products is asked for while the tile before is worked on, a token a thread, and laid down in shared
@@ -181,7 +184,7 @@ fp4_gemm_kernel(const __grid_constant__ F4Maps map, const F4Args a) {
       tc_fence_after();
       const uint32_t tbase = bar.tmem + ((uint32_t)(q * 32) << 16) + ab * (S::MATS * BN);
 #pragma unroll 1
-      for (int b = 16 * half; b < w.rows; b += 32) {               // the two warps of a quarter take 16 tokens each in turn
+      for (int b = 16 * half; b < w.rows && q * 32 < AR; b += 32) {               // the two warps of a quarter take 16 tokens each in turn
         uint32_t v[16], u[DUAL ? 16 : 1];
         tmem_ld16(tbase + b, v);
         if constexpr (DUAL) tmem_ld16(tbase + BN + b, u);
@@ -200,7 +203,7 @@ fp4_gemm_kernel(const __grid_constant__ F4Maps map, const F4Args a) {
             }
           }
         }
-        f4_store16(a, f, &s_row[i & 1][b], w.n0 + q * 32, s_stage[warp - 4], lane);
+        f4_store16(a, f, &s_row[i & 1][b], w.n0 + q * 32, min(a.N, w.n0 + AR), s_stage[warp - 7], lane);
       }
       tc_fence_before();
       __syncwarp();
@@ -225,19 +228,20 @@ struct Fp4GemmCall {
 
 namespace bl {
 
-template <bool DUAL, int BN>
-static int fp4_gemm_go(const Fp4GemmCall& c, const F4Args& a) {
-  using S = F4Shape<DUAL, BN, F4_GEMM_ROOM, F4_GEMM_WARPS>;
+template <bool DUAL, int BN, int AR>
+static int fp4_gemm_go(const Fp4GemmCall& c, F4Args& a) {
+  a.tiles_w = (c.N + AR - 1) / AR;
+  using S = F4Shape<DUAL, BN, F4_GEMM_ROOM, F4_GEMM_WARPS, AR>;
   F4Maps m;
-  const int rc = f4_maps<DUAL, S>(&m, c.x, c.rows_x, c.w, c.w2, c.K, c.N, c.n_groups);
+  const int rc = f4_maps<S>(&m, c.x, c.rows_x, c.w, c.w2, c.K, c.N, c.n_groups);
   if (rc) return rc;
   static PerDevice limit;
   if (limit.due()) {
-    cudaFuncSetAttribute(fp4_gemm_kernel<DUAL, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+    cudaFuncSetAttribute(fp4_gemm_kernel<DUAL, BN, AR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
     limit.mark();
   }
   const long total = (long)c.max_tiles * a.tiles_w;
-  return (int)launch(fp4_gemm_kernel<DUAL, BN>, dim3((unsigned)(total < c.sms ? total : c.sms)), dim3(S::THREADS), S::SMEM, c.stream, m, a);
+  return (int)launch(fp4_gemm_kernel<DUAL, BN, AR>, dim3((unsigned)(total < c.sms ? total : c.sms)), dim3(S::THREADS), S::SMEM, c.stream, m, a);
 }
 
 }  // namespace bl
@@ -254,9 +258,9 @@ int bl_fp4_gemm(const Fp4GemmCall* c) {
   BL_REQUIRE(((uintptr_t)c->x & 15) == 0 && ((uintptr_t)c->w & 15) == 0 && ((uintptr_t)c->w2 & 15) == 0, BL_ERR_ALIGN);
   BL_REQUIRE((c->c_f32 != nullptr) != (c->c_bf16 != nullptr) && c->ldc < 1L << 30 && c->ldr < 1L << 30, BL_ERR_SHAPE);
   F4Args a{};
-  a.N = c->N; a.K = c->K; a.tiles_w = (c->N + 127) / 128; a.tile_rows = c->tile_rows;
+  a.N = c->N; a.K = c->K; a.tile_rows = c->tile_rows;
   a.tiles = (const F4Tile*)c->tiles; a.n_tiles = c->n_tiles; a.max_tiles = c->max_tiles;
-  BL_REQUIRE((long)a.max_tiles * a.tiles_w < 1L << 31, BL_ERR_LIMIT);
+  BL_REQUIRE((long)a.max_tiles * ((c->N + 15) / 16) < 1L << 31, BL_ERR_LIMIT);
   a.x = (const uint8_t*)c->x; a.w = (const uint8_t*)c->w; a.w2 = (const uint8_t*)c->w2;
   a.row_bytes = fp4_row_bytes(c->K); a.group_bytes = a.row_bytes * c->N;
   a.c_f32 = c->c_f32; a.c_bf16 = (__nv_bfloat16*)c->c_bf16; a.ldc = c->ldc;
@@ -264,15 +268,21 @@ int bl_fp4_gemm(const Fp4GemmCall* c) {
   const int es = c->c_f32 ? 4 : 2;
   a.wide = (((uintptr_t)c->c_f32 | (uintptr_t)c->c_bf16 | (uintptr_t)c->resid) & 15) == 0 && c->ldc * es % 16 == 0 && (!c->resid || c->ldr % 4 == 0) &&
            c->N % (c->c_f32 || c->resid ? 4 : 8) == 0;
+  // Weight rows of a tile: as few as still find a processor for each tile at once.
+  auto one_wave = [&](int ar) { return (long)c->max_tiles * ((c->N + ar - 1) / ar) <= c->sms; };
+  const int rows = c->tile_rows, ar = one_wave(16) ? 16 : one_wave(32) ? 32 : one_wave(64) ? 64 : 128;
   if (dual) {
-    if (c->tile_rows == 32) return fp4_gemm_go<true, 32>(*c, a);
-    if (c->tile_rows == 64) return fp4_gemm_go<true, 64>(*c, a);
-    return fp4_gemm_go<true, 128>(*c, a);
+    if (rows == 32) return ar <= 32 ? fp4_gemm_go<true, 32, 32>(*c, a) : ar == 64 ? fp4_gemm_go<true, 32, 64>(*c, a) : fp4_gemm_go<true, 32, 128>(*c, a);
+    if (rows == 64) return ar <= 64 ? fp4_gemm_go<true, 64, 64>(*c, a) : fp4_gemm_go<true, 64, 128>(*c, a);
+    return fp4_gemm_go<true, 128, 128>(*c, a);
   }
-  if (c->tile_rows == 32) return fp4_gemm_go<false, 32>(*c, a);
-  if (c->tile_rows == 64) return fp4_gemm_go<false, 64>(*c, a);
-  if (c->tile_rows == 128) return fp4_gemm_go<false, 128>(*c, a);
-  return fp4_gemm_go<false, 256>(*c, a);
+  if (rows == 32)
+    return ar == 16 ? fp4_gemm_go<false, 32, 16>(*c, a) : ar == 32 ? fp4_gemm_go<false, 32, 32>(*c, a) : ar == 64 ? fp4_gemm_go<false, 32, 64>(*c, a)
+                                                                                                                  : fp4_gemm_go<false, 32, 128>(*c, a);
+  if (rows == 64)
+    return ar <= 32 ? fp4_gemm_go<false, 64, 32>(*c, a) : ar == 64 ? fp4_gemm_go<false, 64, 64>(*c, a) : fp4_gemm_go<false, 64, 128>(*c, a);
+  if (rows == 128) return ar <= 64 ? fp4_gemm_go<false, 128, 64>(*c, a) : fp4_gemm_go<false, 128, 128>(*c, a);
+  return fp4_gemm_go<false, 256, 128>(*c, a);
 }
 
 }  // extern "C"

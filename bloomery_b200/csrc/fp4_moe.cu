@@ -12,14 +12,20 @@
 //   * the CTA that finishes an expert's last tile quantises its rows for the second launch, which reads them as they lie,
 //     expert by expert;
 //   * in the second launch the CTA that finishes the last tile of 128 output columns adds up the slots of every token, in order.
+// CTAs walk tiles next to each other, so that one takes part in two or three experts, or column blocks, and says so once for each.
+// Few tokens (FM_FEW) go without meeting: each CTA quantises the rows that it needs for itself, and the second launch has the columns of a
+// CTA to itself, all experts of them, so that it adds up its slots in shared memory.
 // Rows are claimed and finished by whoever is there, so no CTA waits for one that has not started; the one wait between CTAs (for the tokens'
 // rows) is bounded like all others.  Sums of a slot run in one order: the same bits on every run and with every number of CTAs.
+#include <type_traits>
+
 #include "fp4_pipe.cuh"
 
 namespace bl {
 
 constexpr int FM_TOKENS = 64, FM_SLOTS = 1024, FM_EXPERTS = 512, FM_WIDTH = 8192;
-constexpr int FM_ROOM = 206 * 1024, FM_THREADS = 256;
+constexpr int FM_FEW = 4, FM_FEW_SLOTS = 32;        // tokens and slots of a round that goes without meetings
+constexpr int FM_THREADS = F4_EPILOGUE + 128;
 
 struct FmArgs {
   const void* x; long ldx; int x_type;              // 0 bf16, 2 fp32
@@ -27,9 +33,9 @@ struct FmArgs {
   const int* ids; const float* wts;
   int T, k, E, H, I;
   const uint8_t* wg; const uint8_t* wu; const uint8_t* wd;
-  uint8_t* xq;                                      // [T] NVFP4 rows of H
+  uint8_t* xq;                                      // [T] NVFP4 rows of H; few tokens: as many for each CTA
   float* act;                                       // [T * k][I], expert by expert
-  uint8_t* aq;                                      // the same as NVFP4 rows
+  uint8_t* aq;                                      // the same as NVFP4 rows; few tokens: as many for each CTA
   float* slot_out;                                  // [T * k][H]
   int* claim;                                       // rows taken, rows done, then a ticket for every expert and every 128 columns
   const float* resid; long ldr;
@@ -38,217 +44,336 @@ struct FmArgs {
 };
 
 // Which experts are hit and by which slots: entries of one expert each, at most `most` slots in one.
+template <int SLOTS, int ENTRIES>
 struct FmPlan {
   int n_entries;
-  short id[FM_SLOTS];                               // of every slot, -1: none of ours
-  short slot[FM_SLOTS];                             // expert by expert
-  short place[FM_SLOTS];
-  struct Entry { short expert, rows; int first; } entry[FM_EXPERTS + FM_SLOTS / 32];
-  int count[FM_EXPERTS], first[FM_EXPERTS];
+  struct Entry { short expert, rows; int first; } entry[ENTRIES];
+  short id[SLOTS];                                  // of every slot, -1: none of ours
+  short slot[SLOTS];                                // expert by expert
 };
+using FmFewPlan = FmPlan<FM_FEW_SLOTS, FM_FEW_SLOTS>;
+using FmFullPlan = FmPlan<FM_SLOTS, FM_EXPERTS + FM_SLOTS / 32>;
 
-__device__ __forceinline__ void fm_plan(FmPlan& p, const FmArgs& a, int most) {
+// Up to 32 slots, by one warp: experts in the order in which they appear.
+__device__ __forceinline__ void fm_plan(FmFewPlan& p, const FmArgs& a, int, void*) {
   const int tid = threadIdx.x, n = a.T * a.k;
-  for (int e = tid; e < a.E; e += FM_THREADS) p.count[e] = 0;
-  __syncthreads();
-  for (int s = tid; s < n; s += FM_THREADS) {
-    const int e = a.ids[s];
-    p.id[s] = (short)(e >= 0 && e < a.E ? e : -1);
-  }
-  __syncthreads();
-  // a slot's place among those of its expert: every CTA comes to the same one
-  if (tid < 32)
-    for (int s = tid; s - tid < n; s += 32) {
-      const int e = s < n ? p.id[s] : -1;
-      const unsigned same = __match_any_sync(0xffffffffu, e), before = same & ((1u << tid) - 1);
-      if (e >= 0) p.place[s] = (short)(p.count[e] + __popc(before));
-      __syncwarp();
-      if (e >= 0 && before == 0) p.count[e] += __popc(same);
-      __syncwarp();
-    }
   if (tid < 32) {
-    const int per = (a.E + 31) / 32, e0 = min(a.E, tid * per), e1 = min(a.E, e0 + per);
-    int rows = 0, entries = 0;
-    for (int e = e0; e < e1; ++e) { rows += p.count[e]; entries += (p.count[e] + most - 1) / most; }
-    int ro = rows, en = entries;
+    int e = tid < n ? a.ids[tid] : -1;
+    if (e >= a.E || e < 0) e = -1;
+    const unsigned same = __match_any_sync(0xffffffffu, e), below = (1u << tid) - 1;
+    const bool leads = e >= 0 && (same & below) == 0;
+    const unsigned leaders = __ballot_sync(0xffffffffu, leads);
+    const int rows = leads ? __popc(same) : 0;
+    int before = rows;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int r = __shfl_up_sync(0xffffffffu, ro, d), t = __shfl_up_sync(0xffffffffu, en, d);
-      if (tid >= d) { ro += r; en += t; }
+      const int r = __shfl_up_sync(0xffffffffu, before, d);
+      if (tid >= d) before += r;
     }
-    if (tid == 31) p.n_entries = en;
-    ro -= rows; en -= entries;
-    for (int e = e0; e < e1; ++e) {
-      p.first[e] = ro;
-      for (int r = 0; r < p.count[e]; r += most) p.entry[en++] = FmPlan::Entry{(short)e, (short)min(most, p.count[e] - r), ro + r};
-      ro += p.count[e];
-    }
+    before -= rows;                                 // a leader's: slots of the experts in front of its own
+    const int first = __shfl_sync(0xffffffffu, before, __ffs(same) - 1);
+    if (tid < n) p.id[tid] = (short)e;
+    if (leads) p.entry[__popc(leaders & below)] = FmFewPlan::Entry{(short)e, (short)rows, first};
+    if (e >= 0) p.slot[first + __popc(same & below)] = (short)tid;
+    if (tid == 0) p.n_entries = __popc(leaders);
   }
-  __syncthreads();
-  for (int s = tid; s < n; s += FM_THREADS)
-    if (p.id[s] >= 0) p.slot[p.first[p.id[s]] + p.place[s]] = (short)s;
   __syncthreads();
 }
 
-struct FmUpTiles {
-  const FmPlan& p;
-  int tiles_w, kblocks, T;
-  __device__ __forceinline__ int count() const {
-    const int total = p.n_entries * tiles_w;
-    return total > (int)blockIdx.x ? (total - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+// Any number, by all threads: a warp counts the experts of its own slots (an eighth of them, next to each other), so that a slot's place
+// among those of its expert is the same in every CTA.  `scratch`: FM_EXPERTS * 10 shorts that TMA writes later.
+__device__ __forceinline__ void fm_plan(FmFullPlan& p, const FmArgs& a, int most, void* scratch) {
+  constexpr int W = 8, PER = FM_SLOTS / (32 * W);                  // warps that count
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, n = a.T * a.k;
+  short* count = reinterpret_cast<short*>(scratch);                // [W][FM_EXPERTS], then what lies in front of a warp's slots
+  short *all = count + W * FM_EXPERTS, *first = all + FM_EXPERTS;
+  const int mine = (n + W - 1) / W, lo = min(n, w * mine), hi = min(n, lo + mine);
+  int id[PER], place[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int s = lo + 32 * i + lane;
+    id[i] = s < hi ? a.ids[s] : -1;
   }
-  __device__ __forceinline__ int entry(int i) const { return ((int)blockIdx.x + i * (int)gridDim.x) / tiles_w; }
+  for (int i = tid; i < W * FM_EXPERTS / 2; i += FM_THREADS) reinterpret_cast<int*>(count)[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int s = lo + 32 * i + lane;
+    if (lo + 32 * i >= hi) break;
+    if (id[i] < 0 || id[i] >= a.E) id[i] = -1;
+    const unsigned same = __match_any_sync(0xffffffffu, id[i]), before = same & ((1u << lane) - 1);
+    short* c = count + w * FM_EXPERTS + (id[i] >= 0 ? id[i] : 0);
+    if (id[i] >= 0) place[i] = *c + __popc(before);
+    __syncwarp();
+    if (id[i] >= 0 && before == 0) *c += (short)__popc(same);
+    __syncwarp();
+    if (s < hi) p.id[s] = (short)id[i];
+  }
+  __syncthreads();
+  for (int e = tid; e < a.E; e += FM_THREADS) {
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) { const int c = count[i * FM_EXPERTS + e]; count[i * FM_EXPERTS + e] = (short)sum; sum += c; }
+    all[e] = (short)sum;
+  }
+  __syncthreads();
+  if (w == 0) {
+    const int per = (a.E + 31) / 32, e0 = min(a.E, lane * per), e1 = min(a.E, e0 + per);
+    int rows = 0, entries = 0;
+    for (int e = e0; e < e1; ++e) { rows += all[e]; entries += (all[e] + most - 1) / most; }
+    int both = rows | entries << 16, sum = both;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int r = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += r;
+    }
+    if (lane == 31) p.n_entries = sum >> 16;
+    sum -= both;
+    int ro = sum & 0xffff, en = sum >> 16;
+    for (int e = e0; e < e1; ++e) {
+      const int c = all[e];
+      first[e] = (short)ro;
+      for (int r = 0; r < c; r += most) p.entry[en++] = FmFullPlan::Entry{(short)e, (short)min(most, c - r), ro + r};
+      ro += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (lo + 32 * i + lane < hi && id[i] >= 0) p.slot[first[id[i]] + count[w * FM_EXPERTS + id[i]] + place[i]] = (short)(lo + 32 * i + lane);
+  asm volatile("fence.proxy.async;" ::: "memory");                 // the scratch is a ring's from here on
+  __syncthreads();
+}
+
+// A CTA's share of n tiles: next to each other.
+struct FmShare {
+  int lo, hi;
+  __device__ __forceinline__ explicit FmShare(int n) : lo((int)((long)n * blockIdx.x / gridDim.x)), hi((int)((long)n * (blockIdx.x + 1) / gridDim.x)) {}
+  __device__ __forceinline__ int count() const { return hi - lo; }
+};
+template <class Plan, int AR>
+struct FmUpTiles : FmShare {                        // expert by expert
+  const Plan& p;
+  int tiles_w, kblocks, row0, T;
+  __device__ __forceinline__ FmUpTiles(const Plan& p, int I, int H, int row0, int T)
+      : FmShare(p.n_entries * ((I + AR - 1) / AR)), p(p), tiles_w((I + AR - 1) / AR), kblocks((H + 255) / 256), row0(row0), T(T) {}
+  __device__ __forceinline__ int entry(int i) const { return (lo + i) / tiles_w; }
   __device__ __forceinline__ F4Work at(int i) const {
-    const int t = (int)blockIdx.x + i * (int)gridDim.x;
-    return F4Work{p.entry[t / tiles_w].expert, t % tiles_w * 128, 0, T, 0, kblocks};      // all tokens
+    return F4Work{p.entry[entry(i)].expert, (lo + i) % tiles_w * AR, row0, T, 0, kblocks};      // all tokens
   }
 };
-struct FmDownTiles {
-  const FmPlan& p;
-  int tiles_w, kblocks;
-  __device__ __forceinline__ int count() const {
-    const int total = p.n_entries * tiles_w;
-    return total > (int)blockIdx.x ? (total - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+template <class Plan, int AR, bool FEW>
+struct FmDownTiles : FmShare {                      // columns after columns; few tokens: whole columns
+  const Plan& p;
+  int kblocks, row0;
+  __device__ __forceinline__ FmDownTiles(const Plan& p, int H, int I, int row0)
+      : FmShare(FEW ? (H + AR - 1) / AR : p.n_entries * ((H + AR - 1) / AR)), p(p), kblocks((I + 255) / 256), row0(row0) {
+    if (FEW) { lo *= p.n_entries; hi *= p.n_entries; }
   }
+  __device__ __forceinline__ typename Plan::Entry entry(int i) const { return p.entry[(lo + i) % p.n_entries]; }
   __device__ __forceinline__ F4Work at(int i) const {
-    const int t = (int)blockIdx.x + i * (int)gridDim.x;
-    const FmPlan::Entry e = p.entry[t / tiles_w];
-    return F4Work{e.expert, t % tiles_w * 128, e.first, e.rows, 0, kblocks};
+    const typename Plan::Entry e = entry(i);
+    return F4Work{e.expert, (lo + i) / p.n_entries * AR, row0 + e.first, e.rows, 0, kblocks};
   }
 };
 
-// A token's row in NVFP4, by the 128 threads of the epilogue warps.
-__device__ __forceinline__ void fm_token(const FmArgs& a, int t, double* s_sum, unsigned* s_max) {
-  constexpr int NB = FM_WIDTH / 16 / 128;
-  const int et = threadIdx.x - 128, lane = et & 31, w = et >> 5, blocks = a.H / 16;
-  float v[NB][16];
-#pragma unroll
-  for (int b = 0; b < NB; ++b)
-    if (et + 128 * b < blocks) fp4_load16(a.x, a.x_type, (long)t * a.ldx + 16 * (et + 128 * b), v[b]);
+// A token's row in NVFP4, by the 128 threads of the epilogue warps.  It is run once or twice by a CTA: what counts is little code, which is
+// fetched as it runs, so a thread walks its blocks of 16 three times instead of keeping them.
+__device__ __forceinline__ void fm_token(const FmArgs& a, int t, uint8_t* row, double* s_sum, unsigned* s_max) {
+  const int et = threadIdx.x - F4_EPILOGUE, lane = et & 31, w = et >> 5, blocks = a.H / 16;
+  float v[16], r = 1.0f;
+  auto load = [&](int b) { fp4_load16(a.x, a.x_type, (long)t * a.ldx + 16 * b, v); };
   if (a.gain) {
     double ss = 0.0;
+#pragma unroll 1
+    for (int b = et; b < blocks; b += 128) {
+      load(b);
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-      if (et + 128 * b < blocks) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) ss = fma((double)v[b][i], (double)v[b][i], ss);
-      }
+      for (int i = 0; i < 16; ++i) ss = fma((double)v[i], (double)v[i], ss);
+    }
     ss = warp_sum_d(ss);
     if (lane == 0) s_sum[w] = ss;
     f4_meet<4>();
-    const float r = (float)(1.0 / sqrt((s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) / (double)a.H + a.eps));
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-      if (et + 128 * b < blocks) fp4_scale16(v[b], r, a.gain + 16 * (et + 128 * b));
+    r = (float)(1.0 / sqrt((s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) / (double)a.H + a.eps));
   }
   unsigned top = 0;
-#pragma unroll
-  for (int b = 0; b < NB; ++b)
-    if (et + 128 * b < blocks) top = max(top, fp4_top16(v[b]));
+#pragma unroll 1
+  for (int b = et; b < blocks; b += 128) {
+    if (blocks > 128 || !a.gain) load(b);             // else the one block is still there
+    if (a.gain) fp4_scale16(v, r, a.gain + 16 * b);
+    top = max(top, fp4_top16(v));
+  }
   top = __reduce_max_sync(0xFFFFFFFFu, top);
   if (lane == 0) s_max[w] = top;
   f4_meet<4>();
   const float g = fp4_row_scale(max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3])));
-#pragma unroll
-  for (int b = 0; b < NB; ++b)
-    if (et + 128 * b < blocks) fp4_store_block(a.xq + t * fp4_row_bytes(a.H), a.H, et + 128 * b, v[b], g);
+#pragma unroll 1
+  for (int b = et; b < blocks; b += 128) {
+    if (blocks > 128) {
+      load(b);
+      if (a.gain) fp4_scale16(v, r, a.gain + 16 * b);
+    }
+    fp4_store_block(row, a.H, b, v, g);
+  }
+}
+// The gain's way to this processor, before the launch in front of this one has ended.
+__device__ __forceinline__ void fm_ask_gain(const FmArgs& a) {
+  if (a.gain)
+    for (int i = threadIdx.x * 32; i < a.H; i += FM_THREADS * 32) asm volatile("prefetch.global.L1 [%0];" ::"l"(a.gain + i) : "memory");
 }
 
-// Rows first .. first + rows - 1 of the activations in NVFP4, a warp a row.
-__device__ __forceinline__ void fm_rows(const FmArgs& a, int first, int rows) {
-  const int et = threadIdx.x - 128, lane = et & 31, blocks = a.I / 16;
-  for (int r = et >> 5; r < rows; r += 4) {
-    const float* x = a.act + (long)(first + r) * a.I;
-    uint8_t* out = a.aq + (first + r) * fp4_row_bytes(a.I);
-    float v[4][16];
-    unsigned top = 0;
-    auto load = [&](int from) {
+// Rows first .. first + rows - 1 of the activations in NVFP4 in the rows of `to`: a block of 16 a thread, rows next to each other, up to
+// 32 rows at a time (s_top).
+__device__ __forceinline__ void fm_rows(const FmArgs& a, int first, int rows, uint8_t* to, unsigned* s_top) {
+  const int et = threadIdx.x - F4_EPILOGUE, per = a.I / 16;
+  for (int r0 = 0; r0 < rows; r0 += 32) {
+    const int n = min(32, rows - r0) * per;
+    if (et < 32) s_top[et] = 0;
+    f4_meet<4>();
+    const float4* x = reinterpret_cast<const float4*>(a.act + (long)(first + r0) * a.I);
+    auto load = [&](int b, float* v) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        if (from + 32 * b + lane < blocks) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float4 f = __ldcg(reinterpret_cast<const float4*>(x + 16 * (from + 32 * b + lane)) + i);
-            v[b][4 * i] = f.x; v[b][4 * i + 1] = f.y; v[b][4 * i + 2] = f.z; v[b][4 * i + 3] = f.w;
-          }
-        }
+      for (int i = 0; i < 4; ++i) {
+        const float4 f = x[4 * (long)b + i];
+        v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+      }
     };
-    for (int from = 0; from < blocks; from += 128) {               // 2,048 values at once; wider rows are read again
-      load(from);
+#pragma unroll 1
+    for (int b = et; b < n; b += 512) {
+      float v[4][16];
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        if (from + 32 * b + lane < blocks) top = max(top, fp4_top16(v[b]));
-    }
-    const float g = fp4_row_scale(__reduce_max_sync(0xFFFFFFFFu, top));
-    for (int from = 0; from < blocks; from += 128) {
-      if (blocks > 128) load(from);
+      for (int j = 0; j < 4; ++j)
+        if (b + 128 * j < n) load(b + 128 * j, v[j]);
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        if (from + 32 * b + lane < blocks) fp4_store_block(out, a.I, from + 32 * b + lane, v[b], g);
+      for (int j = 0; j < 4; ++j)
+        if (b + 128 * j < n) atomicMax(&s_top[(b + 128 * j) / per], fp4_top16(v[j]));
     }
+    f4_meet<4>();
+#pragma unroll 1
+    for (int b = et; b < n; b += 128) {
+      float v[16];
+      load(b, v);                                     // from the first cache, mostly
+      fp4_store_block(to + (first + r0 + b / per) * fp4_row_bytes(a.I), a.I, b % per, v, fp4_row_scale(s_top[b / per]));
+    }
+    f4_meet<4>();
   }
 }
 
-template <int BN>
+// Rows that this CTA stores and reads by TMA itself, by an mbarrier that each of the 128 storing threads arrives at.
+__device__ __forceinline__ void fm_rows_stored(uint64_t* bar) {
+  asm volatile("fence.proxy.async;" ::: "memory");
+  mbar_arrive(bar);
+}
+
+// The tokens' rows that other CTAs store, read by TMA: whether all are there; gives up after the limit of all waits.
+__device__ __forceinline__ bool fm_tokens_ready(const FmArgs& a, volatile int* abort_flag) {
+  unsigned long long t0 = 0;
+  for (;;) {
+    int done;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(done) : "l"(a.claim + 1) : "memory");
+    if (done >= a.T) break;
+    const unsigned long long now = globaltimer();
+    if (t0 == 0) t0 = now;
+    else if (now - t0 > WAIT_LIMIT_NS) { *abort_flag = 1; return false; }
+  }
+  asm volatile("fence.proxy.async;" ::: "memory");
+  return true;
+}
+
+// Whether this CTA's `done` parts of `all` were the last; by the 128 threads, whose stores the others see then.
+__device__ __forceinline__ bool fm_last(int* ticket, int done, int all, int* s_word) {
+  __threadfence();
+  f4_meet<4>();
+  if (threadIdx.x == F4_EPILOGUE) {
+    const int last = atomicAdd(ticket, done) + done == all;
+    if (last) *ticket = 0;                          // ready for the next call
+    __threadfence();
+    *s_word = last;
+  }
+  f4_meet<4>();
+  return *s_word != 0;
+}
+
+template <int BN, int AR, bool FEW>
+struct FmShapes {
+  using Up = F4Shape<true, BN, (FEW ? 200 : 206) * 1024, 4, AR, FEW ? 6 : BN == 32 ? 3 : 2>;
+  using Down = F4Shape<false, BN, (FEW ? 200 : 206) * 1024, 4, AR, FEW ? 6 : 3>;
+  using Plan = std::conditional_t<FEW, FmFewPlan, FmFullPlan>;
+};
+
+template <int BN, int AR, bool FEW>
 __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_up_kernel(const __grid_constant__ F4Maps map, const FmArgs a) {
-  using S = F4Shape<true, BN, FM_ROOM, 4>;
+  using S = typename FmShapes<BN, AR, FEW>::Up;
+  using Plan = typename FmShapes<BN, AR, FEW>::Plan;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) F4Bars<S> bar;
-  __shared__ FmPlan plan;
+  __shared__ __align__(8) uint64_t rows_bar;
+  __shared__ Plan plan;
   __shared__ double s_sum[4];
-  __shared__ unsigned s_max[4];
+  __shared__ unsigned s_max[4], s_top[32];
+  __shared__ float s_xs[FM_TOKENS];
   __shared__ int s_word;
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  f4_open<S>(bar);
+  if (threadIdx.x == 0) mbar_init(&rows_bar, 128);
+  f4_open<S>(bar, map);
+  fm_ask_gain(a);
   pdl_wait();
   pdl_launch();
-  fm_plan(plan, a, FM_SLOTS);
-  FmUpTiles tiles{plan, (a.I + 127) / 128, (a.H + 255) / 256, a.T};
+  fm_plan(plan, a, FM_SLOTS, smem);
+  const int row0 = FEW ? blockIdx.x * a.T : 0;                       // few tokens: rows of this CTA's own
+  FmUpTiles<Plan, AR> tiles(plan, a.I, a.H, row0, a.T);
 
   if (warp == 0) {
-    if (lane == 0)
-      f4_produce<true, S>(smem, bar, map, tiles, [&] {
-        unsigned long long t0 = 0;
-        for (;;) {
-          int done;
-          asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(done) : "l"(a.claim + 1) : "memory");
-          if (done >= a.T) break;
-          const unsigned long long now = globaltimer();
-          if (t0 == 0) t0 = now;
-          else if (now - t0 > WAIT_LIMIT_NS) { *(volatile int*)&bar.abort = 1; return false; }
-        }
-        asm volatile("fence.proxy.async;" ::: "memory");             // rows that other CTAs stored, read by TMA
-        return true;
-      });
+    if (lane == 0) f4_weights<S>(smem, bar, map, tiles);
+  } else if (warp == 6) {
+    if (lane == 0 && tiles.count() > 0 && (FEW ? mbar_wait(&rows_bar, 0, &bar.abort) : fm_tokens_ready(a, &bar.abort))) f4_tokens<S>(smem, bar, map, tiles);
   } else if (warp == 1) {
-    f4_issue<true, S>(smem, bar, tiles);
-  } else if (warp < 4) {
-    f4_turn<true, S>(smem, bar, tiles);
+    f4_issue<S>(smem, bar, tiles);
+  } else if (warp < 6) {
+    f4_cells<S>(smem, bar, tiles);
   } else {
-    const int q = warp & 3, et = threadIdx.x - 128;
-    for (;;) {
-      if (et == 0) s_word = atomicAdd(a.claim, 1);
-      f4_meet<4>();
-      const int t = s_word;
-      if (t >= a.T) break;
-      fm_token(a, t, s_sum, s_max);
-      __threadfence();
-      asm volatile("fence.proxy.async;" ::: "memory");
-      f4_meet<4>();
-      if (et == 0) atomicAdd(a.claim + 1, 1);
+    const int q = warp & 3, et = threadIdx.x - F4_EPILOGUE;
+    const long x_bytes = fp4_row_bytes(a.H), x_scale = a.H / 2 + a.H / 16;
+    if (FEW) {
+      if (tiles.count() > 0) {
+        for (int t = 0; t < a.T; ++t) fm_token(a, t, a.xq + (row0 + t) * x_bytes, s_sum, s_max);
+        fm_rows_stored(&rows_bar);
+      }
+    } else {
+      for (;;) {
+        if (et == 0) s_word = atomicAdd(a.claim, 1);
+        f4_meet<4>();
+        const int t = s_word;
+        if (t >= a.T) break;
+        fm_token(a, t, a.xq + t * x_bytes, s_sum, s_max);
+        __threadfence();
+        asm volatile("fence.proxy.async;" ::: "memory");
+        f4_meet<4>();
+        if (et == 0) atomicAdd(a.claim + 1, 1);
+      }
     }
-    f4_meet<4>();                                                       // s_word is read
     uint32_t ab = 0, aphase = 0;
-    const int tiles_w = tiles.tiles_w;
-    for (int i = 0; i < tiles.count(); ++i) {
+    int done = 0;                                                    // tiles of the expert at hand
+    const int n_tiles = tiles.count();
+    auto scale_of = [&](int i, const uint8_t* m) {
       const F4Work mt = tiles.at(i);
-      const FmPlan::Entry e = plan.entry[tiles.entry(i)];
-      const int n = mt.n0 + q * 32 + lane;
-      const long x_scale = a.H / 2 + a.H / 16, wrow = ((long)mt.group * a.I + min(n, a.I - 1)) * fp4_row_bytes(a.H) + x_scale;
-      const float ws = *reinterpret_cast<const float*>(a.wg + wrow), ws2 = *reinterpret_cast<const float*>(a.wu + wrow);
+      return *reinterpret_cast<const float*>(m + ((long)mt.group * a.I + min(mt.n0 + q * 32 + lane, a.I - 1)) * x_bytes + x_scale);
+    };
+    float ws_nxt = 0.0f, ws2_nxt = 0.0f;
+    if (n_tiles > 0) { ws_nxt = scale_of(0, a.wg); ws2_nxt = scale_of(0, a.wu); }
+    for (int i = 0; i < n_tiles; ++i) {
+      const F4Work mt = tiles.at(i);
+      const typename Plan::Entry e = plan.entry[tiles.entry(i)];
+      const int n = mt.n0 + q * 32 + lane, end = min(a.I, mt.n0 + AR);
+      const float ws = ws_nxt, ws2 = ws2_nxt;
+      if (i + 1 < n_tiles) { ws_nxt = scale_of(i + 1, a.wg); ws2_nxt = scale_of(i + 1, a.wu); }
       if (!f4_all<4>(mbar_wait_warp(&bar.acc_full[ab], aphase, &bar.abort))) break;
       tc_fence_after();
+      if (i == 0) {                                                  // the first products are there, and so are all rows
+        if (et < a.T) s_xs[et] = __ldcg(reinterpret_cast<const float*>(a.xq + (row0 + et) * x_bytes + x_scale));
+        f4_meet<4>();
+      }
       const uint32_t tbase = bar.tmem + ((uint32_t)(q * 32) << 16) + ab * (2 * BN);
       for (int r0 = 0; r0 < e.rows; r0 += 4) {
         uint32_t v[4], u[4];
@@ -256,7 +381,7 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_up_kernel(const __grid_
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int t = plan.slot[e.first + min(r0 + j, e.rows - 1)] / a.k;
-          x[j] = __ldcg(reinterpret_cast<const float*>(a.xq + t * fp4_row_bytes(a.H) + x_scale));
+          x[j] = s_xs[t];
           tmem_ld1(tbase + t, v[j]);
           tmem_ld1(tbase + BN + t, u[j]);
         }
@@ -264,125 +389,168 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_up_kernel(const __grid_
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float g = __uint_as_float(v[j]) * ws * x[j], up = __uint_as_float(u[j]) * ws2 * x[j];
-          if (r0 + j < e.rows && n < a.I) a.act[(long)(e.first + r0 + j) * a.I + n] = (g / (1.0f + __expf(-g))) * up;
+          if (r0 + j < e.rows && n < end) a.act[(long)(e.first + r0 + j) * a.I + n] = fp4_silu(g) * up;
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.acc_empty[ab]);
       if (++ab == S::ACCS) { ab = 0; aphase ^= 1; }
-      __threadfence();
-      f4_meet<4>();
-      if (et == 0) {
-        int* ticket = a.claim + 2 + e.expert;
-        const int last = atomicAdd(ticket, 1) == tiles_w - 1;
-        if (last) *ticket = 0;                                       // ready for the next call
-        __threadfence();
-        s_word = last;
+      ++done;
+      if (!FEW && (i + 1 == n_tiles || tiles.entry(i + 1) != tiles.entry(i))) {
+        if (fm_last(a.claim + 2 + e.expert, done, tiles.tiles_w, &s_word)) fm_rows(a, e.first, e.rows, a.aq, s_top);
+        done = 0;
       }
-      f4_meet<4>();
-      if (s_word) fm_rows(a, e.first, e.rows);
     }
   }
   f4_close<S>(bar, a.status);
 }
 
 // 128 columns of the output from column n0 on: the slots of every token, in order.
-__device__ __forceinline__ void fm_combine(const FmArgs& a, const FmPlan& p, int n0) {
-  const int et = threadIdx.x - 128, lane = et & 31, n = n0 + 4 * lane;
+__device__ __forceinline__ void fm_combine(const FmArgs& a, const short* id, int n0) {
+  const int et = threadIdx.x - F4_EPILOGUE, lane = et & 31, n = n0 + 4 * lane;
   if (n >= a.H) return;
-  for (int t = et >> 5; t < a.T; t += 4) {
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (a.resid) {
-      const float* r = a.resid + (long)t * a.ldr + n;
-      s = make_float4(r[0], r[1], r[2], r[3]);
+  for (int t0 = et >> 5; t0 < a.T; t0 += 8) {                       // two tokens of a warp at once
+    float4 s[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int t = t0 + 4 * p;
+      s[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (a.resid && t < a.T) {
+        const float* r = a.resid + (long)t * a.ldr + n;
+        s[p] = make_float4(r[0], r[1], r[2], r[3]);
+      }
     }
     for (int j0 = 0; j0 < a.k; j0 += 8) {
-      float4 v[8];
+      float4 v[2][8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j0 + j < a.k && p.id[t * a.k + j0 + j] >= 0)
-          v[j] = __ldcg(reinterpret_cast<const float4*>(a.slot_out + (long)(t * a.k + j0 + j) * a.H + n));
-        else v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { s.x += v[j].x; s.y += v[j].y; s.z += v[j].z; s.w += v[j].w; }
+        for (int j = 0; j < 8; ++j) {
+          const int at = (t0 + 4 * p) * a.k + j0 + j;
+          v[p][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (t0 + 4 * p < a.T && j0 + j < a.k && id[at] >= 0) v[p][j] = __ldcg(reinterpret_cast<const float4*>(a.slot_out + (long)at * a.H + n));
+        }
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { s[p].x += v[p][j].x; s[p].y += v[p][j].y; s[p].z += v[p][j].z; s[p].w += v[p][j].w; }
     }
-    const float f[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (a.c_f32) a.c_f32[(long)t * a.ldc + n + i] = f[i];
-      else a.c_bf16[(long)t * a.ldc + n + i] = __float2bfloat16_rn(f[i]);
+    for (int p = 0; p < 2; ++p) {
+      const int t = t0 + 4 * p;
+      if (t >= a.T) break;
+      const float f[4] = {s[p].x, s[p].y, s[p].z, s[p].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (a.c_f32) a.c_f32[(long)t * a.ldc + n + i] = f[i];
+        else a.c_bf16[(long)t * a.ldc + n + i] = __float2bfloat16_rn(f[i]);
+      }
     }
   }
 }
 
-template <int BN>
+template <int BN, int AR, bool FEW>
 __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_down_kernel(const __grid_constant__ F4Maps map, const FmArgs a) {
-  using S = F4Shape<false, BN, FM_ROOM, 4>;
+  using S = typename FmShapes<BN, AR, FEW>::Down;
+  using Plan = typename FmShapes<BN, AR, FEW>::Plan;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) F4Bars<S> bar;
-  __shared__ FmPlan plan;
+  __shared__ __align__(8) uint64_t rows_bar;
+  __shared__ Plan plan;
+  __shared__ float s_factor[FEW ? FM_FEW_SLOTS : FM_SLOTS], s_out[FEW ? FM_FEW_SLOTS : 1][AR];
+  __shared__ unsigned s_top[32];
   __shared__ int s_word;
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  f4_open<S>(bar);
+  if (threadIdx.x == 0) mbar_init(&rows_bar, 128);
+  f4_open<S>(bar, map);
   // The ids were there before the launch in front of this one began, and weights always are: both are read before its end is waited for.
-  fm_plan(plan, a, BN);
-  FmDownTiles tiles{plan, (a.H + 127) / 128, (a.I + 255) / 256};
+  fm_plan(plan, a, BN, smem);
+  const int row0 = FEW ? blockIdx.x * a.T * a.k : 0;                 // few tokens: rows of this CTA's own
+  FmDownTiles<Plan, AR, FEW> tiles(plan, a.H, a.I, row0);
 
   if (warp == 0) {
-    if (lane == 0) f4_produce<false, S>(smem, bar, map, tiles, [] { pdl_wait(); pdl_launch(); return true; });
+    if (lane == 0) f4_weights<S>(smem, bar, map, tiles);
+  } else if (warp == 6) {
+    pdl_wait();
+    pdl_launch();
+    if (lane == 0 && tiles.count() > 0 && (!FEW || mbar_wait(&rows_bar, 0, &bar.abort))) f4_tokens<S>(smem, bar, map, tiles);
   } else if (warp == 1) {
-    f4_issue<false, S>(smem, bar, tiles);
-  } else if (warp < 4) {
-    f4_turn<false, S>(smem, bar, tiles);
+    f4_issue<S>(smem, bar, tiles);
+  } else if (warp < 6) {
+    f4_cells<S>(smem, bar, tiles);
   } else {
-    const int q = warp & 3, et = threadIdx.x - 128, tiles_w = tiles.tiles_w;
+    const int q = warp & 3, et = threadIdx.x - F4_EPILOGUE, n_tiles = tiles.count(), n_slots = a.T * a.k;
+    const long a_bytes = fp4_row_bytes(a.I), a_scale = a.I / 2 + a.I / 16;
+    auto scale_of = [&](int i) {
+      const F4Work mt = tiles.at(i);
+      return *reinterpret_cast<const float*>(a.wd + ((long)mt.group * a.H + min(mt.n0 + q * 32 + lane, a.H - 1)) * a_bytes + a_scale);
+    };
+    float ws_nxt = n_tiles > 0 ? scale_of(0) : 0.0f;
     pdl_wait();
     if (blockIdx.x == 0 && et < 2) a.claim[et] = 0;                  // ready for the next call
+    if (FEW && n_tiles > 0) {
+      const typename Plan::Entry last = plan.entry[plan.n_entries - 1];
+      fm_rows(a, 0, last.first + last.rows, a.aq + row0 * a_bytes, s_top);
+      fm_rows_stored(&rows_bar);
+    }
+    for (int s = et; s < n_slots && n_tiles > 0; s += 128) {         // places behind the last slot of an expert of ours are not read
+      const int slot = plan.slot[s];
+      if ((unsigned)slot < (unsigned)n_slots) s_factor[s] = *reinterpret_cast<const volatile float*>(a.aq + (row0 + s) * a_bytes + a_scale) * a.wts[slot];
+    }
+    f4_meet<4>();
     uint32_t ab = 0, aphase = 0;
-    for (int i = 0; i < tiles.count(); ++i) {
+    int done = 0;                                                    // tiles of the columns at hand
+    for (int i = 0; i < n_tiles; ++i) {
       const F4Work mt = tiles.at(i);
-      const int n = mt.n0 + q * 32 + lane;
-      const long a_scale = a.I / 2 + a.I / 16;
-      const float ws = *reinterpret_cast<const float*>(a.wd + ((long)mt.group * a.H + min(n, a.H - 1)) * fp4_row_bytes(a.I) + a_scale);
+      const typename Plan::Entry e = tiles.entry(i);
+      const int col = q * 32 + lane, n = mt.n0 + col, end = min(a.H, mt.n0 + AR);
+      const float ws = ws_nxt;
+      if (i + 1 < n_tiles) ws_nxt = scale_of(i + 1);
       if (!f4_all<4>(mbar_wait_warp(&bar.acc_full[ab], aphase, &bar.abort))) break;
       tc_fence_after();
       const uint32_t tbase = bar.tmem + ((uint32_t)(q * 32) << 16) + ab * BN;
-      for (int r0 = 0; r0 < mt.rows; r0 += 4) {
+      for (int r0 = 0; r0 < e.rows; r0 += 4) {
         uint32_t v[4];
-        float f[4];
-        int slot[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = min(r0 + j, mt.rows - 1);
-          slot[j] = plan.slot[mt.row0 + r];
-          f[j] = *reinterpret_cast<const float*>(a.aq + (mt.row0 + r) * fp4_row_bytes(a.I) + a_scale) * a.wts[slot[j]];
-          tmem_ld1(tbase + r, v[j]);
-        }
+        for (int j = 0; j < 4; ++j) tmem_ld1(tbase + min(r0 + j, e.rows - 1), v[j]);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (r0 + j < mt.rows && n < a.H) a.slot_out[(long)slot[j] * a.H + n] = __uint_as_float(v[j]) * ws * f[j];
+        for (int j = 0; j < 4; ++j) {
+          const int at = e.first + min(r0 + j, e.rows - 1), slot = plan.slot[at];
+          const float f = __uint_as_float(v[j]) * ws * s_factor[at];
+          if (r0 + j < e.rows && n < end) {
+            if (FEW) s_out[slot][col] = f;
+            else a.slot_out[(long)slot * a.H + n] = f;
+          }
+        }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.acc_empty[ab]);
       if (++ab == S::ACCS) { ab = 0; aphase ^= 1; }
-      __threadfence();
-      f4_meet<4>();
-      if (et == 0) {
-        int* ticket = a.claim + 2 + a.E + mt.n0 / 128;
-        const int last = atomicAdd(ticket, 1) == plan.n_entries - 1;
-        if (last) *ticket = 0;
-        __threadfence();
-        s_word = last;
+      ++done;
+      if (i + 1 == n_tiles || tiles.at(i + 1).n0 != mt.n0) {
+        if (FEW) {
+          f4_meet<4>();
+          for (int c = et; c < a.T * AR; c += 128) {
+            const int t = c / AR, m = mt.n0 + c % AR;
+            if (m >= a.H) continue;
+            float s = a.resid ? a.resid[(long)t * a.ldr + m] : 0.0f;
+            for (int j = 0; j < a.k; ++j) s += plan.id[t * a.k + j] >= 0 ? s_out[t * a.k + j][c % AR] : 0.0f;
+            if (a.c_f32) a.c_f32[(long)t * a.ldc + m] = s;
+            else a.c_bf16[(long)t * a.ldc + m] = __float2bfloat16_rn(s);
+          }
+          f4_meet<4>();
+        } else if (fm_last(a.claim + 2 + a.E + mt.n0 / 128, done, plan.n_entries, &s_word)) {
+          fm_combine(a, plan.id, mt.n0);
+        }
+        done = 0;
       }
-      f4_meet<4>();
-      if (s_word) fm_combine(a, plan, mt.n0);
     }
     if (plan.n_entries == 0)                                         // every slot is another tier's
-      for (int j = blockIdx.x; j < tiles_w; j += gridDim.x) fm_combine(a, plan, 128 * j);
+      for (int j = blockIdx.x; j < (a.H + 127) / 128; j += gridDim.x) fm_combine(a, plan.id, 128 * j);
   }
   f4_close<S>(bar, a.status);
 }
@@ -404,41 +572,66 @@ namespace bl {
 // The scratch of calls of up to `rows` tokens: counters, then the buffers, each at a multiple of 128 bytes.
 struct FmWork {
   long xq, act, aq, slot_out, total;
-  FmWork(long rows, long k, long E, long H, long I) {
+  FmWork(long rows, long k, long E, long H, long I, long sms) {
+    const long few = sms * (rows < FM_FEW ? rows : FM_FEW), own = few * k < sms * FM_FEW_SLOTS ? few * k : sms * FM_FEW_SLOTS;
     auto up = [](long n) { return (n + 127) / 128 * 128; };
     xq = up((2 + E + (H + 127) / 128) * 4);
-    act = xq + up(rows * fp4_row_bytes((int)H));
+    act = xq + up((rows > few ? rows : few) * fp4_row_bytes((int)H));
     aq = act + up(rows * k * I * 4);
-    slot_out = aq + up(rows * k * fp4_row_bytes((int)I));
+    slot_out = aq + up((rows * k > own ? rows * k : own) * fp4_row_bytes((int)I));
     total = slot_out + up(rows * k * H * 4);
   }
 };
 
-template <int BN>
-static int fp4_moe_go(const Fp4MoeCall& c, const FmArgs& a) {
-  using SU = F4Shape<true, BN, FM_ROOM, 4>;
-  using SD = F4Shape<false, BN, FM_ROOM, 4>;
-  F4Maps up, down;
-  int rc = f4_maps<true, SU>(&up, a.xq, a.T, a.wg, a.wu, a.H, a.I, a.E);
-  if (!rc) rc = f4_maps<false, SD>(&down, a.aq, (long)a.T * a.k, a.wd, nullptr, a.I, a.H, a.E);
+template <class S>
+static void fm_limit(const void* kernel) { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM); }
+
+// rows_x, rows_a: NVFP4 rows of tokens and of activations that the scratch holds for this call; n: tiles
+template <int BN, int AR, bool FEW>
+static int fm_up(const Fp4MoeCall& c, const FmArgs& a, long rows_x, long n) {
+  using S = typename FmShapes<BN, AR, FEW>::Up;
+  F4Maps m;
+  const int rc = f4_maps<S>(&m, a.xq, rows_x, a.wg, a.wu, a.H, a.I, a.E);
   if (rc) return rc;
   static PerDevice limit;
-  if (limit.due()) {
-    cudaFuncSetAttribute(fp4_moe_up_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SU::SMEM);
-    cudaFuncSetAttribute(fp4_moe_down_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SD::SMEM);
-    limit.mark();
-  }
-  const long hit = a.E < a.T * a.k ? a.E : a.T * a.k, n_up = hit * ((a.I + 127) / 128), n_down = hit * ((a.H + 127) / 128);
-  rc = (int)launch(fp4_moe_up_kernel<BN>, dim3((unsigned)(n_up < c.sms ? n_up : c.sms)), dim3(FM_THREADS), SU::SMEM, c.stream, up, a);
+  if (limit.due()) { fm_limit<S>((const void*)fp4_moe_up_kernel<BN, AR, FEW>); limit.mark(); }
+  return (int)launch(fp4_moe_up_kernel<BN, AR, FEW>, dim3((unsigned)(n < c.sms ? n : c.sms)), dim3(FM_THREADS), S::SMEM, c.stream, m, a);
+}
+template <int BN, int AR, bool FEW>
+static int fm_down(const Fp4MoeCall& c, const FmArgs& a, long rows_a, long n) {
+  using S = typename FmShapes<BN, AR, FEW>::Down;
+  F4Maps m;
+  const int rc = f4_maps<S>(&m, a.aq, rows_a, a.wd, nullptr, a.I, a.H, a.E);
   if (rc) return rc;
-  return (int)launch(fp4_moe_down_kernel<BN>, dim3((unsigned)(n_down < c.sms ? n_down : c.sms)), dim3(FM_THREADS), SD::SMEM, c.stream, down, a);
+  static PerDevice limit;
+  if (limit.due()) { fm_limit<S>((const void*)fp4_moe_down_kernel<BN, AR, FEW>); limit.mark(); }
+  return (int)launch(fp4_moe_down_kernel<BN, AR, FEW>, dim3((unsigned)(n < c.sms ? n : c.sms)), dim3(FM_THREADS), S::SMEM, c.stream, m, a);
+}
+
+static int fp4_moe_few(const Fp4MoeCall& c, const FmArgs& a) {
+  // rows of a tile: as few as still find a processor for each tile at once
+  const long hit = a.E < a.T * a.k ? a.E : a.T * a.k, rows_x = (long)c.sms * a.T, rows_a = rows_x * a.k;
+  auto tiles = [&](long n, int ar) { return (n + ar - 1) / ar; };
+  const int au = hit * tiles(a.I, 32) <= c.sms ? 32 : hit * tiles(a.I, 64) <= c.sms ? 64 : 128;
+  int rc = au == 32 ? fm_up<32, 32, true>(c, a, rows_x, hit * tiles(a.I, 32)) : au == 64 ? fm_up<32, 64, true>(c, a, rows_x, hit * tiles(a.I, 64))
+                                                                                       : fm_up<32, 128, true>(c, a, rows_x, hit * tiles(a.I, 128));
+  if (rc) return rc;
+  const int ad = tiles(a.H, 16) <= c.sms ? 16 : tiles(a.H, 32) <= c.sms ? 32 : 64;
+  return ad == 16 ? fm_down<32, 16, true>(c, a, rows_a, tiles(a.H, 16)) : ad == 32 ? fm_down<32, 32, true>(c, a, rows_a, tiles(a.H, 32))
+                                                                                   : fm_down<32, 64, true>(c, a, rows_a, tiles(a.H, 64));
+}
+template <int BN>
+static int fp4_moe_full(const Fp4MoeCall& c, const FmArgs& a) {
+  const long hit = a.E < a.T * a.k ? a.E : a.T * a.k;
+  const int rc = fm_up<BN, 128, false>(c, a, a.T, hit * ((a.I + 127) / 128));
+  return rc ? rc : fm_down<BN, 128, false>(c, a, (long)a.T * a.k, hit * ((a.H + 127) / 128));
 }
 
 }  // namespace bl
 
 extern "C" {
 
-long bl_fp4_moe_work_bytes(int rows, int k, int E, int H, int I) { return FmWork(rows, k, E, H, I).total; }
+long bl_fp4_moe_work_bytes(int rows, int k, int E, int H, int I, int sms) { return FmWork(rows, k, E, H, I, sms).total; }
 
 // y[t] = resid[t] + sum_j wts[t, j] (NVFP4 of silu(x_t Wg[e]) * (x_t Wu[e])) Wd[e], e = ids[t, j] (none where that is outside 0 .. E - 1),
 // for T rows x (x_type 0 bf16, 2 fp32; gain != null: RMSNorm first), in NVFP4.  Wg, Wu [E, I] rows of H values, Wd [E, H] rows of I; work:
@@ -452,12 +645,13 @@ int bl_fp4_moe(const Fp4MoeCall* c) {
                  ((uintptr_t)c->work & 127) == 0 && ((uintptr_t)c->wg & 15) == 0 && ((uintptr_t)c->wu & 15) == 0 && ((uintptr_t)c->wd & 15) == 0,
              BL_ERR_ALIGN);
   BL_REQUIRE((c->c_f32 != nullptr) != (c->c_bf16 != nullptr), BL_ERR_SHAPE);
-  const FmWork w(c->rows, c->k, c->E, c->H, c->I);
+  const FmWork w(c->rows, c->k, c->E, c->H, c->I, c->sms);
+  const int few = c->T <= FM_FEW && c->T * c->k <= FM_FEW_SLOTS;
   uint8_t* base = (uint8_t*)c->work;
   FmArgs a{c->x, c->ldx, c->x_type, c->gain, c->eps, c->ids, c->wts, c->T, c->k, c->E, c->H, c->I, (const uint8_t*)c->wg, (const uint8_t*)c->wu,
            (const uint8_t*)c->wd, base + w.xq, (float*)(base + w.act), base + w.aq, (float*)(base + w.slot_out), (int*)base, c->resid, c->ldr,
            c->c_f32, (__nv_bfloat16*)c->c_bf16, c->ldc, c->status};
-  return c->T <= 32 ? fp4_moe_go<32>(*c, a) : fp4_moe_go<64>(*c, a);
+  return few ? fp4_moe_few(*c, a) : c->T <= 32 ? fp4_moe_full<32>(*c, a) : fp4_moe_full<64>(*c, a);
 }
 
 }  // extern "C"

@@ -176,7 +176,7 @@ class Fp4MoeWork:
         self.rows, self.used, self.hidden, self.inter, self.n_expert = rows, used, hidden, inter, n_expert
         size = cuda().bl_fp4_moe_work_bytes
         size.restype = ctypes.c_long
-        self.data = torch.zeros(size(rows, used, n_expert, hidden, inter), dtype=torch.uint8, device=device)
+        self.data = torch.zeros(size(rows, used, n_expert, hidden, inter, sm_count(device) if torch.device(device).type == "cuda" else 1), dtype=torch.uint8, device=device)
         self.ptr, self.index = self.data.data_ptr(), self.data.get_device()
 
 
