@@ -109,6 +109,16 @@ __device__ __forceinline__ void fp4_load16(const void* x, int type, long at, flo
     }
   }
 }
+// 1 / sqrt(x) in fp32: two of Newton's steps in 64 bits behind rsqrtf, which leave 2^-52 or so in front of the rounding, are a few
+// instructions where the library's root and quotient are a hundred that have to be fetched.
+__device__ __forceinline__ float fp4_rsqrt(double x) {
+  if (!(x > 1e-30 && x < 1e30)) return (float)(1.0 / sqrt(x));
+  double y = (double)rsqrtf((float)x);
+  const double h = 0.5 * x;
+  y = y * fma(-h * y, y, 1.5);
+  y = y * fma(-h * y, y, 1.5);
+  return (float)y;
+}
 // v * r * gain
 __device__ __forceinline__ void fp4_scale16(float* v, float r, const float* gain) {
   const float4* g4 = reinterpret_cast<const float4*>(gain);
@@ -169,15 +179,12 @@ __device__ __forceinline__ uint4 fp4_raw(const uint8_t* box, int row, int at) {
   return *reinterpret_cast<const uint4*>(box + row * (16 * SPAN) + ((at ^ turn) << 4));
 }
 template <int SPAN, int COLUMNS>
-__device__ __forceinline__ void fp4_cells(uint32_t taddr, const uint8_t* box, int at, int lane, int groups) {
-  uint32_t c[4 * COLUMNS];
+__device__ __forceinline__ void fp4_cells(uint32_t (&c)[4 * COLUMNS], const uint8_t* box, int at, int lane, int groups) {
 #pragma unroll
   for (int j = 0; j < COLUMNS; ++j) {
     const uint4 r = j < groups ? fp4_raw<SPAN>(box, 32 * j + lane, at) : make_uint4(0u, 0u, 0u, 0u);
     c[j] = r.x; c[COLUMNS + j] = r.y; c[2 * COLUMNS + j] = r.z; c[3 * COLUMNS + j] = r.w;
   }
-  if constexpr (COLUMNS == 8) tmem_st32(taddr, c);
-  else fp4_st16(taddr, c);
 }
 
 // Maps of NVFP4 rows [groups][rows][row bytes]: codes in boxes of 256 values (zeros past the row's end), scales in boxes of

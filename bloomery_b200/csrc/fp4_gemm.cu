@@ -21,7 +21,7 @@ struct F4Args {
   int N, K, tiles_w, tile_rows;
   const F4Tile* tiles;
   const int* n_tiles;
-  int max_tiles;
+  int max_tiles, fixed;
   const uint8_t* x;         // the rows, for their fp32 scales
   const uint8_t* w;
   const uint8_t* w2;
@@ -134,9 +134,12 @@ fp4_gemm_kernel(const __grid_constant__ F4Maps map, const F4Args a) {
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   f4_open<S>(bar, map);
-  pdl_wait();
-  pdl_launch();
-  F4GemmTiles<AR> tiles{a, min(*a.n_tiles, a.max_tiles) * a.tiles_w, (a.K + 255) / 256};
+  // A table that the host wrote and the weights are there before the launch in front of this one ends; the rows are not.
+  if (!a.fixed || warp >= 6) {
+    pdl_wait();
+    pdl_launch();
+  }
+  F4GemmTiles<AR> tiles{a, (a.fixed ? a.max_tiles : min(*a.n_tiles, a.max_tiles)) * a.tiles_w, (a.K + 255) / 256};
 
   if (warp == 0) {
     if (lane == 0) f4_weights<S>(smem, bar, map, tiles);
@@ -223,7 +226,7 @@ struct Fp4GemmCall {
   const void* x; const void* w; const void* w2; const void* tiles; const int* n_tiles; float* c_f32; void* c_bf16;
   const int* dst_row; const float* row_scale; const float* resid; unsigned* status; cudaStream_t stream;
   long rows_x, ldc, ldr;
-  int n_groups, N, K, max_tiles, tile_rows, sms;
+  int n_groups, N, K, max_tiles, tile_rows, sms, fixed;
 };
 
 namespace bl {
@@ -250,6 +253,7 @@ extern "C" {
 
 // C[dst_row[t] or t, n] = row_scale[t] * sum_k X[t, k] W[g][n, k] (+ resid) per token tile of the table, of at most tile_rows (32, 64,
 // 128, with one matrix 256) rows.  X [rows_x], W and W2 [n_groups, N] NVFP4 rows of K values; exactly one of c_f32 / c_bf16;
+// fixed: the table has exactly max_tiles tiles, and no launch in flight writes it or the weights.
 // W2 != null: output = row_scale[t] * silu(X W^T) * (X W2^T).
 int bl_fp4_gemm(const Fp4GemmCall* c) {
   const bool dual = c->w2 != nullptr;
@@ -259,7 +263,7 @@ int bl_fp4_gemm(const Fp4GemmCall* c) {
   BL_REQUIRE((c->c_f32 != nullptr) != (c->c_bf16 != nullptr) && c->ldc < 1L << 30 && c->ldr < 1L << 30, BL_ERR_SHAPE);
   F4Args a{};
   a.N = c->N; a.K = c->K; a.tile_rows = c->tile_rows;
-  a.tiles = (const F4Tile*)c->tiles; a.n_tiles = c->n_tiles; a.max_tiles = c->max_tiles;
+  a.tiles = (const F4Tile*)c->tiles; a.n_tiles = c->n_tiles; a.max_tiles = c->max_tiles; a.fixed = c->fixed;
   BL_REQUIRE((long)a.max_tiles * ((c->N + 15) / 16) < 1L << 31, BL_ERR_LIMIT);
   a.x = (const uint8_t*)c->x; a.w = (const uint8_t*)c->w; a.w2 = (const uint8_t*)c->w2;
   a.row_bytes = fp4_row_bytes(c->K); a.group_bytes = a.row_bytes * c->N;

@@ -13,8 +13,7 @@
 //     expert by expert;
 //   * in the second launch the CTA that finishes the last tile of 128 output columns adds up the slots of every token, in order.
 // CTAs walk tiles next to each other, so that one takes part in two or three experts, or column blocks, and says so once for each.
-// Few tokens (FM_FEW) go without meeting: each CTA quantises the rows that it needs for itself, and the second launch has the columns of a
-// CTA to itself, all experts of them, so that it adds up its slots in shared memory.
+// Few tokens (FM_FEW): each CTA quantises the rows that it needs for itself, which is quicker than to wait for another one's.
 // Rows are claimed and finished by whoever is there, so no CTA waits for one that has not started; the one wait between CTAs (for the tokens'
 // rows) is bounded like all others.  Sums of a slot run in one order: the same bits on every run and with every number of CTAs.
 #include <type_traits>
@@ -24,7 +23,7 @@
 namespace bl {
 
 constexpr int FM_TOKENS = 64, FM_SLOTS = 1024, FM_EXPERTS = 512, FM_WIDTH = 8192;
-constexpr int FM_FEW = 4, FM_FEW_SLOTS = 32;        // tokens and slots of a round that goes without meetings
+constexpr int FM_FEW = 4, FM_FEW_SLOTS = 32;        // tokens and slots of a round whose CTAs quantise for themselves
 constexpr int FM_THREADS = F4_EPILOGUE + 128;
 
 struct FmArgs {
@@ -37,7 +36,7 @@ struct FmArgs {
   float* act;                                       // [T * k][I], expert by expert
   uint8_t* aq;                                      // the same as NVFP4 rows; few tokens: as many for each CTA
   float* slot_out;                                  // [T * k][H]
-  int* claim;                                       // rows taken, rows done, then a ticket for every expert and every 128 columns
+  int* claim;                                       // rows taken, rows done, then a ticket for every expert and every block of columns
   const float* resid; long ldr;
   float* c_f32; __nv_bfloat16* c_bf16; long ldc;
   unsigned* status;
@@ -53,6 +52,11 @@ struct FmPlan {
 };
 using FmFewPlan = FmPlan<FM_FEW_SLOTS, FM_FEW_SLOTS>;
 using FmFullPlan = FmPlan<FM_SLOTS, FM_EXPERTS + FM_SLOTS / 32>;
+
+// The plan is made by the warps in front of the epilogue's, which meanwhile quantise tokens and come to it later.
+__device__ __forceinline__ void fm_plan_step() { asm volatile("bar.sync 2, %0;" ::"n"(F4_EPILOGUE) : "memory"); }
+__device__ __forceinline__ void fm_plan_made() { asm volatile("bar.arrive 3, %0;" ::"n"(FM_THREADS) : "memory"); }
+__device__ __forceinline__ void fm_plan_wait() { asm volatile("bar.sync 3, %0;" ::"n"(FM_THREADS) : "memory"); }
 
 // Up to 32 slots, by one warp: experts in the order in which they appear.
 __device__ __forceinline__ void fm_plan(FmFewPlan& p, const FmArgs& a, int, void*) {
@@ -77,13 +81,13 @@ __device__ __forceinline__ void fm_plan(FmFewPlan& p, const FmArgs& a, int, void
     if (e >= 0) p.slot[first + __popc(same & below)] = (short)tid;
     if (tid == 0) p.n_entries = __popc(leaders);
   }
-  __syncthreads();
+  fm_plan_step();
 }
 
-// Any number, by all threads: a warp counts the experts of its own slots (an eighth of them, next to each other), so that a slot's place
-// among those of its expert is the same in every CTA.  `scratch`: FM_EXPERTS * 10 shorts that TMA writes later.
+// Any number: a warp counts the experts of its own slots (a seventh of them, next to each other), so that a slot's place among those of its
+// expert is the same in every CTA.  `scratch`: FM_EXPERTS * 9 shorts that TMA writes later.
 __device__ __forceinline__ void fm_plan(FmFullPlan& p, const FmArgs& a, int most, void* scratch) {
-  constexpr int W = 8, PER = FM_SLOTS / (32 * W);                  // warps that count
+  constexpr int W = F4_EPILOGUE / 32, PER = (FM_SLOTS + 32 * W - 1) / (32 * W);
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, n = a.T * a.k;
   short* count = reinterpret_cast<short*>(scratch);                // [W][FM_EXPERTS], then what lies in front of a warp's slots
   short *all = count + W * FM_EXPERTS, *first = all + FM_EXPERTS;
@@ -94,8 +98,8 @@ __device__ __forceinline__ void fm_plan(FmFullPlan& p, const FmArgs& a, int most
     const int s = lo + 32 * i + lane;
     id[i] = s < hi ? a.ids[s] : -1;
   }
-  for (int i = tid; i < W * FM_EXPERTS / 2; i += FM_THREADS) reinterpret_cast<int*>(count)[i] = 0;
-  __syncthreads();
+  for (int i = tid; i < W * FM_EXPERTS / 2; i += F4_EPILOGUE) reinterpret_cast<int*>(count)[i] = 0;
+  fm_plan_step();
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int s = lo + 32 * i + lane;
@@ -109,14 +113,14 @@ __device__ __forceinline__ void fm_plan(FmFullPlan& p, const FmArgs& a, int most
     __syncwarp();
     if (s < hi) p.id[s] = (short)id[i];
   }
-  __syncthreads();
-  for (int e = tid; e < a.E; e += FM_THREADS) {
+  fm_plan_step();
+  for (int e = tid; e < a.E; e += F4_EPILOGUE) {
     int sum = 0;
 #pragma unroll
     for (int i = 0; i < W; ++i) { const int c = count[i * FM_EXPERTS + e]; count[i * FM_EXPERTS + e] = (short)sum; sum += c; }
     all[e] = (short)sum;
   }
-  __syncthreads();
+  fm_plan_step();
   if (w == 0) {
     const int per = (a.E + 31) / 32, e0 = min(a.E, lane * per), e1 = min(a.E, e0 + per);
     int rows = 0, entries = 0;
@@ -137,12 +141,12 @@ __device__ __forceinline__ void fm_plan(FmFullPlan& p, const FmArgs& a, int most
       ro += c;
     }
   }
-  __syncthreads();
+  fm_plan_step();
 #pragma unroll
   for (int i = 0; i < PER; ++i)
     if (lo + 32 * i + lane < hi && id[i] >= 0) p.slot[first[id[i]] + count[w * FM_EXPERTS + id[i]] + place[i]] = (short)(lo + 32 * i + lane);
   asm volatile("fence.proxy.async;" ::: "memory");                 // the scratch is a ring's from here on
-  __syncthreads();
+  fm_plan_step();
 }
 
 // A CTA's share of n tiles: next to each other.
@@ -162,14 +166,12 @@ struct FmUpTiles : FmShare {                        // expert by expert
     return F4Work{p.entry[entry(i)].expert, (lo + i) % tiles_w * AR, row0, T, 0, kblocks};      // all tokens
   }
 };
-template <class Plan, int AR, bool FEW>
-struct FmDownTiles : FmShare {                      // columns after columns; few tokens: whole columns
+template <class Plan, int AR>
+struct FmDownTiles : FmShare {                      // columns after columns
   const Plan& p;
   int kblocks, row0;
   __device__ __forceinline__ FmDownTiles(const Plan& p, int H, int I, int row0)
-      : FmShare(FEW ? (H + AR - 1) / AR : p.n_entries * ((H + AR - 1) / AR)), p(p), kblocks((I + 255) / 256), row0(row0) {
-    if (FEW) { lo *= p.n_entries; hi *= p.n_entries; }
-  }
+      : FmShare(p.n_entries * ((H + AR - 1) / AR)), p(p), kblocks((I + 255) / 256), row0(row0) {}
   __device__ __forceinline__ typename Plan::Entry entry(int i) const { return p.entry[(lo + i) % p.n_entries]; }
   __device__ __forceinline__ F4Work at(int i) const {
     const typename Plan::Entry e = entry(i);
@@ -194,7 +196,7 @@ __device__ __forceinline__ void fm_token(const FmArgs& a, int t, uint8_t* row, d
     ss = warp_sum_d(ss);
     if (lane == 0) s_sum[w] = ss;
     f4_meet<4>();
-    r = (float)(1.0 / sqrt((s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) / (double)a.H + a.eps));
+    r = fp4_rsqrt((s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) / (double)a.H + a.eps);
   }
   unsigned top = 0;
 #pragma unroll 1
@@ -296,8 +298,8 @@ __device__ __forceinline__ bool fm_last(int* ticket, int done, int all, int* s_w
 
 template <int BN, int AR, bool FEW>
 struct FmShapes {
-  using Up = F4Shape<true, BN, (FEW ? 200 : 206) * 1024, 4, AR, FEW ? 6 : BN == 32 ? 3 : 2>;
-  using Down = F4Shape<false, BN, (FEW ? 200 : 206) * 1024, 4, AR, FEW ? 6 : 3>;
+  using Up = F4Shape<true, BN, 208 * 1024, 4, AR, FEW ? 6 : BN == 32 ? 3 : 2>;
+  using Down = F4Shape<false, BN, 206 * 1024, 4, AR, FEW ? 6 : 3>;
   using Plan = std::conditional_t<FEW, FmFewPlan, FmFullPlan>;
 };
 
@@ -320,26 +322,15 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_up_kernel(const __grid_
   fm_ask_gain(a);
   pdl_wait();
   pdl_launch();
-  fm_plan(plan, a, FM_SLOTS, smem);
-  const int row0 = FEW ? blockIdx.x * a.T : 0;                       // few tokens: rows of this CTA's own
-  FmUpTiles<Plan, AR> tiles(plan, a.I, a.H, row0, a.T);
-
-  if (warp == 0) {
-    if (lane == 0) f4_weights<S>(smem, bar, map, tiles);
-  } else if (warp == 6) {
-    if (lane == 0 && tiles.count() > 0 && (FEW ? mbar_wait(&rows_bar, 0, &bar.abort) : fm_tokens_ready(a, &bar.abort))) f4_tokens<S>(smem, bar, map, tiles);
-  } else if (warp == 1) {
-    f4_issue<S>(smem, bar, tiles);
-  } else if (warp < 6) {
-    f4_cells<S>(smem, bar, tiles);
+  const int row0 = FEW ? blockIdx.x * a.T : 0, et = threadIdx.x - F4_EPILOGUE;         // few tokens: rows of this CTA's own
+  const long x_bytes = fp4_row_bytes(a.H), x_scale = a.H / 2 + a.H / 16;
+  if (et < 0) {
+    fm_plan(plan, a, FM_SLOTS, smem);
+    fm_plan_made();
   } else {
-    const int q = warp & 3, et = threadIdx.x - F4_EPILOGUE;
-    const long x_bytes = fp4_row_bytes(a.H), x_scale = a.H / 2 + a.H / 16;
     if (FEW) {
-      if (tiles.count() > 0) {
-        for (int t = 0; t < a.T; ++t) fm_token(a, t, a.xq + (row0 + t) * x_bytes, s_sum, s_max);
-        fm_rows_stored(&rows_bar);
-      }
+      for (int t = 0; t < a.T; ++t) fm_token(a, t, a.xq + (row0 + t) * x_bytes, s_sum, s_max);
+      fm_rows_stored(&rows_bar);
     } else {
       for (;;) {
         if (et == 0) s_word = atomicAdd(a.claim, 1);
@@ -353,6 +344,20 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_up_kernel(const __grid_
         if (et == 0) atomicAdd(a.claim + 1, 1);
       }
     }
+    fm_plan_wait();
+  }
+  FmUpTiles<Plan, AR> tiles(plan, a.I, a.H, row0, a.T);
+
+  if (warp == 0) {
+    if (lane == 0) f4_weights<S>(smem, bar, map, tiles);
+  } else if (warp == 6) {
+    if (lane == 0 && tiles.count() > 0 && (FEW ? mbar_wait(&rows_bar, 0, &bar.abort) : fm_tokens_ready(a, &bar.abort))) f4_tokens<S>(smem, bar, map, tiles);
+  } else if (warp == 1) {
+    f4_issue<S>(smem, bar, tiles);
+  } else if (warp < 6) {
+    f4_cells<S>(smem, bar, tiles);
+  } else {
+    const int q = warp & 3;
     uint32_t ab = 0, aphase = 0;
     int done = 0;                                                    // tiles of the expert at hand
     const int n_tiles = tiles.count();
@@ -406,15 +411,18 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_up_kernel(const __grid_
   f4_close<S>(bar, a.status);
 }
 
-// 128 columns of the output from column n0 on: the slots of every token, in order.
+// AR columns of the output from column n0 on: the slots of every token, in order.  Four columns a lane, AR / 4 lanes a token, two tokens of
+// a lane at once.
+template <int AR>
 __device__ __forceinline__ void fm_combine(const FmArgs& a, const short* id, int n0) {
-  const int et = threadIdx.x - F4_EPILOGUE, lane = et & 31, n = n0 + 4 * lane;
+  constexpr int LANES = AR / 4, AT_ONCE = 128 / LANES;
+  const int et = threadIdx.x - F4_EPILOGUE, n = n0 + 4 * (et % LANES);
   if (n >= a.H) return;
-  for (int t0 = et >> 5; t0 < a.T; t0 += 8) {                       // two tokens of a warp at once
+  for (int t0 = et / LANES; t0 < a.T; t0 += 2 * AT_ONCE) {
     float4 s[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int t = t0 + 4 * p;
+      const int t = t0 + AT_ONCE * p;
       s[p] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (a.resid && t < a.T) {
         const float* r = a.resid + (long)t * a.ldr + n;
@@ -427,9 +435,9 @@ __device__ __forceinline__ void fm_combine(const FmArgs& a, const short* id, int
       for (int p = 0; p < 2; ++p)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int at = (t0 + 4 * p) * a.k + j0 + j;
+          const int at = (t0 + AT_ONCE * p) * a.k + j0 + j;
           v[p][j] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (t0 + 4 * p < a.T && j0 + j < a.k && id[at] >= 0) v[p][j] = __ldcg(reinterpret_cast<const float4*>(a.slot_out + (long)at * a.H + n));
+          if (t0 + AT_ONCE * p < a.T && j0 + j < a.k && id[at] >= 0) v[p][j] = __ldcg(reinterpret_cast<const float4*>(a.slot_out + (long)at * a.H + n));
         }
 #pragma unroll
       for (int p = 0; p < 2; ++p)
@@ -438,7 +446,7 @@ __device__ __forceinline__ void fm_combine(const FmArgs& a, const short* id, int
     }
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int t = t0 + 4 * p;
+      const int t = t0 + AT_ONCE * p;
       if (t >= a.T) break;
       const float f[4] = {s[p].x, s[p].y, s[p].z, s[p].w};
 #pragma unroll
@@ -458,7 +466,7 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_down_kernel(const __gri
   __shared__ __align__(8) F4Bars<S> bar;
   __shared__ __align__(8) uint64_t rows_bar;
   __shared__ Plan plan;
-  __shared__ float s_factor[FEW ? FM_FEW_SLOTS : FM_SLOTS], s_out[FEW ? FM_FEW_SLOTS : 1][AR];
+  __shared__ float s_factor[FEW ? FM_FEW_SLOTS : FM_SLOTS];
   __shared__ unsigned s_top[32];
   __shared__ int s_word;
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -466,9 +474,14 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_down_kernel(const __gri
   if (threadIdx.x == 0) mbar_init(&rows_bar, 128);
   f4_open<S>(bar, map);
   // The ids were there before the launch in front of this one began, and weights always are: both are read before its end is waited for.
-  fm_plan(plan, a, BN, smem);
+  if (threadIdx.x < F4_EPILOGUE) {
+    fm_plan(plan, a, BN, smem);
+    fm_plan_made();
+  } else {
+    fm_plan_wait();
+  }
   const int row0 = FEW ? blockIdx.x * a.T * a.k : 0;                 // few tokens: rows of this CTA's own
-  FmDownTiles<Plan, AR, FEW> tiles(plan, a.H, a.I, row0);
+  FmDownTiles<Plan, AR> tiles(plan, a.H, a.I, row0);
 
   if (warp == 0) {
     if (lane == 0) f4_weights<S>(smem, bar, map, tiles);
@@ -491,8 +504,7 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_down_kernel(const __gri
     pdl_wait();
     if (blockIdx.x == 0 && et < 2) a.claim[et] = 0;                  // ready for the next call
     if (FEW && n_tiles > 0) {
-      const typename Plan::Entry last = plan.entry[plan.n_entries - 1];
-      fm_rows(a, 0, last.first + last.rows, a.aq + row0 * a_bytes, s_top);
+      for (int i = 0; i < n_tiles && i < plan.n_entries; ++i) fm_rows(a, tiles.entry(i).first, tiles.entry(i).rows, a.aq + row0 * a_bytes, s_top);
       fm_rows_stored(&rows_bar);
     }
     for (int s = et; s < n_slots && n_tiles > 0; s += 128) {         // places behind the last slot of an expert of ours are not read
@@ -505,7 +517,7 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_down_kernel(const __gri
     for (int i = 0; i < n_tiles; ++i) {
       const F4Work mt = tiles.at(i);
       const typename Plan::Entry e = tiles.entry(i);
-      const int col = q * 32 + lane, n = mt.n0 + col, end = min(a.H, mt.n0 + AR);
+      const int n = mt.n0 + q * 32 + lane, end = min(a.H, mt.n0 + AR);
       const float ws = ws_nxt;
       if (i + 1 < n_tiles) ws_nxt = scale_of(i + 1);
       if (!f4_all<4>(mbar_wait_warp(&bar.acc_full[ab], aphase, &bar.abort))) break;
@@ -520,10 +532,7 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_down_kernel(const __gri
         for (int j = 0; j < 4; ++j) {
           const int at = e.first + min(r0 + j, e.rows - 1), slot = plan.slot[at];
           const float f = __uint_as_float(v[j]) * ws * s_factor[at];
-          if (r0 + j < e.rows && n < end) {
-            if (FEW) s_out[slot][col] = f;
-            else a.slot_out[(long)slot * a.H + n] = f;
-          }
+          if (r0 + j < e.rows && n < end) a.slot_out[(long)slot * a.H + n] = f;
         }
       }
       tc_fence_before();
@@ -532,25 +541,12 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_down_kernel(const __gri
       if (++ab == S::ACCS) { ab = 0; aphase ^= 1; }
       ++done;
       if (i + 1 == n_tiles || tiles.at(i + 1).n0 != mt.n0) {
-        if (FEW) {
-          f4_meet<4>();
-          for (int c = et; c < a.T * AR; c += 128) {
-            const int t = c / AR, m = mt.n0 + c % AR;
-            if (m >= a.H) continue;
-            float s = a.resid ? a.resid[(long)t * a.ldr + m] : 0.0f;
-            for (int j = 0; j < a.k; ++j) s += plan.id[t * a.k + j] >= 0 ? s_out[t * a.k + j][c % AR] : 0.0f;
-            if (a.c_f32) a.c_f32[(long)t * a.ldc + m] = s;
-            else a.c_bf16[(long)t * a.ldc + m] = __float2bfloat16_rn(s);
-          }
-          f4_meet<4>();
-        } else if (fm_last(a.claim + 2 + a.E + mt.n0 / 128, done, plan.n_entries, &s_word)) {
-          fm_combine(a, plan.id, mt.n0);
-        }
+        if (fm_last(a.claim + 2 + a.E + mt.n0 / AR, done, plan.n_entries, &s_word)) fm_combine<AR>(a, plan.id, mt.n0);
         done = 0;
       }
     }
     if (plan.n_entries == 0)                                         // every slot is another tier's
-      for (int j = blockIdx.x; j < (a.H + 127) / 128; j += gridDim.x) fm_combine(a, plan.id, 128 * j);
+      for (int j = blockIdx.x; j < (a.H + AR - 1) / AR; j += gridDim.x) fm_combine<AR>(a, plan.id, AR * j);
   }
   f4_close<S>(bar, a.status);
 }
@@ -575,7 +571,7 @@ struct FmWork {
   FmWork(long rows, long k, long E, long H, long I, long sms) {
     const long few = sms * (rows < FM_FEW ? rows : FM_FEW), own = few * k < sms * FM_FEW_SLOTS ? few * k : sms * FM_FEW_SLOTS;
     auto up = [](long n) { return (n + 127) / 128 * 128; };
-    xq = up((2 + E + (H + 127) / 128) * 4);
+    xq = up((2 + E + (H + 31) / 32) * 4);
     act = xq + up((rows > few ? rows : few) * fp4_row_bytes((int)H));
     aq = act + up(rows * k * I * 4);
     slot_out = aq + up((rows * k > own ? rows * k : own) * fp4_row_bytes((int)I));
@@ -616,9 +612,9 @@ static int fp4_moe_few(const Fp4MoeCall& c, const FmArgs& a) {
   int rc = au == 32 ? fm_up<32, 32, true>(c, a, rows_x, hit * tiles(a.I, 32)) : au == 64 ? fm_up<32, 64, true>(c, a, rows_x, hit * tiles(a.I, 64))
                                                                                        : fm_up<32, 128, true>(c, a, rows_x, hit * tiles(a.I, 128));
   if (rc) return rc;
-  const int ad = tiles(a.H, 16) <= c.sms ? 16 : tiles(a.H, 32) <= c.sms ? 32 : 64;
-  return ad == 16 ? fm_down<32, 16, true>(c, a, rows_a, tiles(a.H, 16)) : ad == 32 ? fm_down<32, 32, true>(c, a, rows_a, tiles(a.H, 32))
-                                                                                   : fm_down<32, 64, true>(c, a, rows_a, tiles(a.H, 64));
+  const int ad = hit * tiles(a.H, 32) <= c.sms ? 32 : hit * tiles(a.H, 64) <= c.sms ? 64 : 128;
+  return ad == 32 ? fm_down<32, 32, true>(c, a, rows_a, hit * tiles(a.H, 32)) : ad == 64 ? fm_down<32, 64, true>(c, a, rows_a, hit * tiles(a.H, 64))
+                                                                                        : fm_down<32, 128, true>(c, a, rows_a, hit * tiles(a.H, 128));
 }
 template <int BN>
 static int fp4_moe_full(const Fp4MoeCall& c, const FmArgs& a) {

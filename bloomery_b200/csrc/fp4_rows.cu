@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(512) fp4_rows_kernel(const Fp4RowsArgs a) {
     __syncthreads();
     double all = 0.0;
     for (int w = 0; w < warps; ++w) all += s_sum[w];
-    const float r = (float)(1.0 / sqrt(all / (double)a.K + a.eps));
+    const float r = fp4_rsqrt(all / (double)a.K + a.eps);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
       if (tid + b * nthr < blocks) fp4_scale16(v[b], r, a.gain + 16 * (tid + b * nthr));

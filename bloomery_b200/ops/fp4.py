@@ -18,7 +18,7 @@ from ._lib import check, cuda, raw_stream
 from .decode import QWeight, sm_count
 from .gemm import TileTable
 
-_ROWS, _GEMM, _MOE = struct.Struct("6P2ld4i"), struct.Struct("12P3l6i"), struct.Struct("13P3ld8i")      # Fp4RowsCall, Fp4GemmCall, Fp4MoeCall
+_ROWS, _GEMM, _MOE = struct.Struct("6P2ld4i"), struct.Struct("12P3l7i4x"), struct.Struct("13P3ld8i")      # Fp4RowsCall, Fp4GemmCall, Fp4MoeCall
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_K = 32768                                             # values of a row that fp4_rows holds in registers
 _entries: dict = {}
@@ -156,7 +156,7 @@ def fp4_gemm(X: Fp4Rows, W: QWeight, tiles: TileTable, *, out_f32: Optional[torc
         X.ptr, wp, w2p, tiles.mtiles.data_ptr(), tiles.n_mtiles.data_ptr(), out.data_ptr() if f32 else 0, 0 if f32 else out.data_ptr(),
         0 if dst_row is None else dst_row.data_ptr(), 0 if row_scale is None else row_scale.data_ptr(), rp,
         0 if status is None else status.data_ptr(), raw_stream(index), X.rows, out.stride(0), ldr, G, N, k,
-        tiles.fixed or tiles.max_mtiles, tiles.tile_rows, sm_count()))
+        tiles.fixed or tiles.max_mtiles, tiles.tile_rows, sm_count(), tiles.fixed != 0))
     if code:
         check(code, "bl_fp4_gemm")
 
