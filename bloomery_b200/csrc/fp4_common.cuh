@@ -26,87 +26,106 @@ __device__ __forceinline__ float fp4_row_scale(unsigned amax_bits) {
   return amax_bits < FP4_INF ? fmaxf(__fdiv_rn(__uint_as_float(amax_bits), FP4_ROW), FP4_LEAST) : __uint_as_float(0x7fc00000u);
 }
 
-// E4M3 code nearest to amax / (6 g); its value in `s`
-__device__ __forceinline__ unsigned fp4_block_scale(float amax, float g, float& s) {
-  const float q = __fdiv_rn(amax, 6.0f * g);
-  unsigned c = __nv_cvt_float_to_fp8(fminf(q, 448.0f), __NV_SATFINITE, __NV_E4M3);
-  auto value = [](unsigned code) {                    // also of 0x7f, as the step above 448
-    const unsigned e = code >> 3, m = code & 7;
-    return (float)(e ? 8 + m : m) * __uint_as_float(((e ? e : 1u) + 117u) << 23);
-  };
-  s = value(c);
-  if (c < 0x7eu) {
-    const float up = value(c + 1), r = fmaf(-3.0f * (s + up), g, amax);       // 6 times the midpoint: seven bits
-    if (r > 0.0f || (r == 0.0f && (c & 1))) { ++c; s = up; }
-  }
-  if (c > 0u) {
-    const float down = value(c - 1), r = fmaf(-3.0f * (s + down), g, amax);
-    if (r < 0.0f || (r == 0.0f && (c & 1))) { --c; s = down; }
-  }
+// E4M3 code nearest to amax / (6 g), inv6g next to 1 / (6 g); its value in `s`
+__device__ __forceinline__ unsigned fp4_block_scale(float amax, float g, float inv6g, float& s) {
+  unsigned c = __nv_cvt_float_to_fp8(fminf(amax * inv6g, 448.0f), __NV_SATFINITE, __NV_E4M3);
+  // its neighbours: there is none (NaN, which decides nothing) below 0 and above 448
+  const __half2_raw around = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((c - 1 & 0xff) | (c + 1) << 8), __NV_E4M3);
+  const float2 n = __half22float2(*reinterpret_cast<const __half2*>(&around));
+  const __half_raw mid = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3);
+  s = __half2float(*reinterpret_cast<const __half*>(&mid));
+  const float lo = fmaf(-3.0f * (s + n.x), g, amax), hi = fmaf(-3.0f * (s + n.y), g, amax);       // 6 times the midpoints: seven bits
+  if (hi > 0.0f || (hi == 0.0f && (c & 1))) { ++c; s = n.y; }
+  else if (lo < 0.0f || (lo == 0.0f && (c & 1))) { --c; s = n.x; }
   return c;
 }
 
-// Codes of eight values (value i in bits 4i ..), steps of d.  The quotients are off by less than 2^-21; where 2^-20 to either side gives
-// another code the midpoint is looked at itself.
-__device__ __forceinline__ uint32_t fp4_codes8(const float* x, float d, float lo, float hi) {
-  uint32_t a = 0, b = 0;
+// Two fp32 values in one register pair, and the instruction that works on both
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float2 f2_open(uint64_t v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) { uint64_t r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+
+// Codes of eight values times `f` (value i in bits 4i ..), or of four
+template <int N>
+__device__ __forceinline__ uint32_t fp4_round(const float* x, float f) {
+  const uint64_t ff = f2_pack(f, f);
+  float2 y[N / 2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    a |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(x[2 * i] * lo, x[2 * i + 1] * lo), __NV_E2M1, cudaRoundNearest) << (8 * i);
-    b |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(x[2 * i] * hi, x[2 * i + 1] * hi), __NV_E2M1, cudaRoundNearest) << (8 * i);
-  }
+  for (int i = 0; i < N / 2; ++i) y[i] = f2_open(f2_mul(f2_pack(x[2 * i], x[2 * i + 1]), ff));
+  uint32_t r;
+  if constexpr (N == 8)
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r) : "f"(y[0].x), "f"(y[0].y), "f"(y[1].x), "f"(y[1].y), "f"(y[2].x), "f"(y[2].y), "f"(y[3].x), "f"(y[3].y));
+  else
+    asm("{\n\t.reg .b8 a, b;\n\t.reg .b16 w;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "mov.b16 w, {a, b};\n\tcvt.u32.u16 %0, w;\n\t}"
+        : "=r"(r) : "f"(y[0].x), "f"(y[0].y), "f"(y[1].x), "f"(y[1].y));
+  return r;
+}
+// Codes of N values, steps of d.  The quotients are off by less than 2^-21; where 2^-20 to either side gives another code the midpoint
+// is looked at itself.
+template <int N>
+__device__ __forceinline__ uint32_t fp4_codes(const float* x, float d, float lo, float hi) {
+  uint32_t a = fp4_round<N>(x, lo);
+  const uint32_t b = fp4_round<N>(x, hi);
   if (a != b) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
+#pragma unroll 1
+    for (int i = 0; i < N; ++i) {
       const unsigned c = a >> (4 * i) & 7u;
       if ((b >> (4 * i) & 7u) != c) {                 // one step above: c < 7
         const float mid = c < 4 ? 0.5f * (float)c + 0.25f : c == 4 ? 2.5f : c == 5 ? 3.5f : 5.0f;
-        const float r = fmaf(-mid, d, fabsf(x[i]));
+        float v = x[0];
+#pragma unroll
+        for (int j = 1; j < N; ++j) v = i == j ? x[j] : v;
+        const float r = fmaf(-mid, d, fabsf(v));
         if (r > 0.0f || (r == 0.0f && (c & 1))) a += 1u << (4 * i);
       }
     }
   }
   return a;
 }
+constexpr float FP4_BELOW = 1.0f - 9.5367431640625e-7f, FP4_ABOVE = 1.0f + 9.5367431640625e-7f;      // 2^-20 to either side
 
-// A block of 16 values of a row with scale g: its codes and the byte of its scale.  A row with anything that is not finite has NaN
-// for g and gets zeros: its products are NaN by the row scale alone.
-__device__ __forceinline__ uint2 fp4_block(const float* x, float g, unsigned& scale) {
-  float amax = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));
-  if (!(g > 0.0f)) { scale = 0; return make_uint2(0u, 0u); }
+// A block of 16 values of a row with scale g, the largest of them with the bits `top`: its codes and the byte of its scale.  A row with
+// anything that is not finite has NaN for g and gets zeros: its products are NaN by the row scale alone.
+__device__ __forceinline__ uint2 fp4_block(const float* x, unsigned top, float g, float inv6g, unsigned& scale) {
+  scale = 0;
+  if (!(g > 0.0f)) return make_uint2(0u, 0u);
   float s;
-  scale = fp4_block_scale(amax, g, s);
+  scale = fp4_block_scale(__uint_as_float(top), g, inv6g, s);
   if (scale == 0u) return make_uint2(0u, 0u);
-  const float d = s * g, inv = __frcp_rn(d), lo = inv * (1.0f - 9.5367431640625e-7f), hi = inv * (1.0f + 9.5367431640625e-7f);
-  return make_uint2(fp4_codes8(x, d, lo, hi), fp4_codes8(x + 8, d, lo, hi));
+  const float d = s * g, inv = __fdividef(1.0f, d), lo = inv * FP4_BELOW, hi = inv * FP4_ABOVE;
+  return make_uint2(fp4_codes<8>(x, d, lo, hi), fp4_codes<8>(x + 8, d, lo, hi));
 }
 
 // ---- pieces of a row --------------------------------------------------------------------------------------
-__device__ __forceinline__ void fp4_load16(const void* x, int type, long at, float* v) {       // type: 0 bf16, 1 f16, 2 fp32
+__device__ __forceinline__ void fp4_open16(const uint32_t (&w)[8], int type, float* v) {       // 16 values of type 0 bf16, 1 f16
+  if (type == 0) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { v[2 * j] = __uint_as_float(w[j] << 16); v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u); }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  }
+}
+__device__ __forceinline__ void fp4_load16(const void* x, int type, long at, float* v) {       // 2: fp32
   if (type == 2) {
     const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + at);
 #pragma unroll
     for (int i = 0; i < 4; ++i) { const float4 f = p[i]; v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w; }
   } else {
     const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + at);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 u = p[i];
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (type == 0) {
-          v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
-          v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-          v[8 * i + 2 * j] = f.x;
-          v[8 * i + 2 * j + 1] = f.y;
-        }
-      }
-    }
+    const uint4 lo = p[0], hi = p[1];
+    const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    fp4_open16(w, type, v);
   }
 }
 // 1 / sqrt(x) in fp32: two of Newton's steps in 64 bits behind rsqrtf, which leave 2^-52 or so in front of the rounding, are a few
@@ -129,17 +148,29 @@ __device__ __forceinline__ void fp4_scale16(float* v, float r, const float* gain
     v[4 * i + 2] = v[4 * i + 2] * r * g.z; v[4 * i + 3] = v[4 * i + 3] * r * g.w;
   }
 }
-// The largest magnitude as bits: a NaN is above everything.
-__device__ __forceinline__ unsigned fp4_top16(const float* v) {
-  unsigned top = 0;
+// Sum of squares of 16 values: 16 roundings to 24 bits of a part, of which hundreds are added in 64 bits behind this (two fp32 parts
+// with what each rounding left cost 136 clocks a warp, this 16; the root of the whole then moves by one unit of its last place
+// in one row of twenty or so).
+__device__ __forceinline__ double fp4_squares16(const float* v) {
+  float s = v[0] * v[0];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-  return top;
+  for (int i = 1; i < 16; ++i) s = fmaf(v[i], v[i], s);
+  return (double)s;
 }
+// The largest magnitude as bits: a NaN is above everything.
+template <int N>
+__device__ __forceinline__ unsigned fp4_top(const float* v) {
+  float top = fabsf(v[0]);
+#pragma unroll
+  for (int i = 1; i < N; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(v[i])));
+  return __float_as_uint(top) & 0x7fffffffu;
+}
+// 1 / (6 g), near enough for a first guess at a block's scale
+__device__ __forceinline__ float fp4_inv6(float g) { return __frcp_rn(6.0f * g); }
 // Block `at` of a row of K values with scale g
-__device__ __forceinline__ void fp4_store_block(uint8_t* row, int K, int at, const float* v, float g) {
+__device__ __forceinline__ void fp4_store_block(uint8_t* row, int K, int at, const float* v, unsigned top, float g, float inv6g) {
   unsigned scale;
-  const uint2 codes = fp4_block(v, g, scale);
+  const uint2 codes = fp4_block(v, top, g, inv6g, scale);
   *reinterpret_cast<uint2*>(row + 8 * at) = codes;
   row[K / 2 + at] = (uint8_t)scale;
   if (at == 0) *reinterpret_cast<float*>(row + K / 2 + K / 16) = g;

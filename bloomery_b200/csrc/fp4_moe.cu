@@ -190,8 +190,7 @@ __device__ __forceinline__ void fm_token(const FmArgs& a, int t, uint8_t* row, d
 #pragma unroll 1
     for (int b = et; b < blocks; b += 128) {
       load(b);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) ss = fma((double)v[i], (double)v[i], ss);
+      ss += fp4_squares16(v);
     }
     ss = warp_sum_d(ss);
     if (lane == 0) s_sum[w] = ss;
@@ -203,19 +202,19 @@ __device__ __forceinline__ void fm_token(const FmArgs& a, int t, uint8_t* row, d
   for (int b = et; b < blocks; b += 128) {
     if (blocks > 128 || !a.gain) load(b);             // else the one block is still there
     if (a.gain) fp4_scale16(v, r, a.gain + 16 * b);
-    top = max(top, fp4_top16(v));
+    top = max(top, fp4_top<16>(v));
   }
   top = __reduce_max_sync(0xFFFFFFFFu, top);
   if (lane == 0) s_max[w] = top;
   f4_meet<4>();
-  const float g = fp4_row_scale(max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3])));
+  const float g = fp4_row_scale(max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]))), inv6g = fp4_inv6(g);
 #pragma unroll 1
   for (int b = et; b < blocks; b += 128) {
     if (blocks > 128) {
       load(b);
       if (a.gain) fp4_scale16(v, r, a.gain + 16 * b);
     }
-    fp4_store_block(row, a.H, b, v, g);
+    fp4_store_block(row, a.H, b, v, fp4_top<16>(v), g, inv6g);
   }
 }
 // The gain's way to this processor, before the launch in front of this one has ended.
@@ -248,14 +247,15 @@ __device__ __forceinline__ void fm_rows(const FmArgs& a, int first, int rows, ui
         if (b + 128 * j < n) load(b + 128 * j, v[j]);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (b + 128 * j < n) atomicMax(&s_top[(b + 128 * j) / per], fp4_top16(v[j]));
+        if (b + 128 * j < n) atomicMax(&s_top[(b + 128 * j) / per], fp4_top<16>(v[j]));
     }
     f4_meet<4>();
 #pragma unroll 1
     for (int b = et; b < n; b += 128) {
       float v[16];
       load(b, v);                                     // from the first cache, mostly
-      fp4_store_block(to + (first + r0 + b / per) * fp4_row_bytes(a.I), a.I, b % per, v, fp4_row_scale(s_top[b / per]));
+      const float g = fp4_row_scale(s_top[b / per]);
+      fp4_store_block(to + (first + r0 + b / per) * fp4_row_bytes(a.I), a.I, b % per, v, fp4_top<16>(v), g, fp4_inv6(g));
     }
     f4_meet<4>();
   }
