@@ -111,11 +111,20 @@ def fp4_rows(x: torch.Tensor, out: Fp4Rows, *, gain: Optional[torch.Tensor] = No
         check(code, "bl_fp4_rows")
 
 
+def fp4_supports(w: QWeight) -> bool:
+    """Whether the products here take a matrix or stack: NVFP4 whose block scales are without a sign, as checkpoints have them (looks at
+    all of them and waits for the answer: once, when a model is set up)."""
+    if w.qtype != "NVFP4" or w.k % 64 or w.k > MAX_K:
+        return False
+    return not bool((w.data[..., w.k // 2:w.k // 2 + w.k // 16] >= 0x80).any())
+
+
 class Fp4Work:
-    """Partial sums and tickets of products that split their depth: one per stream that runs them."""
+    """What a program keeps for the dense products of one stream.  Products with few tiles take narrower ones instead of sharing their depth, so
+    there is nothing in it yet; it is part of the call so that a program that keeps one per stream stays as it is."""
 
     def __init__(self, device):
-        pass
+        self.device = device
 
 
 def _matrix(name: str, w: QWeight, k: int, index: int) -> int:

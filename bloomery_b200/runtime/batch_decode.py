@@ -25,6 +25,7 @@ from typing import Dict, List, Sequence, Tuple
 import torch
 
 from ..ops import decode as K
+from ..ops import fp4 as Q
 from ..ops import gemm as G
 from ..ops.prefix import prefix_attention
 
@@ -131,6 +132,9 @@ class BatchDecode:
         self._work = [G.QgemmWork(dev) for _ in range(3)]
         from ..utils import levers
         self.fp8_native = bool(levers.get("BLOOMERY_FP8_NATIVE"))
+        self.fp4_native = bool(levers.get("BLOOMERY_FP4_NATIVE"))
+        self._fp4_ok: Dict[int, bool] = {}      # of a matrix of the model: whether its block scales allow it
+        self._moe_work = None
         # the engine's own stream: its 8-row passes and prompts and these passes touch the same KV pages in order
         self._stream = getattr(engine, "_stream", None) or torch.cuda.Stream(device=dev)
         self._side = [torch.cuda.Stream(device=dev), torch.cuda.Stream(device=dev)]
@@ -153,12 +157,36 @@ class BatchDecode:
     def _native_fp8(self, Wq) -> bool:
         return self.fp8_native and Wq.qtype == "FP8_B128" and Wq.k % 128 == 0
 
+    def _native_fp4(self, *weights) -> bool:
+        """Whether all of these matrices multiply NVFP4 rows (looked up once for a matrix: before the pass is captured)."""
+        if not self.fp4_native or any(w.qtype != "NVFP4" for w in weights):
+            return False
+        for w in weights:
+            if id(w) not in self._fp4_ok:
+                self._fp4_ok[id(w)] = Q.fp4_supports(w)
+        return all(self._fp4_ok[id(w)] for w in weights)
+
+    def _q4(self, X: torch.Tensor, gain=None) -> "Q.Fp4Rows":
+        """NVFP4 rows of X (one launch; ``gain``: of fp32 rows behind their norm), in a buffer of X's own."""
+        key = ("q4", X.data_ptr(), X.shape[1])
+        buf = self._scratch_w.get(key)
+        if buf is None:                              # for the largest bucket: passes captured before go on with it
+            buf = self._scratch_w[key] = Q.Fp4Rows(max(X.shape[0], self.R), X.shape[1], self.e.device)
+        Q.fp4_rows(X, buf, gain=gain, eps=self.e.spec.rms_eps)
+        return buf
+
     def _mm(self, X, Wq, tiles, M, x8=None, W2=None, branch=0, room=0, **kw):
         """X [rows, K] bf16 times a resident matrix (or, with W2, the SwiGLU pair): FP8 weights against E4M3 rows on the
         tensor cores, other quantised types expanded in flight, the rest through a bf16 expansion launch.  ``x8``: the
         rows' E4M3 form when the caller already made it (several products of one input).  ``branch``: 0 on the pass's own
-        stream, 1 / 2 on its side streams; ``room``: processors that a split product may take (0: all).  Returns the launch
-        count."""
+        stream, 1 / 2 on its side streams; ``room``: processors that a split product may take (0: all).  NVFP4 weights take NVFP4 rows where
+        that is asked for (``x8`` then holds those).  Returns the launch count."""
+        if self._native_fp4(Wq, *([W2] if W2 is not None else [])):
+            n = 0
+            if not isinstance(x8, Q.Fp4Rows):
+                x8 = self._q4(X); n += 1
+            Q.fp4_gemm(x8, Wq, tiles if tiles.tile_rows <= 64 else self._dense32(M), W2=W2, status=self.status, **kw)
+            return n + 1
         if self._native_fp8(Wq):
             n = 0
             if x8 is None:
@@ -243,6 +271,15 @@ class BatchDecode:
         n = self._mm(xn, w.q[b + "ffn_gate.weight"], tiles, M, W2=w.q[b + "ffn_up.weight"], out_bf16=self.dact[:M])
         yield n + self._mm(self.dact[:M], w.q[b + "ffn_down.weight"], tiles, M, out_f32=x, resid=x)
 
+    def _experts_in_fp4(self, *stacks) -> bool:
+        s = self.e.spec
+        if not self._native_fp4(*stacks) or s.n_used > Q.MOE_USED or s.n_expert > Q.MOE_EXPERTS or \
+                any(n % 64 or n > Q.MOE_WIDTH for n in (s.hidden, s.moe_inter)):
+            return False
+        if self._moe_work is None:
+            self._moe_work = Q.Fp4MoeWork(self.R, s.n_used, s.hidden, s.moe_inter, s.n_expert, self.e.device)
+        return True
+
     def experts(self, il: int, M: int, x: torch.Tensor, xn: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, tiles):
         """Routed experts (and the shared one) of layer il on the routed rows; a generator of launch counts (it yields
         where ranks of a several-GPU pass must meet; here it never does)."""
@@ -252,10 +289,19 @@ class BatchDecode:
         E, k = s.n_expert, s.n_used
         mark = self.timing.mark
         n = 0
+        qg, qu, qd = (w.q[b + f"ffn_{nm}_exps.weight"] for nm in ("gate", "up", "down"))
+        if self._experts_in_fp4(qg, qu, qd):
+            # the norm, the plan, both products and the sum over a token's experts are two launches
+            gain = w.f[b + "ffn_norm.weight"]
+            Q.fp4_moe(x, ids, wts, qg, qu, qd, self._moe_work, gain=gain, eps=s.rms_eps, out_f32=x, resid=x, status=self.status); n += 2
+            if s.n_shared:
+                n += self.shared_expert(il, M, xn, tiles, x, x)
+            mark(il, "experts")
+            yield n
+            return
         G.moe_plan(ids, wts, E, self.moe_tiles, self.pos_of, self.dst_row, self.row_scale); n += 1
         G.gather_rows_bf16(xn, self.dst_row, self.moe_tiles.offsets[E:E + 1], self.cap, k, self.Ap); n += 1
         mark(il, "route_plan_gather")
-        qg, qu, qd = (w.q[b + f"ffn_{nm}_exps.weight"] for nm in ("gate", "up", "down"))
         n += self._mm(self.Ap, qg, self.moe_tiles, M, W2=qu, out_bf16=self.act)
         mark(il, "gate_up")
         n += self._mm(self.act, qd, self.moe_tiles, M, out_f32=self.slot_out, dst_row=self.dst_row, row_scale=self.row_scale)
@@ -272,6 +318,11 @@ class BatchDecode:
             mark(il, "shared_expert")
         yield n
 
+    def _rows_in_fp4(self, il: int) -> bool:
+        """Whether the projections of layer il take NVFP4 rows made of the residual stream, so that nobody reads its normed rows."""
+        w, b = self.e.w, f"blk.{il}."
+        return not self.e.spec.mla and self._native_fp4(*(w.q[b + nm] for nm in ("attn_q.weight", "attn_k.weight", "attn_v.weight")))
+
     def _attn_gqa(self, il: int, M: int, xn: torch.Tensor, tiles) -> int:
         """Grouped-query attention of layer il up to the bf16 rows of the o product."""
         e = self.e
@@ -287,6 +338,9 @@ class BatchDecode:
         x8 = None
         if any(self._native_fp8(w.q[b + nm]) for nm in ("attn_q.weight", "attn_k.weight", "attn_v.weight")):
             x8 = self._q8(xn); n += 1                            # one E4M3 form of the rows for the three products
+        elif self._rows_in_fp4(il):
+            # one NVFP4 form, with the norm in front of it
+            x8 = self._q4(self.x[:M], w.f[b + "attn_norm.weight"]); n += 1
         fork = torch.cuda.Event()
         fork.record(main)
         joins = []
@@ -370,7 +424,7 @@ class BatchDecode:
             b = f"blk.{il}."
             mark = self.timing.mark
             mark(il, "ffn_tail")
-            if not self._normed:
+            if not self._normed and not self._rows_in_fp4(il):
                 G.rmsnorm_bf16(x, w.f[b + "attn_norm.weight"], s.rms_eps, xn); n += 1
             self._normed = False
             mark(il, "norm")

@@ -27,6 +27,7 @@ import os
 import torch
 
 from ..ops import decode as K
+from ..ops import fp4 as Q
 from ..ops import gemm as G
 from .engine import GEMM_THRESHOLD
 from .kv import PAGE
@@ -96,6 +97,9 @@ class GemmPrefill:
         # 33.5, 46.4).
         self.pair_rows = 128
         self._direct_ok = None
+        self.fp4_native = bool(levers.get("BLOOMERY_FP4_NATIVE"))       # NVFP4 weights multiply NVFP4 rows: no copies, nothing expanded
+        self._fp4_ok = None
+        self._rows4 = {}
         self._block_limit = None
         self._work = None
         self._flash_work = G.FlashWork(engine.device)
@@ -111,6 +115,27 @@ class GemmPrefill:
                 b.fill_(float("nan") if dtype.is_floating_point else -1)
             self._buf[name] = b
         return b[:n].view(*shape)
+
+    def _q4(self, name: str, X: torch.Tensor, rows: int = 0, **kw) -> "Q.Fp4Rows":
+        """NVFP4 rows of X in the buffer ``name`` (of ``rows`` rows, where they are scattered)."""
+        rows = rows or X.shape[0]
+        buf = self._rows4.get(name)
+        if buf is None or buf.rows < rows:
+            buf = self._rows4[name] = Q.Fp4Rows(rows, X.shape[1], self.e.device)
+        Q.fp4_rows(X, buf, eps=self.e.spec.rms_eps, **kw)
+        return buf
+
+    def _native_fp4(self) -> bool:
+        """Whether prompts run on NVFP4 rows: where that is asked for, of a model whose layers are all routed and whose matrices are all
+        NVFP4 and on the card."""
+        if not self.fp4_native or self.expert_source is not None:
+            return False
+        if self._fp4_ok is None:
+            s, w = self.e.spec, self.e.w
+            names = ("attn_q", "attn_k", "attn_v", "attn_output", "ffn_gate_exps", "ffn_up_exps", "ffn_down_exps")
+            self._fp4_ok = all(s.layer_is_moe(il) for il in range(s.n_layer)) and \
+                all(Q.fp4_supports(w.q[f"blk.{il}.{n}.weight"]) for il in range(s.n_layer) for n in names)
+        return self._fp4_ok
 
     def run(self, slot: int, tokens: Sequence[int], start: int = 0) -> None:
         """Append ``tokens`` at positions start.. of ``slot``; leaves the last row's hidden
@@ -147,13 +172,14 @@ class GemmPrefill:
         qkv = self._get("qkv", (T, qkv_w), f32)
         # Quantised weights are expanded to bf16 one layer AHEAD of their use, on a side stream: the expansion is bound
         # by HBM traffic, the products by the tensor cores, so the two overlap.  Two sets of bf16 buffers alternate.
-        direct = fine or self._direct(T)
-        blocks = direct or self._expert_blocks(T)           # the routed experts' weights are multiplied as they are
-        resident = not direct and self._use_resident(experts=not blocks)
-        ahead = self.expert_source is None and self.expand_ahead and not resident and not direct
+        native = not fine and self._native_fp4()            # every product of NVFP4 rows with the weights as they are
+        direct = fine or (not native and self._direct(T))
+        blocks = direct or native or self._expert_blocks(T) # the routed experts' weights are multiplied as they are
+        resident = not direct and not native and self._use_resident(experts=not blocks)
+        ahead = self.expert_source is None and self.expand_ahead and not resident and not direct and not native
         nset = 2 if ahead else 1
-        wqkv_s = [None if direct else self._get(f"wqkv{i}", (qkv_w, H), bf) for i in range(nset)]
-        wo_s = [None if direct else self._get(f"wo{i}", (H, s.q_rows), bf) for i in range(nset)]
+        wqkv_s = [None if direct or native else self._get(f"wqkv{i}", (qkv_w, H), bf) for i in range(nset)]
+        wo_s = [None if direct or native else self._get(f"wo{i}", (H, s.q_rows), bf) for i in range(nset)]
         form = dict(fine=True) if fine else dict(exact=True)
         if fine:
             # key segments as in a decode round: about eight blocks a processor
@@ -172,6 +198,8 @@ class GemmPrefill:
             dense_tiles = G.TileTable.dense(T, dev, host=True)
             on_pairs = {n for n in (qkv_w, H) if G.pairs_pay(T, n)}       # widths of the projections that go to pairs of CTAs
             pair_tiles = G.TileTable.dense(T, dev, G.PAIR_ROWS, host=True) if on_pairs else None
+            if native:
+                rows_tiles, on_pairs = Q.fp4_tiles(T, dev), ()
 
         def project(X, W, **out):
             """A dense product over a bf16 copy."""
@@ -206,7 +234,7 @@ class GemmPrefill:
             act = self._get("act", (cap, I_), bf)
             slot_out = self._get("slot_out", (nslot, H), f32)
             pairs = not blocks and nslot >= self.pair_rows * E
-            moe_tiles = G.TileTable(nslot, E, dev, (32 if direct or nslot <= 8 * E else 64) if blocks else G.PAIR_ROWS if pairs else G.BM)
+            moe_tiles = G.TileTable(nslot, E, dev, Q.fp4_tile_rows(nslot, E, True) if native else (32 if direct or nslot <= 8 * E else 64) if blocks else G.PAIR_ROWS if pairs else G.BM)
         if s.dense_inter and (s.first_dense > 0 or not s.is_moe):
             Id = s.dense_inter
             dg_s = [self._get(f"dg{i}", (Id, H), bf) for i in range(nset)]
@@ -290,10 +318,17 @@ class GemmPrefill:
                         expand(il + 1, "all")
                         ready[il + 1].record(side)
                 main.wait_event(ready[il])
-            if not normed:
+            if not normed and not native:
                 G.rmsnorm_bf16(x, w.f[b + "attn_norm.weight"], s.rms_eps, xn)
             normed = False
-            if direct:
+            if native:
+                rows = self._q4("hidden", x, gain=w.f[b + "attn_norm.weight"])
+                lo = 0
+                for nm in ("attn_q", "attn_k", "attn_v"):
+                    wq = w.q[b + nm + ".weight"]
+                    Q.fp4_gemm(rows, wq, rows_tiles, out_f32=qkv[:, lo:lo + wq.rows], status=st)
+                    lo += wq.rows
+            elif direct:
                 lo = 0
                 for nm in ("attn_q", "attn_k", "attn_v"):
                     wq = w.q[b + nm + ".weight"]
@@ -338,7 +373,9 @@ class GemmPrefill:
                     G.gemm_bf16(P, Vt, pv_tiles, out_bf16=attn.view(T * s.n_q, s.head_dim), dst_row=map_o, status=st)
                     self.timing.mark(il, "values")
             self.timing.mark(il, "attention")
-            if direct:
+            if native:
+                Q.fp4_gemm(self._q4("attention", attn), w.q[b + "attn_output.weight"], rows_tiles, out_f32=x, resid=x, status=st)
+            elif direct:
                 G.qgemm(attn, w.q[b + "attn_output.weight"], dense_tiles, out_f32=x, resid=x, status=st, work=self._work,
                         **form)
             else:
@@ -363,9 +400,17 @@ class GemmPrefill:
                 self.timing.mark(il, "route")
                 G.moe_plan(ids, wts, E, moe_tiles, pos_of, dst_row, row_scale)
                 self.timing.mark(il, "count_scatter")
-                G.gather_rows_bf16(rows_in, dst_row, moe_tiles.offsets[E:E + 1], cap, k, Ap)
+                if native:
+                    rows = self._q4("experts", rows_in, nslot, pos_of=pos_of)           # to their places, once for each expert
+                else:
+                    G.gather_rows_bf16(rows_in, dst_row, moe_tiles.offsets[E:E + 1], cap, k, Ap)
                 self.timing.mark(il, "dispatch")
-                if blocks:
+                if native:
+                    qg, qu, qd = (w.q[b + f"ffn_{n}_exps.weight"] for n in ("gate", "up", "down"))
+                    Q.fp4_gemm(rows, qg, moe_tiles, out_bf16=act, W2=qu, status=st)
+                    self.timing.mark(il, "gemm_gate_up")
+                    Q.fp4_gemm(self._q4("inter", act[:nslot]), qd, moe_tiles, out_f32=slot_out, dst_row=dst_row, row_scale=row_scale, status=st)
+                elif blocks:
                     qg, qu, qd = (w.q[b + f"ffn_{n}_exps.weight"] for n in ("gate", "up", "down"))
                     G.qgemm(Ap, qg, moe_tiles, out_bf16=act, W2=qu, status=st, **form)
                     self.timing.mark(il, "gemm_gate_up")
@@ -385,7 +430,7 @@ class GemmPrefill:
                     (G.gemm_pair if pairs else G.gemm_bf16)(act, wd, moe_tiles, out_f32=slot_out, dst_row=dst_row,
                                                             row_scale=row_scale, status=st)
                 self.timing.mark(il, "gemm_down")
-                if il + 1 < s.n_layer and H <= 8192:
+                if il + 1 < s.n_layer and H <= 8192 and not native:
                     G.moe_combine_norm(slot_out, pos_of, T, k, x, x, w.f[f"blk.{il + 1}.attn_norm.weight"], s.rms_eps, xn)
                     normed = True
                 else:
