@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_up_kernel(const __grid_
       for (int t = 0; t < a.T; ++t) fm_token(a, t, a.xq + (row0 + t) * x_bytes, s_sum, s_max);
       fm_rows_stored(&rows_bar);
     } else {
-      for (;;) {
+      for (int tries = 0; tries <= a.T; ++tries) {
         if (et == 0) s_word = atomicAdd(a.claim, 1);
         f4_meet<4>();
         const int t = s_word;
@@ -351,7 +351,8 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_up_kernel(const __grid_
   if (warp == 0) {
     if (lane == 0) f4_weights<S>(smem, bar, map, tiles);
   } else if (warp == 6) {
-    if (lane == 0 && tiles.count() > 0 && (FEW ? mbar_wait(&rows_bar, 0, &bar.abort) : fm_tokens_ready(a, &bar.abort))) f4_tokens<S>(smem, bar, map, tiles);
+    const bool go = tiles.count() > 0 && (!FEW || mbar_wait_warp(&rows_bar, 0, &bar.abort));
+    if (lane == 0 && go && (FEW || fm_tokens_ready(a, &bar.abort))) f4_tokens<S>(smem, bar, map, tiles);
   } else if (warp == 1) {
     f4_issue<S>(smem, bar, tiles);
   } else if (warp < 6) {
@@ -488,7 +489,8 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_down_kernel(const __gri
   } else if (warp == 6) {
     pdl_wait();
     pdl_launch();
-    if (lane == 0 && tiles.count() > 0 && (!FEW || mbar_wait(&rows_bar, 0, &bar.abort))) f4_tokens<S>(smem, bar, map, tiles);
+    const bool go = tiles.count() > 0 && (!FEW || mbar_wait_warp(&rows_bar, 0, &bar.abort));
+    if (lane == 0 && go) f4_tokens<S>(smem, bar, map, tiles);
   } else if (warp == 1) {
     f4_issue<S>(smem, bar, tiles);
   } else if (warp < 6) {

@@ -19,7 +19,8 @@ __device__ __forceinline__ bool f4_all(bool ok) {
   return r != 0;
 }
 
-// mbar_wait_warp with one try in front of its loop (54 clocks instead of 94 where the phase has ended, as it mostly has)
+// mbar_wait_warp, whose limit holds, with one try in front of its loop (54 clocks instead of 94 where the phase has ended, as it mostly
+// has)
 __device__ __forceinline__ bool f4_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   uint32_t ok;
   asm volatile(

@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from ..formats.resident import resident_row_bytes
-from ._lib import check, cuda, raw_stream
+from ._lib import check, cuda, fault_ptr, raw_stream
 from .decode import QWeight, sm_count
 from .gemm import TileTable
 
@@ -133,12 +133,18 @@ def _matrix(name: str, w: QWeight, k: int, index: int) -> int:
     return w.data.data_ptr()
 
 
+def _of_rows(name: str, t: torch.Tensor, dtype, rows: int, index: int) -> int:
+    if t.dtype is not dtype or t.numel() < rows or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"{name}: contiguous {dtype}, {rows} values at least, on the device of the rest")
+    return t.data_ptr()
+
+
 def fp4_gemm(X: Fp4Rows, W: QWeight, tiles: TileTable, *, out_f32: Optional[torch.Tensor] = None,
              out_bf16: Optional[torch.Tensor] = None, W2: Optional[QWeight] = None, dst_row=None, row_scale=None, resid=None,
              status: Optional[torch.Tensor] = None, work: Optional[Fp4Work] = None) -> None:
     """C = X @ W[g].T per token tile, codes by codes on tcgen05 ``kind::mxf4nvf4`` with fp32 sums: ``X`` NVFP4 rows, W (and W2)
     resident NVFP4 matrices [N, bytes] or stacks [G, N, bytes]; tiles of 32, 64 or 128 rows, without W2 of 256 too
-    (:func:`fp4_tile_rows`).  With W2 the output is silu(X W^T) * (X W2^T).  Epilogue options as :func:`gemm.qgemm`.  Block scales are
+    (:func:`fp4_tile_rows`; :func:`fp4_tiles` for one matrix).  With W2 the output is silu(X W^T) * (X W2^T).  Epilogue options as :func:`gemm.qgemm`.  Block scales are
     taken without their sign, which no checkpoint sets (:func:`fp4_supports`)."""
     index, k = X.index, X.k
     wp = _matrix("W", W, k, index)
@@ -159,12 +165,21 @@ def fp4_gemm(X: Fp4Rows, W: QWeight, tiles: TileTable, *, out_f32: Optional[torc
         if resid.dtype is not torch.float32 or resid.shape != out.shape or (resid.stride(1) != 1 and N > 1) or resid.get_device() != index:
             raise ValueError("resid: fp32, shaped like the output")
         rp, ldr = resid.data_ptr(), resid.stride(0)
+    rows = tiles.rows
+    if out.shape[0] > 1 and out.stride(0) < N:
+        raise ValueError("the output's rows lie over each other")
+    if tiles.n_groups > G or tiles.tile_rows not in (32, 64, 128, 256) or (w2p and tiles.tile_rows == 256) or tiles.mtiles.get_device() != index:
+        raise ValueError(f"tiles: of 32, 64 or 128 rows (256 without W2) over at most {G} matrices, on the device of the rest")
+    if rows > X.rows or (dst_row is None and rows > out.shape[0]):
+        raise ValueError(f"the tiles reach {rows} rows")
+    dp = _of_rows("dst_row", dst_row, torch.int32, rows, index) if dst_row is not None else 0
+    fp = _of_rows("row_scale", row_scale, torch.float32, rows, index) if row_scale is not None else 0
+    sp = fault_ptr(status, index) if status is not None else 0
     if index < 0:
         raise ValueError("the kernels need a CUDA device")
     code = _fn("bl_fp4_gemm")(_GEMM.pack(
         X.ptr, wp, w2p, tiles.mtiles.data_ptr(), tiles.n_mtiles.data_ptr(), out.data_ptr() if f32 else 0, 0 if f32 else out.data_ptr(),
-        0 if dst_row is None else dst_row.data_ptr(), 0 if row_scale is None else row_scale.data_ptr(), rp,
-        0 if status is None else status.data_ptr(), raw_stream(index), X.rows, out.stride(0), ldr, G, N, k,
+        dp, fp, rp, sp, raw_stream(index), X.rows, out.stride(0), ldr, G, N, k,
         tiles.fixed or tiles.max_mtiles, tiles.tile_rows, sm_count(), tiles.fixed != 0))
     if code:
         check(code, "bl_fp4_gemm")
@@ -222,11 +237,14 @@ def fp4_moe(x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, gate: QWeight
         if kind != 2 or gain.dtype is not torch.float32 or gain.numel() != H or not gain.is_contiguous() or gain.get_device() != index:
             raise ValueError(f"gain: contiguous fp32 [{H}] beside fp32 rows")
         gain_at = gain.data_ptr()
+    sp = fault_ptr(status, index) if status is not None else 0
+    if T > 1 and (out.stride(0) < H or (resid is not None and resid.stride(0) < H)):
+        raise ValueError("rows lie over each other")
     if index < 0:
         raise ValueError("the kernels need a CUDA device")
     ldx = x.stride(0) if T > 1 else H
     code = _fn("bl_fp4_moe")(_MOE.pack(x.data_ptr(), gain_at, ids.data_ptr(), wts.data_ptr(), *at, work.ptr, rp, out.data_ptr() if f32 else 0,
-                                       0 if f32 else out.data_ptr(), 0 if status is None else status.data_ptr(), raw_stream(index), ldx, ldr,
+                                       0 if f32 else out.data_ptr(), sp, raw_stream(index), ldx, ldr,
                                        out.stride(0), eps, kind, T, k, E, H, I_, work.rows, sm_count()))
     if code:
         check(code, "bl_fp4_moe")

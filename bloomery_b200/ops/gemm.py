@@ -18,6 +18,7 @@ class TileTable:
 
     def __init__(self, max_rows: int, n_groups: int, device, tile_rows: int = BM):
         self.tile_rows = tile_rows
+        self.rows = max_rows                    # rows that the tiles reach at most
         self.max_mtiles = max_rows // tile_rows + n_groups + 1
         self.n_groups = n_groups
         self.mtiles = torch.zeros(self.max_mtiles, 4, dtype=torch.int32, device=device)

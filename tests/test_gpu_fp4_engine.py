@@ -4,6 +4,8 @@ A value in four bits is off by a tenth of itself or so (a step is half of the va
 the block's rms).  A pass of the tiny model has 16 such products on the way of the residual stream, whose errors add up like
 noise: 0.4 of the logits' own size at most, a cosine of 0.92.  The bits of the operators are tested elsewhere; here the passes are
 held to themselves, and to the 16-bit ones within that."""
+import gc
+
 import pytest
 import torch
 
@@ -11,6 +13,13 @@ from test_gpu_fp4 import DEV
 from test_gpu_fp4_moe import oracle
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_engine_left():
+    """Engines hold their prompt paths and those the engines: their graphs must not be taken down while a later test captures one."""
+    yield
+    gc.collect()
 
 
 def engine(n_slots, native=True, seed=3, spec=None):
