@@ -72,19 +72,20 @@ template <int N>
 __device__ __forceinline__ uint32_t fp4_codes(const float* x, float d, float lo, float hi) {
   uint32_t a = fp4_round<N>(x, lo);
   const uint32_t b = fp4_round<N>(x, hi);
-  if (a != b) {
-#pragma unroll 1
-    for (int i = 0; i < N; ++i) {
-      const unsigned c = a >> (4 * i) & 7u;
-      if ((b >> (4 * i) & 7u) != c) {                 // one step above: c < 7
-        const float mid = c < 4 ? 0.5f * (float)c + 0.25f : c == 4 ? 2.5f : c == 5 ? 3.5f : 5.0f;
-        float v = x[0];
+  // 16-bit values meet midpoints often (their quotients are ratios of small numbers): one value at a time, and only those
+  for (uint32_t m = a ^ b; m;) {
+    const int i = (__ffs(m) - 1) >> 2;
+    m &= ~(0xfu << (4 * i));
+    const unsigned c = a >> (4 * i) & 7u;             // b's is one step above: c < 7
+    float v[N];
 #pragma unroll
-        for (int j = 1; j < N; ++j) v = i == j ? x[j] : v;
-        const float r = fmaf(-mid, d, fabsf(v));
-        if (r > 0.0f || (r == 0.0f && (c & 1))) a += 1u << (4 * i);
-      }
-    }
+    for (int j = 0; j < N; ++j) v[j] = x[j];
+#pragma unroll
+    for (int n = N / 2; n > 0; n /= 2)
+#pragma unroll
+      for (int j = 0; j < n; ++j) v[j] = i & n ? v[j + n] : v[j];
+    const float mid = c < 4 ? 0.5f * (float)c + 0.25f : c == 4 ? 2.5f : c == 5 ? 3.5f : 5.0f, r = fmaf(-mid, d, fabsf(v[0]));
+    if (r > 0.0f || (r == 0.0f && (c & 1))) a += 1u << (4 * i);
   }
   return a;
 }
