@@ -48,7 +48,7 @@ struct F4Shape {
   static constexpr int RAWS = RAWS_;                               // slots of scales
   static constexpr int WARPS = WARPS_, THREADS = F4_EPILOGUE + 32 * WARPS, BN = BN_, AR = AR_;
   static constexpr int MATS = DUAL ? 2 : 1;
-  static constexpr int FEW = BN / 4;                               // rows of the smaller box of tokens
+  static constexpr int FEW = BN > 32 ? BN / 4 : BN;                // rows of the smaller box of tokens
   static constexpr int SPAN = DUAL || BN > 128 ? 2 : 4;
   static constexpr int A_BYTES = AR * 128, B = MATS * A_BYTES;
   static constexpr int B_CELLS = BN > 128 ? 8 : 4;                 // columns of an instruction's token scales
@@ -251,7 +251,8 @@ __device__ __forceinline__ void f4_cells(uint8_t* smem, F4Bars<S>& bar, Tiles& t
 template <class S>
 static int f4_maps(F4Maps* m, const void* x, long rows_x, const void* w, const void* w2, int K, int N, int groups) {
   int rc = fp4_maps(&m->x, &m->xs, x, K, rows_x, 1, S::BN, S::SPAN);
-  if (!rc) rc = fp4_maps(&m->few, &m->fews, x, K, rows_x, 1, S::FEW, S::SPAN);
+  m->few = m->x; m->fews = m->xs;
+  if (!rc && S::FEW < S::BN) rc = fp4_maps(&m->few, &m->fews, x, K, rows_x, 1, S::FEW, S::SPAN);
   if (!rc) rc = fp4_maps(&m->w, &m->ws, w, K, N, groups, S::AR, S::SPAN);
   m->w2 = m->w; m->ws2 = m->ws;
   if (!rc && S::DUAL) rc = fp4_maps(&m->w2, &m->ws2, w2, K, N, groups, S::AR, S::SPAN);

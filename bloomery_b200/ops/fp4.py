@@ -22,6 +22,7 @@ _ROWS, _GEMM, _MOE = struct.Struct("6P2ld4i"), struct.Struct("12P3l7i4x"), struc
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_K = 32768                                             # values of a row that fp4_rows holds in registers
 _entries: dict = {}
+_processors: dict = {}
 
 
 def _fn(name):
@@ -32,12 +33,11 @@ def _fn(name):
     return fn
 
 
-def _index(device) -> int:
-    """The device's number as ``Tensor.get_device`` says it."""
-    device = torch.device(device)
-    if device.type != "cuda":
-        return -1
-    return torch.cuda.current_device() if device.index is None else device.index
+def _sms(index: int) -> int:
+    n = _processors.get(index)
+    if n is None:
+        n = _processors[index] = sm_count(torch.device("cuda", index))
+    return n
 
 
 class Fp4Rows:
@@ -168,7 +168,7 @@ def fp4_gemm(X: Fp4Rows, W: QWeight, tiles: TileTable, *, out_f32: Optional[torc
     rows = tiles.rows
     if out.shape[0] > 1 and out.stride(0) < N:
         raise ValueError("the output's rows lie over each other")
-    if tiles.n_groups > G or tiles.tile_rows not in (32, 64, 128, 256) or (w2p and tiles.tile_rows == 256) or tiles.mtiles.get_device() != index:
+    if tiles.n_groups > G or tiles.tile_rows not in (32, 64, 128, 256) or (w2p and tiles.tile_rows == 256) or tiles.index != index:
         raise ValueError(f"tiles: of 32, 64 or 128 rows (256 without W2) over at most {G} matrices, on the device of the rest")
     if rows > X.rows or (dst_row is None and rows > out.shape[0]):
         raise ValueError(f"the tiles reach {rows} rows")
@@ -178,9 +178,9 @@ def fp4_gemm(X: Fp4Rows, W: QWeight, tiles: TileTable, *, out_f32: Optional[torc
     if index < 0:
         raise ValueError("the kernels need a CUDA device")
     code = _fn("bl_fp4_gemm")(_GEMM.pack(
-        X.ptr, wp, w2p, tiles.mtiles.data_ptr(), tiles.n_mtiles.data_ptr(), out.data_ptr() if f32 else 0, 0 if f32 else out.data_ptr(),
+        X.ptr, wp, w2p, tiles.mtiles_ptr, tiles.n_mtiles_ptr, out.data_ptr() if f32 else 0, 0 if f32 else out.data_ptr(),
         dp, fp, rp, sp, raw_stream(index), X.rows, out.stride(0), ldr, G, N, k,
-        tiles.fixed or tiles.max_mtiles, tiles.tile_rows, sm_count(), tiles.fixed != 0))
+        tiles.fixed or tiles.max_mtiles, tiles.tile_rows, _sms(index), tiles.fixed != 0))
     if code:
         check(code, "bl_fp4_gemm")
 
@@ -245,6 +245,6 @@ def fp4_moe(x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, gate: QWeight
     ldx = x.stride(0) if T > 1 else H
     code = _fn("bl_fp4_moe")(_MOE.pack(x.data_ptr(), gain_at, ids.data_ptr(), wts.data_ptr(), *at, work.ptr, rp, out.data_ptr() if f32 else 0,
                                        0 if f32 else out.data_ptr(), sp, raw_stream(index), ldx, ldr,
-                                       out.stride(0), eps, kind, T, k, E, H, I_, work.rows, sm_count()))
+                                       out.stride(0), eps, kind, T, k, E, H, I_, work.rows, _sms(index)))
     if code:
         check(code, "bl_fp4_moe")

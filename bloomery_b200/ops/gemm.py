@@ -2,6 +2,7 @@
 (``csrc/prefill_aux.cu``)."""
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import torch
@@ -23,6 +24,7 @@ class TileTable:
         self.n_groups = n_groups
         self.mtiles = torch.zeros(self.max_mtiles, 4, dtype=torch.int32, device=device)
         self.n_mtiles = torch.zeros(1, dtype=torch.int32, device=device)
+        self.mtiles_ptr, self.n_mtiles_ptr, self.index = self.mtiles.data_ptr(), self.n_mtiles.data_ptr(), self.mtiles.get_device()
         self.offsets = torch.zeros(n_groups + 1, dtype=torch.int32, device=device)
         self.fixed = 0                          # number of tiles when the host wrote the table once and for all
 
@@ -186,15 +188,24 @@ def localize_ids(ids: torch.Tensor, e_lo: int, e_hi: int, out: torch.Tensor) -> 
     check(cuda().bl_localize_ids(p(ids), I(ids.numel()), I(e_lo), I(e_hi), p(out), stream()), "bl_localize_ids")
 
 
+_dequant = None
+
+
 def dequant_bf16(w: QWeight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Expand a resident quantised weight (matrix or stack) to bf16 [..., rows, K]."""
-    lead = w.data.shape[:-1]
-    rows = 1
-    for d in lead:
-        rows *= d
+    data, k = w.data, w.k
     if out is None:
-        out = torch.empty(*lead, w.k, dtype=torch.bfloat16, device=w.data.device)
-    check(cuda().bl_dequant_bf16(p(w.data), I(w.wt), L(rows), I(w.k), p(out), stream()), "bl_dequant_bf16")
+        out = torch.empty(*data.shape[:-1], k, dtype=torch.bfloat16, device=data.device)
+    rows = 1
+    for d in data.shape[:-1]:
+        rows *= d
+    global _dequant
+    if _dequant is None:
+        _dequant = cuda().bl_dequant_bf16
+        _dequant.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]
+    code = _dequant(data.data_ptr(), w.wt, rows, k, out.data_ptr(), torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+    if code:
+        check(code, "bl_dequant_bf16")
     return out
 
 
