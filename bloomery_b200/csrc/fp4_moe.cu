@@ -270,13 +270,15 @@ __device__ __forceinline__ void fm_rows_stored(uint64_t* bar) {
 // The tokens' rows that other CTAs store, read by TMA: whether all are there; gives up after the limit of all waits.
 __device__ __forceinline__ bool fm_tokens_ready(const FmArgs& a, volatile int* abort_flag) {
   unsigned long long t0 = 0;
-  for (;;) {
+  for (uint32_t it = 0;; ++it) {
     int done;
     asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(done) : "l"(a.claim + 1) : "memory");
     if (done >= a.T) break;
-    const unsigned long long now = globaltimer();
-    if (t0 == 0) t0 = now;
-    else if (now - t0 > WAIT_LIMIT_NS) { *abort_flag = 1; return false; }
+    if ((it & 63) == 63) {                          // the timer takes longer than a look at the word
+      const unsigned long long now = globaltimer();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > WAIT_LIMIT_NS) { *abort_flag = 1; return false; }
+    }
   }
   asm volatile("fence.proxy.async;" ::: "memory");
   return true;

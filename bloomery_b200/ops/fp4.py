@@ -40,6 +40,10 @@ def _sms(index: int) -> int:
     return n
 
 
+class RowsAsWeight(QWeight):
+    """Rows that a launch in flight may still be writing, where weights are there before: a product waits before it reads them."""
+
+
 class Fp4Rows:
     """Buffer of ``rows`` NVFP4 rows of ``k`` values."""
 
@@ -53,7 +57,7 @@ class Fp4Rows:
     @property
     def weight(self) -> QWeight:
         """The rows as a resident NVFP4 matrix (what expands or dots one takes them too)."""
-        return QWeight(self.data, "NVFP4", self.k)
+        return RowsAsWeight(self.data, "NVFP4", self.k)
 
 
 def fp4_tile_rows(rows: int, groups: int = 1, gated: bool = False) -> int:
@@ -71,7 +75,8 @@ def fp4_rows(x: torch.Tensor, out: Fp4Rows, *, gain: Optional[torch.Tensor] = No
              tensor_scale: Optional[torch.Tensor] = None, pos_of: Optional[torch.Tensor] = None) -> None:
     """NVFP4 rows of ``x`` [M, k] (bf16, f16 or fp32; rows may be strided) in the first M rows of ``out``.
 
-    A row's scale takes its largest magnitude to 6 x 448 (or is ``tensor_scale``, one fp32 on the device; larger values saturate), a
+    A row's scale takes its largest magnitude to 6 x 448 (or is ``tensor_scale``, one positive fp32 on the
+    device; larger values saturate), a
     block's scale takes its own to 6; scales and codes are the nearest, ties go to the even code.  A row with a NaN or an
     infinity becomes one whose products are all NaN.  ``gain`` fp32 [k] (fp32 rows): RMSNorm first.  ``pos_of`` int32 [M * copies]:
     row m goes to the rows ``pos_of[m * copies + j]`` of ``out`` (none where that is negative or past the end), as ``moe_plan``
@@ -83,7 +88,7 @@ def fp4_rows(x: torch.Tensor, out: Fp4Rows, *, gain: Optional[torch.Tensor] = No
     M = x.shape[0]
     copies, at = 1, 0
     if pos_of is not None:
-        copies, rest = divmod(pos_of.numel(), M) if M else (0, 0)
+        copies, rest = divmod(pos_of.numel(), M) if M else (1, pos_of.numel())
         if pos_of.dtype is not torch.int32 or not pos_of.is_contiguous() or rest or copies < 1 or pos_of.get_device() != index:
             raise ValueError("pos_of: contiguous int32, as many places for every row, on the device of the rest")
         at = pos_of.data_ptr()
@@ -180,7 +185,8 @@ def fp4_gemm(X: Fp4Rows, W: QWeight, tiles: TileTable, *, out_f32: Optional[torc
     code = _fn("bl_fp4_gemm")(_GEMM.pack(
         X.ptr, wp, w2p, tiles.mtiles_ptr, tiles.n_mtiles_ptr, out.data_ptr() if f32 else 0, 0 if f32 else out.data_ptr(),
         dp, fp, rp, sp, raw_stream(index), X.rows, out.stride(0), ldr, G, N, k,
-        tiles.fixed or tiles.max_mtiles, tiles.tile_rows, _sms(index), tiles.fixed != 0))
+        tiles.fixed or tiles.max_mtiles, tiles.tile_rows, _sms(index),
+        tiles.fixed != 0 and type(W) is QWeight and (W2 is None or type(W2) is QWeight)))
     if code:
         check(code, "bl_fp4_gemm")
 

@@ -253,3 +253,80 @@ def test_gated_and_scattered_products_of_experts(T, E, k, inter, H, tile_rows):
         off = (out[i].double().cpu() - f * (v @ dv[e].T)[0]).abs()
         assert bool((off <= f * allowed(v, dv[e], H)[0] + 1e-30).all())
     assert int(status) == 0
+
+
+@gpu
+def test_rows_times_rows_made_right_before():
+    """Both sides of a product out of the launches in front of it, again and again: it reads none of them before they are written."""
+    from bloomery_b200.ops.fp4 import Fp4Rows, fp4_gemm, fp4_rows, fp4_tiles
+    M, N, K = 20, 300, 2048
+    tiles, a, b = fp4_tiles(M, DEV), Fp4Rows(M, K, DEV), Fp4Rows(N, K, DEV)
+    xs = [make(M, K, seed=s) for s in range(3)]
+    ys = [make(N, K, seed=10 + s) for s in range(3)]
+    outs = [torch.empty(M, N, device=DEV) for _ in range(12)]
+    for i, out in enumerate(outs):
+        fp4_rows(xs[i % 3], a)
+        fp4_rows(ys[(i * 2) % 3], b)
+        fp4_gemm(a, b.weight, tiles, out_f32=out)
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        xv, yv = quantised(xs[i % 3])[3], quantised(ys[(i * 2) % 3])[3]
+        off = (out.double().cpu() - xv @ yv.T).abs()
+        assert bool((off <= allowed(xv, yv, K)).all()), i
+
+
+@gpu
+def test_no_rows_and_no_tiles():
+    from bloomery_b200.ops.fp4 import Fp4Rows, fp4_gemm, fp4_rows
+    rows = Fp4Rows(8, 128, DEV)
+    rows.data.fill_(0x55)
+    fp4_rows(torch.zeros(0, 128, device=DEV), rows)
+    fp4_rows(torch.zeros(0, 128, device=DEV), rows, pos_of=torch.zeros(0, dtype=torch.int32, device=DEV))
+    assert bool((rows.data == 0x55).all())
+    ids, wts, tiles, pos_of, dst_row, row_scale = plan(4, 5, 2, 32, 1, elsewhere=8)          # every slot is another tier's
+    fp4_rows(make(4, 128), rows, pos_of=pos_of)
+    assert bool((rows.data == 0x55).all())
+    w, _ = weight(64, 128, 1, 5)
+    out = torch.full((8, 64), 3.0, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    fp4_gemm(rows, w, tiles, out_f32=out, dst_row=dst_row, status=status)
+    assert (out == 3).all() and int(status) == 0
+
+
+@gpu
+def test_products_in_place_on_streams_and_in_graphs():
+    """The residual stream as addend and output; a captured pair replayed with other rows; two streams at once."""
+    from bloomery_b200.ops.fp4 import Fp4Rows, fp4_gemm, fp4_rows, fp4_tiles
+    M, N, K = 48, 512, 1024
+    w, wv = weight(N, K, seed=4)
+    x, tiles = make(M, K, seed=6), fp4_tiles(M, DEV)
+    rows, y = Fp4Rows(M, K, DEV), torch.randn(M, N, device=DEV)
+    y0 = y.clone()
+    fp4_rows(x, rows)
+    fp4_gemm(rows, w, tiles, out_f32=y, resid=y)
+    xv = quantised(x)[3]
+    off = (y.double().cpu() - (xv @ wv.T + y0.double().cpu())).abs()
+    assert bool((off <= allowed(xv, wv, K) + 2.0 ** -23 * y.double().cpu().abs()).all())
+    out = torch.empty(M, N, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fp4_rows(x, rows)
+        fp4_gemm(rows, w, tiles, out_f32=out)
+    other = make(M, K, seed=7)
+    x.copy_(other)
+    graph.replay()
+    ref, rows2 = torch.empty(M, N, device=DEV), Fp4Rows(M, K, DEV)
+    fp4_rows(other, rows2)
+    fp4_gemm(rows2, w, tiles, out_f32=ref)
+    torch.cuda.synchronize()
+    assert torch.equal(out, ref)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs, bufs = [torch.empty(M, N, device=DEV) for _ in streams], [Fp4Rows(M, K, DEV) for _ in streams]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, o, b in zip(streams, outs, bufs):
+            with torch.cuda.stream(s):
+                fp4_rows(other, b)
+                fp4_gemm(b, w, tiles, out_f32=o)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, ref) for o in outs)

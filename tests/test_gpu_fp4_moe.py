@@ -61,7 +61,7 @@ def run(x, ids, wts, g, u, d, work=None, **kw):
 @gpu
 @pytest.mark.parametrize("T,E,k,inter,H,away", [(1, 16, 4, 256, 512, 0), (5, 16, 4, 256, 512, 6), (32, 16, 4, 192, 320, 0), (33, 7, 3, 128, 1024, 20),
                                                 (64, 24, 8, 320, 576, 0), (64, 3, 2, 64, 64, 5), (2, 130, 16, 64, 192, 0), (9, 4, 1, 2112, 2048, 1),
-                                                (3, 4, 2, 64, 192, 6)])
+                                                (3, 4, 2, 64, 192, 6), (64, 512, 16, 64, 64, 100), (7, 2, 2, 64, 8192, 0), (4, 3, 1, 8192, 64, 0)])
 def test_tokens_through_their_experts(T, E, k, inter, H, away):
     c = case(T, E, k, inter, H, seed=T, away=away)
     out = torch.full((T + 1, H + 4), 5.0, device=DEV)
@@ -152,3 +152,21 @@ def test_calls_on_two_streams_and_in_graphs():
     ref = torch.empty(40, 512, device=DEV)
     fp4_moe(x, ids, wts, *on[0][3:], Fp4MoeWork(40, 8, 512, 256, 64, DEV), out_f32=ref)
     assert torch.equal(outs[0], ref) and torch.equal(outs[1], ref)
+
+
+@gpu
+def test_a_wait_that_runs_out_is_reported():
+    """Rows that are said to be taken and never come: the launch gives up after its limit, says so and leaves the card as it was."""
+    from bloomery_b200.ops.fp4 import Fp4MoeWork, fp4_moe
+    c = case(8, 16, 4, 256, 512, seed=4)
+    args = (c[0], c[1].to(DEV), c[2].to(DEV), c[3][0], c[4][0], c[5][0])
+    want, out = torch.empty(8, 512, device=DEV), torch.empty(8, 512, device=DEV)
+    work, status = Fp4MoeWork(8, 4, 512, 256, 16, DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    fp4_moe(*args, work, out_f32=want, status=status)
+    assert int(status) == 0
+    work.data[:4].view(torch.int32).fill_(8)
+    fp4_moe(*args, work, out_f32=out, status=status)
+    assert int(status) == 1
+    status.zero_()
+    fp4_moe(*args, Fp4MoeWork(8, 4, 512, 256, 16, DEV), out_f32=out, status=status)
+    assert int(status) == 0 and torch.equal(out, want)
