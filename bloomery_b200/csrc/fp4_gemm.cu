@@ -13,7 +13,7 @@
 
 namespace bl {
 
-constexpr int F4_GEMM_ROOM = 190 * 1024, F4_GEMM_WARPS = 8;
+constexpr int F4_GEMM_ROOM = 200 * 1024, F4_GEMM_WARPS = 8;
 
 struct F4Tile { int group, row0, row_end, pad; };
 

@@ -49,7 +49,7 @@ struct F4Shape {
   static constexpr int WARPS = WARPS_, THREADS = F4_EPILOGUE + 32 * WARPS, BN = BN_, AR = AR_;
   static constexpr int MATS = DUAL ? 2 : 1;
   static constexpr int FEW = BN > 32 ? BN / 4 : BN;                // rows of the smaller box of tokens
-  static constexpr int SPAN = DUAL || BN > 128 ? 2 : 4;
+  static constexpr int SPAN = DUAL ? 2 : 4;
   static constexpr int A_BYTES = AR * 128, B = MATS * A_BYTES;
   static constexpr int B_CELLS = BN > 128 ? 8 : 4;                 // columns of an instruction's token scales
   static constexpr int STAGE = B + BN * 128;
