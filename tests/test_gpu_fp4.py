@@ -330,3 +330,30 @@ def test_products_in_place_on_streams_and_in_graphs():
                 fp4_gemm(b, w, tiles, out_f32=o)
     torch.cuda.synchronize()
     assert all(torch.equal(o, ref) for o in outs)
+
+
+@gpu
+@pytest.mark.parametrize("rows,K", [(1, 64), (37, 320), (9, 4096)])
+def test_expansion_of_every_code_and_scale(rows, K):
+    """Exact: fp32(E4M3 * g / 2) times the doubled code, rounded once; negative, zero, infinite and NaN scales among them.  The halving takes
+    no rounding of its own (E4M3 * g / 2 has 28 bits, exact in 64): twice as much may pass fp32's largest value where the half does not."""
+    from bloomery_b200.ops.gemm import dequant_bf16
+
+    gen = torch.Generator().manual_seed(K)
+    codes = torch.randint(0, 16, (rows, K), generator=gen)
+    sc = torch.randint(0, 256, (rows, K // 16), generator=gen, dtype=torch.uint8)
+    g = torch.randn(rows, generator=gen) * 1e-3
+    odd = torch.tensor([0.0, -0.0, 1e-40, 3e38, math.inf, -math.inf, math.nan, -1.0])
+    g[:min(rows - 1, 8)] = odd[:min(rows - 1, 8)]
+    data = torch.zeros(rows, (K // 2 + K // 16 + 4 + 15) // 16 * 16, dtype=torch.uint8)
+    data[:, :K // 2] = (codes[:, ::2] | codes[:, 1::2] << 4).to(torch.uint8)
+    data[:, K // 2:K // 2 + K // 16] = sc
+    data[:, K // 2 + K // 16:K // 2 + K // 16 + 4] = g.view(rows, 1).view(torch.uint8)
+    out = torch.empty(rows, K, dtype=torch.bfloat16, device=DEV)
+    dequant_bf16(QWeight(data.to(DEV), "NVFP4", K), out)
+    doubled = torch.tensor([int(2 * v) for v in E2M1] + [-int(2 * v) for v in E2M1]).float()
+    step = (planes.e4m3_decode(sc).double() * g[:, None].double() * 0.5).float()
+    want = (step.repeat_interleave(16, 1) * doubled[codes]).to(torch.bfloat16)
+    nan = want.isnan()
+    assert torch.equal(out.cpu().isnan(), nan)
+    assert torch.equal(out.cpu()[~nan].view(torch.int16), want[~nan].view(torch.int16))
