@@ -34,6 +34,7 @@ struct F4Args {
   const float* resid;
   long ldr;
   unsigned* status;
+  int rows_out;             // of the output: others are none
   int wide;                 // rows of the output (and of resid) start at 16 bytes and hold whole 16 bytes
 };
 
@@ -177,7 +178,7 @@ fp4_gemm_kernel(const __grid_constant__ F4Maps map, const F4Args a) {
       w1 = w2;
       const float ws = nxt.ws, ws2 = nxt.ws2;
       if (et < BN) {
-        s_row[i & 1][et] = nxt.row;
+        s_row[i & 1][et] = nxt.row < a.rows_out ? nxt.row : -1;           // here, where it has arrived
         s_xs[i & 1][et] = DUAL ? nxt.xs : nxt.xs * nxt.factor;
         if (DUAL) s_factor[i & 1][et] = nxt.factor;
       }
@@ -226,7 +227,7 @@ struct Fp4GemmCall {
   const void* x; const void* w; const void* w2; const void* tiles; const int* n_tiles; float* c_f32; void* c_bf16;
   const int* dst_row; const float* row_scale; const float* resid; unsigned* status; cudaStream_t stream;
   long rows_x, ldc, ldr;
-  int n_groups, N, K, max_tiles, tile_rows, sms, fixed;
+  int n_groups, N, K, max_tiles, tile_rows, sms, fixed, rows_out;
 };
 
 namespace bl {
@@ -251,6 +252,7 @@ static int fp4_gemm_go(const Fp4GemmCall& c, F4Args& a) {
 
 extern "C" {
 
+// Rows of C from 0 to rows_out - 1, others nowhere:
 // C[dst_row[t] or t, n] = row_scale[t] * sum_k X[t, k] W[g][n, k] (+ resid) per token tile of the table, of at most tile_rows (32, 64,
 // 128, with one matrix 256) rows.  X [rows_x], W and W2 [n_groups, N] NVFP4 rows of K values; exactly one of c_f32 / c_bf16;
 // fixed: the table has exactly max_tiles tiles, and no launch in flight writes it or the weights.
@@ -268,7 +270,7 @@ int bl_fp4_gemm(const Fp4GemmCall* c) {
   a.x = (const uint8_t*)c->x; a.w = (const uint8_t*)c->w; a.w2 = (const uint8_t*)c->w2;
   a.row_bytes = fp4_row_bytes(c->K); a.group_bytes = a.row_bytes * c->N;
   a.c_f32 = c->c_f32; a.c_bf16 = (__nv_bfloat16*)c->c_bf16; a.ldc = c->ldc;
-  a.dst_row = c->dst_row; a.row_scale = c->row_scale; a.resid = c->resid; a.ldr = c->ldr; a.status = c->status;
+  a.dst_row = c->dst_row; a.row_scale = c->row_scale; a.resid = c->resid; a.ldr = c->ldr; a.status = c->status; a.rows_out = c->rows_out;
   const int es = c->c_f32 ? 4 : 2;
   a.wide = (((uintptr_t)c->c_f32 | (uintptr_t)c->c_bf16 | (uintptr_t)c->resid) & 15) == 0 && c->ldc * es % 16 == 0 && (!c->resid || c->ldr % 4 == 0) &&
            c->N % (c->c_f32 || c->resid ? 4 : 8) == 0;

@@ -18,7 +18,7 @@ from ._lib import check, cuda, fault_ptr, raw_stream
 from .decode import QWeight, sm_count
 from .gemm import TileTable
 
-_ROWS, _GEMM, _MOE = struct.Struct("6P2ld4i"), struct.Struct("12P3l7i4x"), struct.Struct("13P3ld8i")      # Fp4RowsCall, Fp4GemmCall, Fp4MoeCall
+_ROWS, _GEMM, _MOE = struct.Struct("6P2ld4i"), struct.Struct("12P3l8i"), struct.Struct("13P3ld8i")      # Fp4RowsCall, Fp4GemmCall, Fp4MoeCall
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_K = 32768                                             # values of a row that fp4_rows holds in registers
 _entries: dict = {}
@@ -149,7 +149,8 @@ def fp4_gemm(X: Fp4Rows, W: QWeight, tiles: TileTable, *, out_f32: Optional[torc
              status: Optional[torch.Tensor] = None, work: Optional[Fp4Work] = None) -> None:
     """C = X @ W[g].T per token tile, codes by codes on tcgen05 ``kind::mxf4nvf4`` with fp32 sums: ``X`` NVFP4 rows, W (and W2)
     resident NVFP4 matrices [N, bytes] or stacks [G, N, bytes]; tiles of 32, 64 or 128 rows, without W2 of 256 too
-    (:func:`fp4_tile_rows`; :func:`fp4_tiles` for one matrix).  With W2 the output is silu(X W^T) * (X W2^T).  Epilogue options as :func:`gemm.qgemm`.  Block scales are
+    (:func:`fp4_tile_rows`; :func:`fp4_tiles` for one matrix).  With W2 the output is silu(X W^T) * (X W2^T).  Epilogue options as :func:`gemm.qgemm`; a row
+    that ``dst_row`` sends below 0 or past the output goes nowhere.  Block scales are
     taken without their sign, which no checkpoint sets (:func:`fp4_supports`)."""
     index, k = X.index, X.k
     wp = _matrix("W", W, k, index)
@@ -186,7 +187,7 @@ def fp4_gemm(X: Fp4Rows, W: QWeight, tiles: TileTable, *, out_f32: Optional[torc
         X.ptr, wp, w2p, tiles.mtiles_ptr, tiles.n_mtiles_ptr, out.data_ptr() if f32 else 0, 0 if f32 else out.data_ptr(),
         dp, fp, rp, sp, raw_stream(index), X.rows, out.stride(0), ldr, G, N, k,
         tiles.fixed or tiles.max_mtiles, tiles.tile_rows, _sms(index),
-        tiles.fixed != 0 and type(W) is QWeight and (W2 is None or type(W2) is QWeight)))
+        tiles.fixed != 0 and type(W) is QWeight and (W2 is None or type(W2) is QWeight), min(out.shape[0], 2 ** 31 - 1)))
     if code:
         check(code, "bl_fp4_gemm")
 

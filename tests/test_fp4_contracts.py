@@ -35,7 +35,7 @@ def test_rows_are_refused_before_they_are_launched():
 
 
 def gemm(x=A, w=A, w2=0, f32=A, bf16=0, rows_x=64, ldc=256, groups=1, N=256, K=1024, tiles=4, tile_rows=32, sms=148):
-    return call("bl_fp4_gemm", Q._GEMM.pack(x, w, w2, A, A, f32, bf16, 0, 0, 0, 0, 0, rows_x, ldc, 0, groups, N, K, tiles, tile_rows, sms, 0))
+    return call("bl_fp4_gemm", Q._GEMM.pack(x, w, w2, A, A, f32, bf16, 0, 0, 0, 0, 0, rows_x, ldc, 0, groups, N, K, tiles, tile_rows, sms, 0, 0))
 
 
 def test_products_are_refused_before_they_are_launched():

@@ -357,3 +357,29 @@ def test_expansion_of_every_code_and_scale(rows, K):
     nan = want.isnan()
     assert torch.equal(out.cpu().isnan(), nan)
     assert torch.equal(out.cpu()[~nan].view(torch.int16), want[~nan].view(torch.int16))
+
+
+@gpu
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("M,N,K", [(5, 24, 128), (40, 130, 320), (300, 136, 64)])
+def test_rows_sent_past_the_output_go_nowhere(M, N, K, f32):
+    """A third of the rows below 0, a third past the end; the rest as without the sending, bit for bit."""
+    from bloomery_b200.ops.fp4 import Fp4Rows, fp4_gemm, fp4_rows, fp4_tiles
+    rows, (w, _) = Fp4Rows(M, K, DEV), weight(N, K, 4)
+    fp4_rows(make(M, K, seed=3), rows)
+    dtype = torch.float32 if f32 else torch.bfloat16
+    kw = lambda t: dict(out_f32=t) if f32 else dict(out_bf16=t)
+    plain, whole = torch.empty(M, N, dtype=dtype, device=DEV), torch.full((2 * M, N), 3.0, dtype=dtype, device=DEV)
+    fp4_gemm(rows, w, fp4_tiles(M, DEV), **kw(plain))
+    dst = torch.arange(M, dtype=torch.int32)
+    dst[1::3], dst[2::3] = -1 - dst[1::3], M + dst[2::3] % 7
+    dst[2] = 2 ** 31 - 1
+    resid = torch.zeros(M, N, device=DEV)
+    fp4_gemm(rows, w, fp4_tiles(M, DEV), **kw(whole[:M]), dst_row=dst.to(DEV))
+    assert torch.equal(whole[0:M:3], plain[::3])
+    whole[0:M:3] = 3.0
+    assert (whole == 3).all()
+    fp4_gemm(rows, w, fp4_tiles(M, DEV), **kw(whole[:M]), dst_row=dst.to(DEV), resid=resid)
+    assert torch.equal(whole[0:M:3], plain[::3])
+    whole[0:M:3] = 3.0
+    assert (whole == 3).all()
