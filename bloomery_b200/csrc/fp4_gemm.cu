@@ -43,10 +43,12 @@ struct F4GemmTiles {
   const F4Args& a;
   int total, kblocks;
   __device__ __forceinline__ int count() const { return total > (int)blockIdx.x ? (total - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0; }
+  __device__ __forceinline__ F4Work work(const F4Tile& mt, int column) const {
+    return F4Work{mt.group, column * AR, mt.row0, min(a.tile_rows, mt.row_end - mt.row0), 0, kblocks};
+  }
   __device__ __forceinline__ F4Work at(int i) const {
     const int t = (int)blockIdx.x + i * (int)gridDim.x;
-    const F4Tile mt = a.tiles[t / a.tiles_w];
-    return F4Work{mt.group, t % a.tiles_w * AR, mt.row0, min(a.tile_rows, mt.row_end - mt.row0), 0, kblocks};
+    return work(a.tiles[t / a.tiles_w], t % a.tiles_w);
   }
 };
 
@@ -155,7 +157,8 @@ fp4_gemm_kernel(const __grid_constant__ F4Maps map, const F4Args a) {
     const int n_tiles = tiles.count();
     const long scale_at = a.K / 2 + a.K / 16;
     // What a tile needs beside its products is asked for while the tile before is worked on, a token a thread, and laid down in shared
-    // memory behind it; the entry of the table a tile earlier.
+    // memory behind it; the entry of the table a tile earlier.  Where K is short these warps are what a tile waits for: the entry is not looked
+    // into before it is used, and the places of the tiles are walked without divisions (down of 4,096 ids 98.8 -> 96.2 us).
     struct Beside { int row; float xs, factor, ws, ws2; } nxt{};
     auto open = [&](const F4Work& w) {
       const int r = w.row0 + et;
@@ -170,12 +173,23 @@ fp4_gemm_kernel(const __grid_constant__ F4Maps map, const F4Args a) {
       if (DUAL) nxt.ws2 = *reinterpret_cast<const float*>(a.w2 + at);
     };
     uint32_t ab = 0, aphase = 0;
-    F4Work w{}, w1{}, w2{};                                        // this tile, the next one and the one behind it
+    F4Work w{}, w1{};                                              // this tile and the next one, behind it an entry and its column
+    F4Tile t2{};
+    int c2 = 0;
     if (n_tiles > 0) { w1 = tiles.at(0); open(w1); }
-    if (n_tiles > 1) w2 = tiles.at(1);
+    const int m_step = (int)gridDim.x / a.tiles_w, c_step = (int)gridDim.x % a.tiles_w;
+    int m = (int)blockIdx.x / a.tiles_w, c = (int)blockIdx.x % a.tiles_w;
+    auto ask = [&]() {                                             // the entry of the tile one further
+      m += m_step;
+      c += c_step;
+      if (c >= a.tiles_w) { c -= a.tiles_w; ++m; }
+      t2 = a.tiles[m];
+      c2 = c;
+    };
+    if (n_tiles > 1) ask();
     for (int i = 0; i < n_tiles; ++i) {
       w = w1;
-      w1 = w2;
+      if (i + 1 < n_tiles) w1 = tiles.work(t2, c2);
       const float ws = nxt.ws, ws2 = nxt.ws2;
       if (et < BN) {
         s_row[i & 1][et] = nxt.row < a.rows_out ? nxt.row : -1;           // here, where it has arrived
@@ -183,7 +197,7 @@ fp4_gemm_kernel(const __grid_constant__ F4Maps map, const F4Args a) {
         if (DUAL) s_factor[i & 1][et] = nxt.factor;
       }
       if (i + 1 < n_tiles) open(w1);
-      if (i + 2 < n_tiles) w2 = tiles.at(i + 2);
+      if (i + 2 < n_tiles) ask();
       if (!f4_all<F4_GEMM_WARPS>(mbar_wait_warp(&bar.acc_full[ab], aphase, &bar.abort))) break;
       tc_fence_after();
       const uint32_t tbase = bar.tmem + ((uint32_t)(q * 32) << 16) + ab * (S::MATS * BN);
