@@ -8,6 +8,9 @@
 // add in fp32.  Eight epilogue warps apply the two fp32 scales.
 //   * "dual" mode runs gate and up in one main loop; the epilogue writes silu(gate) * up;
 //   * the epilogue scatters and scales like the other GEMMs (dst_row / row_scale / resid).
+// 4,096 tokens x 8,192 x 4,096: 100 us (2.75 PFLOP/s), bound by TMA's way from L2 (85 without an epilogue); gate and up of 2,000 ids on 128
+// experts of 768 x 2,048: 63 us (249 MB, 4.0 TB/s; 54 without an epilogue, which one accumulator of each matrix leaves no room to
+// overlap); down of 4,096 ids: 96 us, of which the stores of 268 MB are 20.
 // Every wait is bounded; on expiry the CTA raises status word 1, leaves its loops, frees its TMEM and returns.
 #include "fp4_pipe.cuh"
 
