@@ -182,7 +182,8 @@ struct FmDownTiles : FmShare {                      // columns after columns
 };
 
 // A token's row in NVFP4, by the 128 threads of the epilogue warps.  It is run once or twice by a CTA: what counts is little code, which is
-// fetched as it runs, so a thread walks its blocks of 16 three times instead of keeping them.
+// fetched as it runs, so a thread walks its blocks of 16 three times instead of keeping them.  s_sum and s_max are read behind its last
+// meeting: the threads meet once more before another row.
 __device__ __forceinline__ void fm_token(const FmArgs& a, int t, uint8_t* row, double* s_sum, unsigned* s_max) {
   const int et = threadIdx.x - F4_EPILOGUE, lane = et & 31, w = et >> 5, blocks = a.H / 16;
   float v[16], r = 1.0f;
@@ -333,7 +334,10 @@ __global__ void __launch_bounds__(FM_THREADS, 1) fp4_moe_up_kernel(const __grid_
     fm_plan_made();
   } else {
     if (FEW) {
-      for (int t = 0; t < a.T; ++t) fm_token(a, t, a.xq + (row0 + t) * x_bytes, s_sum, s_max);
+      for (int t = 0; t < a.T; ++t) {
+        if (t) f4_meet<4>();                        // the row before's maxima have been read
+        fm_token(a, t, a.xq + (row0 + t) * x_bytes, s_sum, s_max);
+      }
       fm_rows_stored(&rows_bar);
     } else {
       for (int tries = 0; tries <= a.T; ++tries) {
