@@ -175,17 +175,19 @@ class BatchDecode:
         Q.fp4_rows(X, buf, gain=gain, eps=self.e.spec.rms_eps)
         return buf
 
-    def _mm(self, X, Wq, tiles, M, x8=None, W2=None, branch=0, room=0, **kw):
+    def _mm(self, X, Wq, tiles, M, x8=None, x4=None, W2=None, branch=0, room=0, **kw):
         """X [rows, K] bf16 times a resident matrix (or, with W2, the SwiGLU pair): FP8 weights against E4M3 rows on the
         tensor cores, other quantised types expanded in flight, the rest through a bf16 expansion launch.  ``x8``: the
         rows' E4M3 form when the caller already made it (several products of one input).  ``branch``: 0 on the pass's own
         stream, 1 / 2 on its side streams; ``room``: processors that a split product may take (0: all).  NVFP4 weights take NVFP4 rows where
-        that is asked for (``x8`` then holds those).  Returns the launch count."""
+        that is asked for; ``x4``: those rows when the caller already made them, as it has to for products of one input on several
+        streams, since the rows of an input have one buffer.  Returns the launch count."""
         if self._native_fp4(Wq, *([W2] if W2 is not None else [])):
             n = 0
-            if not isinstance(x8, Q.Fp4Rows):
-                x8 = self._q4(X); n += 1
-            Q.fp4_gemm(x8, Wq, tiles if tiles.tile_rows <= 64 else self._dense32(M), W2=W2, status=self.status, **kw)
+            if x4 is None:
+                assert branch == 0, "a side stream does not fill the buffer that the pass's own stream may be reading"
+                x4 = self._q4(X); n += 1
+            Q.fp4_gemm(x4, Wq, tiles if tiles.tile_rows <= 64 else self._dense32(M), W2=W2, status=self.status, **kw)
             return n + 1
         if self._native_fp8(Wq):
             n = 0
@@ -335,12 +337,15 @@ class BatchDecode:
         main = torch.cuda.current_stream(e.device)
         n_tiles = lambda rows: tiles.fixed * ((rows + 127) // 128)                                    # noqa: E731
         q_room, kv_room = G.qkv_rooms(n_tiles(s.q_rows), n_tiles(s.kv_rows), s.hidden // 256, K.sm_count(e.device))
-        x8 = None
-        if any(self._native_fp8(w.q[b + nm]) for nm in ("attn_q.weight", "attn_k.weight", "attn_v.weight")):
+        x8 = x4 = None
+        three = [w.q[b + nm] for nm in ("attn_q.weight", "attn_k.weight", "attn_v.weight")]
+        if any(self._native_fp8(q) for q in three):
             x8 = self._q8(xn); n += 1                            # one E4M3 form of the rows for the three products
-        elif self._rows_in_fp4(il):
+        if self._rows_in_fp4(il):
             # one NVFP4 form, with the norm in front of it
-            x8 = self._q4(self.x[:M], w.f[b + "attn_norm.weight"]); n += 1
+            x4 = self._q4(self.x[:M], w.f[b + "attn_norm.weight"]); n += 1
+        elif any(self._native_fp4(q) for q in three):
+            x4 = self._q4(xn); n += 1                            # for those that take it, of the rows that the others read
         fork = torch.cuda.Event()
         fork.record(main)
         joins = []
@@ -349,11 +354,11 @@ class BatchDecode:
             side = self._side[branch - 1]
             side.wait_event(fork)
             with torch.cuda.stream(side):
-                n += self._mm(xn, w.q[b + name], tiles, M, x8=x8, branch=branch, room=kv_room, out_f32=self.qkv[:M, lo:hi])
+                n += self._mm(xn, w.q[b + name], tiles, M, x8=x8, x4=x4, branch=branch, room=kv_room, out_f32=self.qkv[:M, lo:hi])
                 ev = torch.cuda.Event()
                 ev.record(side)
                 joins.append(ev)
-        n += self._mm(xn, w.q[b + "attn_q.weight"], tiles, M, x8=x8, room=q_room, out_f32=self.qkv[:M, :s.q_rows])
+        n += self._mm(xn, w.q[b + "attn_q.weight"], tiles, M, x8=x8, x4=x4, room=q_room, out_f32=self.qkv[:M, :s.q_rows])
         for ev in joins:
             main.wait_event(ev)
         kvp = e.kv
@@ -380,20 +385,23 @@ class BatchDecode:
         n = 0
         main = torch.cuda.current_stream(e.device)
         first = w.q[b + "attn_q_a.weight"] if s.q_lora else w.q[b + "attn_q.weight"]
-        x8 = None
-        if self._native_fp8(first) or self._native_fp8(w.q[b + "attn_kv_a_mqa.weight"]):
+        x8 = x4 = None
+        both = first, w.q[b + "attn_kv_a_mqa.weight"]
+        if any(self._native_fp8(q) for q in both):
             x8 = self._q8(xn); n += 1                            # one E4M3 form of the rows for both products
+        if any(self._native_fp4(q) for q in both):
+            x4 = self._q4(xn); n += 1                            # and one NVFP4 form
         fork = torch.cuda.Event()
         fork.record(main)
         side = self._side[0]
         side.wait_event(fork)
         with torch.cuda.stream(side):
-            n += self._mm(xn, w.q[b + "attn_kv_a_mqa.weight"], tiles, M, x8=x8, branch=1, out_f32=self.qkv[:M, self.qa_w:])
+            n += self._mm(xn, w.q[b + "attn_kv_a_mqa.weight"], tiles, M, x8=x8, x4=x4, branch=1, out_f32=self.qkv[:M, self.qa_w:])
             K.mla_kv_append(self.qkv[:, self.qa_w:], w.f[b + "attn_kv_a_norm.weight"], e.inv_freq, s.rms_eps, M, self.row_pos,
                             self.row_seq, kvp.table, kvp.n_pages, kvp.k[il], e.fault, il); n += 1
             join = torch.cuda.Event()
             join.record(side)
-        n += self._mm(xn, first, tiles, M, x8=x8, out_f32=self.qkv[:M, :self.qa_w])
+        n += self._mm(xn, first, tiles, M, x8=x8, x4=x4, out_f32=self.qkv[:M, :self.qa_w])
         if s.q_lora:
             G.rmsnorm_bf16(self.qkv[:M, :s.q_lora], w.f[b + "attn_q_a_norm.weight"], s.rms_eps, self.qn[:M]); n += 1
             n += self._mm(self.qn[:M], w.q[b + "attn_q_b.weight"], tiles, M, out_f32=self.q_full[:M])

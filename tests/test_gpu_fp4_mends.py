@@ -1,8 +1,11 @@
 """Calls of the NVFP4 operators that were answered wrongly once, or could be."""
+import gc
+
 import pytest
 import torch
 
-from test_gpu_fp4 import DEV
+from bloomery_b200.formats import planes
+from test_gpu_fp4 import DEV, allowed, quantised
 from test_gpu_fp4_moe import case, oracle, run
 
 gpu = pytest.mark.gpu
@@ -27,3 +30,101 @@ def test_few_tokens_without_a_norm_keep_their_own_scales(T, k, dtype):
     for _ in range(40):
         work = run(*c, work=work, out_f32=out)
         assert torch.equal(out, alone)
+
+
+# ---- products of one input on several streams -----------------------------------------------------------------------
+def engine(kind, n_slots=12):
+    """Tiny models: every matrix NVFP4, but the v projections in Q8_0 (``mixed``) or one projection of a layer with signs in its block
+    scales (``signs``); latent attention with a shared expert and a dense layer (``latent``)."""
+    from bloomery_b200.models.spec import tiny_deepseek, tiny_qwen3moe
+    from bloomery_b200.models.weights import Weights, synth_tensors
+    from bloomery_b200.runtime.engine import DecodeEngine
+    spec = tiny_deepseek() if kind == "latent" else tiny_qwen3moe()
+    items = list(synth_tensors(spec, DEV, seed=3, mix="NVFP4"))
+    if kind == "mixed":
+        items = [b if a[0].endswith("attn_v.weight") else a for a, b in zip(items, synth_tensors(spec, DEV, seed=3, mix="Q8_0"))]
+    w = Weights.from_items(spec, iter(items), DEV)
+    if kind == "signs":
+        q = w.q["blk.0.attn_k.weight"]
+        q.data[3, q.k // 2 + 1] |= 0x80
+    eng = DecodeEngine(w, n_slots=n_slots, slot_ctx=256)
+    g = torch.Generator().manual_seed(7)
+    prompts = [torch.randint(0, spec.vocab, (5 + 3 * (i % 7),), generator=g).tolist() for i in range(n_slots)]
+    return spec, eng, [(slot, eng.prefill(slot, p, gemm=False), len(p)) for slot, p in enumerate(prompts)]
+
+
+@pytest.fixture(autouse=True)
+def no_engine_left():
+    """Engines hold their prompt paths and those the engines: their graphs must not be taken down while a later test captures one."""
+    yield
+    gc.collect()
+
+
+def values(q):
+    flat = q.data.reshape(-1, q.data.shape[-1]).cpu()
+    ts = flat[:, q.k // 2 + q.k // 16:q.k // 2 + q.k // 16 + 4].contiguous().view(torch.float32).double()
+    return planes.nvfp4_dequantize(flat[:, :q.k // 2], flat[:, q.k // 2:q.k // 2 + q.k // 16], 1.0).double() * ts
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["mixed", "signs", "latent"])
+def test_rows_of_one_input_are_made_on_one_stream(kind, monkeypatch):
+    """Two streams that fill one buffer while either reads it have no order between them.  The first pass, of plain launches, gives the
+    bits of the captured one."""
+    from bloomery_b200.ops import fp4 as Q
+    from bloomery_b200.runtime.batch_decode import BatchDecode
+    spec, eng, rows = engine(kind)
+    bd = BatchDecode(eng, max_rows=16)
+    bd.fp4_native = True
+    streams, plain = {}, Q.fp4_rows
+
+    def recorded(x, out, **kw):
+        streams.setdefault(out.ptr, set()).add(torch.cuda.current_stream().cuda_stream)
+        plain(x, out, **kw)
+    monkeypatch.setattr(Q, "fp4_rows", recorded)
+    M = bd.set_rows(rows)
+    with torch.cuda.stream(bd._stream):
+        bd.enqueue(M)
+    torch.cuda.synchronize()
+    first = bd.logits[:len(rows)].clone()
+    assert streams and all(s == {bd._stream.cuda_stream} for s in streams.values())
+    monkeypatch.setattr(Q, "fp4_rows", plain)
+    for _ in range(3):
+        bd.step(rows)
+        assert torch.equal(bd.logits[:len(rows)], first)
+    assert first.isfinite().all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["mixed", "signs", "latent"])
+def test_projections_beside_others_of_another_type(kind):
+    """Those that take NVFP4 rows against the definition, the others as without."""
+    from bloomery_b200.ops import gemm as G
+    from bloomery_b200.runtime.batch_decode import BatchDecode
+    spec, eng, rows = engine(kind)
+    bd = BatchDecode(eng, max_rows=16)
+    M = bd.set_rows(rows)
+    x = torch.randn(M, spec.hidden, generator=torch.Generator().manual_seed(1)).to(DEV)
+    names = ("attn_q_a", "attn_kv_a_mqa") if spec.mla else ("attn_q", "attn_k", "attn_v")
+    got = {}
+    for native in (False, True):
+        bd.fp4_native = native
+        with torch.cuda.stream(bd._stream):
+            bd.x[:M].copy_(x)
+            G.rmsnorm_bf16(bd.x[:M], eng.w.f["blk.0.attn_norm.weight"], spec.rms_eps, bd.xn[:M])
+            (bd._attn_mla if spec.mla else bd._attn_gqa)(0, M, bd.xn[:M], bd.dense_tiles[M])
+        torch.cuda.synchronize()
+        got[native] = bd.qkv[:M].clone()
+    xv, lo, taken = quantised(bd.xn[:M])[3], 0, 0
+    for n in names:
+        q = eng.w.q[f"blk.0.{n}.weight"]
+        a, b = got[False][:, lo:lo + q.rows], got[True][:, lo:lo + q.rows]
+        if kind == "mixed" and n == "attn_v" or kind == "signs" and n == "attn_k":
+            assert torch.equal(a, b)
+        else:
+            w = values(q)
+            off = (b.double().cpu() - xv @ w.T).abs()
+            assert bool((off <= allowed(xv, w, q.k)).all()), n
+            taken += 1
+        lo += q.rows
+    assert taken == 2
