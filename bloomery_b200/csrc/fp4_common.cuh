@@ -158,6 +158,15 @@ __device__ __forceinline__ double fp4_squares16(const float* v) {
   for (int i = 1; i < 16; ++i) s = fmaf(v[i], v[i], s);
   return (double)s;
 }
+// Whether a row's sum of those can stand: a part past fp32's largest is infinite, and squares below its normal numbers lose bits that count
+// where there is little else.  Else it is made again in 64 bits throughout.
+__device__ __forceinline__ bool fp4_sum_holds(double ss) { return ss > 0x1p-100 && ss < 0x1p200; }
+__device__ __forceinline__ double fp4_squares16_wide(const float* v) {
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s = fma((double)v[i], (double)v[i], s);
+  return s;
+}
 // The largest magnitude as bits: a NaN is above everything.
 template <int N>
 __device__ __forceinline__ unsigned fp4_top(const float* v) {

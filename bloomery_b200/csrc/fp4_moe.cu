@@ -189,16 +189,30 @@ __device__ __forceinline__ void fm_token(const FmArgs& a, int t, uint8_t* row, d
   float v[16], r = 1.0f;
   auto load = [&](int b) { fp4_load16(a.x, a.x_type, (long)t * a.ldx + 16 * b, v); };
   if (a.gain) {
+    auto whole = [&](double ss) {
+      ss = warp_sum_d(ss);
+      if (lane == 0) s_sum[w] = ss;
+      f4_meet<4>();
+      return s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+    };
     double ss = 0.0;
 #pragma unroll 1
     for (int b = et; b < blocks; b += 128) {
       load(b);
       ss += fp4_squares16(v);
     }
-    ss = warp_sum_d(ss);
-    if (lane == 0) s_sum[w] = ss;
-    f4_meet<4>();
-    r = fp4_rsqrt((s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) / (double)a.H + a.eps);
+    double all = whole(ss);
+    if (__builtin_expect(!fp4_sum_holds(all), 0)) {
+      f4_meet<4>();
+      ss = 0.0;
+#pragma unroll 1
+      for (int b = et; b < blocks; b += 128) {
+        load(b);
+        ss += fp4_squares16_wide(v);
+      }
+      all = whole(ss);
+    }
+    r = fp4_rsqrt(all / (double)a.H + a.eps);
   }
   unsigned top = 0;
 #pragma unroll 1

@@ -53,15 +53,26 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, NB == 1 ? (!F32 ? (WARP ? 8 
   }
   if constexpr (F32) {
     if (a.gain) {
+      auto whole = [&](double ss) {
+        ss = warp_sum_d(ss);
+        if (!WARP) {
+          if (lane == 0) s_sum[warp] = ss;
+          __syncthreads();
+          ss = 0.0;
+          for (int w = 0; w < warps; ++w) ss += s_sum[w];
+        }
+        return ss;
+      };
       double ss = 0.0;
 #pragma unroll
       for (int b = 0; b < NB; ++b) ss += fp4_squares16(v[b]);
-      ss = warp_sum_d(ss);
-      if (!WARP) {
-        if (lane == 0) s_sum[warp] = ss;
-        __syncthreads();
+      ss = whole(ss);
+      if (!fp4_sum_holds(ss)) {                       // the same for all threads of the row
+        if (!WARP) __syncthreads();
         ss = 0.0;
-        for (int w = 0; w < warps; ++w) ss += s_sum[w];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) ss += fp4_squares16_wide(v[b]);
+        ss = whole(ss);
       }
       const float r = fp4_rsqrt(ss / (double)a.K + a.eps);
 #pragma unroll

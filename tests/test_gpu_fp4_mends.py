@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from bloomery_b200.formats import planes
-from test_gpu_fp4 import DEV, allowed, quantised
+from test_gpu_fp4 import DEV, allowed, make, parts, quantised, same
 from test_gpu_fp4_moe import case, oracle, run
 
 gpu = pytest.mark.gpu
@@ -128,3 +128,45 @@ def test_projections_beside_others_of_another_type(kind):
             taken += 1
         lo += q.rows
     assert taken == 2
+
+
+# ---- norms of large and of small rows -------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("K", [64, 512, 1024, 2048, 4096, 16384])
+def test_norms_of_rows_whose_squares_pass_32_bits(K):
+    """Squares of 2^70 and of 2^-80 are no fp32 numbers, their norm is.  One large value among ordinary ones, and blocks that vanish beside
+    others, too."""
+    from bloomery_b200.ops.fp4 import Fp4Rows, fp4_rows
+    x = make(7, K, torch.float32, seed=K)
+    x[1] *= 2.0 ** 70
+    x[2] *= 2.0 ** -80
+    x[3, K // 2] = 3e38
+    x[4, :K // 2] *= 2.0 ** -75
+    x[5] = x[5].sign() * 2.0 ** -62
+    x[6] = 2.0 ** 127
+    gain = (1 + 0.3 * torch.randn(K, generator=torch.Generator().manual_seed(1))).to(DEV)
+    out = Fp4Rows(7, K, DEV)
+    fp4_rows(x, out, gain=gain)
+    r = (1 / x.double().square().mean(1, keepdim=True).sqrt()).float()
+    want = quantised(x * r * gain)
+    # ordinary rows (0, 4): their root may be the next fp32 number, 2^-23 away, and with it the largest value and the scale
+    g = parts(out.data, K)[2].double()
+    assert bool(((g - want[2].double()).abs() <= 2.0 ** -22 * want[2].double()).all())
+    odd = [1, 2, 3, 5, 6]
+    same(out.data[odd], K, tuple(t[odd] for t in want))
+
+
+@gpu
+@pytest.mark.parametrize("T", [3, 9])
+def test_experts_of_tokens_whose_squares_pass_32_bits(T):
+    c = case(T, 16, 4, 256, 512, seed=70 + T)
+    x, rest = c[0], c[1:]
+    x[1] *= 2.0 ** 70
+    x[2] *= 2.0 ** -80
+    gain = (1 + 0.3 * torch.randn(512, generator=torch.Generator().manual_seed(1))).to(DEV)
+    r = (1 / x.double().square().mean(1, keepdim=True).sqrt()).float()
+    want, tol = oracle(x * r * gain, *rest[:2], *(w[1] for w in rest[2:]))
+    out = torch.empty(T, 512, device=DEV)
+    run(x, *rest, out_f32=out, gain=gain)
+    off = (out.double().cpu() - want).abs()
+    assert bool((off <= tol + 5 * 2.0 ** -24 * want.abs()).all())
