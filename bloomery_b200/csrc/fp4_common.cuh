@@ -175,8 +175,8 @@ __device__ __forceinline__ unsigned fp4_top(const float* v) {
   for (int i = 1; i < N; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(v[i])));
   return __float_as_uint(top) & 0x7fffffffu;
 }
-// 1 / (6 g), near enough for a first guess at a block's scale
-__device__ __forceinline__ float fp4_inv6(float g) { return __frcp_rn(6.0f * g); }
+// 1 / (6 g), near enough for a first guess at a block's scale (6 g itself may be past fp32's largest)
+__device__ __forceinline__ float fp4_inv6(float g) { return __frcp_rn(g) * (1.0f / 6.0f); }
 // Block `at` of a row of K values with scale g
 __device__ __forceinline__ void fp4_store_block(uint8_t* row, int K, int at, const float* v, unsigned top, float g, float inv6g) {
   unsigned scale;

@@ -113,7 +113,10 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, NB == 1 ? (!F32 ? (WARP ? 8 
     top = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? s_max[lane] : 0u);
   }
   float g = fp4_row_scale(top);
-  if (a.tensor_scale && top < FP4_INF) g = fmaxf(*a.tensor_scale, FP4_LEAST);
+  if (a.tensor_scale && top < FP4_INF) {
+    g = *a.tensor_scale;
+    g = g < __uint_as_float(FP4_INF) ? fmaxf(g, FP4_LEAST) : __uint_as_float(0x7fc00000u);        // NaN where it is no finite number
+  }
   const float inv6g = fp4_inv6(g);
   auto places = [&](auto&& store) {
     for (int j = 0; j < a.copies; ++j) {
@@ -191,7 +194,7 @@ struct Fp4RowsCall {
 extern "C" {
 
 // NVFP4 rows of M rows of x (type 0 bf16, 1 f16, 2 fp32; ldx elements); gain != null: RMSNorm with that gain first (fp32 rows);
-// tensor_scale != null: that scale for every row; pos_of != null: row m goes to rows pos_of[m * copies + j] < rows_out (others
+// tensor_scale != null: that scale for every row (2^-100 at least; NaN where it is not finite); pos_of != null: row m goes to rows pos_of[m * copies + j] < rows_out (others
 // nowhere).
 int bl_fp4_rows(const Fp4RowsCall* c) {
   BL_REQUIRE(c->M >= 1 && c->K >= 64 && c->K % 64 == 0 && c->copies >= 1 && c->rows_out >= 1, BL_ERR_SHAPE);

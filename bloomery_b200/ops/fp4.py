@@ -75,10 +75,11 @@ def fp4_rows(x: torch.Tensor, out: Fp4Rows, *, gain: Optional[torch.Tensor] = No
              tensor_scale: Optional[torch.Tensor] = None, pos_of: Optional[torch.Tensor] = None) -> None:
     """NVFP4 rows of ``x`` [M, k] (bf16, f16 or fp32; rows may be strided) in the first M rows of ``out``.
 
-    A row's scale takes its largest magnitude to 6 x 448 (or is ``tensor_scale``, one positive fp32 on the
-    device; larger values saturate), a
+    A row's scale takes its largest magnitude to 6 x 448, or is ``tensor_scale``, one fp32 on the device (values too large for it
+    saturate; 2^-100 where it is below that, and with one that is no finite number all rows' products are NaN); a
     block's scale takes its own to 6; scales and codes are the nearest, ties go to the even code.  A row with a NaN or an
-    infinity becomes one whose products are all NaN.  ``gain`` fp32 [k] (fp32 rows): RMSNorm first.  ``pos_of`` int32 [M * copies]:
+    infinity becomes one whose products are all NaN.  ``gain`` fp32 [k] (fp32 rows): RMSNorm first, with 1 / sqrt(mean square + eps)
+    in fp32 (rows that are all zeros, or too small for that, need an ``eps``).  ``pos_of`` int32 [M * copies]:
     row m goes to the rows ``pos_of[m * copies + j]`` of ``out`` (none where that is negative or past the end), as ``moe_plan``
     deals the slots of M tokens."""
     kind = _TYPES.get(x.dtype)

@@ -1,5 +1,6 @@
 """Calls of the NVFP4 operators that were answered wrongly once, or could be."""
 import gc
+import math
 
 import pytest
 import torch
@@ -170,3 +171,32 @@ def test_experts_of_tokens_whose_squares_pass_32_bits(T):
     run(x, *rest, out_f32=out, gain=gain)
     off = (out.double().cpu() - want).abs()
     assert bool((off <= tol + 5 * 2.0 ** -24 * want.abs()).all())
+
+
+# ---- one scale for all rows -----------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_given_scales_over_the_whole_range(dtype):
+    """Six times a scale past 5.6e37 is no fp32 number."""
+    from bloomery_b200.ops.fp4 import Fp4Rows, fp4_rows
+    K = 256
+    x = make(24, K, torch.float32, seed=4)
+    x *= torch.exp2(torch.linspace(-40, 125, 24)).to(DEV)[:, None] / x.abs().amax(1, keepdim=True)
+    x = x.to(dtype)
+    for scale in (2.0 ** -100, 1e-20, 1.0, 5e37, 5.7e37, 1e38, 2.0 ** 127, 3.4e38):
+        out, s = Fp4Rows(24, K, DEV), torch.tensor([scale], device=DEV)
+        fp4_rows(x, out, tensor_scale=s)
+        same(out.data, K, quantised(x, s.item()))
+
+
+@gpu
+def test_given_scales_that_are_no_number():
+    """Every row becomes one whose products are NaN, as one with a value that is none."""
+    from bloomery_b200.ops.fp4 import Fp4Rows, fp4_rows
+    x = make(5, 128, torch.float32)
+    for scale in (math.nan, math.inf):
+        out = Fp4Rows(5, 128, DEV)
+        out.data.fill_(0x55)
+        fp4_rows(x, out, tensor_scale=torch.tensor([scale], device=DEV))
+        codes, scales, g = parts(out.data, 128)
+        assert g.isnan().all() and not codes.any() and not scales.any()
