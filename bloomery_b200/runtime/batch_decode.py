@@ -187,7 +187,7 @@ class BatchDecode:
             if x4 is None:
                 assert branch == 0, "a side stream does not fill the buffer that the pass's own stream may be reading"
                 x4 = self._q4(X); n += 1
-            Q.fp4_gemm(x4, Wq, tiles if tiles.tile_rows <= 64 else self._dense32(M), W2=W2, status=self.status, **kw)
+            Q.fp4_gemm(x4, Wq, tiles, W2=W2, status=self.status, **kw)
             return n + 1
         if self._native_fp8(Wq):
             n = 0

@@ -200,3 +200,42 @@ def test_given_scales_that_are_no_number():
         fp4_rows(x, out, tensor_scale=torch.tensor([scale], device=DEV))
         codes, scales, g = parts(out.data, 128)
         assert g.isnan().all() and not codes.any() and not scales.any()
+
+
+# ---- stacks of a type of their own behind a layer of bf16 ones ------------------------------------------------------
+@gpu
+def test_grouped_products_keep_their_tiles():
+    """A first routed layer in bf16 makes token tiles of 128 rows; the NVFP4 gate and up of the next one, whose down is Q8_0, run on the
+    experts' tiles all the same."""
+    from bloomery_b200.models.spec import tiny_qwen3moe
+    from bloomery_b200.models.weights import Weights, synth_tensors
+    from bloomery_b200.runtime.batch_decode import BatchDecode
+    from bloomery_b200.runtime.engine import DecodeEngine
+    spec = tiny_qwen3moe()
+    kinds = {m: list(synth_tensors(spec, DEV, seed=3, mix=m)) for m in ("NVFP4", "BF16", "Q8_0")}
+
+    def kind(name):
+        return "NVFP4" if "_exps" not in name else "BF16" if name.startswith("blk.0.") else "Q8_0" if "down" in name else "NVFP4"
+    items = (kinds[kind(a[0])][i] for i, a in enumerate(kinds["NVFP4"]))
+    eng = DecodeEngine(Weights.from_items(spec, items, DEV), n_slots=1, slot_ctx=256)
+    bd = BatchDecode(eng, max_rows=64)
+    assert bd.moe_tiles.tile_rows == 128
+    bd.fp4_native = True
+    M, k, gen = 64, spec.n_used, torch.Generator().manual_seed(5)
+    xn = torch.randn(M, spec.hidden, generator=gen).bfloat16().to(DEV)
+    ids = torch.stack([torch.randperm(spec.n_expert, generator=gen)[:k] for _ in range(M)]).to(torch.int32)
+    bd.x.zero_()
+    for _ in bd.experts(1, M, bd.x[:M], xn.clone(), ids.to(DEV), torch.rand(M, k, generator=gen).to(DEV), bd.dense_tiles[M]):
+        pass
+    act, slot = bd.act[:M * k].double().cpu(), bd.dst_row[:M * k].cpu()
+    xv, H = quantised(xn)[3], spec.hidden
+    g_, u_ = (values(eng.w.q[f"blk.1.ffn_{n}_exps.weight"]).view(spec.n_expert, -1, H) for n in ("gate", "up"))
+    assert slot.sort().values.tolist() == list(range(M * k))
+    for i, s in enumerate(slot.tolist()):
+        v, e = xv[s // k:s // k + 1], int(ids[s // k, s % k])
+        g, u = v @ g_[e].T, v @ u_[e].T
+        want = g * torch.sigmoid(g) * u
+        # the factor's slope is at most 1.1; the exponential and the quotient are off by a few units of 2^-22
+        tg, tu = allowed(v, g_[e], H), allowed(v, u_[e], H)
+        tol = 1.1 * tg * (u.abs() + tu) + (g.abs() + tg) * tu + (2.0 ** -8 + 2.0 ** -19) * want.abs() + 1e-30
+        assert bool(((act[i] - want[0]).abs() <= tol[0]).all()), i
