@@ -189,8 +189,8 @@ class BatchDecode:
                 x4 = self._q4(X); n += 1
             Q.fp4_gemm(x4, Wq, tiles, W2=W2, status=self.status, **kw)
             return n + 1
-        if self._native_fp8(Wq):
-            n = 0
+        if self._native_fp8(Wq) and (tiles.fixed or tiles.tile_rows == TILE):
+            n = 0                                                # (experts' tiles of 128 rows, behind a bf16 layer, are expanded below)
             if x8 is None:
                 x8 = self._q8(X); n += 1
             if tiles.tile_rows != 32:                            # the dense table of a 64-row bucket

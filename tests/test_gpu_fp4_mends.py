@@ -239,3 +239,30 @@ def test_grouped_products_keep_their_tiles():
         tg, tu = allowed(v, g_[e], H), allowed(v, u_[e], H)
         tol = 1.1 * tg * (u.abs() + tu) + (g.abs() + tg) * tu + (2.0 ** -8 + 2.0 ** -19) * want.abs() + 1e-30
         assert bool(((act[i] - want[0]).abs() <= tol[0]).all()), i
+
+
+@gpu
+def test_grouped_fp8_products_keep_their_tiles():
+    """The same layers with FP8 gate and up: tiles of 128 rows are no case of the E4M3 kernel, so they run as without it."""
+    from bloomery_b200.models.spec import tiny_qwen3moe
+    from bloomery_b200.models.weights import Weights, synth_tensors
+    from bloomery_b200.runtime.batch_decode import BatchDecode
+    from bloomery_b200.runtime.engine import DecodeEngine
+    spec = tiny_qwen3moe()
+    kinds = {m: list(synth_tensors(spec, DEV, seed=3, mix=m)) for m in ("FP8_B128", "BF16")}
+    items = (kinds["BF16" if "_exps" in a[0] and a[0].startswith("blk.0.") else "FP8_B128"][i] for i, a in enumerate(kinds["BF16"]))
+    eng = DecodeEngine(Weights.from_items(spec, items, DEV), n_slots=1, slot_ctx=256)
+    bd = BatchDecode(eng, max_rows=64)
+    assert bd.moe_tiles.tile_rows == 128
+    M, k, gen = 64, spec.n_used, torch.Generator().manual_seed(5)
+    xn = torch.randn(M, spec.hidden, generator=gen).bfloat16().to(DEV)
+    ids = torch.stack([torch.randperm(spec.n_expert, generator=gen)[:k] for _ in range(M)]).to(torch.int32).to(DEV)
+    wts = torch.rand(M, k, generator=gen).to(DEV)
+    got = []
+    for native in (False, True):
+        bd.fp8_native = native
+        bd.x.zero_()
+        for _ in bd.experts(1, M, bd.x[:M], xn.clone(), ids, wts, bd.dense_tiles[M]):
+            pass
+        got.append(bd.x[:M].clone())
+    assert bool((got[0] != 0).any()) and torch.equal(*got)
