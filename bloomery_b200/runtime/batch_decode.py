@@ -98,9 +98,8 @@ class BatchDecode:
             self.Ap = torch.zeros(self.cap, H, **bf)
             self.act = torch.zeros(self.cap, I_, **bf)
             self.slot_out = torch.zeros(n, H, **f32)
-            # bf16 expert stacks multiply as they are through the bf16 GEMM, whose token tiles are 128 rows
-            moe0 = next(il for il in range(s.n_layer) if s.layer_is_moe(il))
-            self.float_experts = e.w.q[f"blk.{moe0}.ffn_gate_exps.weight"].qtype == "BF16"
+            # bf16 expert stacks, of any layer, multiply as they are through the bf16 GEMM, whose token tiles are 128 rows
+            self.float_experts = any(e.w.q[f"blk.{il}.ffn_gate_exps.weight"].qtype == "BF16" for il in range(s.n_layer) if s.layer_is_moe(il))
             self.moe_tiles = G.TileTable(n, E, dev, 128 if self.float_experts else TILE)
         # widths come from the weights: a rank of a several-GPU engine holds a slice of the dense and shared widths
         wq = e.w.q

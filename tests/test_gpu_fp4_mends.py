@@ -266,3 +266,28 @@ def test_grouped_fp8_products_keep_their_tiles():
             pass
         got.append(bd.x[:M].clone())
     assert bool((got[0] != 0).any()) and torch.equal(*got)
+
+
+@gpu
+def test_bf16_stacks_behind_a_quantised_layer():
+    """A second routed layer in bf16 gives what it gives behind a bf16 one."""
+    from bloomery_b200.models.spec import tiny_qwen3moe
+    from bloomery_b200.models.weights import Weights, synth_tensors
+    from bloomery_b200.runtime.batch_decode import BatchDecode
+    from bloomery_b200.runtime.engine import DecodeEngine
+    spec = tiny_qwen3moe()
+    kinds = {m: list(synth_tensors(spec, DEV, seed=3, mix=m)) for m in ("Q8_0", "BF16")}
+    M, k, gen = 64, spec.n_used, torch.Generator().manual_seed(5)
+    xn = torch.randn(M, spec.hidden, generator=gen).bfloat16().to(DEV)
+    ids = torch.stack([torch.randperm(spec.n_expert, generator=gen)[:k] for _ in range(M)]).to(torch.int32).to(DEV)
+    wts = torch.rand(M, k, generator=gen).to(DEV)
+    got = []
+    for first in ("Q8_0", "BF16"):
+        items = (kinds[first if a[0].startswith("blk.0.") else "BF16"][i] for i, a in enumerate(kinds["BF16"]))
+        eng = DecodeEngine(Weights.from_items(spec, items, DEV), n_slots=1, slot_ctx=256)
+        bd = BatchDecode(eng, max_rows=64)
+        bd.x.zero_()
+        for _ in bd.experts(1, M, bd.x[:M], xn.clone(), ids, wts, bd.dense_tiles[M]):
+            pass
+        got.append(bd.x[:M].clone())
+    assert bool((got[0] != 0).any()) and torch.equal(*got)
