@@ -120,7 +120,7 @@ def fp4_rows(x: torch.Tensor, out: Fp4Rows, *, gain: Optional[torch.Tensor] = No
 def fp4_supports(w: QWeight) -> bool:
     """Whether the products here take a matrix or stack: NVFP4 whose block scales are without a sign, as checkpoints have them (looks at
     all of them and waits for the answer: once, when a model is set up)."""
-    if w.qtype != "NVFP4" or w.k % 64 or w.k > MAX_K:
+    if w.qtype != "NVFP4" or w.k % 64 or w.k > MAX_K or not _rows_of(w.data, w.k):
         return False
     return not bool((w.data[..., w.k // 2:w.k // 2 + w.k // 16] >= 0x80).any())
 
@@ -133,10 +133,17 @@ class Fp4Work:
         self.device = device
 
 
+def _rows_of(data: torch.Tensor, k: int) -> bool:
+    """Whether these are one matrix, or a stack, of NVFP4 rows of k values."""
+    shape = data.shape
+    return 2 <= len(shape) <= 3 and shape[-1] == (k // 2 + k // 16 + 19) // 16 * 16 and data.dtype is torch.uint8 and data.numel() > 0
+
+
 def _matrix(name: str, w: QWeight, k: int, index: int) -> int:
-    if w.qtype != "NVFP4" or w.k != k or not w.data.is_contiguous() or w.data.get_device() != index:
+    data = w.data
+    if w.qtype != "NVFP4" or w.k != k or not _rows_of(data, k) or not data.is_contiguous() or data.get_device() != index:
         raise ValueError(f"{name}: contiguous NVFP4 rows of {k} values on the device of the rest")
-    return w.data.data_ptr()
+    return data.data_ptr()
 
 
 def _of_rows(name: str, t: torch.Tensor, dtype, rows: int, index: int) -> int:

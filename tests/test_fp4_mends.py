@@ -1,0 +1,29 @@
+"""What the NVFP4 calls took, or kept, wrongly once; without a card."""
+import pytest
+import torch
+
+from bloomery_b200.ops import fp4 as Q
+from bloomery_b200.ops.decode import QWeight
+from test_fp4_contracts import w
+
+
+@pytest.mark.parametrize("data", [torch.zeros(16, 48, dtype=torch.uint8), torch.zeros(16, 96, dtype=torch.uint8), torch.zeros(2, 2, 16, 80, dtype=torch.uint8),
+                                  torch.zeros(80, dtype=torch.uint8), torch.zeros(16, 80, dtype=torch.int8), torch.zeros(0, 80, dtype=torch.uint8)],
+                         ids=["short rows", "long rows", "four dimensions", "one row", "signed", "no rows"])
+def test_weights_that_are_not_rows_of_their_width(data):
+    """Rows of 128 values are 80 bytes: others would be read past their end."""
+    bad, rows = QWeight(data, "NVFP4", 128), Q.Fp4Rows(4, 128, "cpu")
+    for kw in (dict(W=bad), dict(W=w(16, 128), W2=bad)):
+        with pytest.raises(ValueError, match="W2?: "):
+            Q.fp4_gemm(rows, kw.pop("W"), Q.fp4_tiles(4, "cpu"), out_f32=torch.zeros(4, 16), **kw)
+    assert not Q.fp4_supports(bad)
+
+
+def test_stacks_that_are_not_rows_of_their_width():
+    good = dict(gate=w(64, 128, 3), up=w(64, 128, 3), down=w(128, 64, 3))
+    for name, k in (("gate", 128), ("up", 128), ("down", 64)):
+        q = good[name]
+        bad = QWeight(q.data[..., :-16].contiguous(), "NVFP4", k)
+        with pytest.raises(ValueError, match=name + ": "):
+            Q.fp4_moe(torch.zeros(2, 128), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, 2), *{**good, name: bad}.values(),
+                      Q.Fp4MoeWork(2, 2, 128, 64, 3, "cpu"), out_f32=torch.zeros(2, 128))
