@@ -132,7 +132,7 @@ class BatchDecode:
         from ..utils import levers
         self.fp8_native = bool(levers.get("BLOOMERY_FP8_NATIVE"))
         self.fp4_native = bool(levers.get("BLOOMERY_FP4_NATIVE"))
-        self._fp4_ok: Dict[int, bool] = {}      # of a matrix of the model: whether its block scales allow it
+        self._fp4_ok: Dict[int, tuple] = {}     # of a matrix of the model: itself, and whether its block scales allow it
         self._moe_work = None
         # the engine's own stream: its 8-row passes and prompts and these passes touch the same KV pages in order
         self._stream = getattr(engine, "_stream", None) or torch.cuda.Stream(device=dev)
@@ -161,9 +161,9 @@ class BatchDecode:
         if not self.fp4_native or any(w.qtype != "NVFP4" for w in weights):
             return False
         for w in weights:
-            if id(w) not in self._fp4_ok:
-                self._fp4_ok[id(w)] = Q.fp4_supports(w)
-        return all(self._fp4_ok[id(w)] for w in weights)
+            if id(w) not in self._fp4_ok:            # which is its own as long as it is kept here
+                self._fp4_ok[id(w)] = w, Q.fp4_supports(w)
+        return all(self._fp4_ok[id(w)][1] for w in weights)
 
     def _q4(self, X: torch.Tensor, gain=None) -> "Q.Fp4Rows":
         """NVFP4 rows of X (one launch; ``gain``: of fp32 rows behind their norm), in a buffer of X's own."""

@@ -27,3 +27,18 @@ def test_stacks_that_are_not_rows_of_their_width():
         with pytest.raises(ValueError, match=name + ": "):
             Q.fp4_moe(torch.zeros(2, 128), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, 2), *{**good, name: bad}.values(),
                       Q.Fp4MoeWork(2, 2, 128, 64, 3, "cpu"), out_f32=torch.zeros(2, 128))
+
+
+def test_what_was_said_of_a_matrix_is_not_said_of_the_next_one():
+    """A matrix that took the place of another, address and all, is looked at itself."""
+    from types import SimpleNamespace
+    from bloomery_b200.runtime.batch_decode import BatchDecode
+    asks = SimpleNamespace(fp4_native=True, _fp4_ok={})
+    native = lambda q: BatchDecode._native_fp4(asks, q)                                          # noqa: E731
+    signed = w(16, 128).data
+    signed[3, 64 + 2] = 0x80
+    for _ in range(200):
+        good = QWeight(w(1, 128).data, "NVFP4", 128)
+        assert native(good)
+        del good
+        assert not native(QWeight(signed, "NVFP4", 128))
