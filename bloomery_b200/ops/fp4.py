@@ -68,6 +68,8 @@ def fp4_tile_rows(rows: int, groups: int = 1, gated: bool = False) -> int:
 
 def fp4_tiles(rows: int, device) -> TileTable:
     """The table of a product of ``rows`` rows with one matrix."""
+    if rows == 0:
+        return TileTable(0, 1, device, 32)
     return TileTable.dense(rows, device, fp4_tile_rows(rows), host=True)
 
 
@@ -191,6 +193,8 @@ def fp4_gemm(X: Fp4Rows, W: QWeight, tiles: TileTable, *, out_f32: Optional[torc
     sp = fault_ptr(status, index) if status is not None else 0
     if index < 0:
         raise ValueError("the kernels need a CUDA device")
+    if out.shape[0] == 0:
+        return                                   # no row of it to write
     code = _fn("bl_fp4_gemm")(_GEMM.pack(
         X.ptr, wp, w2p, tiles.mtiles_ptr, tiles.n_mtiles_ptr, out.data_ptr() if f32 else 0, 0 if f32 else out.data_ptr(),
         dp, fp, rp, sp, raw_stream(index), X.rows, out.stride(0), ldr, G, N, k,

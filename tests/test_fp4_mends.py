@@ -42,3 +42,10 @@ def test_what_was_said_of_a_matrix_is_not_said_of_the_next_one():
         assert native(good)
         del good
         assert not native(QWeight(signed, "NVFP4", 128))
+
+
+def test_tables_of_no_rows():
+    t = Q.fp4_tiles(0, "cpu")
+    assert t.rows == 0 and t.fixed == 0 and int(t.n_mtiles) == 0
+    with pytest.raises(ValueError, match="CUDA"):                 # the last check
+        Q.fp4_gemm(Q.Fp4Rows(1, 128, "cpu"), w(16, 128), t, out_f32=torch.zeros(0, 16))

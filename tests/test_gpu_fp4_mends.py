@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from bloomery_b200.formats import planes
-from test_gpu_fp4 import DEV, allowed, make, parts, quantised, same
+from test_gpu_fp4 import DEV, allowed, make, parts, quantised, same, weight
 from test_gpu_fp4_moe import case, oracle, run
 
 gpu = pytest.mark.gpu
@@ -291,3 +291,15 @@ def test_bf16_stacks_behind_a_quantised_layer():
             pass
         got.append(bd.x[:M].clone())
     assert bool((got[0] != 0).any()) and torch.equal(*got)
+
+
+# ---- no rows --------------------------------------------------------------------------------------------------------
+@gpu
+def test_products_of_no_rows():
+    from bloomery_b200.ops.fp4 import Fp4Rows, fp4_gemm, fp4_rows, fp4_tiles
+    rows, (q, _) = Fp4Rows(4, 128, DEV), weight(16, 128)
+    fp4_rows(torch.zeros(0, 128, device=DEV), rows)
+    fp4_gemm(rows, q, fp4_tiles(0, DEV), out_f32=torch.empty(0, 16, device=DEV))
+    out = torch.full((3, 16), 7.0, device=DEV)
+    fp4_gemm(rows, q, fp4_tiles(0, DEV), out_f32=out)
+    assert (out == 7).all()
