@@ -34,6 +34,7 @@ class ShardedBatchDecode(BatchDecode):
 
     def __init__(self, engine, rank: int, world: int, group=None, max_rows: int = 64, local_only: bool = False):
         super().__init__(engine, max_rows)
+        self.fp4_native = False                      # activations in four bits are the one-GPU pass's
         s = engine.spec
         if not s.is_moe or s.n_expert % world:
             raise ValueError(f"{world} ranks do not divide {s.n_expert} experts")

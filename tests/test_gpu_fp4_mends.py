@@ -303,3 +303,22 @@ def test_products_of_no_rows():
     out = torch.full((3, 16), 7.0, device=DEV)
     fp4_gemm(rows, q, fp4_tiles(0, DEV), out_f32=out)
     assert (out == 7).all()
+
+
+# ---- the lever ------------------------------------------------------------------------------------------------------
+@gpu
+def test_the_pass_over_ranks_keeps_16_bits():
+    from bloomery_b200.models.spec import tiny_qwen3moe
+    from bloomery_b200.models.weights import Weights, synth_tensors
+    from bloomery_b200.parallel.batch_dist import ShardedBatchDecode
+    from bloomery_b200.runtime.batch_decode import BatchDecode
+    from bloomery_b200.runtime.engine import DecodeEngine
+    from bloomery_b200.utils import levers
+    spec = tiny_qwen3moe()
+    eng = DecodeEngine(Weights.from_items(spec, synth_tensors(spec, DEV, seed=3, mix="NVFP4"), DEV), n_slots=1, slot_ctx=256)
+    try:
+        levers.at_main({"BLOOMERY_FP4_NATIVE": "1"})
+        assert BatchDecode(eng, max_rows=16).fp4_native
+        assert not ShardedBatchDecode(eng, 0, 1, max_rows=16, local_only=True).fp4_native
+    finally:
+        levers.at_main()
