@@ -230,7 +230,7 @@ class GemmPrefill:
             pos_of = self._get("pos_of", (nslot,), i32)
             dst_row = self._get("dst_row", (cap,), i32)
             row_scale = self._get("row_scale", (cap,), f32)
-            Ap = self._get("Ap", (cap, H), bf)
+            Ap = None if native else self._get("Ap", (cap, H), bf)
             act = self._get("act", (cap, I_), bf)
             slot_out = self._get("slot_out", (nslot, H), f32)
             pairs = not blocks and nslot >= self.pair_rows * E

@@ -322,3 +322,69 @@ def test_the_pass_over_ranks_keeps_16_bits():
         assert not ShardedBatchDecode(eng, 0, 1, max_rows=16, local_only=True).fp4_native
     finally:
         levers.at_main()
+
+
+def by_definition(X, W):
+    """(X [rows, K] in NVFP4) W^T in 64 bits, and how far fp32 sums may be off."""
+    xv = quantised(X)[3]
+    return xv @ W.T, allowed(xv, W, W.shape[1])
+
+
+@gpu
+@pytest.mark.parametrize("T,experts", [(64, 16), (131, 16), (300, 16), (131, 32)])
+def test_a_layer_of_a_prompt_is_the_sum_of_its_parts(T, experts):
+    """A model of one layer: every product of a prompt against the definition, of the rows that the path itself has in front of it."""
+    from dataclasses import replace
+    from bloomery_b200.models.spec import tiny_qwen3moe
+    from bloomery_b200.models.weights import Weights, synth_tensors
+    from bloomery_b200.runtime.engine import DecodeEngine
+    from bloomery_b200.runtime.prefill import GemmPrefill
+    spec = replace(tiny_qwen3moe(), n_layer=1, n_expert=experts)
+    eng = DecodeEngine(Weights.from_items(spec, synth_tensors(spec, DEV, seed=3, mix="NVFP4"), DEV), n_slots=1, slot_ctx=1024)
+    pf = GemmPrefill(eng)
+    pf.fp4_native = True
+    ids = torch.randint(0, spec.vocab, (T,), generator=torch.Generator().manual_seed(T)).tolist()
+    pf.run(0, ids)
+    torch.cuda.synchronize()
+    eng.check_fault()
+    assert "Ap" not in pf._buf and not pf._resident               # nothing is laid out, or kept, that this path does not read
+    w, H, E, k, n = eng.w, spec.hidden, spec.n_expert, spec.n_used, T * spec.n_used
+    get = lambda name, *shape: pf._buf[name][:math.prod(shape)].view(*shape).double().cpu()       # noqa: E731
+    normed = lambda v, gain: v * (1 / (v.double().square().mean(1, keepdim=True) + spec.rms_eps).sqrt()).float() * gain      # noqa: E731
+    from bloomery_b200.ops import decode as K
+    x0 = torch.empty(T, H, device=DEV)
+    K.embed_rows(torch.tensor(ids, dtype=torch.int32, device=DEV), T, w.q["token_embd.weight"], spec.vocab, x0, eng.fault)
+    # the projections, of the embeddings behind their norm: its root may be the next fp32 number
+    W = torch.cat([values(w.q[f"blk.0.attn_{m}.weight"]) for m in "qkv"])
+    want, tol = by_definition(normed(x0, w.f["blk.0.attn_norm.weight"]), W)
+    off = (get("qkv", T, W.shape[0]) - want).abs()
+    assert bool((off <= tol + 2.0 ** -21 * want.abs()).all())
+    # the o projection, seen behind the experts: x = embeddings + o + experts
+    attn = pf._buf["attn"][:T * spec.q_rows].view(T, spec.q_rows)
+    o, tol_o = by_definition(attn, values(w.q["blk.0.attn_output.weight"]))
+    x1 = x0.double().cpu() + o
+    # the experts' rows: the router's input, in bf16
+    split = T >= 128 and E % 32 == 0                              # the router's product in two halves: the rows are the high ones
+    rows = (pf._buf["xn3"][:T * 3 * H].view(T, 3 * H)[:, :H] if split else pf._buf["xn"][:T * H].view(T, H)).contiguous()
+    ref = normed(x1.float().to(DEV), w.f["blk.0.ffn_norm.weight"]).double().cpu()
+    assert bool(((rows.double().cpu() - ref).abs() <= (2.0 ** -8 + 2.0 ** -12) * ref.abs() + 1e-4).all())
+    sel, wts, slot = get("ids", T, k).long(), get("wts", T, k), get("dst_row", n).long()
+    act, out = get("act", n, spec.moe_inter), get("slot_out", n, H)
+    gate, up, down = (values(w.q[f"blk.0.ffn_{m}_exps.weight"]).view(E, -1, kk) for m, kk in (("gate", H), ("up", H), ("down", spec.moe_inter)))
+    xv, av = quantised(rows)[3], quantised(act.bfloat16())[3]
+    for e in range(E):
+        at = (sel.view(-1)[slot] == e).nonzero().flatten()       # places of this expert's slots
+        if not len(at):
+            continue
+        v = xv[slot[at] // k]
+        g, u = v @ gate[e].T, v @ up[e].T
+        tg, tu, a = allowed(v, gate[e], H), allowed(v, up[e], H), g * torch.sigmoid(g) * u
+        # the factor's slope is at most 1.1; the exponential and the quotient are off by a few units of 2^-22
+        tol = 1.1 * tg * (u.abs() + tu) + (g.abs() + tg) * tu + (2.0 ** -8 + 2.0 ** -19) * a.abs() + 1e-30
+        assert bool(((act[at] - a).abs() <= tol).all()), e
+        f = wts.view(-1)[slot[at], None]
+        d = f * (av[at] @ down[e].T)
+        assert bool(((out[slot[at]] - d).abs() <= f * allowed(av[at], down[e], spec.moe_inter) + 2.0 ** -23 * d.abs() + 1e-30).all()), e
+    x2 = x1 + out.view(T, k, H).sum(1)
+    tol = tol_o + (k + 2) * 2.0 ** -23 * (x1.abs() + out.view(T, k, H).abs().sum(1))
+    assert bool(((get("x", T, H) - x2).abs() <= tol).all())
