@@ -388,3 +388,81 @@ def test_a_layer_of_a_prompt_is_the_sum_of_its_parts(T, experts):
     x2 = x1 + out.view(T, k, H).sum(1)
     tol = tol_o + (k + 2) * 2.0 ** -23 * (x1.abs() + out.view(T, k, H).abs().sum(1))
     assert bool(((get("x", T, H) - x2).abs() <= tol).all())
+
+
+# ---- every form of the kernels --------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("N", [2040, 4096, 8200, 20000])
+@pytest.mark.parametrize("M", [20, 60, 100, 200])
+def test_products_in_every_tile(M, N, gated):
+    """Tiles of 16 to 128 weight rows, by how many find a processor at once, and of 32 to 256 tokens."""
+    from bloomery_b200.ops.fp4 import Fp4Rows, fp4_gemm, fp4_rows, fp4_tile_rows
+    from bloomery_b200.ops.gemm import TileTable
+    K = 192
+    x, rows, status = make(M, K, seed=N), Fp4Rows(M, K, DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    fp4_rows(x, rows)
+    (w1, v1), (w2, v2) = weight(N, K, 1), weight(N, K, 2)
+    out = torch.empty(M, N, dtype=torch.bfloat16, device=DEV)
+    tiles = TileTable.dense(M, DEV, fp4_tile_rows(M, gated=gated), host=True)
+    fp4_gemm(rows, w1, tiles, W2=w2 if gated else None, out_bf16=out, status=status)
+    xv = quantised(x)[3]
+    g, tg = xv @ v1.T, allowed(xv, v1, K)
+    want, tol = g, tg
+    if gated:
+        u, tu = xv @ v2.T, allowed(xv, v2, K)
+        want = g * torch.sigmoid(g) * u
+        # the factor's slope is at most 1.1; the exponential and the quotient are off by a few units of 2^-22
+        tol = 1.1 * tg * (u.abs() + tu) + (g.abs() + tg) * tu + 2.0 ** -19 * want.abs()
+    assert int(status) == 0
+    assert bool(((out.double().cpu() - want).abs() <= tol + 2.0 ** -8 * (want.abs() + tol)).all())
+
+
+@gpu
+@pytest.mark.parametrize("T,E,k,inter,H", [(1, 4, 2, 256, 512), (2, 4, 2, 256, 2048), (1, 16, 8, 768, 2048), (4, 32, 8, 768, 512), (3, 5, 3, 2048, 4096),
+                                           (3, 20, 16, 128, 512), (4, 40, 16, 64, 4096), (5, 9, 4, 320, 4096)])
+def test_few_tokens_behind_their_norm(T, E, k, inter, H):
+    """Every height of a tile of one to four tokens, and more slots than that form has room for."""
+    c = case(T, E, k, inter, H, seed=20 + T)
+    gain = (1 + 0.3 * torch.randn(H, generator=torch.Generator().manual_seed(1))).to(DEV)
+    x, rest = c[0], c[1:]
+    r = (1 / (x.double().square().mean(1, keepdim=True) + 1e-6).sqrt()).float()
+    want, tol = oracle(x * r * gain, *rest[:2], *(w[1] for w in rest[2:]))
+    want = want + x.double().cpu()
+    out = x.clone()
+    work = run(out, *rest, out_f32=out, resid=out, gain=gain, eps=1e-6)
+    # twice the oracle's: its rows may differ by a unit of the root's last place (and a code on the edge with it)
+    off = (out.double().cpu() - want).abs()
+    assert bool((off <= 2 * tol + (k + 1) * 2.0 ** -24 * (want.abs() + x.double().cpu().abs())).all()), float((off / tol).max())
+    again = torch.empty(T, H, device=DEV)
+    for _ in range(3):
+        run(x, *rest, work=work, out_f32=again, resid=x, gain=gain, eps=1e-6)
+        assert torch.equal(again, out)
+
+
+@gpu
+def test_the_dense_layers_and_the_shared_expert():
+    """Both halves of a SwiGLU pair against the definition, in a model with latent attention."""
+    from bloomery_b200.runtime.batch_decode import BatchDecode
+    spec, eng, rows = engine("latent")
+    bd = BatchDecode(eng, max_rows=16)
+    bd.fp4_native = True
+    M, gen = 16, torch.Generator().manual_seed(5)
+    xn = torch.randn(M, spec.hidden, generator=gen).bfloat16().to(DEV)
+    x = torch.randn(M, spec.hidden, generator=gen).to(DEV)
+    q = lambda name: values(eng.w.q[name + ".weight"])                                            # noqa: E731
+    for stem, suffix, act in (("blk.0.ffn_", "", bd.dact), ("blk.1.ffn_", "_shexp", bd.sh_act)):
+        bd.x[:M].copy_(x)
+        if suffix:
+            bd.shared_expert(1, M, xn, bd.dense_tiles[M], bd.x[:M], bd.x[:M])
+        else:
+            for _ in bd.dense_ffn(0, M, bd.x[:M], xn, bd.dense_tiles[M]):
+                pass
+        torch.cuda.synchronize()
+        (g, tg), (u, tu) = (by_definition(xn, q(stem + n + suffix)) for n in ("gate", "up"))
+        a = g * torch.sigmoid(g) * u
+        tol = 1.1 * tg * (u.abs() + tu) + (g.abs() + tg) * tu + (2.0 ** -8 + 2.0 ** -19) * a.abs() + 1e-30
+        assert bool(((act[:M].double().cpu() - a).abs() <= tol).all())
+        y, tol = by_definition(act[:M], q(stem + "down" + suffix))
+        want = y + x.double().cpu()
+        assert bool(((bd.x[:M].double().cpu() - want).abs() <= tol + 2.0 ** -23 * want.abs()).all())
