@@ -302,6 +302,8 @@ def softmax_causal(S, rows: int, Tq: int, pos0: int, T_pad: int, P) -> None:
 def moe_plan(ids, wts, E: int, tiles: "TileTable", pos_of, dst_row, row_scale) -> None:
     """Count, offsets, tile table and scatter of a micro-batch's routed slots in one launch (``ids`` / ``wts`` flat)."""
     n = ids.numel()
+    if n > tiles.rows or E > tiles.n_groups:     # what a product over the table trusts
+        raise ValueError(f"{n} slots of {E} experts in a table of {tiles.rows} rows and {tiles.n_groups} matrices")
     tiles.fixed = 0
     rc = cuda().bl_moe_plan(p(ids), p(wts), I(n), I(E), I(dst_row.numel()), p(tiles.offsets), p(pos_of), p(dst_row),
                             p(row_scale), p(tiles.mtiles), p(tiles.n_mtiles), I(tiles.max_mtiles), I(tiles.tile_rows),

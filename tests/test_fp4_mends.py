@@ -49,3 +49,13 @@ def test_tables_of_no_rows():
     assert t.rows == 0 and t.fixed == 0 and int(t.n_mtiles) == 0
     with pytest.raises(ValueError, match="CUDA"):                 # the last check
         Q.fp4_gemm(Q.Fp4Rows(1, 128, "cpu"), w(16, 128), t, out_f32=torch.zeros(0, 16))
+
+
+def test_plans_of_more_slots_than_their_table_has_rows():
+    """A product trusts the rows that the table was made for."""
+    from bloomery_b200.ops import gemm as G
+    ids, i32 = torch.zeros(65, dtype=torch.int32), torch.zeros(200, dtype=torch.int32)
+    with pytest.raises(ValueError, match="65 slots"):
+        G.moe_plan(ids, ids.float(), 4, G.TileTable(64, 4, "cpu", 32), i32, i32, i32.float())
+    with pytest.raises(ValueError, match="5 experts"):
+        G.moe_plan(ids[:64], ids.float()[:64], 5, G.TileTable(64, 4, "cpu", 32), i32, i32, i32.float())
