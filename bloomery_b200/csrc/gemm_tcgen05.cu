@@ -423,7 +423,7 @@ static int gemm_splits(long tiles, int K, int sm_count) {
 // query heads of one KV head).
 __global__ void build_mtiles_kernel(const int* group_rows, int n_groups, MTile* mtiles, int* n_mtiles, int max_mtiles,
                                     int* group_offset_out, int group_div, int group_stride, int base, int src_rows,
-                                    int causal_pos0, int causal_kind) {
+                                    int causal_pos0, int causal_kind, int tile_rows) {
   pdl_wait();
   pdl_launch();
   if (threadIdx.x != 0 || blockIdx.x != 0) return;
@@ -434,7 +434,7 @@ __global__ void build_mtiles_kernel(const int* group_rows, int n_groups, MTile* 
     const int rows = group_rows[g];
     if (group_stride > 0) off = base + g * group_stride;
     if (group_offset_out) group_offset_out[g] = off;
-    for (int r = 0; r < rows; r += BM) {
+    for (int r = 0; r < rows; r += tile_rows) {
       // src_rows > 0: A is row-sharded over ranks in blocks of src_rows; the tile reads rank (row / src_rows)'s map
       if (n < max_mtiles) {
         if (src_rows > 0) {
@@ -467,12 +467,12 @@ using namespace bl;
 
 extern "C" {
 
-// Fill the tile table for a grouped GEMM from per-group row counts on the device.
+// Fill the tile table for a grouped GEMM from per-group row counts on the device, tile_rows rows a tile.
 int bl_gemm_build_tiles(const int* group_rows, int n_groups, void* mtiles, int* n_mtiles, int max_mtiles,
-                        int* group_offsets, int group_div, int group_stride, int base, cudaStream_t st) {
-  BL_REQUIRE(n_groups >= 1 && max_mtiles >= 1 && group_div >= 1, BL_ERR_SHAPE);
+                        int* group_offsets, int group_div, int group_stride, int base, int tile_rows, cudaStream_t st) {
+  BL_REQUIRE(n_groups >= 1 && max_mtiles >= 1 && group_div >= 1 && tile_rows >= 8, BL_ERR_SHAPE);
   return (int)launch(build_mtiles_kernel, dim3(1), dim3(32), 0, st, group_rows, n_groups, (MTile*)mtiles, n_mtiles,
-                     max_mtiles, group_offsets, group_div, group_stride, base, 0, 0, 0);
+                     max_mtiles, group_offsets, group_div, group_stride, base, 0, 0, 0, tile_rows);
 }
 
 // The same with causal limits: kind 1 = columns are keys (scores), kind 2 = depth is keys (values); a group's row r is
@@ -482,7 +482,7 @@ int bl_gemm_build_tiles_causal(const int* group_rows, int n_groups, void* mtiles
                                cudaStream_t st) {
   BL_REQUIRE(n_groups >= 1 && max_mtiles >= 1 && group_div >= 1 && (kind == 1 || kind == 2) && causal_pos0 >= 0, BL_ERR_SHAPE);
   return (int)launch(build_mtiles_kernel, dim3(1), dim3(32), 0, st, group_rows, n_groups, (MTile*)mtiles, n_mtiles,
-                     max_mtiles, group_offsets, group_div, group_stride, base, 0, causal_pos0, kind);
+                     max_mtiles, group_offsets, group_div, group_stride, base, 0, causal_pos0, kind, BM);
 }
 
 // Tile table of a dense product whose A rows are sharded over ranks in blocks of src_rows (a multiple of 128).
@@ -490,7 +490,7 @@ int bl_gemm_build_tiles_sharded(const int* total_rows, void* mtiles, int* n_mtil
                                 cudaStream_t st) {
   BL_REQUIRE(max_mtiles >= 1 && src_rows >= BM && src_rows % BM == 0, BL_ERR_SHAPE);
   return (int)launch(build_mtiles_kernel, dim3(1), dim3(32), 0, st, total_rows, 1, (MTile*)mtiles, n_mtiles, max_mtiles,
-                     (int*)nullptr, 1, 0, 0, src_rows, 0, 0);
+                     (int*)nullptr, 1, 0, 0, src_rows, 0, 0, BM);
 }
 
 // C = A * B[g]^T per 128-row tile of the table.  A: [rows_a, K] bf16 (lda elements);

@@ -30,7 +30,7 @@ class TileTable:
 
     def build(self, group_rows: torch.Tensor, group_div: int = 1, group_stride: int = 0, base: int = 0,
               causal_pos0: int = -1, causal_kind: int = 0) -> None:
-        """group_rows int32 [n_groups] on the device.  Rows of group g follow group g-1 in A
+        """group_rows int32 [n_groups] on the device, together the table's rows at most; causal ones in tiles of 128.  Rows of group g follow group g-1 in A
         (or start at ``base + g * group_stride`` when ``group_stride`` > 0) and use B matrix
         ``g // group_div``."""
         self.fixed = 0                          # a launch writes the table now, and its number of tiles is on the device
@@ -44,7 +44,7 @@ class TileTable:
             return
         check(cuda().bl_gemm_build_tiles(p(group_rows), I(self.n_groups), p(self.mtiles), p(self.n_mtiles),
                                          I(self.max_mtiles), p(self.offsets), I(group_div), I(group_stride), I(base),
-                                         stream()), "bl_gemm_build_tiles")
+                                         I(self.tile_rows), stream()), "bl_gemm_build_tiles")
 
     @classmethod
     def sharded(cls, total_rows: int, src_rows: int, device) -> "TileTable":

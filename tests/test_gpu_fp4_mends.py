@@ -466,3 +466,30 @@ def test_the_dense_layers_and_the_shared_expert():
         y, tol = by_definition(act[:M], q(stem + "down" + suffix))
         want = y + x.double().cpu()
         assert bool(((bd.x[:M].double().cpu() - want).abs() <= tol + 2.0 ** -23 * want.abs()).all())
+
+
+# ---- tables built from rows a group ---------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("tile_rows", [32, 64, 128, 256])
+def test_tables_have_tiles_of_their_own_rows(tile_rows):
+    """Every row of ragged groups is in one tile, and the product over the table has them all."""
+    from bloomery_b200.ops.fp4 import Fp4Rows, fp4_gemm, fp4_rows
+    from bloomery_b200.ops.gemm import TileTable
+    groups, K, N = [0, 1, 300, 33, 128, 64, 0, 7], 128, 72
+    M = sum(groups)
+    t = TileTable(M, len(groups), DEV, tile_rows)
+    t.build(torch.tensor(groups, dtype=torch.int32, device=DEV))
+    want, lo = [], 0
+    for g, n in enumerate(groups):
+        want += [[g, lo + r, lo + n, 0] for r in range(0, n, tile_rows)]
+        lo += n
+    assert t.mtiles[:int(t.n_mtiles)].tolist() == want
+    x, rows, (q, v) = make(M, K, seed=2), Fp4Rows(M, K, DEV), weight(N, K, 3, len(groups))
+    fp4_rows(x, rows)
+    out = torch.empty(M, N, device=DEV)
+    fp4_gemm(rows, q, t, out_f32=out)
+    xv, lo = quantised(x)[3], 0
+    for g, n in enumerate(groups):
+        a = xv[lo:lo + n]
+        assert bool(((out[lo:lo + n].double().cpu() - a @ v[g].T).abs() <= allowed(a, v[g], K)).all())
+        lo += n
