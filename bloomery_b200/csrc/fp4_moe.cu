@@ -13,7 +13,10 @@
 //     expert by expert;
 //   * in the second launch the CTA that finishes the last tile of 128 output columns adds up the slots of every token, in order.
 // CTAs walk tiles next to each other, so that one takes part in two or three experts, or column blocks, and says so once for each.
-// Few tokens (FM_FEW): each CTA quantises the rows that it needs for itself, which is quicker than to wait for another one's.
+// One token or two (FM_FEW): each CTA quantises the rows that it needs for itself, which is quicker than to wait for another one's.  Rows of
+// each CTA's own / one form for all, us, eight experts a token: 30B shape 1 token 18.8 / 21.1, 2 tokens 23.3 / 23.5, 3 tokens 28.6 / 27.7; 235B
+// shape 32.1 / 35.3, 57.8 / 60.3, 71.2 / 70.3; 32 experts of 2,048 x 7,168 57.5 / 61.5, 90.9 / 89.2, 140.5 / 128.9; 4 tokens on the 30B
+// shape 36.5 / 32.9.
 // Rows are claimed and finished by whoever is there, so no CTA waits for one that has not started; the one wait between CTAs (for the tokens'
 // rows) is bounded like all others.  Sums of a slot run in one order: the same bits on every run and with every number of CTAs.
 // 24 tokens on the 30B shape (258 MB of weights): 66.5 us, 3.9 TB/s; 64 tokens on the 235B shape (1.38 GB): 283 to 297 us, 4.8 TB/s; one token
@@ -25,7 +28,9 @@
 namespace bl {
 
 constexpr int FM_TOKENS = 64, FM_SLOTS = 1024, FM_EXPERTS = 512, FM_WIDTH = 8192;
-constexpr int FM_FEW = 4, FM_FEW_SLOTS = 32;        // tokens and slots of a round whose CTAs quantise for themselves
+constexpr int FM_USED = 16;                         // experts of a token
+constexpr int FM_FEW = 2, FM_FEW_SLOTS = 32;        // tokens of a round whose CTAs quantise for themselves, and slots that one warp plans
+static_assert(FM_FEW * FM_USED <= FM_FEW_SLOTS, "the few-token plan has room for every slot");
 constexpr int FM_THREADS = F4_EPILOGUE + 128;
 
 struct FmArgs {
@@ -593,7 +598,7 @@ namespace bl {
 struct FmWork {
   long xq, act, aq, slot_out, total;
   FmWork(long rows, long k, long E, long H, long I, long sms) {
-    const long few = sms * (rows < FM_FEW ? rows : FM_FEW), own = few * k < sms * FM_FEW_SLOTS ? few * k : sms * FM_FEW_SLOTS;
+    const long few = sms * (rows < FM_FEW ? rows : FM_FEW), own = few * k;
     auto up = [](long n) { return (n + 127) / 128 * 128; };
     xq = up((2 + E + (H + 31) / 32) * 4);
     act = xq + up((rows > few ? rows : few) * fp4_row_bytes((int)H));
@@ -659,14 +664,14 @@ long bl_fp4_moe_work_bytes(int rows, int k, int E, int H, int I, int sms) { retu
 int bl_fp4_moe(const Fp4MoeCall* c) {
   BL_REQUIRE(c->T >= 1 && c->k >= 1 && c->E >= 1 && c->rows >= c->T && c->sms >= 1, BL_ERR_SHAPE);
   BL_REQUIRE(c->H >= 64 && c->H % 64 == 0 && c->I >= 64 && c->I % 64 == 0, BL_ERR_SHAPE);
-  BL_REQUIRE(c->rows <= FM_TOKENS && c->k <= 16 && c->E <= FM_EXPERTS && c->H <= FM_WIDTH && c->I <= FM_WIDTH, BL_ERR_LIMIT);
+  BL_REQUIRE(c->rows <= FM_TOKENS && c->k <= FM_USED && c->E <= FM_EXPERTS && c->H <= FM_WIDTH && c->I <= FM_WIDTH, BL_ERR_LIMIT);
   BL_REQUIRE((c->x_type == 0 || c->x_type == 2) && (!c->gain || c->x_type == 2), BL_ERR_TYPE);
   BL_REQUIRE(c->ldx >= c->H && c->ldx % (c->x_type == 2 ? 4 : 8) == 0 && ((uintptr_t)c->x & 15) == 0 && ((uintptr_t)c->gain & 15) == 0 &&
                  ((uintptr_t)c->work & 127) == 0 && ((uintptr_t)c->wg & 15) == 0 && ((uintptr_t)c->wu & 15) == 0 && ((uintptr_t)c->wd & 15) == 0,
              BL_ERR_ALIGN);
   BL_REQUIRE((c->c_f32 != nullptr) != (c->c_bf16 != nullptr), BL_ERR_SHAPE);
   const FmWork w(c->rows, c->k, c->E, c->H, c->I, c->sms);
-  const int few = c->T <= FM_FEW && c->T * c->k <= FM_FEW_SLOTS;
+  const int few = c->T <= FM_FEW;
   uint8_t* base = (uint8_t*)c->work;
   FmArgs a{c->x, c->ldx, c->x_type, c->gain, c->eps, c->ids, c->wts, c->T, c->k, c->E, c->H, c->I, (const uint8_t*)c->wg, (const uint8_t*)c->wu,
            (const uint8_t*)c->wd, base + w.xq, (float*)(base + w.act), base + w.aq, (float*)(base + w.slot_out), (int*)base, c->resid, c->ldr,
