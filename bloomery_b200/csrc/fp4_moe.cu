@@ -19,8 +19,9 @@
 // shape 36.5 / 32.9.
 // Rows are claimed and finished by whoever is there, so no CTA waits for one that has not started; the one wait between CTAs (for the tokens'
 // rows) is bounded like all others.  Sums of a slot run in one order: the same bits on every run and with every number of CTAs.
-// 24 tokens on the 30B shape (258 MB of weights): 66.5 us, 3.9 TB/s; 64 tokens on the 235B shape (1.38 GB): 283 to 297 us, 4.8 TB/s; one token
-// 19 us, latency.  The stream runs at 0.93 of the copy rate; the plan and first rows in front of it, and the last tickets, are the rest.
+// 24 tokens on the 30B shape (258 MB of weights): 66.8 us, 3.9 TB/s, 0.59 of the copy rate; 64 tokens on the 235B shape (1.38 GB): 284 to 300 us,
+// 4.6 to 4.9 TB/s under the power cap; one token 18.9 us, latency.  The plan and first rows stand in front of the weights' stream, the last tickets
+// behind it.
 #include <type_traits>
 
 #include "fp4_pipe.cuh"

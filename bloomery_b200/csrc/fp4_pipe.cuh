@@ -39,7 +39,10 @@ struct F4Work {
 
 // What a stage holds, in bytes from its start, and what it has in tensor memory, in columns.  Scales arrive for SPAN stages at once, in a
 // ring of their own: a box of 16 bytes a row costs TMA as much as one of 128.
-// ROOM: bytes of shared memory for both; WARPS: of the epilogue, four or eight; AR: weight rows of a tile.  The instruction multiplies 128
+// ROOM: bytes of shared memory for both; RAWS: slots of scales, two of which do: single matrices of 128 rows lose a stage to a third and are
+// slower (queries of 4,096 tokens 114 us with two, 120.5 with three, 121 with four; gate and up of 2,000 ids 70.7, 74.1, 74.2), smaller tiles and
+// rounds have room for more and are no different with them (one token 19.5 us with six or three, 20.1 with two).
+// WARPS: of the epilogue, four or eight; AR: weight rows of a tile.  The instruction multiplies 128
 // rows in any case; where few tokens meet few weights, tiles of fewer rows give more processors a share of the weights' way from
 // memory, and what the instruction reads behind the tile's rows ends in lanes that nobody reads.
 template <bool DUAL_, int BN_, int ROOM, int WARPS_, int AR_ = 128, int RAWS_ = AR_ < 128 ? 6 : 2>

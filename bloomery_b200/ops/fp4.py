@@ -61,7 +61,14 @@ class Fp4Rows:
 
 
 def fp4_tile_rows(rows: int, groups: int = 1, gated: bool = False) -> int:
-    """Rows of a tile of :func:`fp4_gemm` for ``rows`` rows dealt to ``groups`` matrices; ``gated``: with a second matrix."""
+    """Rows of a tile of :func:`fp4_gemm` for ``rows`` rows dealt to ``groups`` matrices; ``gated``: with a second matrix.
+
+    The smallest tile that holds a group's rows: a second tile of a group reads its weights again.  us, gate and up of 128 experts of
+    768 x 2,048: 32 rows each in tiles of 32 / 64: 44.3 / 45.7, 33 rows 61.6 / 45.8; 64 rows in tiles of 64 / 128: 47.7 / 51.8, 65 rows 71.2 /
+    55.5.  256 rows a tile halve what many rows ask of the weights and pad ragged groups more.  Tiles of 128 / 256: 4,096 x 8,192 for 512
+    rows 19.3 / 16.2, for 4,096 rows 119 / 101, but for 256 rows 11.1 / 15.4; 16 matrices of 512 x 512 with 256 rows each 6.2 / 8.1, with 1,024
+    11.4 / 10.8, with 1,100 11.5 / 14.1, with 1,500 15.4 / 14.2; eight of 4,096 x 4,096 with 512 rows each 63.9 / 61.4, with 1,100 149 / 137, with
+    2,048 263 / 223.  (Two limits could lie closer: a single matrix gains from 256 rows a tile past some 300 rows, wide groups past 128.)"""
     per = -(-rows // groups)
     return 32 if per <= 32 else 64 if per <= 64 else 128 if per <= (128 if groups == 1 else 1024) or gated else 256
 
@@ -82,8 +89,8 @@ def fp4_rows(x: torch.Tensor, out: Fp4Rows, *, gain: Optional[torch.Tensor] = No
     block's scale takes its own to 6; scales and codes are the nearest, ties go to the even code.  A row with a NaN or an
     infinity becomes one whose products are all NaN.  ``gain`` fp32 [k] (fp32 rows): RMSNorm first, with 1 / sqrt(mean square + eps)
     in fp32 (rows that are all zeros, or too small for that, need an ``eps``).  ``pos_of`` int32 [M * copies]:
-    row m goes to the rows ``pos_of[m * copies + j]`` of ``out`` (none where that is negative or past the end), as ``moe_plan``
-    deals the slots of M tokens."""
+    row m goes to the rows ``pos_of[m * copies + j]`` of ``out`` (none where that is negative or past the end; no place twice), as
+    ``moe_plan`` deals the slots of M tokens."""
     kind = _TYPES.get(x.dtype)
     index = out.index
     if kind is None or x.dim() != 2 or x.shape[1] != out.k or x.stride(1) != 1:
@@ -160,7 +167,7 @@ def fp4_gemm(X: Fp4Rows, W: QWeight, tiles: TileTable, *, out_f32: Optional[torc
     """C = X @ W[g].T per token tile, codes by codes on tcgen05 ``kind::mxf4nvf4`` with fp32 sums: ``X`` NVFP4 rows, W (and W2)
     resident NVFP4 matrices [N, bytes] or stacks [G, N, bytes]; tiles of 32, 64 or 128 rows, without W2 of 256 too
     (:func:`fp4_tile_rows`; :func:`fp4_tiles` for one matrix).  With W2 the output is silu(X W^T) * (X W2^T).  Epilogue options as :func:`gemm.qgemm`; a row
-    that ``dst_row`` sends below 0 or past the output goes nowhere.  Block scales are
+    that ``dst_row`` sends below 0 or past the output goes nowhere, and no two go to one place.  Block scales are
     taken without their sign, which no checkpoint sets (:func:`fp4_supports`)."""
     index, k = X.index, X.k
     wp = _matrix("W", W, k, index)

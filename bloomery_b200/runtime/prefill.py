@@ -127,7 +127,9 @@ class GemmPrefill:
 
     def _native_fp4(self) -> bool:
         """Whether prompts run on NVFP4 rows: where that is asked for, of a model whose layers are all routed and whose matrices are all
-        NVFP4 and on the card."""
+        NVFP4 and on the card.  At any length from the GEMM threshold on: next to kept bf16 copies of every weight prompts of 64 to 512 ids take
+        longer (30B shape, 128 ids 10.6 ms against 9.3, 512 10.7 against 10.0, 640 10.8 against 12.2, 4,096 32.3 against 41.8), next to none they
+        do not (11.4, 23.6, 24.4, 56.1), and this path is there to do without copies."""
         if not self.fp4_native or self.expert_source is not None:
             return False
         if self._fp4_ok is None:

@@ -51,7 +51,7 @@ REGISTRY: List[LeverSpec] = [
     LeverSpec("BLOOMERY_PREFILL", "word", "batch", "prompt path", ("batch", "steps")),
     LeverSpec("BLOOMERY_PREFILL_BF16", "word", "auto", "resident bf16 copy of the weights for the prompt path (auto = when it leaves a quarter of the card free)", ("auto", "0", "1")),
     LeverSpec("BLOOMERY_FP8_NATIVE", "bool", True, "batched pass: FP8 128x128 weights multiply E4M3 activations on the tensor cores (off = expand the weights to bf16 in flight)"),
-    LeverSpec("BLOOMERY_FP4_NATIVE", "bool", False, "batched pass and prompts: NVFP4 weights multiply NVFP4 activations on the tensor cores (off = activations keep 16 bits and the weights are expanded in flight)"),
+    LeverSpec("BLOOMERY_FP4_NATIVE", "bool", False, "one GPU, rounds of more than eight rows and prompts of 64 ids on: NVFP4 weights multiply NVFP4 activations on the tensor cores (off, and in shorter ones: activations keep 16 bits and the weights are expanded in flight)"),
     LeverSpec("BLOOMERY_NEED_HOOK", "str", "", "absolute path of a program run once per placed load with the need line on its standard input (exit 0 goes on, 75 = ask again later)"),
     LeverSpec("BLOOMERY_HOST_NATIVE", "bool", True, "-dev none: decode through the native host step where it covers the model (off = the plain PyTorch model)"),
     LeverSpec("BLOOMERY_PDL", "bool", True, "programmatic dependent launch between decode kernels"),
