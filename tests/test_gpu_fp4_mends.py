@@ -150,9 +150,10 @@ def test_norms_of_rows_whose_squares_pass_32_bits(K):
     fp4_rows(x, out, gain=gain)
     r = (1 / x.double().square().mean(1, keepdim=True).sqrt()).float()
     want = quantised(x * r * gain)
-    # ordinary rows (0, 4): their root may be the next fp32 number, 2^-23 away, and with it the largest value and the scale
+    # ordinary rows (0, 4): their root may be the next fp32 number, 2^-23 away; behind it two products and a quotient round on either side,
+    # 2^-24 each
     g = parts(out.data, K)[2].double()
-    assert bool(((g - want[2].double()).abs() <= 2.0 ** -22 * want[2].double()).all())
+    assert bool(((g - want[2].double()).abs() <= 2.0 ** -21 * want[2].double()).all())
     odd = [1, 2, 3, 5, 6]
     same(out.data[odd], K, tuple(t[odd] for t in want))
 
