@@ -145,7 +145,7 @@ class Fp4Work:
 def _rows_of(data: torch.Tensor, k: int) -> bool:
     """Whether these are one matrix, or a stack, of NVFP4 rows of k values."""
     shape = data.shape
-    return shape[-1] == (k // 2 + k // 16 + 19) // 16 * 16 and 2 <= len(shape) <= 3 and 0 not in shape and data.dtype is torch.uint8
+    return 2 <= len(shape) <= 3 and shape[-1] == (k // 2 + k // 16 + 19) // 16 * 16 and 0 not in shape and data.dtype is torch.uint8
 
 
 def _matrix(name: str, w: QWeight, k: int, index: int) -> int:

@@ -8,8 +8,8 @@ from test_fp4_contracts import w
 
 
 @pytest.mark.parametrize("data", [torch.zeros(16, 48, dtype=torch.uint8), torch.zeros(16, 96, dtype=torch.uint8), torch.zeros(2, 2, 16, 80, dtype=torch.uint8),
-                                  torch.zeros(80, dtype=torch.uint8), torch.zeros(16, 80, dtype=torch.int8), torch.zeros(0, 80, dtype=torch.uint8)],
-                         ids=["short rows", "long rows", "four dimensions", "one row", "signed", "no rows"])
+                                  torch.zeros(80, dtype=torch.uint8), torch.zeros(16, 80, dtype=torch.int8), torch.zeros(0, 80, dtype=torch.uint8), torch.zeros((), dtype=torch.uint8)],
+                         ids=["short rows", "long rows", "four dimensions", "one row", "signed", "no rows", "one byte"])
 def test_weights_that_are_not_rows_of_their_width(data):
     """Rows of 128 values are 80 bytes: others would be read past their end."""
     bad, rows = QWeight(data, "NVFP4", 128), Q.Fp4Rows(4, 128, "cpu")
